@@ -19,14 +19,18 @@ STATUS = {
 for _code, _name in STATUS.items():
     globals()[_name] = _code
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
 TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K, TYPE_IQ1_S, TYPE_MXFP4 = 8, 12, 14, 15, 19, 39
 POLICY_AUTO, POLICY_UNIFORM, POLICY_PLAN, POLICY_FREQUENCY, POLICY_LRU = range(5)
 ACT_SWIGLU, ACT_SWIGLU_OAI = 0, 1
 
-BLOCK_BYTES = {TYPE_Q8_0: 34, TYPE_Q8_K: 292, TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_MXFP4: 17, TYPE_IQ1_S: 50}
-BLOCK_ELEMS = {TYPE_Q8_0: 32, TYPE_Q8_K: 256, TYPE_Q4_K: 256, TYPE_Q6_K: 256, TYPE_MXFP4: 32, TYPE_IQ1_S: 256}
+BLOCK_BYTES = {TYPE_Q8_0: 34, TYPE_Q8_K: 292, TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_MXFP4: 17, TYPE_IQ1_S: 50,
+               TYPE_F32: 4, TYPE_F16: 2, TYPE_BF16: 2}
+BLOCK_ELEMS = {TYPE_Q8_0: 32, TYPE_Q8_K: 256, TYPE_Q4_K: 256, TYPE_Q6_K: 256, TYPE_MXFP4: 32, TYPE_IQ1_S: 256,
+               TYPE_F32: 1, TYPE_F16: 1, TYPE_BF16: 1}
 TYPE_NAMES = {TYPE_Q8_0: "q8_0", TYPE_Q4_K: "q4_K", TYPE_Q6_K: "q6_K", TYPE_Q8_K: "q8_K",
-              TYPE_IQ1_S: "iq1_s", TYPE_MXFP4: "mxfp4"}
+              TYPE_IQ1_S: "iq1_s", TYPE_MXFP4: "mxfp4",
+              TYPE_F32: "f32", TYPE_F16: "f16", TYPE_BF16: "bf16"}
 
 
 def row_bytes(t: int, n: int) -> int:
@@ -173,6 +177,11 @@ _SIGS = {
                                      C.POINTER(_P), _I64, _I64, C.POINTER(_P), _P, C.POINTER(gx_serve_stats)]),
     "gx_moe_ffn_noalloc": (C.c_int, [C.POINTER(gx_layer_desc), _P, C.c_uint64, C.c_uint32, _P, _P, _P, _I64, _I64,
                                      _P, _P]),
+    "gx_group_rows": (C.c_int, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "gx_mul_mat_grouped": (C.c_int, [C.c_int, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64,
+                                     C.c_int, C.c_int, _P, _I64, _P]),
+    "gx_mul_mat_grouped_glu": (C.c_int, [C.c_int, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
+                                         _I64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _I64, _P]),
     "gx_synth_normal": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
     "gx_synth_weights": (C.c_int, [C.c_int, _P, _I64, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
 }

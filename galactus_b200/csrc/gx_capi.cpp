@@ -252,7 +252,10 @@ int gx_device_init(int device) {
 int gx_device_error(int32_t * code_out) {
     return guarded([&] {
         int code = 0;
+        int grouped = 0;
         ck(gx::read_and_clear_device_error(&code));
+        ck(gx::read_and_clear_grouped_error(&grouped));
+        if (code == 0) code = grouped;
         if (code_out) *code_out = code;
         return GX_OK;
     });
@@ -668,6 +671,16 @@ int gx_mul_mat_id(int type, const void * as, int64_t ne00, int64_t ne01, int64_t
 
 int gx_quantize_rows(int vdt, const float * src, int64_t ne0, int64_t nrows, int64_t nb1, void * dst, int64_t dst_row_stride,
                      void * stream) {
+    if (vdt == GX_TYPE_F16 || vdt == GX_TYPE_BF16) {
+        if (src == nullptr || dst == nullptr || ne0 <= 0 || nrows < 0 || nb1 % 4) return GX_ERR_INVALID;
+        if (ne0 > 0x7fffffff || nrows > 0x7fffffff || nb1 < 0 || dst_row_stride < 2 * ne0) return GX_ERR_INVALID;
+        if (dst_row_stride % 2 || reinterpret_cast<uintptr_t>(dst) % 2 || reinterpret_cast<uintptr_t>(src) % 4) return GX_ERR_ALIGN;
+        return guarded([&] {
+            ck(gx::launch_round_rows(vdt == GX_TYPE_BF16, src, ne0, nrows, nb1, static_cast<uint8_t *>(dst),
+                                     dst_row_stride, reinterpret_cast<cudaStream_t>(stream)));
+            return GX_OK;
+        });
+    }
     if (vdt != GX_TYPE_Q8_0 && vdt != GX_TYPE_Q8_K) return GX_ERR_TYPE;
     if (src == nullptr || dst == nullptr || ne0 <= 0 || nrows < 0 || nb1 % 4) return GX_ERR_INVALID;
     if (ne0 % (vdt == GX_TYPE_Q8_0 ? 32 : 256) != 0) return GX_ERR_ALIGN;

@@ -1,0 +1,249 @@
+// Entry points of the operators on grouped rows: the grouping, the products
+// with unquantised experts and the adapters' low-rank deltas. No C++
+// exception crosses this boundary; every entry point returns GX_*.
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "../../include/galactus_b200.h"
+#include "gx_gmm.cuh"
+#include "gx_group.cuh"
+#include "gx_kernels.h"
+
+namespace gx {
+
+cudaError_t read_and_clear_grouped_error(int * code) {
+    int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_dev_error, sizeof(int));
+    if (e != cudaSuccess) return e;
+    return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int));
+}
+
+namespace {
+
+// One CTA per row and 1024 elements, four elements a thread. Bound by HBM.
+__global__ void __launch_bounds__(256) k_round_rows(bool bf16, const float * src, int ne0, int64_t nb1, uint8_t * dst,
+                                                    int64_t stride) {
+    const float * s = reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(src) + (int64_t)blockIdx.x * nb1);
+    uint8_t * d = dst + (int64_t)blockIdx.x * stride;
+    for (int64_t i = (int64_t)blockIdx.y * 1024 + threadIdx.x; i < ne0 && i < (int64_t)(blockIdx.y + 1) * 1024; i += 256)
+        store_out(d, (int)i, s[i], bf16 ? GMM_BF16 : GMM_F16);
+}
+
+}  // namespace
+
+cudaError_t launch_round_rows(bool bf16, const float * src, int64_t ne0, int64_t nrows, int64_t nb1, uint8_t * dst,
+                              int64_t stride, cudaStream_t stream) {
+    if (nrows == 0) return cudaSuccess;
+    const int64_t cols = (ne0 + 1023) / 1024;
+    if (cols > 65535) return cudaErrorInvalidValue;
+    k_round_rows<<<dim3((unsigned)nrows, (unsigned)cols), 256, 0, stream>>>(bf16, src, (int)ne0, nb1, dst, stride);
+    return cudaGetLastError();
+}
+
+}  // namespace gx
+
+namespace {
+
+int cuda_status(cudaError_t e) {
+    if (e == cudaSuccess) return GX_OK;
+    std::fprintf(stderr, "galactus_b200: CUDA error: %s\n", cudaGetErrorString(e));
+    return e == cudaErrorMemoryAllocation ? GX_ERR_NOMEM : GX_ERR_CUDA;
+}
+
+constexpr int kMaxDevices = 64;
+
+// multiprocessors of the current device
+int device_sms() {
+    static int sms[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+    if (sms[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        sms[dev] = n;
+    }
+    return sms[dev];
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void * f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// rows of K 16-bit elements, 128-byte swizzled boxes of 64 elements by `box` rows
+bool encode_rows(CUtensorMap * map, bool bf16, const void * base, int64_t K, int64_t rows, int64_t nb1, int64_t mats,
+                 int64_t nb2, uint32_t box) {
+    const auto enc = map_encoder();
+    if (enc == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)mats};
+    const cuuint64_t strides[2] = {(cuuint64_t)nb1, (cuuint64_t)nb2};
+    const cuuint32_t boxes[3] = {(cuuint32_t)gx::kGmmK, box, 1u};
+    const cuuint32_t elem[3] = {1u, 1u, 1u};
+    return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, mats > 0 ? 3 : 2,
+               const_cast<void *>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool misaligned(const void * p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+int out_kind(int type) {
+    return type == GX_TYPE_F32 ? gx::GMM_F32 : type == GX_TYPE_F16 ? gx::GMM_F16 : type == GX_TYPE_BF16 ? gx::GMM_BF16 : -1;
+}
+
+constexpr int64_t kMaxIndex = 0x7fffffff;
+constexpr int64_t kMaxStride = 1ll << 40;      // of a tensor map
+
+// The shared checks and the launch of the plain (up == NULL) and gated products.
+int grouped_product(int type, const void * as, const void * up, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02,
+                    int64_t n_as, const void * b, int64_t ne11, int64_t nb11, const int32_t * offsets,
+                    const int32_t * order, int64_t n_rows, int64_t gather, int scatter, int act, float alpha, float limit,
+                    int type_dst, void * dst, int64_t nbd1, void * stream) {
+    if (type != GX_TYPE_F16 && type != GX_TYPE_BF16) return GX_ERR_TYPE;
+    const int out = out_kind(type_dst);
+    if (out < 0) return GX_ERR_TYPE;
+    if (act != GX_ACT_SWIGLU && act != GX_ACT_SWIGLU_OAI) return GX_ERR_INVALID;
+    if (ne00 <= 0 || ne01 <= 0 || n_as <= 0 || ne11 < 0 || n_rows < 0 || gather < 0 || scatter < 0 || scatter > 1)
+        return GX_ERR_INVALID;
+    if (n_as > gx::kGroupMaxGroups || ne00 > kMaxIndex || ne01 > kMaxIndex || ne11 > kMaxIndex || n_rows > kMaxIndex ||
+        gather > kMaxIndex)
+        return GX_ERR_INVALID;
+    if (n_rows == 0) return GX_OK;
+    if (as == nullptr || b == nullptr || offsets == nullptr || dst == nullptr || ne11 == 0) return GX_ERR_INVALID;
+    if (order == nullptr && (gather != 0 || scatter != 0)) return GX_ERR_INVALID;
+    if (gather == 0 && ne11 < n_rows) return GX_ERR_INVALID;
+    const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
+    if (nb01 < 0 || nb02 < 0 || nb11 < 0 || nbd1 < 0 || nb01 >= kMaxStride || nb02 >= kMaxStride || nb11 >= kMaxStride)
+        return GX_ERR_INVALID;
+    if (n_as == 1) nb02 = nb01;                    // (never used to reach a second expert)
+    if (nb01 % 16 || nb02 % 16 || nb11 % 16 || misaligned(as, 16) || misaligned(b, 16) || (up && misaligned(up, 16)))
+        return GX_ERR_ALIGN;
+    if (nbd1 % esz || misaligned(dst, esz) || misaligned(offsets, 4) || (order && misaligned(order, 4))) return GX_ERR_ALIGN;
+    if (nb01 < 2 * ne00 || (n_as > 1 && nb02 < (ne01 - 1) * nb01 + 2 * ne00) || nb11 < 2 * ne00 || nbd1 < esz * ne01)
+        return GX_ERR_INVALID;
+    const bool glu = up != nullptr;
+
+    gx::GmmParams p{};
+    p.bf16 = type == GX_TYPE_BF16;
+    p.offsets = offsets;
+    p.order = order;
+    p.G = (int32_t)n_as;
+    p.n_rows = (int32_t)n_rows;
+    p.x_rows = (int32_t)ne11;
+    p.N = (int32_t)ne01;
+    p.K = (int32_t)ne00;
+    p.gather = (int32_t)gather;
+    p.scatter = scatter;
+    p.out = out;
+    p.dst = static_cast<uint8_t *>(dst);
+    p.nbd1 = nbd1;
+    p.act = act;
+    p.alpha = alpha;
+    p.limit = limit;
+    p.mt = (int32_t)((ne01 + gx::kGmmRows - 1) / gx::kGmmRows);
+    const int64_t touched = std::min(n_rows, n_as);
+    const int64_t avg = (n_rows + touched - 1) / touched;
+    p.nt = 32;
+    while (p.nt < (glu ? 128 : 256) && p.nt < 2 * avg) p.nt *= 2;
+    const uint32_t pre = (uint32_t)(n_as + 1) * 4u;
+    const uint32_t room = gx::kMaxSmem - 2048u - pre;
+    p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, room / gx::gmm_stage_bytes(glu, p.nt));
+    const uint32_t smem = 1024u + (uint32_t)p.stages * gx::gmm_stage_bytes(glu, p.nt) + pre;
+    if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows) ||
+        (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows)) ||
+        !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)gx::kGmmBox))
+        return GX_ERR_ALIGN;
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
+    const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
+    if (most > kMaxIndex) return GX_ERR_INVALID;
+    const dim3 grid((unsigned)std::min<int64_t>(sms, most));
+    const void * fn = glu ? (const void *)gx::k_gmm<true> : (const void *)gx::k_gmm<false>;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (glu) gx::k_gmm<true><<<grid, gx::kGmmThreads, smem, s>>>(p);
+    else gx::k_gmm<false><<<grid, gx::kGmmThreads, smem, s>>>(p);
+    return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+extern "C" {
+
+int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1, const int32_t * adapter, int64_t n_as,
+                  int64_t n_adapters, int32_t * order, int32_t * offsets, void * stream) {
+    if (ne20 <= 0 || ne21 < 0 || n_as <= 0 || n_adapters < 0) return GX_ERR_INVALID;
+    if (offsets == nullptr) return GX_ERR_INVALID;
+    if (ne21 > 0) {
+        if (order == nullptr || (adapter == nullptr) != (n_adapters == 0)) return GX_ERR_INVALID;
+        if (ids == nullptr && (adapter == nullptr || ne20 != 1 || n_as != 1)) return GX_ERR_INVALID;
+    }
+    if (ids != nullptr && (nbi1 < 4 * ne20 || nbi1 % 4)) return GX_ERR_INVALID;
+    if (n_as > gx::kGroupMaxGroups || n_adapters > gx::kGroupMaxGroups) return GX_ERR_INVALID;
+    const int64_t G = n_as * std::max<int64_t>(1, n_adapters);
+    if (G > gx::kGroupMaxGroups || ne20 > kMaxIndex || ne21 > kMaxIndex || ne20 * ne21 > kMaxIndex - 65536) return GX_ERR_INVALID;
+    if (misaligned(order, 4) || misaligned(offsets, 4) || misaligned(ids, 4) || misaligned(adapter, 4)) return GX_ERR_ALIGN;
+    gx::GroupParams p{};
+    p.ids = ids;
+    p.nbi1 = nbi1;
+    p.adapter = adapter;
+    p.k = (int32_t)ne20;
+    p.n_as = (int32_t)n_as;
+    p.n_adapters = (int32_t)n_adapters;
+    p.G = (int32_t)G;
+    p.P = (int32_t)(ne20 * ne21);
+    p.order = order;
+    p.offsets = offsets;
+    const uint32_t bins = (uint32_t)(G + 1) * 4u;
+    const int ncta = p.P <= 2048 ? 1 : gx::kGroupCluster;
+    const int most = (int)std::min<uint32_t>(32u, (gx::kGroupSmem - 2u * bins) / bins);
+    const int64_t steps = ((int64_t)p.P + 31) / 32;
+    p.warps = (int)std::max<int64_t>(1, std::min<int64_t>(most, (steps + ncta - 1) / ncta));
+    p.seg = (int)((steps + (int64_t)ncta * p.warps - 1) / ((int64_t)ncta * p.warps) * 32);
+    const int threads = std::max(32 * p.warps, G > 1024 ? 1024 : 256);
+    const uint32_t smem = (2u + (uint32_t)p.warps) * bins;
+    cudaError_t e = cudaFuncSetAttribute(gx::k_group_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ncta);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)ncta;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, gx::k_group_rows, p));
+}
+
+int gx_mul_mat_grouped(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as,
+                       const void * b, int64_t ne11, int64_t nb11, const int32_t * offsets, const int32_t * order,
+                       int64_t n_rows, int64_t gather, int scatter, int type_dst, void * dst, int64_t nbd1,
+                       void * stream) {
+    return grouped_product(type, as, nullptr, ne00, ne01, nb01, nb02, n_as, b, ne11, nb11, offsets, order, n_rows, gather,
+                           scatter, GX_ACT_SWIGLU, 0.0f, 0.0f, type_dst, dst, nbd1, stream);
+}
+
+int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t ne00, int64_t ne01, int64_t nb01,
+                           int64_t nb02, int64_t n_as, const void * b, int64_t ne11, int64_t nb11,
+                           const int32_t * offsets, const int32_t * order, int64_t n_rows, int64_t gather, int scatter,
+                           int act, float alpha, float limit, int type_dst, void * dst, int64_t nbd1, void * stream) {
+    if (up == nullptr && n_rows > 0) return GX_ERR_INVALID;
+    return grouped_product(type, gate, up, ne00, ne01, nb01, nb02, n_as, b, ne11, nb11, offsets, order, n_rows, gather,
+                           scatter, act, alpha, limit, type_dst, dst, nbd1, stream);
+}
+
+}  // extern "C"

@@ -303,6 +303,11 @@ cudaError_t launch_synth_normal(float * dst, int64_t n, uint64_t seed, uint64_t 
 cudaError_t launch_synth_weights(int type, void * dst, int64_t ne00, int64_t n_rows, uint64_t seed, uint64_t stream_id,
                                  float sigma, cudaStream_t stream);
 cudaError_t read_and_clear_device_error(int * code);
+cudaError_t read_and_clear_grouped_error(int * code);
+
+// rows of ne0 f32 rounded to F16 / BF16
+cudaError_t launch_round_rows(bool bf16, const float * src, int64_t ne0, int64_t nrows, int64_t nb1, uint8_t * dst,
+                              int64_t dst_row_stride, cudaStream_t stream);
 uint64_t synth_key(uint64_t seed, uint64_t stream_id);
 
 }  // namespace gx

@@ -45,6 +45,9 @@ extern "C" {
 #define GX_ERR_COMM      -13  /* an NCCL call failed or NCCL could not be loaded */
 
 /* ggml type ids (ggml.h numbering) of the formats this library computes on */
+#define GX_TYPE_F32    0   /* results of the operators on grouped rows */
+#define GX_TYPE_F16    1   /* unquantised experts and adapters, their rows and results */
+#define GX_TYPE_BF16  30
 #define GX_TYPE_Q8_0   8
 #define GX_TYPE_Q4_K  12
 #define GX_TYPE_Q6_K  14
@@ -238,7 +241,9 @@ int gx_mul_mat_id(int type, const void * as, int64_t ne00, int64_t ne01, int64_t
                   float * dst, void * stream);
 
 /* Activation quantization alone (quantize_row_q8_0 / quantize_row_q8_K):
- * rows of ne0 f32 at src + i*nb1 -> blocks at dst + i*dst_row_stride. */
+ * rows of ne0 f32 at src + i*nb1 -> blocks at dst + i*dst_row_stride. With
+ * GX_TYPE_F16 or GX_TYPE_BF16 the rows are rounded to that type (to nearest,
+ * ties to even), ggml's activation type of F16 / BF16 weights. */
 int gx_quantize_rows(int vec_dot_type, const float * src, int64_t ne0, int64_t nrows, int64_t nb1,
                      void * dst, int64_t dst_row_stride, void * stream);
 
@@ -250,6 +255,67 @@ int gx_swiglu_oai(const float * g, const float * u, float * out, int64_t n, floa
 int gx_combine(const float * y, const float * w, float * out, int64_t H, int64_t k, int64_t T, void * stream);
 /* The library's exp, elementwise (the one SiLU uses) */
 int gx_expf(const float * x, float * y, int64_t n, void * stream);
+
+/* ----------------------------------------------------------- grouped rows
+ * The routed FFN of experts that are not quantised (ggml F16 and BF16), and
+ * the low-rank adapters of many requests beside a projection they share, on
+ * rows grouped by expert, by adapter, or by both. Everything is read on the
+ * device: no call waits for the host to learn a group's size, so the calls can
+ * be captured into a graph and follow gx_router_forward or gx_remap_serve's
+ * slots on one stream. All pointers belong to the current device; no call
+ * allocates or keeps anything, so calls on different streams are independent.
+ * One layer:
+ *   gx_router_forward(logits)                      -> ids, weights
+ *   gx_group_rows(ids)                             -> order, offsets
+ *   gx_mul_mat_grouped_glu(gate, up, x, gather=k)  -> h, rows in expert order
+ *   gx_mul_mat_grouped(down, h, scatter)           -> y [T, k, H]
+ *   gx_combine(y, weights)                         -> out [T, H]
+ *
+ * gx_group_rows: the P = ne20 * ne21 (slot s, token t) pairs p = t*ne20 + s by
+ * ascending key, pairs of one key by ascending p:
+ *   key = adapter[t] * n_as + ids[t, s]
+ * ids: device i32 [ne20, ne21], nbi1 bytes between tokens (NULL with ne20 = 1
+ * and n_as = 1: dense adapters). adapter: device i32 [ne21], or NULL with
+ * n_adapters = 0. A negative id or adapter takes the pair out of every group.
+ * order: device i32 [P], the pairs in group order, pairs of no group last, by
+ * ascending p; offsets: device i32 [G + 1], G = n_as * max(1, n_adapters) <=
+ * 8192, group g's pairs are order[offsets[g] .. offsets[g+1]). An id >= n_as or
+ * an adapter >= n_adapters is reported (gx_device_error) and its pair dropped. */
+int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1, const int32_t * adapter, int64_t n_as,
+                  int64_t n_adapters, int32_t * order, int32_t * offsets, void * stream);
+
+/* Products of the groups with their experts' matrices:
+ *   dst row of j = W_g (b row of j)      for offsets[g] <= j < offsets[g+1]
+ *   as       F16 or BF16, row r of expert g at as + g*nb02 + r*nb01, ne00 x ne01
+ *            per expert, n_as experts (an arena's slots are experts here:
+ *            nb02 = the record)
+ *   b        ne11 rows of ne00 elements of the same type, nb11 bytes apart: the
+ *            caller rounds f32 activations to the weight type as ggml does
+ *            (gx_quantize_rows with GX_TYPE_F16 / GX_TYPE_BF16)
+ *   gather   0: row j of b; n > 0: row order[j] / n (n = k when b has one row
+ *            per token, 1 when it has one per pair)
+ *   scatter  0: row j of dst; 1: row order[j]
+ *   dst      rows of ne01 elements of type_dst (F32, F16, BF16), nbd1 bytes apart
+ * Products and sums are f32; the result is rounded once. order may be NULL
+ * when neither gather nor scatter reads it. offsets ascend from >= 0 to <=
+ * n_rows (the length of order; without gather b has at least n_rows rows).
+ * Rows of dst outside every group are left as they were. A group whose borders
+ * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped;
+ * a row index outside b or dst is reported and its result is NaN or dropped.
+ * Requires 16-byte aligned as, b and strides nb01, nb02, nb11 (so ne00 * 2 may
+ * need padded rows), n_as <= 8192. */
+int gx_mul_mat_grouped(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as,
+                       const void * b, int64_t ne11, int64_t nb11, const int32_t * offsets, const int32_t * order,
+                       int64_t n_rows, int64_t gather, int scatter, int type_dst, void * dst, int64_t nbd1,
+                       void * stream);
+/* The gate and up products and the activation in one pass (gate and up share
+ * their strides): dst row of j = act(G_g b_j, U_g b_j), act GX_ACT_SWIGLU or
+ * GX_ACT_SWIGLU_OAI (alpha, limit) as gx_swiglu / gx_swiglu_oai compute them,
+ * in f32 on the f32 sums, rounded once to type_dst. */
+int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t ne00, int64_t ne01, int64_t nb01,
+                           int64_t nb02, int64_t n_as, const void * b, int64_t ne11, int64_t nb11,
+                           const int32_t * offsets, const int32_t * order, int64_t n_rows, int64_t gather, int scatter,
+                           int act, float alpha, float limit, int type_dst, void * dst, int64_t nbd1, void * stream);
 
 /* ------------------------------------------------------------- MoE layer
  * One routed-expert FFN layer, end to end on the device:
