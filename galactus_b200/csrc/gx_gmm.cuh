@@ -17,19 +17,24 @@
 
 namespace gx {
 
-constexpr int kGmmRows = 128;                  // matrix rows of a tile (MMA M)
+constexpr int kGmmRows = 128;                  // matrix rows of a CTA's tile: TMEM lanes (gated: 64 gate and 64 up rows)
 constexpr int kGmmK = 64;                      // elements of K per stage: one 128-byte swizzled row
 constexpr uint32_t kGmmATile = kGmmRows * 128u;
 constexpr int kGmmMaxStages = 12;
-constexpr int kGmmThreads = 192;               // producer, MMA issuer, 4 epilogue warps
-constexpr int kGmmBox = 32;                    // rows of one TMA box of x (rows in place)
+constexpr int kGmmGatherWarps = 8;
+constexpr int kGmmEpiWarps = 4;
+constexpr int kGmmThreads = 32 * (2 + kGmmGatherWarps + kGmmEpiWarps);
+constexpr uint32_t kGmmStaging = kGmmEpiWarps * 32u * 32u * 4u;   // results of 32 columns per epilogue warp
+constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer][warp pair][direction][column][lane] f32
 
 enum : int { GMM_F32 = 0, GMM_F16 = 1, GMM_BF16 = 2 };
 
 struct GmmParams {
-    CUtensorMap wmap;         // W (or G): [K, N, G], boxes 64 x 128
+    CUtensorMap wmap;         // W (or G): [K, N, G], boxes 64 x 128 (gated: 64 x 64)
     CUtensorMap umap;         // U
-    CUtensorMap xmap;         // x: [K, rows], boxes 64 x 32, or 64 x 1 for gathers
+    CUtensorMap xmap;         // x in place: [K, rows], boxes 64 x box
+    const uint8_t * x;
+    int64_t nb11;
     const int32_t * offsets;  // [G + 1]
     const int32_t * order;    // [n_rows] or NULL
     int32_t G, n_rows, x_rows;
@@ -42,20 +47,57 @@ struct GmmParams {
     int64_t nbd1;
     int32_t act;              // GX_ACT_*
     float alpha, limit;
-    int32_t nt;               // rows of a group per tile (multiple of 16)
+    int32_t nt;               // rows of a group per tile (multiple of 32)
     int32_t stages;
-    int32_t mt;               // tiles of 128 matrix rows
+    int32_t box;              // rows of one TMA box of x in place (divides nt / CTAs)
+    int32_t mt;               // tiles of the matrix rows
 };
 
 // ------------------------------------------------------------ PTX helpers
 
-// D[tmem] (+)= A x B^T, f16 or bf16 operands, f32 accumulators, one thread
+template <int CTAS>
+__device__ __forceinline__ void gmm_tmem_alloc(uint32_t * dst, uint32_t cols) {
+    if constexpr (CTAS == 1) {
+        tmem_alloc(dst, cols);
+        tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void gmm_tmem_free(uint32_t addr, uint32_t cols) {
+    if constexpr (CTAS == 1) tmem_dealloc(addr, cols);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+
+// D[tmem] (+)= A x B^T, f16 or bf16 operands, f32 accumulators, one thread (of
+// the leading CTA; a pair's A is 2 x 128 rows and each CTA holds half of B's rows)
+template <int CTAS>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
-        : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+            : "memory");
+}
+
+// the barrier (in both CTAs of a pair) arrives once this thread's MMAs so far are done
+template <int CTAS>
+__device__ __forceinline__ void gmm_commit(uint64_t * bar) {
+    if constexpr (CTAS == 1) mma_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
 }
 
 // instruction descriptor of kind::f16: f32 accumulator, A and B of one type, both K-major
@@ -63,26 +105,62 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(bool bf16, uint32_t M, uin
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_load_2d(void * dst, const CUtensorMap * map, int x, int y, uint64_t * bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
+// TMA tiles into this CTA's shared memory. In a pair the bytes are counted on
+// the leading CTA's barrier: bit 24 of a shared-memory address tells the
+// CTAs of a pair apart, and cta_group::2 lets a copy signal its peer.
+constexpr uint32_t kLeaderMask = 0xFEFFFFFFu;
+
+template <int CTAS>
+__device__ __forceinline__ void gmm_tma_3d(void * dst, const CUtensorMap * map, int x, int y, int z, uint64_t * bar) {
+    if constexpr (CTAS == 1) tma_load_3d(dst, map, x, y, z, bar);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+            "%4}], [%5];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar) & kLeaderMask)
+            : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void gmm_tma_2d(void * dst, const CUtensorMap * map, int x, int y, uint64_t * bar) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar) & kLeaderMask)
+            : "memory");
 }
 
-// four rows of a one-row-box map (no multicast: this GPU's own memory)
-__device__ __forceinline__ void tma_gather4(void * dst, const CUtensorMap * map, int x, int r0, int r1, int r2, int r3,
-                                            uint64_t * bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
-        : "memory");
-}
-
+// arrive on the barrier of the leading CTA
+template <int CTAS>
 __device__ __forceinline__ void gmm_arrive(uint64_t * bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar))
+            : "memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// the first `bytes` of them, zeros behind
+__device__ __forceinline__ void cp_async16_part(uint32_t dst, const void * src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 __device__ __forceinline__ uint64_t global_ns() {
@@ -91,22 +169,49 @@ __device__ __forceinline__ uint64_t global_ns() {
     return t;
 }
 
-// Bounded wait: gives up after two seconds, or once another role of the CTA has.
+// one poll of a phase, with what the peer CTA's arrivals released (suspends for a while)
+template <int CTAS>
+__device__ __forceinline__ bool gmm_poll(uint64_t * bar, uint32_t parity) {
+    if constexpr (CTAS == 1) return mbar_try_wait(bar, parity);
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, "
+        "p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// Bounded wait of a warp: gives up after two seconds, or once another role of the CTA has.
+template <int CTAS>
 __device__ __forceinline__ bool gmm_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
-    if (mbar_test_wait(bar, parity)) return true;
+    bool ok = false;
     uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+    for (uint32_t i = 1; !(ok = gmm_poll<CTAS>(bar, parity)); ++i) {
         if ((i & 63u) == 0u) {
-            if (*abort_flag != 0) return false;
+            if (*abort_flag != 0) break;
             const uint64_t t = global_ns();
             if (t0 == 0) t0 = t;
-            else if (t - t0 > 2000000000ull) break;
+            else if (t - t0 > 2000000000ull) {
+                *abort_flag = 1;
+                record_error(GX_DEVERR_TIMEOUT);
+                break;
+            }
         }
     }
-    *abort_flag = 1;
-    record_error(GX_DEVERR_TIMEOUT);
-    return false;
+    return __all_sync(0xffffffffu, ok);
+}
+
+// and of a value over the two warps that share a named barrier
+__device__ __forceinline__ bool pair_agrees(int id, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "r"(id)
+        : "memory");
+    return r != 0;
 }
 
 #define kNan __int_as_float(0x7fc00000)
@@ -162,12 +267,13 @@ struct GmmTile {
     int g, m0, row0, cnt;
 };
 
-// tile t of the launch: the 128-row tiles of the matrix run fastest, so that
-// CTAs at work together read the same rows and one expert's weights
-__device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t * pre, int t) {
+// tile t of the launch: the tiles of the matrix run fastest, so that CTAs at
+// work together read the same rows and one expert's weights (m0: its first
+// matrix row, `rows` per tile)
+__device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t * pre, int t, int rows) {
     GmmTile r;
     const int tt = t / p.mt;
-    r.m0 = (t - tt * p.mt) * kGmmRows;
+    r.m0 = (t - tt * p.mt) * rows;
     r.g = tile_group(pre, p.G, tt);
     const int lo = p.offsets[r.g], hi = p.offsets[r.g + 1];
     r.row0 = lo + (tt - pre[r.g]) * p.nt;
@@ -203,15 +309,104 @@ __device__ __forceinline__ void store_out(uint8_t * row, int n, float v, int out
     else reinterpret_cast<__half *>(row)[n] = __float2half_rn(v);
 }
 
+// e^x without branches: x is clamped to where the result leaves the normal
+// range (n = 128 makes the scale infinite), n = x log2 e to nearest, r = x -
+// n ln 2 with ln 2 in two parts (Cody and Waite, 1980), e^r by its Taylor
+// polynomial; within 2 f32 steps on the normal range
+__device__ __forceinline__ float gmm_exp(float x) {
+    x = fminf(fmaxf(x, -87.0f), 89.0f);
+    const float t = __fmaf_rn(x, 1.44269502162933349609375f, 12582912.0f);
+    const float n = __fsub_rn(t, 12582912.0f);
+    float r = __fmaf_rn(-n, 0.693145751953125f, x);
+    r = __fmaf_rn(-n, 1.428606765330187045e-06f, r);
+    float q = __fmaf_rn(r, 1.98412701138295233249664306640625e-04f, 1.3888889225199818611145019531250e-03f);
+    q = __fmaf_rn(q, r, 8.3333337679505348205566406250000e-03f);
+    q = __fmaf_rn(q, r, 4.1666667908430099487304687500000e-02f);
+    q = __fmaf_rn(q, r, 1.6666667163372039794921875000000e-01f);
+    q = __fmaf_rn(q, r, 0.5f);
+    q = __fmaf_rn(q, r, 1.0f);
+    q = __fmaf_rn(q, r, 1.0f);
+    return __fmul_rn(q, __uint_as_float((__float_as_uint(t) + 127u) << 23));
+}
+
+// The activation on f32 sums. The quotient is CUDA's fast division (2 steps):
+// the sums are not those of the bit-exact formats anyway, and a full division
+// per value kept the epilogue behind the tensor cores.
 __device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) {
-    return p.act == 0 ? act_swiglu(g, u) : act_swiglu_oai(g, u, p.alpha, p.limit);
+    if (p.act == 0) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, gmm_exp(-g))), u);
+    const float x = p.limit < g ? p.limit : g;
+    const float y = u < -p.limit ? -p.limit : (p.limit < u ? p.limit : u);
+    return __fmul_rn(__fdividef(x, __fadd_rn(1.0f, gmm_exp(__fmul_rn(p.alpha, -x)))), __fadd_rn(y, 1.0f));
 }
 
-__host__ __device__ constexpr uint32_t gmm_stage_bytes(bool glu, int nt) {
-    return kGmmATile * (glu ? 2u : 1u) + (uint32_t)nt * 128u;
+// bytes of a ring stage: the matrix tile and the CTA's rows
+__host__ __device__ constexpr uint32_t gmm_stage_bytes(int ctas, int nt) { return kGmmATile + (uint32_t)(nt / ctas) * 128u; }
+
+// position in the ring of stages: stage, and how often the ring was gone round
+struct RingPos {
+    int s = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++s == stages) {
+            s = 0;
+            ++round;
+        }
+    }
+};
+
+// 32 (or 16) columns of a warp's 32 matrix rows, staged as [column][row], to
+// their result rows: 16-byte pieces where rows allow them (`vec`), element by
+// element at a ragged edge. `my` is lane i's result row of column i.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_rows(const GmmParams & p, const uint8_t * stage, int my, int n0, bool vec) {
+    constexpr int kPer = 16 / (int)sizeof(T);                 // elements of a piece
+    constexpr int kLanes = 32 / kPer;                         // lanes of a row
+    const int lane = threadIdx.x & 31, sub = lane % kLanes;
+    const int n = n0 + sub * kPer;
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32 / kLanes) {
+        const int col = c + lane / kLanes;
+        const int row = __shfl_sync(0xffffffffu, my, col);
+        if (row < 0) continue;
+        const uint4 v = *reinterpret_cast<const uint4 *>(stage + (uint32_t)(col * 32 + sub * kPer) * sizeof(T));
+        T * out = reinterpret_cast<T *>(p.dst + (int64_t)row * p.nbd1) + n;
+        if (vec && n + kPer <= p.N) *reinterpret_cast<uint4 *>(out) = v;
+        else {
+            const T * e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (n + i < p.N) out[i] = e[i];
+        }
+    }
 }
 
-template <bool GLU>
+template <typename T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// lane's COLS values, rounded, through the warp's staging area to the result rows
+template <typename T, int COLS>
+__device__ __forceinline__ void put_rows(const GmmParams & p, uint8_t * stage, const float (&v)[COLS], int my, int n0, bool vec) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) reinterpret_cast<T *>(stage)[i * 32 + lane] = round_to<T>(v[i]);
+    __syncwarp();
+    store_rows<T, COLS>(p, stage, my, n0, vec);
+}
+template <int COLS>
+__device__ __forceinline__ void put_rows_as(const GmmParams & p, uint8_t * stage, const float (&v)[COLS], int my, int n0, bool vec) {
+    if (p.out == GMM_F32) put_rows<float, COLS>(p, stage, v, my, n0, vec);
+    else if (p.out == GMM_BF16) put_rows<__nv_bfloat16, COLS>(p, stage, v, my, n0, vec);
+    else put_rows<__half, COLS>(p, stage, v, my, n0, vec);
+}
+
+template <int CTAS, bool GLU>
 __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ GmmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], drained;
@@ -219,167 +414,244 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     __shared__ int32_t wsum[kGmmThreads / 32];
     __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);              // CTA of the pair; 0 leads
+    const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const uint32_t stage_bytes = gmm_stage_bytes(GLU, p.nt);
-    int32_t * pre = reinterpret_cast<int32_t *>(ring + (uint32_t)p.stages * stage_bytes);
-    constexpr uint32_t kB = kGmmATile * (GLU ? 2u : 1u);   // the rows' tile inside a stage
-    // TMEM columns: two accumulator buffers of (one or two) nt columns
-    const uint32_t acc_cols = (uint32_t)p.nt * (GLU ? 2u : 1u);
+    const uint32_t stage_bytes = gmm_stage_bytes(CTAS, p.nt);
+    uint8_t * staging = ring + (uint32_t)p.stages * stage_bytes;
+    float * xchg = reinterpret_cast<float *>(staging + kGmmStaging);
+    int32_t * pre = reinterpret_cast<int32_t *>(staging + kGmmStaging + (GLU ? kGmmXchg : 0u));
+    constexpr int kOut = GLU ? kGmmRows / 2 : kGmmRows;                  // result rows of a CTA's tile
+    constexpr int kRound = 16 * CTAS;                                    // MMA N: a multiple of this
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1);
+            mbar_init(full + i, 1 + (p.gather ? CTAS : 0));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, 4);
+            mbar_init(acc_empty + i, kGmmEpiWarps * CTAS);
         }
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 1) {
-        tmem_alloc(&tslot, 512);
-        tmem_relinquish();
-    }
+    if (warp == 1) gmm_tmem_alloc<CTAS>(&tslot, 512);
     tile_prefix(pre, wsum, p.offsets, p.G, p.n_rows, p.nt);
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CTAS == 1) __syncthreads(); else cluster_sync_all();
     tc_fence_after();
     const uint32_t tbase = tslot;
     const int tiles = pre[p.G] * p.mt;
     const int nk = (p.K + kGmmK - 1) / kGmmK;
 
     if (warp == 0) {
-        // ------------------------------------------------------- producer
+        // ------------------------------------------- weights, rows in place
         int c = 0, done = 0;           // chunks started; chunks whose stage was handed back
+        RingPos at;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const GmmTile q = gmm_tile(p, pre, t);
-            const int quads = (q.cnt + 3) >> 2;                  // rows in fours (the last repeats its final row)
-            const int boxes = (q.cnt + kGmmBox - 1) / kGmmBox;
-            const uint32_t bytes = kB + (p.gather ? (uint32_t)quads * 512u : (uint32_t)boxes * (kGmmBox * 128u));
-            int r[2][4];
-            if (p.gather) {
-                for (int h = 0; h < 2; ++h)
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = min((h * 32 + lane) * 4 + i, q.cnt - 1);
-                        r[h][i] = gmm_src_row(p, q.row0 + j);
-                    }
+        for (int t = unit; t < tiles && ok; t += units) {
+            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+            const int m0 = q.m0 + rank * kOut;
+            const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
+            const int r0 = q.row0 + rank * half;
+            uint32_t bytes = (uint32_t)CTAS * kGmmATile;
+            int boxes = 0;
+            if (!p.gather) {
+                for (int r = 0; r < CTAS; ++r) {
+                    const int b = (max(0, min(half, q.cnt - r * half)) + p.box - 1) / p.box;
+                    bytes += (uint32_t)b * (p.box * 128u);
+                    if (r == rank) boxes = b;
+                }
             }
-            for (int kc = 0; kc < nk; ++kc, ++c) {
-                const int s = c % p.stages;
-                if (c >= p.stages) {
-                    ok = __all_sync(0xffffffffu, gmm_wait(empty + s, (uint32_t)((c / p.stages - 1) & 1), &abort_flag));
+            for (int kc = 0; kc < nk; ++kc, ++c, at.next(p.stages)) {
+                const int s = at.s;
+                if (at.round != 0) {
+                    ok = gmm_wait<CTAS>(empty + s, (at.round - 1u) & 1u, &abort_flag);
                     if (!ok) break;
                     ++done;
                 }
                 uint8_t * st = ring + (uint32_t)s * stage_bytes;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(full + s, bytes);
-                    tma_load_3d(st, &p.wmap, kc * kGmmK, q.m0, q.g, full + s);
-                    if (GLU) tma_load_3d(st + kGmmATile, &p.umap, kc * kGmmK, q.m0, q.g, full + s);
-                    if (!p.gather)
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(st + kB + (uint32_t)b * (kGmmBox * 128u), &p.xmap, kc * kGmmK, q.row0 + b * kGmmBox,
-                                        full + s);
+                    if (rank == 0) mbar_arrive_expect_tx(full + s, bytes);
+                    gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, full + s);
+                    if (GLU) gmm_tma_3d<CTAS>(st + kGmmATile / 2, &p.umap, kc * kGmmK, m0, q.g, full + s);
+                    for (int b = 0; b < boxes; ++b)
+                        gmm_tma_2d<CTAS>(st + kGmmATile + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box,
+                                         full + s);
                 }
                 __syncwarp();
-                if (p.gather) {
-                    if (lane < quads)
-                        tma_gather4(st + kB + (uint32_t)lane * 512u, &p.xmap, kc * kGmmK, r[0][0], r[0][1], r[0][2], r[0][3],
-                                    full + s);
-                    if (lane + 32 < quads)
-                        tma_gather4(st + kB + (uint32_t)(lane + 32) * 512u, &p.xmap, kc * kGmmK, r[1][0], r[1][1], r[1][2],
-                                    r[1][3], full + s);
-                }
             }
         }
-        if (!ok) {
+        if (!ok && rank == 0) {
             // copies in flight land before the CTA leaves
             volatile int none = 0;
-            for (int i = done; i < c; ++i) gmm_wait(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
+            for (int i = done; i < c; ++i) gmm_wait<CTAS>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------ MMA issuer
-        int c = 0, it = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++it) {
-            const GmmTile q = gmm_tile(p, pre, t);
-            const uint32_t n = (uint32_t)((q.cnt + 15) & ~15);
-            const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows, n);
+        int it = 0;
+        RingPos at;
+        bool ok = rank == 0;
+        for (int t = unit; t < tiles && ok; t += units, ++it) {
+            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+            const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
+            const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
             const int b = it & 1;
-            if (it >= 2) ok = __all_sync(0xffffffffu, gmm_wait(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag));
-            const uint32_t d = tbase + (uint32_t)b * acc_cols;
-            for (int kc = 0; kc < nk && ok; ++kc, ++c) {
-                const int s = c % p.stages;
-                ok = __all_sync(0xffffffffu, gmm_wait(full + s, (uint32_t)((c / p.stages) & 1), &abort_flag));
+            if (it >= 2) ok = gmm_wait<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
+            const uint32_t d = tbase + (uint32_t)b * 256u;
+            for (int kc = 0; kc < nk && ok; ++kc, at.next(p.stages)) {
+                const int s = at.s;
+                ok = gmm_wait<CTAS>(full + s, at.round & 1u, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 uint8_t * st = ring + (uint32_t)s * stage_bytes;
                 if (lane == 0) {
-                    const uint64_t da = umma_desc_sw128(st, 1024u), db = umma_desc_sw128(st + kB, 1024u);
-                    const uint64_t du = umma_desc_sw128(st + kGmmATile, 1024u);
+                    const uint64_t da = umma_desc_sw128(st, 1024u), db = umma_desc_sw128(st + kGmmATile, 1024u);
 #pragma unroll
-                    for (int i = 0; i < kGmmK / 16; ++i) {
-                        mma_f16(d, da + (uint64_t)(2 * i), db + (uint64_t)(2 * i), idesc, kc | i);
-                        if (GLU) mma_f16(d + p.nt, du + (uint64_t)(2 * i), db + (uint64_t)(2 * i), idesc, kc | i);
-                    }
-                    mma_commit(empty + s);
-                    if (kc == nk - 1) mma_commit(acc_full + b);
+                    for (int i = 0; i < kGmmK / 16; ++i)
+                        mma_f16<CTAS>(d, da + (uint64_t)(2 * i), db + (uint64_t)(2 * i), idesc, kc | i);
+                    gmm_commit<CTAS>(empty + s);
+                    if (kc == nk - 1) gmm_commit<CTAS>(acc_full + b);
                 }
                 __syncwarp();
             }
         }
-        if (!ok) {
+        if (!ok && rank == 0) {
             volatile int none = 0;
-            if (lane == 0) mma_commit(&drained);
+            if (lane == 0) gmm_commit<CTAS>(&drained);
             __syncwarp();
-            gmm_wait(&drained, 0, &none);
+            gmm_wait<CTAS>(&drained, 0, &none);
+        }
+    } else if (warp < 2 + kGmmGatherWarps) {
+        // -------------------------------------------------- gathered rows
+        // each warp fetches whole chunks of its own, every kGmmGatherWarps-th
+        // one, four rows of 128 bytes per step. The fence that shows a chunk
+        // to the tensor cores waits for all of the warp's copies in flight,
+        // so it is the warps, not one warp's chunks, that overlap.
+        if (p.gather) {
+            const int gw = warp - 2, sub = lane & 7, r4 = lane >> 3;
+            // 16-byte piece `sub` of rows r4, r4 + 4 (mod 8), swizzled
+            const uint32_t at0 = kGmmATile + (uint32_t)r4 * 128u + (uint32_t)((sub ^ r4) << 4);
+            const uint32_t at1 = kGmmATile + (uint32_t)(r4 + 4) * 128u + (uint32_t)((sub ^ (r4 + 4)) << 4);
+            const uint32_t pitch = (uint32_t)(p.nb11 >> 4);
+            int turn = 0;                                                         // whose chunk is next
+            RingPos at;
+            bool ok = true;
+            for (int t = unit; t < tiles && ok; t += units) {
+                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+                const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
+                const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
+                uint32_t mine[4];                                                 // x rows of rows lane + 32 i
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mine[i] = 0;
+                    if (i * 32 + lane < n) {
+                        const int o = p.order[q.row0 + rank * half + i * 32 + lane];
+                        const int row = o / p.gather;
+                        if (o < 0 || row >= p.x_rows) record_error(GX_DEVERR_DOMAIN);
+                        else mine[i] = (uint32_t)row;
+                    }
+                }
+                for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
+                    const bool skip = turn != gw;
+                    turn = turn + 1 == kGmmGatherWarps ? 0 : turn + 1;
+                    if (skip) continue;
+                    const int s = at.s;
+                    if (at.round != 0) {
+                        ok = gmm_wait<CTAS>(empty + s, (at.round - 1u) & 1u, &abort_flag);
+                        if (!ok) break;
+                    }
+                    const uint32_t dst = smem_u32(ring) + (uint32_t)s * stage_bytes;
+                    const uint8_t * col = p.x + (int64_t)kc * 128 + sub * 16;
+                    const int left = (p.K - kc * kGmmK) * 2 - sub * 16;           // bytes of the row from this piece on
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        if (h * 32 >= n) break;
+                        const uint8_t * src[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[h], i * 4 + r4) * pitch << 4);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t to = dst + ((i & 1) ? at1 : at0) + (uint32_t)(h * 4 + (i >> 1)) * 1024u;
+                            if (h * 32 + i * 4 + r4 < n) {
+                                // the last chunk of rows that end inside it: zeros behind the end
+                                if (left >= 16) cp_async16(to, src[i]);
+                                else cp_async16_part(to, left > 0 ? src[i] : p.x, (uint32_t)max(0, left));
+                            }
+                        }
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) gmm_arrive<CTAS>(full + s);
+                }
+            }
         }
     } else {
         // -------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lanes 32 * quad ..
-        int it = 0;
+        uint8_t * stage = staging + (uint32_t)quad * (kGmmStaging / kGmmEpiWarps);
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | (uintptr_t)p.nbd1) & 15u) == 0;
+        int it = 0, xb = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++it) {
-            const GmmTile q = gmm_tile(p, pre, t);
+        for (int t = unit; t < tiles && ok; t += units, ++it) {
+            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
             const int b = it & 1;
-            ok = __all_sync(0xffffffffu, gmm_wait(acc_full + b, (uint32_t)((it / 2) & 1), &abort_flag));
+            ok = gmm_wait<CTAS>(acc_full + b, (uint32_t)((it / 2) & 1), &abort_flag);
+            if constexpr (GLU) ok = pair_agrees(1 + (quad & 1), ok);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d = tbase + (uint32_t)b * acc_cols + ((uint32_t)quad << 21);
-            const int n = q.m0 + quad * 32 + lane;
-            for (int c0 = 0; c0 < q.cnt; c0 += 16) {
-                uint32_t v[16], u[16];
-                tmem_ld16(d + (uint32_t)c0, v);
-                if (GLU) tmem_ld16(d + (uint32_t)(p.nt + c0), u);
-                const int j = q.row0 + c0 + lane;
+            const uint32_t d = tbase + (uint32_t)b * 256u + ((uint32_t)quad << 21);
+            const int n0 = q.m0 + rank * kOut + (GLU ? quad & 1 : quad) * 32;
+            for (int c0 = 0; c0 < q.cnt; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld32(d + (uint32_t)c0, v);
                 bool nan = false;
-                const int my = (lane < 16 && c0 + lane < q.cnt) ? gmm_dst_row(p, j, nan) : -1;
+                int my = c0 + lane < q.cnt ? gmm_dst_row(p, q.row0 + c0 + lane, nan) : -1;
                 const unsigned nans = __ballot_sync(0xffffffffu, nan);
-                tmem_wait_ld();
+                if constexpr (GLU) {
+                    // quads 0, 1 hold gate rows, quads 2, 3 the same up rows:
+                    // each of a pair finishes 16 of the 32 columns
+                    const int pair = quad & 1, up = quad >> 1;
+                    float * sendp = xchg + (((xb * 2 + pair) * 2 + up) * 16) * 32 + lane;
+                    const float * recvp = xchg + (((xb * 2 + pair) * 2 + (up ^ 1)) * 16) * 32 + lane;
+                    float own[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int row = __shfl_sync(0xffffffffu, my, i);
-                    if (row >= 0 && n < p.N) {
-                        float a = __uint_as_float(v[i]);
-                        if (GLU) a = gmm_act(p, a, __uint_as_float(u[i]));
-                        store_out(p.dst + (int64_t)row * p.nbd1, n, (nans >> i) & 1u ? kNan : a, p.out);
+                    for (int i = 0; i < 16; ++i) {
+                        sendp[i * 32] = __uint_as_float(up ? v[i] : v[16 + i]);
+                        own[i] = __uint_as_float(up ? v[16 + i] : v[i]);
                     }
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
+                    my = __shfl_sync(0xffffffffu, my, (lane & 15) + 16 * up);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float other = recvp[i * 32];
+                        own[i] = gmm_act(p, up ? other : own[i], up ? own[i] : other);
+                        if ((nans >> (i + 16 * up)) & 1u) own[i] = kNan;
+                    }
+                    xb ^= 1;
+                    put_rows_as<16>(p, stage, own, my, n0, vec);
+                } else {
+                    float own[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) own[i] = (nans >> i) & 1u ? kNan : __uint_as_float(v[i]);
+                    put_rows_as<32>(p, stage, own, my, n0, vec);
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) gmm_arrive(acc_empty + b);
+            if (lane == 0) gmm_arrive<CTAS>(acc_empty + b);
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (CTAS == 1) __syncthreads(); else cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tbase, 512);
+        gmm_tmem_free<CTAS>(tbase, 512);
     }
 }
 

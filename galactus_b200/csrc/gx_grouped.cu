@@ -123,7 +123,8 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (order == nullptr && (gather != 0 || scatter != 0)) return GX_ERR_INVALID;
     if (gather == 0 && ne11 < n_rows) return GX_ERR_INVALID;
     const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
-    if (nb01 < 0 || nb02 < 0 || nb11 < 0 || nbd1 < 0 || nb01 >= kMaxStride || nb02 >= kMaxStride || nb11 >= kMaxStride)
+    if (nb01 < 0 || nb02 < 0 || nb11 < 0 || nbd1 < 0 || nb01 >= kMaxStride || nb02 >= kMaxStride ||
+        nb11 >= (1ll << 35))
         return GX_ERR_INVALID;
     if (n_as == 1) nb02 = nb01;                    // (never used to reach a second expert)
     if (nb01 % 16 || nb02 % 16 || nb11 % 16 || misaligned(as, 16) || misaligned(b, 16) || (up && misaligned(up, 16)))
@@ -135,6 +136,8 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
 
     gx::GmmParams p{};
     p.bf16 = type == GX_TYPE_BF16;
+    p.x = static_cast<const uint8_t *>(b);
+    p.nb11 = nb11;
     p.offsets = offsets;
     p.order = order;
     p.G = (int32_t)n_as;
@@ -150,31 +153,45 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     p.act = act;
     p.alpha = alpha;
     p.limit = limit;
-    p.mt = (int32_t)((ne01 + gx::kGmmRows - 1) / gx::kGmmRows);
     const int64_t touched = std::min(n_rows, n_as);
     const int64_t avg = (n_rows + touched - 1) / touched;
+    const int ctas = avg >= 96 ? 2 : 1;
     p.nt = 32;
-    while (p.nt < (glu ? 128 : 256) && p.nt < 2 * avg) p.nt *= 2;
-    const uint32_t pre = (uint32_t)(n_as + 1) * 4u;
-    const uint32_t room = gx::kMaxSmem - 2048u - pre;
-    p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, room / gx::gmm_stage_bytes(glu, p.nt));
-    const uint32_t smem = 1024u + (uint32_t)p.stages * gx::gmm_stage_bytes(glu, p.nt) + pre;
-    if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows) ||
-        (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows)) ||
-        !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)gx::kGmmBox))
+    if (ctas == 2) p.nt = 256;
+    else
+        while (p.nt < 128 && p.nt < 2 * avg) p.nt *= 2;
+    p.box = std::min(64, p.nt / ctas);
+    const int out_rows = (glu ? gx::kGmmRows / 2 : gx::kGmmRows) * ctas;
+    p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
+    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (glu ? gx::kGmmXchg : 0u);
+    const uint32_t stage = gx::gmm_stage_bytes(ctas, p.nt);
+    p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, (gx::kMaxSmem - 2048u - fixed) / stage);
+    const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
+    if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, glu ? gx::kGmmRows / 2 : gx::kGmmRows) ||
+        (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows / 2)) ||
+        (gather == 0 && !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, (uint32_t)p.box)))
         return GX_ERR_ALIGN;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
     const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
     if (most > kMaxIndex) return GX_ERR_INVALID;
-    const dim3 grid((unsigned)std::min<int64_t>(sms, most));
-    const void * fn = glu ? (const void *)gx::k_gmm<true> : (const void *)gx::k_gmm<false>;
+    const void * fn = ctas == 2 ? (glu ? (const void *)gx::k_gmm<2, true> : (const void *)gx::k_gmm<2, false>)
+                                : (glu ? (const void *)gx::k_gmm<1, true> : (const void *)gx::k_gmm<1, false>);
     cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_status(e);
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (glu) gx::k_gmm<true><<<grid, gx::kGmmThreads, smem, s>>>(p);
-    else gx::k_gmm<false><<<grid, gx::kGmmThreads, smem, s>>>(p);
-    return cuda_status(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(sms / ctas, most)));
+    cfg.blockDim = dim3(gx::kGmmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    void * args[] = {&p};
+    return cuda_status(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
 }  // namespace
