@@ -21,7 +21,7 @@ constexpr int kGmmRows = 128;                  // matrix rows of a CTA's tile: T
 constexpr int kGmmK = 64;                      // elements of K per stage: one 128-byte swizzled row
 constexpr uint32_t kGmmATile = kGmmRows * 128u;
 constexpr int kGmmMaxStages = 12;
-constexpr int kGmmGatherWarps = 8;
+constexpr int kGmmGatherWarps = 12, kGmmGatherSplit = 2;   // copying warps; warps that share a chunk
 constexpr int kGmmEpiWarps = 4;
 constexpr int kGmmThreads = 32 * (2 + kGmmGatherWarps + kGmmEpiWarps);
 constexpr uint32_t kGmmStaging = kGmmEpiWarps * 32u * 32u * 4u;   // results of 32 columns per epilogue warp
@@ -183,24 +183,32 @@ __device__ __forceinline__ bool gmm_poll(uint64_t * bar, uint32_t parity) {
     return done != 0;
 }
 
-// Bounded wait of a warp: gives up after two seconds, or once another role of the CTA has.
+// Bounded wait of a thread: gives up after two seconds, or once another role of the CTA has.
 template <int CTAS>
-__device__ __forceinline__ bool gmm_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
-    bool ok = false;
+__device__ __noinline__ bool gmm_wait_long(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
     uint64_t t0 = 0;
-    for (uint32_t i = 1; !(ok = gmm_poll<CTAS>(bar, parity)); ++i) {
+    for (uint32_t i = 1;; ++i) {
+        if (gmm_poll<CTAS>(bar, parity)) return true;
         if ((i & 63u) == 0u) {
-            if (*abort_flag != 0) break;
+            if (*abort_flag != 0) return false;
             const uint64_t t = global_ns();
             if (t0 == 0) t0 = t;
             else if (t - t0 > 2000000000ull) {
                 *abort_flag = 1;
                 record_error(GX_DEVERR_TIMEOUT);
-                break;
+                return false;
             }
         }
     }
-    return __all_sync(0xffffffffu, ok);
+}
+template <int CTAS>
+__device__ __forceinline__ bool gmm_wait_one(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
+    return gmm_poll<CTAS>(bar, parity) || gmm_wait_long<CTAS>(bar, parity, abort_flag);
+}
+// the same by a whole warp
+template <int CTAS>
+__device__ __forceinline__ bool gmm_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
+    return __all_sync(0xffffffffu, gmm_wait_one<CTAS>(bar, parity, abort_flag));
 }
 
 // and of a value over the two warps that share a named barrier
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1 + (p.gather ? CTAS : 0));
+            mbar_init(full + i, 1 + (p.gather ? CTAS * kGmmGatherSplit : 0));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -448,86 +456,84 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
 
     if (warp == 0) {
         // ------------------------------------------- weights, rows in place
-        int c = 0, done = 0;           // chunks started; chunks whose stage was handed back
-        RingPos at;
-        bool ok = true;
-        for (int t = unit; t < tiles && ok; t += units) {
-            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
-            const int m0 = q.m0 + rank * kOut;
-            const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
-            const int r0 = q.row0 + rank * half;
-            uint32_t bytes = (uint32_t)CTAS * kGmmATile;
-            int boxes = 0;
-            if (!p.gather) {
-                for (int r = 0; r < CTAS; ++r) {
-                    const int b = (max(0, min(half, q.cnt - r * half)) + p.box - 1) / p.box;
-                    bytes += (uint32_t)b * (p.box * 128u);
-                    if (r == rank) boxes = b;
+        if (lane == 0) {
+            int c = 0, done = 0;       // chunks started; chunks whose stage was handed back
+            RingPos at;
+            bool ok = true;
+            for (int t = unit; t < tiles && ok; t += units) {
+                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+                const int m0 = q.m0 + rank * kOut;
+                const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
+                const int r0 = q.row0 + rank * half;
+                uint32_t bytes = (uint32_t)CTAS * kGmmATile;
+                int boxes = 0;
+                if (!p.gather) {
+                    for (int r = 0; r < CTAS; ++r) {
+                        const int b = (max(0, min(half, q.cnt - r * half)) + p.box - 1) / p.box;
+                        bytes += (uint32_t)b * (p.box * 128u);
+                        if (r == rank) boxes = b;
+                    }
                 }
-            }
-            for (int kc = 0; kc < nk; ++kc, ++c, at.next(p.stages)) {
-                const int s = at.s;
-                if (at.round != 0) {
-                    ok = gmm_wait<CTAS>(empty + s, (at.round - 1u) & 1u, &abort_flag);
-                    if (!ok) break;
-                    ++done;
-                }
-                uint8_t * st = ring + (uint32_t)s * stage_bytes;
-                if (lane == 0) {
-                    if (rank == 0) mbar_arrive_expect_tx(full + s, bytes);
-                    gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, full + s);
-                    if (GLU) gmm_tma_3d<CTAS>(st + kGmmATile / 2, &p.umap, kc * kGmmK, m0, q.g, full + s);
+                for (int kc = 0; kc < nk; ++kc, ++c, at.next(p.stages)) {
+                    uint64_t * bar = full + at.s;
+                    if (at.round != 0) {
+                        ok = gmm_wait_one<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
+                        if (!ok) break;
+                        ++done;
+                    }
+                    uint8_t * st = ring + (uint32_t)at.s * stage_bytes;
+                    if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
+                    gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
+                    if (GLU) gmm_tma_3d<CTAS>(st + kGmmATile / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
                     for (int b = 0; b < boxes; ++b)
-                        gmm_tma_2d<CTAS>(st + kGmmATile + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box,
-                                         full + s);
+                        gmm_tma_2d<CTAS>(st + kGmmATile + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
                 }
-                __syncwarp();
+            }
+            if (!ok && rank == 0) {
+                // copies in flight land before the CTA leaves
+                volatile int none = 0;
+                for (int i = done; i < c; ++i) gmm_wait_one<CTAS>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
             }
         }
-        if (!ok && rank == 0) {
-            // copies in flight land before the CTA leaves
-            volatile int none = 0;
-            for (int i = done; i < c; ++i) gmm_wait<CTAS>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
-        }
+        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------ MMA issuer
-        int it = 0;
-        RingPos at;
-        bool ok = rank == 0;
-        for (int t = unit; t < tiles && ok; t += units, ++it) {
-            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
-            const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
-            const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
-            const int b = it & 1;
-            if (it >= 2) ok = gmm_wait<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
-            const uint32_t d = tbase + (uint32_t)b * 256u;
-            for (int kc = 0; kc < nk && ok; ++kc, at.next(p.stages)) {
-                const int s = at.s;
-                ok = gmm_wait<CTAS>(full + s, at.round & 1u, &abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                uint8_t * st = ring + (uint32_t)s * stage_bytes;
-                if (lane == 0) {
-                    const uint64_t da = umma_desc_sw128(st, 1024u), db = umma_desc_sw128(st + kGmmATile, 1024u);
+        if (lane == 0 && rank == 0) {
+            int it = 0;
+            RingPos at;
+            bool ok = true;
+            const uint64_t da0 = umma_desc_sw128(ring, 1024u), db0 = umma_desc_sw128(ring + kGmmATile, 1024u);
+            for (int t = unit; t < tiles && ok; t += units, ++it) {
+                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+                const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
+                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
+                const int b = it & 1;
+                if (it >= 2) ok = gmm_wait_one<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
+                const uint32_t d = tbase + (uint32_t)b * 256u;
+                for (int kc = 0; kc < nk && ok; ++kc, at.next(p.stages)) {
+                    ok = gmm_wait_one<CTAS>(full + at.s, at.round & 1u, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    // (a stage's address only touches the low word: 14 bits of 16 bytes)
+                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
 #pragma unroll
                     for (int i = 0; i < kGmmK / 16; ++i)
-                        mma_f16<CTAS>(d, da + (uint64_t)(2 * i), db + (uint64_t)(2 * i), idesc, kc | i);
-                    gmm_commit<CTAS>(empty + s);
-                    if (kc == nk - 1) gmm_commit<CTAS>(acc_full + b);
+                        mma_f16<CTAS>(d, da0 + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i), idesc, kc | i);
+                    gmm_commit<CTAS>(empty + at.s);
                 }
-                __syncwarp();
+                if (ok) gmm_commit<CTAS>(acc_full + b);
+            }
+            if (!ok) {
+                volatile int none = 0;
+                gmm_commit<CTAS>(&drained);
+                gmm_wait_one<CTAS>(&drained, 0, &none);
             }
         }
-        if (!ok && rank == 0) {
-            volatile int none = 0;
-            if (lane == 0) gmm_commit<CTAS>(&drained);
-            __syncwarp();
-            gmm_wait<CTAS>(&drained, 0, &none);
-        }
+        __syncwarp();
     } else if (warp < 2 + kGmmGatherWarps) {
         // -------------------------------------------------- gathered rows
-        // each warp fetches whole chunks of its own, every kGmmGatherWarps-th
-        // one, four rows of 128 bytes per step. The fence that shows a chunk
+        // a pair of warps fetches every kGmmGatherWarps/2-th chunk, 32-row
+        // blocks in turn, four rows of 128 bytes per step. The fence that shows a chunk
         // to the tensor cores waits for all of the warp's copies in flight,
         // so it is the warps, not one warp's chunks, that overlap.
         if (p.gather) {
@@ -543,20 +549,21 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                 const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
-                uint32_t mine[4];                                                 // x rows of rows lane + 32 i
+                uint32_t mine[4 / kGmmGatherSplit];                               // x rows of this warp's 32-row blocks
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 4 / kGmmGatherSplit; ++i) {
+                    const int r = (i * kGmmGatherSplit + gw % kGmmGatherSplit) * 32 + lane;
                     mine[i] = 0;
-                    if (i * 32 + lane < n) {
-                        const int o = p.order[q.row0 + rank * half + i * 32 + lane];
+                    if (r < n) {
+                        const int o = p.order[q.row0 + rank * half + r];
                         const int row = o / p.gather;
                         if (o < 0 || row >= p.x_rows) record_error(GX_DEVERR_DOMAIN);
                         else mine[i] = (uint32_t)row;
                     }
                 }
                 for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
-                    const bool skip = turn != gw;
-                    turn = turn + 1 == kGmmGatherWarps ? 0 : turn + 1;
+                    const bool skip = turn != gw / kGmmGatherSplit;
+                    turn = turn + 1 == kGmmGatherWarps / kGmmGatherSplit ? 0 : turn + 1;
                     if (skip) continue;
                     const int s = at.s;
                     if (at.round != 0) {
@@ -567,12 +574,13 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     const uint8_t * col = p.x + (int64_t)kc * 128 + sub * 16;
                     const int left = (p.K - kc * kGmmK) * 2 - sub * 16;           // bytes of the row from this piece on
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    for (int hh = 0; hh < 4 / kGmmGatherSplit; ++hh) {
+                        const int h = hh * kGmmGatherSplit + gw % kGmmGatherSplit;
                         if (h * 32 >= n) break;
                         const uint8_t * src[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[h], i * 4 + r4) * pitch << 4);
+                            src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[hh], i * 4 + r4) * pitch << 4);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const uint32_t to = dst + ((i & 1) ? at1 : at0) + (uint32_t)(h * 4 + (i >> 1)) * 1024u;

@@ -160,7 +160,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (ctas == 2) p.nt = 256;
     else
         while (p.nt < 128 && p.nt < 2 * avg) p.nt *= 2;
-    p.box = std::min(64, p.nt / ctas);
+    p.box = std::min(128, p.nt / ctas);
     const int out_rows = (glu ? gx::kGmmRows / 2 : gx::kGmmRows) * ctas;
     p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
     const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (glu ? gx::kGmmXchg : 0u);
