@@ -17,12 +17,12 @@ from .models import MODELS, ModelShape  # noqa: F401
 
 __all__ = [
     "Arena", "LayerShape", "SlotPolicy", "mul_mat_id", "record_layout", "MODELS", "ModelShape", "lib", "check",
-    "GxError", "group_rows", "mul_mat_grouped", "mul_mat_grouped_glu", "round_rows",
+    "GxError", "group_rows", "lora_mul_mat", "mul_mat_grouped", "mul_mat_grouped_glu", "round_rows",
 ]
 
 
 # the operators on grouped rows take torch tensors: torch is imported with the first of them
-_GROUPED = ("group_rows", "mul_mat_grouped", "mul_mat_grouped_glu", "round_rows")
+_GROUPED = ("group_rows", "lora_mul_mat", "mul_mat_grouped", "mul_mat_grouped_glu", "round_rows")
 
 
 def __getattr__(name):

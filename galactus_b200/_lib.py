@@ -101,6 +101,12 @@ class gx_shared_expert(C.Structure):
     _fields_ = [("record", C.c_void_p), ("desc", gx_layer_desc)]
 
 
+class gx_lora_desc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("rank", C.c_int32), ("ne00", C.c_int64), ("ne01", C.c_int64), ("n_as", C.c_int64),
+                ("n_adapters", C.c_int64), ("a", C.c_void_p), ("nba1", C.c_int64), ("nba2", C.c_int64), ("b", C.c_void_p),
+                ("nbb1", C.c_int64), ("nbb2", C.c_int64), ("ranks", C.c_void_p), ("scale", C.c_void_p)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _SIGS = {
@@ -182,6 +188,8 @@ _SIGS = {
                                      C.c_int, C.c_int, _P, _I64, _P]),
     "gx_mul_mat_grouped_glu": (C.c_int, [C.c_int, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64,
                                          _I64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _I64, _P]),
+    "gx_lora_mul_mat": (C.c_int, [C.POINTER(gx_lora_desc), _P, _I64, _I64, _P, _P, _I64, _I64, C.c_int, _P, _I64, _P, _I64,
+                                  _P]),
     "gx_synth_normal": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
     "gx_synth_weights": (C.c_int, [C.c_int, _P, _I64, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
 }

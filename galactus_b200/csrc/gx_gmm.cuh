@@ -235,15 +235,16 @@ __device__ __forceinline__ int2 group_rows_of(const int32_t * offsets, int g, in
     return make_int2(lo, hi);
 }
 
-// pre[g] = tiles of nt rows in the groups before g (G + 1 values), by the whole block
-__device__ __forceinline__ void tile_prefix(int32_t * pre, int32_t * wsum, const int32_t * offsets, int G, int n_rows,
-                                            int nt) {
+// pre[g] = tiles of nt rows in the groups before g (G + 1 values), by the
+// whole block; rows(g) are the rows of group g
+template <typename F>
+__device__ __forceinline__ void tile_prefix(int32_t * pre, int32_t * wsum, int G, int nt, F && rows) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = blockDim.x;
     const int per = (G + n - 1) / n;
     const int g0 = min(tid * per, G), g1 = min(g0 + per, G);
     int sum = 0;
     for (int g = g0; g < g1; ++g) {
-        const int2 r = group_rows_of(offsets, g, n_rows);
+        const int2 r = rows(g);
         pre[g] = sum;
         sum += (r.y - r.x + nt - 1) / nt;
     }
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
         mbar_fence_init();
     }
     if (warp == 1) gmm_tmem_alloc<CTAS>(&tslot, 512);
-    tile_prefix(pre, wsum, p.offsets, p.G, p.n_rows, p.nt);
+    tile_prefix(pre, wsum, p.G, p.nt, [&](int g) { return group_rows_of(p.offsets, g, p.n_rows); });
     tc_fence_before();
     if constexpr (CTAS == 1) __syncthreads(); else cluster_sync_all();
     tc_fence_after();

@@ -11,6 +11,7 @@
 #include "gx_gmm.cuh"
 #include "gx_group.cuh"
 #include "gx_kernels.h"
+#include "gx_lora.cuh"
 
 namespace gx {
 
@@ -261,6 +262,101 @@ int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t
     if (up == nullptr && n_rows > 0) return GX_ERR_INVALID;
     return grouped_product(type, gate, up, ne00, ne01, nb01, nb02, n_as, b, ne11, nb11, offsets, order, n_rows, gather,
                            scatter, act, alpha, limit, type_dst, dst, nbd1, stream);
+}
+
+int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_t nb11, const int32_t * offsets,
+                    const int32_t * order, int64_t n_rows, int64_t gather, int type_dst, const void * base, int64_t nbb,
+                    void * dst, int64_t nbd, void * stream) {
+    if (d == nullptr) return GX_ERR_INVALID;
+    if (d->type != GX_TYPE_F16 && d->type != GX_TYPE_BF16) return GX_ERR_TYPE;
+    const int out = out_kind(type_dst);
+    if (out < 0) return GX_ERR_TYPE;
+    const int64_t K = d->ne00, N = d->ne01;
+    int64_t nba2 = d->nba2, nbb2 = d->nbb2;
+    if (K <= 0 || N <= 0 || d->rank <= 0 || d->rank > GX_LORA_MAX_RANK || d->n_as <= 0 || d->n_adapters <= 0 || ne11 < 0 ||
+        n_rows < 0 || gather <= 0)
+        return GX_ERR_INVALID;
+    if (d->n_as > gx::kGroupMaxGroups || d->n_adapters > gx::kGroupMaxGroups || K > kMaxIndex || N > kMaxIndex ||
+        ne11 > kMaxIndex || n_rows > kMaxIndex || gather > kMaxIndex)
+        return GX_ERR_INVALID;
+    const int64_t G = d->n_as * d->n_adapters;
+    if (G > gx::kGroupMaxGroups) return GX_ERR_INVALID;
+    if (n_rows == 0) return GX_OK;
+    if (d->a == nullptr || d->b == nullptr || x == nullptr || offsets == nullptr || base == nullptr || dst == nullptr || ne11 == 0)
+        return GX_ERR_INVALID;
+    const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
+    if (d->nba1 < 0 || nba2 < 0 || d->nbb1 < 0 || nbb2 < 0 || nb11 < 0 || nbb < 0 || nbd < 0 || d->nba1 >= kMaxStride ||
+        nba2 >= kMaxStride || d->nbb1 >= kMaxStride || nbb2 >= kMaxStride || nb11 >= (1ll << 35))
+        return GX_ERR_INVALID;
+    if (G == 1) {                                      // (never used to reach a second adapter)
+        nba2 = d->nba1;
+        nbb2 = d->nbb1;
+    }
+    if (d->nba1 % 16 || nba2 % 16 || d->nbb1 % 16 || nbb2 % 16 || nb11 % 16 || misaligned(d->a, 16) || misaligned(d->b, 16) ||
+        misaligned(x, 16))
+        return GX_ERR_ALIGN;
+    if (nbb % esz || nbd % esz || misaligned(base, esz) || misaligned(dst, esz) || misaligned(offsets, 4) ||
+        misaligned(order, 4) || misaligned(d->ranks, 4) || misaligned(d->scale, 4))
+        return GX_ERR_ALIGN;
+    if (d->nba1 < 2 * K || d->nbb1 < 2 * d->rank || nb11 < 2 * K || nbb < esz * N || nbd < esz * N) return GX_ERR_INVALID;
+    if (G > 1 && (nba2 < (d->rank - 1) * d->nba1 + 2 * K || nbb2 < (N - 1) * d->nbb1 + 2 * d->rank)) return GX_ERR_INVALID;
+
+    gx::LoraParams p{};
+    p.x = static_cast<const uint8_t *>(x);
+    p.nb11 = nb11;
+    p.offsets = offsets;
+    p.order = order;
+    p.ranks = d->ranks;
+    p.scale = d->scale;
+    p.base = static_cast<const uint8_t *>(base);
+    p.dst = static_cast<uint8_t *>(dst);
+    p.nbb = nbb;
+    p.nbd = nbd;
+    p.G = (int32_t)G;
+    p.n_as = (int32_t)d->n_as;
+    p.n_rows = (int32_t)n_rows;
+    p.x_rows = (int32_t)ne11;
+    p.gather = (int32_t)gather;
+    p.N = (int32_t)N;
+    p.K = (int32_t)K;
+    p.rank = (int32_t)d->rank;
+    p.ra = 16;
+    while (p.ra < p.rank) p.ra *= 2;
+    p.bf16 = d->type == GX_TYPE_BF16;
+    p.out = out;
+    p.copy = base != dst;
+    if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
+    if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
+        !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u))
+        return GX_ERR_ALIGN;
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
+    // small ranks leave room for two CTAs per SM, whose phases overlap
+    const uint32_t fixed = gx::lora_fixed_bytes(p.ra, p.G), stage = gx::lora_stage_bytes(p.ra);
+    const int per_sm = fixed + 1024u + 4u * stage <= 113u * 1024u ? 2 : 1;
+    const uint32_t room = (per_sm == 2 ? 113u * 1024u : gx::kMaxSmem - 2048u) - 1024u - fixed;
+    p.stages = (int32_t)std::min<uint32_t>(gx::kLoraMaxStages, room / stage);
+    const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
+    const int64_t most = n_rows / gx::kLoraRows + std::min(n_rows, G);
+    // a cluster per tile of rows, of as many CTAs as still give every tile one
+    // at once (whether or not base is dst: the split of K sets the result's bits)
+    const int64_t slots = (int64_t)sms * per_sm;
+    int ctas = 8;
+    while (ctas > 1 && (most * ctas > slots || ctas > std::max((K + 63) / 64, (N + 127) / 128))) ctas /= 2;
+    cudaError_t e = cudaFuncSetAttribute(gx::k_lora, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(slots / ctas, most + (p.copy ? n_rows / gx::kLoraRows + 1 : 0))));
+    cfg.blockDim = dim3(gx::kLoraThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)ctas;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, gx::k_lora, p));
 }
 
 }  // extern "C"

@@ -1,0 +1,581 @@
+// Low-rank deltas of many requests' adapters beside a projection they share
+// (sm_100a, tcgen05 + TMA):
+//
+//   y_j = base_j + B_g (s_g A_g x_j)          j in the rows of group g
+//
+// A_g [rank, K] and B_g [N, rank] are F16 or BF16, x of the same type, base
+// and y F32, F16 or BF16.
+//
+// ONE kernel does both products: a cluster of C CTAs takes up to 64 rows of a
+// group. Each CTA multiplies its share of K (A_g on the M side, the rows on
+// the N side), the partial h of the CTAs meet in shared memory over the
+// cluster and are summed in CTA order, and each CTA then forms its share of
+// the N results, adds base and writes them. h never leaves the SMs, and a
+// call with one row still uses eight SMs.
+//
+// h is held in 32 bits. For the second product it is split into parts of the
+// operand type that sum to it (three BF16 parts: 24 bits; two F16 parts: 22
+// bits below the row's largest value, the row scaled by a power of two first
+// so that no h overflows F16), all multiplied with the same B tile in shared
+// memory: the deltas keep f32 accuracy for two extra MMAs per 16 ranks, which
+// the memory-bound kernel has time for.
+//
+// Ranks differ by adapter: rows of A and columns of B behind an adapter's
+// rank may hold anything and do not reach the result.
+#pragma once
+
+#include "gx_gmm.cuh"
+
+namespace gx {
+
+constexpr int kLoraRows = 64;                   // rows of a tile (MMA N)
+constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxStages = 8;
+constexpr int kLoraGatherWarps = 4;
+constexpr int kLoraEpiWarps = 4;
+constexpr int kLoraThreads = 32 * (2 + kLoraGatherWarps + kLoraEpiWarps);
+constexpr uint32_t kLoraXTile = kLoraRows * 128u;
+constexpr uint32_t kLoraBTile = 128u * 128u;    // 128 rows of B, 64 ranks
+constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
+
+struct LoraParams {
+    CUtensorMap amap;         // A: [K, rank, G], boxes 64 x ra
+    CUtensorMap bmap;         // B: [rank, N, G], boxes 64 x 128
+    const uint8_t * x;
+    int64_t nb11;
+    const int32_t * offsets;  // [G + 1]
+    const int32_t * order;    // [n_rows] or NULL: rows in place
+    const int32_t * ranks;    // [G / n_as] or NULL: all `rank`
+    const float * scale;      // [G / n_as] or NULL: 1
+    const uint8_t * base;
+    uint8_t * dst;
+    int64_t nbb, nbd;
+    int32_t G, n_as, n_rows, x_rows, gather;
+    int32_t N, K, rank;
+    int32_t ra;               // rank rounded up to 16, 32, 64 or 128
+    int32_t bf16, out;
+    int32_t copy;             // base is not dst: rows without an adapter are copied
+    int32_t stages;
+};
+
+__host__ __device__ constexpr uint32_t lora_stage_bytes(int ra) { return kLoraXTile + (uint32_t)ra * 128u; }
+__host__ __device__ constexpr uint32_t lora_blocks(int ra) { return ra > 64 ? 2u : 1u; }    // of 64 ranks
+__host__ __device__ constexpr uint32_t lora_h_bytes(int ra) { return 3u * lora_blocks(ra) * kLoraXTile; }
+__host__ __device__ constexpr uint32_t lora_fixed_bytes(int ra, int groups) {
+    return lora_h_bytes(ra) + 2u * lora_blocks(ra) * kLoraBTile + (uint32_t)kLoraRows * ra * 4u + kLoraStaging +
+           kLoraRows * 4u + ((uint32_t)groups + 2u) * 4u;
+}
+
+// arrive on the same barrier of every CTA of the cluster (lane c of the warp: CTA c)
+__device__ __forceinline__ void arrive_all(uint64_t * bar, int ctas) {
+    const int lane = threadIdx.x & 31;
+    if (lane < ctas)
+        asm volatile(
+            "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar)),
+            "r"(lane)
+            : "memory");
+}
+
+__device__ __forceinline__ float4 ld_peer4(const float * p, int cta) {
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        : "r"(smem_u32(p)), "r"(cta)
+        : "memory");
+    return v;
+}
+
+struct LoraTile {
+    int g, row0, cnt;
+    int rank;         // 0: the rows have no adapter
+};
+
+__device__ __forceinline__ int2 lora_rows(const LoraParams & p, int g) {
+    if (g < p.G) return group_rows_of(p.offsets, g, p.n_rows);
+    const int lo = p.offsets[p.G];
+    if (lo < 0 || lo > p.n_rows || p.offsets[0] != 0) {
+        record_error(GX_DEVERR_DOMAIN);
+        return make_int2(0, 0);
+    }
+    return p.copy ? make_int2(lo, p.n_rows) : make_int2(0, 0);
+}
+
+__device__ __forceinline__ LoraTile lora_tile(const LoraParams & p, const int32_t * pre, int t) {
+    LoraTile q;
+    q.g = tile_group(pre, p.G + 1, t);
+    const int lo = p.offsets[q.g], hi = q.g < p.G ? p.offsets[q.g + 1] : p.n_rows;
+    q.row0 = lo + (t - pre[q.g]) * kLoraRows;
+    q.cnt = min(kLoraRows, hi - q.row0);
+    q.rank = 0;
+    if (q.g < p.G) {
+        q.rank = p.ranks != nullptr ? p.ranks[q.g / p.n_as] : p.rank;
+        if (q.rank < 0 || q.rank > p.rank) {
+            record_error(GX_DEVERR_DOMAIN);
+            q.rank = 0;
+        }
+    }
+    return q;
+}
+
+// whether the last step of 16 ranks reaches columns of B behind the adapter's
+// rank (behind the pool's own rank TMA fills in zeros)
+__device__ __forceinline__ bool lora_ragged(const LoraParams & p, const LoraTile & q) {
+    return (q.rank & 15) != 0 && q.rank < p.rank;
+}
+
+// y row of grouped row j (-1: none), and whether its x row exists
+__device__ __forceinline__ int lora_row(const LoraParams & p, int j, bool & bad_x) {
+    const int row = p.order != nullptr ? p.order[j] : j;
+    bad_x = row < 0 || row / p.gather >= p.x_rows;
+    if (row >= 0 && row < p.n_rows) return row;
+    record_error(GX_DEVERR_DOMAIN);
+    return -1;
+}
+
+// 16 staged columns of f32 deltas ([column][32 rows of B]) plus base, rounded, to the result rows
+template <typename T>
+__device__ __forceinline__ void lora_add(const LoraParams & p, const float * stage, int my, int n0, bool vec) {
+    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 32 / kPer, kCols = 32 / kLanes;
+    const int lane = threadIdx.x & 31, sub = lane % kLanes;
+    const int n = n0 + sub * kPer;
+    uint4 old[16 / kCols];
+    int rows[16 / kCols];
+    const bool whole = vec && n + kPer <= p.N;
+#pragma unroll
+    for (int i = 0; i < 16 / kCols; ++i) {
+        rows[i] = __shfl_sync(0xffffffffu, my, i * kCols + lane / kLanes);
+        if (whole && rows[i] >= 0)
+            old[i] = *reinterpret_cast<const uint4 *>(p.base + (int64_t)rows[i] * p.nbb + (int64_t)n * (int)sizeof(T));
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / kCols; ++i) {
+        if (rows[i] < 0) continue;
+        float d[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4)
+            *reinterpret_cast<float4 *>(d + e) =
+                *reinterpret_cast<const float4 *>(stage + (i * kCols + lane / kLanes) * 32 + sub * kPer + e);
+        T * out = reinterpret_cast<T *>(p.dst + (int64_t)rows[i] * p.nbd) + n;
+        const T * was = reinterpret_cast<const T *>(p.base + (int64_t)rows[i] * p.nbb) + n;
+        if (whole) {
+            T * v = reinterpret_cast<T *>(&old[i]);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] = round_to<T>((float)v[e] + d[e]);
+            *reinterpret_cast<uint4 *>(out) = old[i];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (n + e < p.N) out[e] = round_to<T>((float)was[e] + d[e]);
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void lora_copy_row(const LoraParams & p, int row, int first, int step) {
+    const T * s = reinterpret_cast<const T *>(p.base + (int64_t)row * p.nbb);
+    T * d = reinterpret_cast<T *>(p.dst + (int64_t)row * p.nbd);
+    const bool vec = ((reinterpret_cast<uintptr_t>(s) | reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const int pieces = vec ? p.N / kPer : 0;
+    for (int i = first; i < pieces; i += step) reinterpret_cast<uint4 *>(d)[i] = reinterpret_cast<const uint4 *>(s)[i];
+    for (int i = pieces * kPer + first; i < p.N; i += step) d[i] = s[i];
+}
+
+// eight values of h as `parts` vectors of the operand type that sum to them
+__device__ __forceinline__ void split_h(const float (&h)[8], bool bf16, uint4 (&out)[3]) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = h[i];
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+        if (bf16) {
+            __nv_bfloat16 * v = reinterpret_cast<__nv_bfloat16 *>(&out[part]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = __float2bfloat16_rn(rest[i]);
+                const float d = __fsub_rn(rest[i], __bfloat162float(v[i]));
+                rest[i] = fabsf(d) < __int_as_float(0x7f800000) ? d : 0.0f;      // (an infinity or NaN stays in the first part)
+            }
+        } else {
+            __half * v = reinterpret_cast<__half *>(&out[part]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = __float2half_rn(rest[i]);
+                const float d = __fsub_rn(rest[i], __half2float(v[i]));
+                rest[i] = fabsf(d) < __int_as_float(0x7f800000) ? d : 0.0f;
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant__ LoraParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[kLoraMaxStages], empty[kLoraMaxStages], b_full[2], b_empty[2], b_fixed[2], d2_full[2], d2_empty[2];
+    __shared__ uint64_t d1_full, d1_empty, part_full, part_free, h_full, h_empty, drained;
+    __shared__ uint32_t tslot;
+    __shared__ int32_t wsum[kLoraThreads / 32];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t ctas, rank_of;
+    asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(ctas));
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank_of));
+    const int C = (int)ctas, me = (int)rank_of;
+    const int unit = (int)blockIdx.x / C, units = (int)gridDim.x / C;
+    const uint32_t blocks = lora_blocks(p.ra), stage_bytes = lora_stage_bytes(p.ra), b_bytes = blocks * kLoraBTile;
+    // the ring comes first: an MMA over 128 rows of A reads past the last
+    // stage's rows into what follows (lanes that nobody looks at)
+    uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t * bring = ring + (uint32_t)p.stages * stage_bytes;
+    uint8_t * hbuf = bring + 2u * b_bytes;
+    float * part = reinterpret_cast<float *>(hbuf + lora_h_bytes(p.ra));       // [row][ra]
+    float * staging = part + kLoraRows * p.ra;
+    float * esc = staging + kLoraStaging / 4;                                  // [row] power of two of its h
+    int32_t * pre = reinterpret_cast<int32_t *>(esc + kLoraRows);
+
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(full + i, 2);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(b_full + i, 1);
+            mbar_init(b_empty + i, 1);
+            mbar_init(b_fixed + i, kLoraGatherWarps);
+            mbar_init(d2_full + i, 1);
+            mbar_init(d2_empty + i, kLoraEpiWarps);
+        }
+        mbar_init(&d1_full, 1);
+        mbar_init(&d1_empty, kLoraEpiWarps);
+        mbar_init(&part_full, (uint32_t)(kLoraEpiWarps * C));
+        mbar_init(&part_free, (uint32_t)(kLoraEpiWarps * C));
+        mbar_init(&h_full, kLoraEpiWarps);
+        mbar_init(&h_empty, 1);
+        mbar_init(&drained, 1);
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) gmm_tmem_alloc<1>(&tslot, 256);
+    tile_prefix(pre, wsum, p.G + 1, kLoraRows, [&](int g) { return lora_rows(p, g); });
+    tc_fence_before();
+    if (C > 1) cluster_sync_all(); else __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = tslot;
+    const uint32_t d1 = tbase, d2 = tbase + 64u;
+    const int tiles = pre[p.G + 1];
+    const int nk = (p.K + kGmmK - 1) / kGmmK;
+    const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
+    const int nn = (p.N + 127) / 128;                                          // result tiles; this CTA's: me, me + C, ..
+
+    if (warp == 0) {
+        // ------------------------------------------------ A and B by TMA
+        if (lane == 0) {
+            int c = 0, done = 0, bc = 0;
+            RingPos at;
+            bool ok = true;
+            for (int t = unit; t < tiles && ok; t += units) {
+                const LoraTile q = lora_tile(p, pre, t);
+                if (q.rank == 0) continue;
+                for (int kc = k0; kc < k1; ++kc, ++c, at.next(p.stages)) {
+                    if (at.round != 0) {
+                        ok = gmm_wait_one<1>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
+                        if (!ok) break;
+                        ++done;
+                    }
+                    mbar_arrive_expect_tx(full + at.s, (uint32_t)p.ra * 128u);
+                    tma_load_3d(ring + (uint32_t)at.s * stage_bytes + kLoraXTile, &p.amap, kc * kGmmK, 0, q.g, full + at.s);
+                }
+                for (int i = me; i < nn && ok; i += C, ++bc) {
+                    const int b = bc & 1;
+                    if (bc >= 2) ok = gmm_wait_one<1>(b_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
+                    if (!ok) break;
+                    const int nb = q.rank > 64 ? 2 : 1;
+                    mbar_arrive_expect_tx(b_full + b, (uint32_t)nb * kLoraBTile);
+                    for (int j = 0; j < nb; ++j)
+                        tma_load_3d(bring + (uint32_t)b * b_bytes + (uint32_t)j * kLoraBTile, &p.bmap, j * 64, i * 128, q.g,
+                                    b_full + b);
+                }
+            }
+            if (!ok) {
+                // copies in flight land before the CTA leaves
+                volatile int none = 0;
+                for (int i = done; i < c; ++i) gmm_wait_one<1>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
+                for (int i = max(0, bc - 2); i < bc; ++i) gmm_wait_one<1>(b_full + (i & 1), (uint32_t)((i / 2) & 1), &none);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ----------------------------------------------------- MMA issuer
+        if (lane == 0) {
+            int it = 0, bc = 0, fixes = 0;
+            RingPos at;
+            bool ok = true;
+            const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
+            const uint64_t b0 = umma_desc_sw128(bring, 1024u), h0 = umma_desc_sw128(hbuf, 1024u);
+            const int parts = p.bf16 ? 3 : 2;
+            for (int t = unit; t < tiles && ok; t += units) {
+                const LoraTile q = lora_tile(p, pre, t);
+                if (q.rank == 0) continue;
+                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, 128, (uint32_t)((q.cnt + 15) & ~15));
+                if (it > 0) ok = gmm_wait_one<1>(&d1_empty, (uint32_t)((it - 1) & 1), &abort_flag);
+                for (int kc = k0; kc < k1 && ok; ++kc, at.next(p.stages)) {
+                    ok = gmm_wait_one<1>(full + at.s, at.round & 1u, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
+#pragma unroll
+                    for (int i = 0; i < kGmmK / 16; ++i)
+                        mma_f16<1>(d1, a0 + off + (uint64_t)(2 * i), x0 + off + (uint64_t)(2 * i), idesc, (uint32_t)((kc - k0) | i));
+                    gmm_commit<1>(empty + at.s);
+                }
+                if (!ok) break;
+                gmm_commit<1>(&d1_full);
+                ok = gmm_wait_one<1>(&h_full, (uint32_t)(it & 1), &abort_flag);
+                const int steps = (q.rank + 15) / 16;
+                for (int i = me; i < nn && ok; i += C, ++bc) {
+                    const int b = bc & 1;
+                    if (lora_ragged(p, q)) {
+                        ok = gmm_wait_one<1>(b_fixed + (fixes & 1), (uint32_t)((fixes / 2) & 1), &abort_flag);
+                        ++fixes;
+                    } else {
+                        ok = gmm_wait_one<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
+                    }
+                    if (ok && bc >= 2) ok = gmm_wait_one<1>(d2_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int st = 0; st < steps; ++st) {
+                        const uint64_t blk = (uint64_t)(st >> 2), in = (uint64_t)(2 * (st & 3));
+                        const uint64_t bd = b0 + (uint64_t)((uint32_t)b * b_bytes >> 4) + blk * (kLoraBTile >> 4) + in;
+                        for (int part_i = 0; part_i < parts; ++part_i)
+                            mma_f16<1>(d2 + (uint32_t)b * 64u, bd,
+                                       h0 + ((uint64_t)part_i * blocks + blk) * (kLoraXTile >> 4) + in, idesc,
+                                       (uint32_t)(st | part_i));
+                    }
+                    gmm_commit<1>(b_empty + b);
+                    gmm_commit<1>(d2_full + b);
+                }
+                if (ok) gmm_commit<1>(&h_empty);
+                ++it;
+            }
+            if (!ok) {
+                volatile int none = 0;
+                gmm_commit<1>(&drained);
+                gmm_wait_one<1>(&drained, 0, &none);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 2 + kLoraGatherWarps) {
+        // --------------------------------------- rows of x, a warp per chunk
+        const int gw = warp - 2, sub = lane & 7, r4 = lane >> 3;
+        const uint32_t at0 = (uint32_t)r4 * 128u + (uint32_t)((sub ^ r4) << 4);
+        const uint32_t at1 = (uint32_t)(r4 + 4) * 128u + (uint32_t)((sub ^ (r4 + 4)) << 4);
+        const uint32_t pitch = (uint32_t)(p.nb11 >> 4);
+        int turn = 0, bc = 0, fixes = 0;
+        RingPos at;
+        bool ok = true;
+        for (int t = unit; t < tiles && ok; t += units) {
+            const LoraTile q = lora_tile(p, pre, t);
+            if (q.rank == 0) continue;
+            uint32_t mine[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                mine[i] = 0;
+                if (i * 32 + lane < q.cnt) {
+                    bool bad = false;
+                    const int row = lora_row(p, q.row0 + i * 32 + lane, bad);
+                    if (bad) record_error(GX_DEVERR_DOMAIN);
+                    else if (row >= 0) mine[i] = (uint32_t)(row / p.gather);
+                }
+            }
+            for (int kc = k0; kc < k1; ++kc, at.next(p.stages)) {
+                const bool skip = turn != gw;
+                turn = turn + 1 == kLoraGatherWarps ? 0 : turn + 1;
+                if (skip) continue;
+                if (at.round != 0) {
+                    ok = gmm_wait<1>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
+                    if (!ok) break;
+                }
+                const uint32_t dst = smem_u32(ring) + (uint32_t)at.s * stage_bytes;
+                const uint8_t * col = p.x + (int64_t)kc * 128 + sub * 16;
+                const int left = (p.K - kc * kGmmK) * 2 - sub * 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h * 32 >= q.cnt) break;
+                    const uint8_t * src[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[h], i * 4 + r4) * pitch << 4);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t to = dst + ((i & 1) ? at1 : at0) + (uint32_t)(h * 4 + (i >> 1)) * 1024u;
+                        if (h * 32 + i * 4 + r4 < q.cnt) {
+                            if (left >= 16) cp_async16(to, src[i]);
+                            else cp_async16_part(to, left > 0 ? src[i] : p.x, (uint32_t)max(0, left));
+                        }
+                    }
+                }
+                cp_async_commit();
+                cp_async_wait<0>();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<1>(full + at.s);
+            }
+            // where the rank ends inside a step of 16, B's columns behind it are
+            // cleared in shared memory: a zero in h does not silence a NaN
+            for (int i = me; i < nn && ok; i += C, ++bc) {
+                if (!lora_ragged(p, q)) continue;
+                const int b = bc & 1, row = gw * 32 + lane;
+                ok = gmm_wait<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
+                if (!ok) break;
+                uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * kLoraBTile + (uint32_t)row * 128u;
+                for (int r = q.rank; r < ((q.rank + 15) & ~15); ++r)
+                    *reinterpret_cast<uint16_t *>(tile + ((((r & 63) >> 3) ^ (row & 7)) << 4) + (r & 7) * 2) = 0;
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<1>(b_fixed + (fixes & 1));
+                ++fixes;
+            }
+        }
+    } else {
+        // ------------------------------------------------- h and results
+        const int quad = warp & 3, ew = warp - 2 - kLoraGatherWarps;
+        float * stage = staging + quad * (16 * 32);
+        const int esz = p.out == GMM_F32 ? 4 : 2;
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.nbd |
+                           (uintptr_t)p.nbb) & 15u) == 0;
+        int it = 0, bc = 0;
+        bool ok = true;
+        for (int t = unit; t < tiles && ok; t += units) {
+            const LoraTile q = lora_tile(p, pre, t);
+            if (q.rank == 0) {
+                if (p.copy) {
+                    for (int j = ew * C + me; j < q.cnt; j += kLoraEpiWarps * C) {
+                        bool bad = false;
+                        const int row = lora_row(p, q.row0 + j, bad);
+                        if (row < 0) continue;
+                        if (esz == 4) lora_copy_row<float>(p, row, lane, 32);
+                        else lora_copy_row<uint16_t>(p, row, lane, 32);
+                    }
+                }
+                continue;
+            }
+            // the partial h of this CTA's share of K: lanes are ranks, columns rows
+            ok = gmm_wait<1>(&d1_full, (uint32_t)(it & 1), &abort_flag);
+            if (ok && it > 0) ok = gmm_wait<2>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            if (quad * 32 < p.ra) {
+                const int r = quad * 32 + lane;
+                for (int c0 = 0; c0 < q.cnt; c0 += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(d1 + (uint32_t)c0 + ((uint32_t)quad << 21), v);
+                    tmem_wait_ld();
+                    if (r < p.ra) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) part[(c0 + i) * p.ra + r] = k0 < k1 ? __uint_as_float(v[i]) : 0.0f;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) gmm_arrive<1>(&d1_empty);
+            arrive_all(&part_full, C);
+            ok = gmm_wait<2>(&part_full, (uint32_t)(it & 1), &abort_flag);
+            if (ok && it > 0) ok = gmm_wait<1>(&h_empty, (uint32_t)((it - 1) & 1), &abort_flag);
+            if (!ok) break;
+            // sum over the cluster in CTA order, scale, split, store as an MMA operand
+            {
+                const int a = q.g / p.n_as;
+                const float s = p.scale != nullptr ? p.scale[a] : 1.0f;
+                const int per = p.ra / 8;                              // eight ranks per thread; a power of two <= 16
+                const int rows16 = (q.cnt + 15) & ~15;
+                const int items = rows16 * per;                        // a multiple of 32
+                for (int i = ew * 32 + lane; i < items; i += kLoraEpiWarps * 32) {
+                    const int row = i / per, r0 = (i - row * per) * 8;
+                    float h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[e] = 0.0f;
+                    for (int c = 0; c < C; ++c) {
+                        const float4 lo = ld_peer4(part + row * p.ra + r0, c), hi = ld_peer4(part + row * p.ra + r0 + 4, c);
+                        h[0] += lo.x; h[1] += lo.y; h[2] += lo.z; h[3] += lo.w;
+                        h[4] += hi.x; h[5] += hi.y; h[6] += hi.z; h[7] += hi.w;
+                    }
+                    float big = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        h[e] = r0 + e < q.rank && row < q.cnt ? __fmul_rn(h[e], s) : 0.0f;
+                        big = fmaxf(big, fabsf(h[e]));
+                    }
+                    if (!p.bf16) {
+                        // the row's largest |h| to [2^13, 2^14)
+                        for (int m = 1; m < per; m <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
+                        const int e2 = big > 0.0f && big < __int_as_float(0x7f800000)
+                                           ? min(max((int)(__float_as_uint(big) >> 23) - 127 - 13, -100), 114) : 0;
+                        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = __fmul_rn(h[e], down);
+                        if (r0 == 0) esc[row] = __uint_as_float((uint32_t)(127 + e2) << 23);
+                    }
+                    uint4 v[3];
+                    split_h(h, p.bf16 != 0, v);
+                    uint8_t * to = hbuf + (uint32_t)(r0 >> 6) * kLoraXTile + (uint32_t)row * 128u +
+                                   (uint32_t)((((r0 & 63) >> 3) ^ (row & 7)) << 4);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(to + (uint32_t)k * blocks * kLoraXTile) = v[k];
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) gmm_arrive<1>(&h_full);
+            arrive_all(&part_free, C);
+            ok = gmm_wait<1>(&h_full, (uint32_t)(it & 1), &abort_flag);       // (every row's power of two)
+            int my[2];
+            unsigned nans[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                bool bad = false;
+                my[i] = i * 32 + lane < q.cnt ? lora_row(p, q.row0 + i * 32 + lane, bad) : -1;
+                nans[i] = __ballot_sync(0xffffffffu, bad);
+            }
+            for (int nt = me; nt < nn && ok; nt += C, ++bc) {
+                const int b = bc & 1;
+                ok = gmm_wait<1>(d2_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const int n0 = nt * 128 + quad * 32;
+                for (int c0 = 0; c0 < q.cnt; c0 += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(d2 + (uint32_t)b * 64u + (uint32_t)c0 + ((uint32_t)quad << 21), v);
+                    tmem_wait_ld();
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float f = __uint_as_float(v[i]);
+                        if (!p.bf16) f = __fmul_rn(f, esc[c0 + i]);
+                        if ((nans[c0 >> 5] >> ((c0 & 31) + i)) & 1u) f = kNan;
+                        stage[i * 32 + lane] = f;
+                    }
+                    __syncwarp();
+                    const int rows = __shfl_sync(0xffffffffu, my[c0 >> 5], (c0 & 16) + (lane & 15));
+                    if (p.out == GMM_F32) lora_add<float>(p, stage, rows, n0, vec);
+                    else if (p.out == GMM_BF16) lora_add<__nv_bfloat16>(p, stage, rows, n0, vec);
+                    else lora_add<__half>(p, stage, rows, n0, vec);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<1>(d2_empty + b);
+            }
+            ++it;
+        }
+    }
+    tc_fence_before();
+    if (C > 1) cluster_sync_all(); else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        gmm_tmem_free<1>(tbase, 256);
+    }
+}
+
+}  // namespace gx

@@ -1,5 +1,6 @@
 """The operators on grouped rows, on torch tensors: rows ordered by expert or
-adapter, products with unquantised (F16 / BF16) experts, rows rounded for them.
+adapter, products with unquantised (F16 / BF16) experts, low-rank adapters of
+many requests, rows rounded for them.
 
 Every tensor lives on the current CUDA device. The calls run on `stream` (a
 cudaStream_t handle or a torch stream), torch's current stream by default, wait
@@ -7,6 +8,8 @@ for nothing and can be captured into a graph; results they allocate belong to
 torch's current stream.
 """
 from __future__ import annotations
+
+import ctypes as C
 
 import torch
 
@@ -157,4 +160,45 @@ def mul_mat_grouped_glu(gate, up, x, offsets, *, order=None, n_rows: int | None 
     rc = L.lib().gx_mul_mat_grouped_glu(_TYPE.get(gate.dtype, -1), gate.data_ptr(), up.data_ptr(), *tail, act, alpha, limit,
                                         _TYPE[out.dtype], out.data_ptr(), _row_stride(out, 0), _raw_stream(stream, dev))
     L.check(rc, "gx_mul_mat_grouped_glu")
+    return out
+
+
+def lora_mul_mat(a, b, x, offsets, *, order=None, gather: int = 1, n_as: int | None = None, ranks=None, scale=None, base,
+                 out=None, stream=None):
+    """gx_lora_mul_mat: base + the rows' low-rank deltas, in a new tensor, in
+    `out`, or in place (out=base). a [G, rank, K] and b [G, N, rank] hold the
+    adapters (G = adapters * n_as, expert minor), x [rows, K] the projection's
+    input of their type, base [n_rows, N] its output; ranks i32 and scale f32
+    [adapters] (n_as defaults to G // len(ranks or scale), else 1). order and
+    offsets as group_rows gives them; row r of base belongs to x[r // gather]."""
+    dev = _device(a, b, x, offsets, order, ranks, scale, base, out)
+    for t, name, dims in ((a, "a", 3), (b, "b", 3), (x, "x", 2), (base, "base", 2)):
+        _matrix(t, name, dims)
+    G, rank, K = a.shape
+    if b.shape[0] != G or b.shape[2] != rank or not a.dtype == b.dtype == x.dtype or x.shape[1] != K:
+        raise ValueError("a [G, rank, K], b [G, N, rank] and x [rows, K] of one type expected")
+    if n_as is None:
+        per = ranks if ranks is not None else scale
+        n_as = 1 if per is None else G // max(1, per.shape[0])
+    if n_as <= 0 or G % n_as:
+        raise ValueError("n_as: a divisor of the number of matrices")
+    adapters = G // n_as
+    _index(offsets, "offsets", G + 1)
+    _index(order, "order", base.shape[0])
+    _index(ranks, "ranks", adapters)
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous()):
+        raise ValueError(f"scale: contiguous float32 vector of {adapters} expected")
+    if out is None:
+        out = torch.empty(base.shape, dtype=base.dtype, device=base.device)
+    _matrix(out, "out", 2)
+    if base.shape[1] != b.shape[1] or out.shape != base.shape or out.dtype != base.dtype or base.dtype not in _TYPE:
+        raise ValueError(f"base and out: rows of {b.shape[1]} elements of one result type expected")
+    desc = L.gx_lora_desc(_TYPE.get(a.dtype, -1), rank, K, b.shape[1], n_as, adapters, a.data_ptr(), _row_stride(a, 1),
+                          _row_stride(a, 0), b.data_ptr(), _row_stride(b, 1), _row_stride(b, 0),
+                          None if ranks is None else ranks.data_ptr(), None if scale is None else scale.data_ptr())
+    rc = L.lib().gx_lora_mul_mat(C.byref(desc), x.data_ptr(), x.shape[0], _row_stride(x, 0), offsets.data_ptr(),
+                                 0 if order is None else order.data_ptr(), base.shape[0], gather, _TYPE[base.dtype],
+                                 base.data_ptr(), _row_stride(base, 0), out.data_ptr(), _row_stride(out, 0),
+                                 _raw_stream(stream, dev))
+    L.check(rc, "gx_lora_mul_mat")
     return out

@@ -317,6 +317,47 @@ int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t
                            const int32_t * offsets, const int32_t * order, int64_t n_rows, int64_t gather, int scatter,
                            int act, float alpha, float limit, int type_dst, void * dst, int64_t nbd1, void * stream);
 
+/* Low-rank adapters of many requests on the output of a projection they share
+ * (llama.cpp's build_lora_mm and, on routed experts, build_lora_mm_id):
+ *   dst row = base row + B_g (scale A_g x row)   for the rows of group g
+ * on rows grouped by gx_group_rows with adapter (and ids, where the adapters
+ * are those of experts: n_as experts per adapter, group adapter * n_as + id).
+ * Row j of the order is row r = order[j] of base and dst (n_rows of them; r = j
+ * when order is NULL) and row r / gather of x. base is the projection's output,
+ * gx_mul_mat_id's f32 rows for instance; dst may be base (rows without an
+ * adapter are then left alone) or lie apart from it (they are copied). dst and
+ * base may not overlap in any other way.
+ *   a      group g's A at a + g*nba2, `rank` rows of ne00 elements, nba1 apart
+ *   b      group g's B at b + g*nbb2, ne01 rows of `rank` elements, nbb1 apart
+ *   ranks  device i32 [n_adapters], each 0 .. rank (0: no adapter), or NULL:
+ *          all of rank `rank`. Rows of A and columns of B behind an adapter's
+ *          rank may hold anything.
+ *   scale  device f32 [n_adapters] (alpha / rank, ...), or NULL: 1
+ * x has the adapters' type; sums, h = A x and the deltas are f32 (h enters the
+ * second product in parts that keep at least 22 bits), the result is rounded
+ * once to type_dst. offsets: [n_as * n_adapters + 1], offsets[0] = 0. Errors
+ * found on the device are reported (gx_device_error): borders that do not
+ * ascend or leave [0, n_rows] (the group is skipped), a rank above `rank` (as
+ * 0), a row outside dst (dropped) or x (NaN). rank <= GX_LORA_MAX_RANK; 16-byte
+ * aligned a, b, x and strides nba1, nba2, nbb1, nbb2, nb11. */
+#define GX_LORA_MAX_RANK 128
+typedef struct gx_lora_desc {
+    int32_t type;           /* GX_TYPE_F16 or GX_TYPE_BF16 */
+    int32_t rank;           /* of the pool: the largest */
+    int64_t ne00, ne01;     /* K, N of the projection */
+    int64_t n_as;           /* experts per adapter (1: dense projection) */
+    int64_t n_adapters;
+    const void * a;
+    int64_t nba1, nba2;
+    const void * b;
+    int64_t nbb1, nbb2;
+    const int32_t * ranks;
+    const float * scale;
+} gx_lora_desc;
+int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int64_t nb11, const int32_t * offsets,
+                    const int32_t * order, int64_t n_rows, int64_t gather, int type_dst, const void * base, int64_t nbb,
+                    void * dst, int64_t nbd, void * stream);
+
 /* ------------------------------------------------------------- MoE layer
  * One routed-expert FFN layer, end to end on the device:
  *   remap (policy + miss copies) -> gate/up mul_mat_id + activation

@@ -70,3 +70,30 @@ def test_group_refusals(gxlib, over, want):
 ])
 def test_round_rows_refusals(gxlib, args, want):
     assert gxlib.lib().gx_quantize_rows(*args, None) == want
+
+
+@pytest.mark.parametrize("over,want", [
+    (dict(type=F32), TYPE), (dict(type_dst=8), TYPE), (dict(rank=0), INVALID), (dict(rank=129), INVALID), (dict(ne00=0), INVALID),
+    (dict(ne01=0), INVALID), (dict(n_as=0), INVALID), (dict(n_adapters=0), INVALID), (dict(n_as=4096, n_adapters=3), INVALID),
+    (dict(a=None), INVALID), (dict(b=None), INVALID), (dict(x=None), INVALID), (dict(offsets=None), INVALID),
+    (dict(base=None), INVALID), (dict(dst=None), INVALID), (dict(ne11=0), INVALID), (dict(n_rows=-1), INVALID),
+    (dict(gather=0), INVALID), (dict(nba1=112), INVALID), (dict(nba2=128), INVALID), (dict(nbb1=16), INVALID),
+    (dict(nbb2=64), INVALID), (dict(nb11=112), INVALID), (dict(nbb=188), INVALID), (dict(nbd=188), INVALID),
+    (dict(nb11=1 << 35), INVALID), (dict(nbb=256, dst=65536), INVALID),       # in place with two strides
+    (dict(nba1=136), ALIGN), (dict(nbb1=40), ALIGN), (dict(nba2=16 * 128 + 8), ALIGN), (dict(nbb2=48 * 32 + 8), ALIGN),
+    (dict(nb11=136), ALIGN), (dict(a=4104), ALIGN), (dict(b=4104), ALIGN), (dict(x=4104), ALIGN), (dict(base=4098), ALIGN),
+    (dict(dst=4098), ALIGN), (dict(offsets=4098), ALIGN), (dict(order=4098), ALIGN), (dict(ranks=4098), ALIGN),
+    (dict(scale=4098), ALIGN), (dict(nbd=194), ALIGN), (dict(n_rows=0, x=None, base=None, dst=None), OK),
+])
+def test_lora_refusals(gxlib, over, want):
+    import ctypes as C
+    a = dict(type=F16, rank=16, ne00=64, ne01=48, n_as=2, n_adapters=4, a=4096, nba1=128, nba2=16 * 128, b=4096, nbb1=32,
+             nbb2=48 * 32, ranks=4096, scale=4096)
+    c = dict(x=4096, ne11=10, nb11=128, offsets=4096, order=4096, n_rows=10, gather=1, type_dst=F32, base=65536, nbb=192, dst=4096,
+             nbd=192)
+    assert set(over) <= set(a) | set(c)
+    for k, v in over.items():
+        (a if k in a else c)[k] = v
+    desc = gxlib._lib.gx_lora_desc(*a.values())
+    assert gxlib.lib().gx_lora_mul_mat(C.byref(desc), *c.values(), None) == want
+    assert gxlib.lib().gx_lora_mul_mat(None, *c.values(), None) == INVALID
