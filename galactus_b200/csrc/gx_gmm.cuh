@@ -21,7 +21,7 @@ constexpr int kGmmRows = 128;                  // matrix rows of a CTA's tile: T
 constexpr int kGmmK = 64;                      // elements of K per stage: one 128-byte swizzled row
 constexpr uint32_t kGmmATile = kGmmRows * 128u;
 constexpr int kGmmMaxStages = 12;
-constexpr int kGmmGatherWarps = 12, kGmmGatherSplit = 2;   // copying warps; warps that share a chunk
+constexpr int kGmmGatherWarps = 4;             // 32 rows each
 constexpr int kGmmEpiWarps = 4;
 constexpr int kGmmThreads = 32 * (2 + kGmmGatherWarps + kGmmEpiWarps);
 constexpr uint32_t kGmmStaging = kGmmEpiWarps * 32u * 32u * 4u;   // results of 32 columns per epilogue warp
@@ -32,9 +32,7 @@ enum : int { GMM_F32 = 0, GMM_F16 = 1, GMM_BF16 = 2 };
 struct GmmParams {
     CUtensorMap wmap;         // W (or G): [K, N, G], boxes 64 x 128 (gated: 64 x 64)
     CUtensorMap umap;         // U
-    CUtensorMap xmap;         // x in place: [K, rows], boxes 64 x box
-    const uint8_t * x;
-    int64_t nb11;
+    CUtensorMap xmap;         // x: [K, rows], boxes 64 x box, 64 x 1 for gathers
     const int32_t * offsets;  // [G + 1]
     const int32_t * order;    // [n_rows] or NULL
     int32_t G, n_rows, x_rows;
@@ -136,6 +134,24 @@ __device__ __forceinline__ void gmm_tma_2d(void * dst, const CUtensorMap * map, 
             : "memory");
 }
 
+// four rows of a map with boxes of one row (no multicast: this GPU's own memory)
+template <int CTAS>
+__device__ __forceinline__ void gmm_gather4(void * dst, const CUtensorMap * map, int x, int r0, int r1, int r2, int r3,
+                                            uint64_t * bar) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+            "%4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, "
+            "{%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar) & kLeaderMask)
+            : "memory");
+}
+
 // arrive on the barrier of the leading CTA
 template <int CTAS>
 __device__ __forceinline__ void gmm_arrive(uint64_t * bar) {
@@ -146,6 +162,14 @@ __device__ __forceinline__ void gmm_arrive(uint64_t * bar) {
             "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
             "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar))
             : "memory");
+}
+
+// one thread of a whole warp (the compiler then knows that values of the
+// branch belong to one thread, as the TMA and MMA operands need)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
@@ -361,6 +385,11 @@ struct RingPos {
             ++round;
         }
     }
+    __device__ __forceinline__ void skip(int n, int stages) {
+        s += n;
+        round += (uint32_t)(s / stages);
+        s %= stages;
+    }
 };
 
 // 32 (or 16) columns of a warp's 32 matrix rows, staged as [column][row], to
@@ -420,8 +449,10 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tslot;
+    __shared__ int4 gather_mem[kGmmGatherWarps * 8];
     __shared__ int32_t wsum[kGmmThreads / 32];
     __shared__ int abort_flag;
+    int32_t * gather_rows = reinterpret_cast<int32_t *>(gather_mem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);              // CTA of the pair; 0 leads
     const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
@@ -435,7 +466,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1 + (p.gather ? CTAS * kGmmGatherSplit : 0));
+            mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -457,7 +488,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
 
     if (warp == 0) {
         // ------------------------------------------- weights, rows in place
-        if (lane == 0) {
+        if (elect_one()) {
             int c = 0, done = 0;       // chunks started; chunks whose stage was handed back
             RingPos at;
             bool ok = true;
@@ -468,9 +499,12 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                 const int r0 = q.row0 + rank * half;
                 uint32_t bytes = (uint32_t)CTAS * kGmmATile;
                 int boxes = 0;
-                if (!p.gather) {
-                    for (int r = 0; r < CTAS; ++r) {
-                        const int b = (max(0, min(half, q.cnt - r * half)) + p.box - 1) / p.box;
+                for (int r = 0; r < CTAS; ++r) {
+                    const int n = max(0, min(half, q.cnt - r * half));
+                    if (p.gather) {
+                        bytes += (uint32_t)((n + 3) >> 2) * 512u;
+                    } else {
+                        const int b = (n + p.box - 1) / p.box;
                         bytes += (uint32_t)b * (p.box * 128u);
                         if (r == rank) boxes = b;
                     }
@@ -499,7 +533,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------ MMA issuer
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             int it = 0;
             RingPos at;
             bool ok = true;
@@ -533,71 +567,50 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
         __syncwarp();
     } else if (warp < 2 + kGmmGatherWarps) {
         // -------------------------------------------------- gathered rows
-        // a pair of warps fetches every kGmmGatherWarps/2-th chunk, 32-row
-        // blocks in turn, four rows of 128 bytes per step. The fence that shows a chunk
-        // to the tensor cores waits for all of the warp's copies in flight,
-        // so it is the warps, not one warp's chunks, that overlap.
+        // four rows of 128 bytes per copy (tile::gather4), up to 32 rows per
+        // warp: the warp looks its rows up, one thread issues the copies
         if (p.gather) {
-            const int gw = warp - 2, sub = lane & 7, r4 = lane >> 3;
-            // 16-byte piece `sub` of rows r4, r4 + 4 (mod 8), swizzled
-            const uint32_t at0 = kGmmATile + (uint32_t)r4 * 128u + (uint32_t)((sub ^ r4) << 4);
-            const uint32_t at1 = kGmmATile + (uint32_t)(r4 + 4) * 128u + (uint32_t)((sub ^ (r4 + 4)) << 4);
-            const uint32_t pitch = (uint32_t)(p.nb11 >> 4);
-            int turn = 0;                                                         // whose chunk is next
+            const int gw = warp - 2;
+            int32_t * rows = gather_rows + gw * 32;
             RingPos at;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
                 const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
-                uint32_t mine[4 / kGmmGatherSplit];                               // x rows of this warp's 32-row blocks
-#pragma unroll
-                for (int i = 0; i < 4 / kGmmGatherSplit; ++i) {
-                    const int r = (i * kGmmGatherSplit + gw % kGmmGatherSplit) * 32 + lane;
-                    mine[i] = 0;
-                    if (r < n) {
-                        const int o = p.order[q.row0 + rank * half + r];
-                        const int row = o / p.gather;
-                        if (o < 0 || row >= p.x_rows) record_error(GX_DEVERR_DOMAIN);
-                        else mine[i] = (uint32_t)row;
+                const int quads = max(0, min(32, n - gw * 32) + 3) >> 2;          // this warp's, in fours
+                const int r = min(gw * 32 + lane, n - 1);                         // (the last four repeat the final row)
+                int row = 0;
+                if (r >= 0) {
+                    const int o = p.order[q.row0 + rank * half + r];
+                    row = o / p.gather;
+                    if (o < 0 || row >= p.x_rows) {
+                        record_error(GX_DEVERR_DOMAIN);
+                        row = 0;
                     }
                 }
-                for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
-                    const bool skip = turn != gw / kGmmGatherSplit;
-                    turn = turn + 1 == kGmmGatherWarps / kGmmGatherSplit ? 0 : turn + 1;
-                    if (skip) continue;
-                    const int s = at.s;
-                    if (at.round != 0) {
-                        ok = gmm_wait<CTAS>(empty + s, (at.round - 1u) & 1u, &abort_flag);
-                        if (!ok) break;
-                    }
-                    const uint32_t dst = smem_u32(ring) + (uint32_t)s * stage_bytes;
-                    const uint8_t * col = p.x + (int64_t)kc * 128 + sub * 16;
-                    const int left = (p.K - kc * kGmmK) * 2 - sub * 16;           // bytes of the row from this piece on
+                __syncwarp();
+                rows[lane] = row;
+                __syncwarp();
+                if (elect_one()) {
+                    int4 of[8];
 #pragma unroll
-                    for (int hh = 0; hh < 4 / kGmmGatherSplit; ++hh) {
-                        const int h = hh * kGmmGatherSplit + gw % kGmmGatherSplit;
-                        if (h * 32 >= n) break;
-                        const uint8_t * src[8];
+                    for (int i = 0; i < 8; ++i) of[i] = *reinterpret_cast<const int4 *>(rows + i * 4);
+                    RingPos on = at;
+                    for (int kc = 0; kc < nk; ++kc, on.next(p.stages)) {
+                        if (on.round != 0) {
+                            ok = gmm_wait_one<CTAS>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
+                            if (!ok) break;
+                        }
+                        uint8_t * to = ring + (uint32_t)on.s * stage_bytes + kGmmATile + (uint32_t)gw * 4096u;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[hh], i * 4 + r4) * pitch << 4);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t to = dst + ((i & 1) ? at1 : at0) + (uint32_t)(h * 4 + (i >> 1)) * 1024u;
-                            if (h * 32 + i * 4 + r4 < n) {
-                                // the last chunk of rows that end inside it: zeros behind the end
-                                if (left >= 16) cp_async16(to, src[i]);
-                                else cp_async16_part(to, left > 0 ? src[i] : p.x, (uint32_t)max(0, left));
-                            }
-                        }
+                            if (i < quads)
+                                gmm_gather4<CTAS>(to + i * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
                     }
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) gmm_arrive<CTAS>(full + s);
                 }
+                ok = __all_sync(0xffffffffu, ok);
+                at.skip(nk, p.stages);
             }
         }
     } else {

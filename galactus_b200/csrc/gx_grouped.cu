@@ -125,7 +125,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (gather == 0 && ne11 < n_rows) return GX_ERR_INVALID;
     const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
     if (nb01 < 0 || nb02 < 0 || nb11 < 0 || nbd1 < 0 || nb01 >= kMaxStride || nb02 >= kMaxStride ||
-        nb11 >= (1ll << 35))
+        nb11 >= kMaxStride)
         return GX_ERR_INVALID;
     if (n_as == 1) nb02 = nb01;                    // (never used to reach a second expert)
     if (nb01 % 16 || nb02 % 16 || nb11 % 16 || misaligned(as, 16) || misaligned(b, 16) || (up && misaligned(up, 16)))
@@ -137,8 +137,6 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
 
     gx::GmmParams p{};
     p.bf16 = type == GX_TYPE_BF16;
-    p.x = static_cast<const uint8_t *>(b);
-    p.nb11 = nb11;
     p.offsets = offsets;
     p.order = order;
     p.G = (int32_t)n_as;
@@ -170,7 +168,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
     if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, glu ? gx::kGmmRows / 2 : gx::kGmmRows) ||
         (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows / 2)) ||
-        (gather == 0 && !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, (uint32_t)p.box)))
+        !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)p.box))
         return GX_ERR_ALIGN;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
