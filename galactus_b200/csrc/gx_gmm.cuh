@@ -172,17 +172,6 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void * src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// the first `bytes` of them, zeros behind
-__device__ __forceinline__ void cp_async16_part(uint32_t dst, const void * src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
@@ -314,16 +303,8 @@ __device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t *
     return r;
 }
 
-// x row of grouped row j (a bad index is reported; its result is not stored)
-__device__ __forceinline__ int gmm_src_row(const GmmParams & p, int j) {
-    if (p.gather == 0) return j;
-    const int r = p.order[j] / p.gather;
-    if (p.order[j] < 0 || r >= p.x_rows) {
-        record_error(GX_DEVERR_DOMAIN);
-        return 0;
-    }
-    return r;
-}
+// fours of rows that gathering warp w copies of a CTA's n
+__device__ __forceinline__ int gather_quads(int n, int w) { return max(1, (min(32, n - w * 32) + 3) >> 2); }
 
 // y row of grouped row j, -1 to skip it (no such row); nan: its x row does not exist
 __device__ __forceinline__ int gmm_dst_row(const GmmParams & p, int j, bool & nan) {
@@ -485,6 +466,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     const uint32_t tbase = tslot;
     const int tiles = pre[p.G] * p.mt;
     const int nk = (p.K + kGmmK - 1) / kGmmK;
+    const int gathering = p.gather ? (p.nt / CTAS + 31) / 32 : 0;        // warps that gather
 
     if (warp == 0) {
         // ------------------------------------------- weights, rows in place
@@ -502,7 +484,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                 for (int r = 0; r < CTAS; ++r) {
                     const int n = max(0, min(half, q.cnt - r * half));
                     if (p.gather) {
-                        bytes += (uint32_t)((n + 3) >> 2) * 512u;
+                        for (int w = 0; w < gathering; ++w) bytes += (uint32_t)gather_quads(n, w) * 512u;
                     } else {
                         const int b = (n + p.box - 1) / p.box;
                         bytes += (uint32_t)b * (p.box * 128u);
@@ -568,9 +550,12 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     } else if (warp < 2 + kGmmGatherWarps) {
         // -------------------------------------------------- gathered rows
         // four rows of 128 bytes per copy (tile::gather4), up to 32 rows per
-        // warp: the warp looks its rows up, one thread issues the copies
-        if (p.gather) {
-            const int gw = warp - 2;
+        // warp: the warp looks its rows up, one thread issues the copies. A
+        // warp without rows in a tile still copies four: a stage that does not
+        // wait for it could go round the ring twice before it looks, and the
+        // parity of its barrier would then say the opposite.
+        const int gw = warp - 2;
+        if (gw < gathering) {
             int32_t * rows = gather_rows + gw * 32;
             RingPos at;
             bool ok = true;
@@ -578,16 +563,13 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                 const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
-                const int quads = max(0, min(32, n - gw * 32) + 3) >> 2;          // this warp's, in fours
-                const int r = min(gw * 32 + lane, n - 1);                         // (the last four repeat the final row)
-                int row = 0;
-                if (r >= 0) {
-                    const int o = p.order[q.row0 + rank * half + r];
-                    row = o / p.gather;
-                    if (o < 0 || row >= p.x_rows) {
-                        record_error(GX_DEVERR_DOMAIN);
-                        row = 0;
-                    }
+                const int quads = gather_quads(n, gw);
+                // (rows behind the last repeat it)
+                const int o = p.order[q.row0 + min(rank * half + min(gw * 32 + lane, max(n - 1, 0)), q.cnt - 1)];
+                int row = o / p.gather;
+                if (o < 0 || row >= p.x_rows) {
+                    record_error(GX_DEVERR_DOMAIN);
+                    row = 0;
                 }
                 __syncwarp();
                 rows[lane] = row;

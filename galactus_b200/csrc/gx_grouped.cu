@@ -284,7 +284,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
         return GX_ERR_INVALID;
     const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
     if (d->nba1 < 0 || nba2 < 0 || d->nbb1 < 0 || nbb2 < 0 || nb11 < 0 || nbb < 0 || nbd < 0 || d->nba1 >= kMaxStride ||
-        nba2 >= kMaxStride || d->nbb1 >= kMaxStride || nbb2 >= kMaxStride || nb11 >= (1ll << 35))
+        nba2 >= kMaxStride || d->nbb1 >= kMaxStride || nbb2 >= kMaxStride || nb11 >= kMaxStride)
         return GX_ERR_INVALID;
     if (G == 1) {                                      // (never used to reach a second adapter)
         nba2 = d->nba1;
@@ -300,8 +300,6 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (G > 1 && (nba2 < (d->rank - 1) * d->nba1 + 2 * K || nbb2 < (N - 1) * d->nbb1 + 2 * d->rank)) return GX_ERR_INVALID;
 
     gx::LoraParams p{};
-    p.x = static_cast<const uint8_t *>(x);
-    p.nb11 = nb11;
     p.offsets = offsets;
     p.order = order;
     p.ranks = d->ranks;
@@ -325,7 +323,8 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     p.copy = base != dst;
     if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
     if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
-        !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u))
+        !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u) ||
+        !encode_rows(&p.xmap, p.bf16, x, K, ne11, nb11, 0, 0, 1u))
         return GX_ERR_ALIGN;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;

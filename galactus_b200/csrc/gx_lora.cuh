@@ -31,9 +31,10 @@ namespace gx {
 constexpr int kLoraRows = 64;                   // rows of a tile (MMA N)
 constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxStages = 8;
-constexpr int kLoraGatherWarps = 4;
+constexpr int kLoraGatherWarps = kLoraRows / 32;
+constexpr int kLoraFixWarps = 2;
 constexpr int kLoraEpiWarps = 4;
-constexpr int kLoraThreads = 32 * (2 + kLoraGatherWarps + kLoraEpiWarps);
+constexpr int kLoraThreads = 32 * (2 + kLoraGatherWarps + kLoraFixWarps + kLoraEpiWarps);
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
 constexpr uint32_t kLoraBTile = 128u * 128u;    // 128 rows of B, 64 ranks
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
@@ -41,8 +42,7 @@ constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
 struct LoraParams {
     CUtensorMap amap;         // A: [K, rank, G], boxes 64 x ra
     CUtensorMap bmap;         // B: [rank, N, G], boxes 64 x 128
-    const uint8_t * x;
-    int64_t nb11;
+    CUtensorMap xmap;         // x: [K, rows], boxes 64 x 1, gathered
     const int32_t * offsets;  // [G + 1]
     const int32_t * order;    // [n_rows] or NULL: rows in place
     const int32_t * ranks;    // [G / n_as] or NULL: all `rank`
@@ -118,12 +118,6 @@ __device__ __forceinline__ LoraTile lora_tile(const LoraParams & p, const int32_
         }
     }
     return q;
-}
-
-// whether the last step of 16 ranks reaches columns of B behind the adapter's
-// rank (behind the pool's own rank TMA fills in zeros)
-__device__ __forceinline__ bool lora_ragged(const LoraParams & p, const LoraTile & q) {
-    return (q.rank & 15) != 0 && q.rank < p.rank;
 }
 
 // y row of grouped row j (-1: none), and whether its x row exists
@@ -215,6 +209,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kLoraMaxStages], empty[kLoraMaxStages], b_full[2], b_empty[2], b_fixed[2], d2_full[2], d2_empty[2];
     __shared__ uint64_t d1_full, d1_empty, part_full, part_free, h_full, h_empty, drained;
+    __shared__ int4 gather_mem[kLoraRows / 4];
     __shared__ uint32_t tslot;
     __shared__ int32_t wsum[kLoraThreads / 32];
     __shared__ int abort_flag;
@@ -237,13 +232,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 2);
+            mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
-            mbar_init(b_fixed + i, kLoraGatherWarps);
+            mbar_init(b_fixed + i, kLoraFixWarps);
             mbar_init(d2_full + i, 1);
             mbar_init(d2_empty + i, kLoraEpiWarps);
         }
@@ -271,20 +266,22 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
 
     if (warp == 0) {
         // ------------------------------------------------ A and B by TMA
-        if (lane == 0) {
+        if (elect_one()) {
             int c = 0, done = 0, bc = 0;
             RingPos at;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
                 const LoraTile q = lora_tile(p, pre, t);
                 if (q.rank == 0) continue;
+                uint32_t bytes = (uint32_t)p.ra * 128u;
+                for (int w = 0; w < kLoraGatherWarps; ++w) bytes += (uint32_t)gather_quads(q.cnt, w) * 512u;
                 for (int kc = k0; kc < k1; ++kc, ++c, at.next(p.stages)) {
                     if (at.round != 0) {
                         ok = gmm_wait_one<1>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
                         if (!ok) break;
                         ++done;
                     }
-                    mbar_arrive_expect_tx(full + at.s, (uint32_t)p.ra * 128u);
+                    mbar_arrive_expect_tx(full + at.s, bytes);
                     tma_load_3d(ring + (uint32_t)at.s * stage_bytes + kLoraXTile, &p.amap, kc * kGmmK, 0, q.g, full + at.s);
                 }
                 for (int i = me; i < nn && ok; i += C, ++bc) {
@@ -308,8 +305,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         __syncwarp();
     } else if (warp == 1) {
         // ----------------------------------------------------- MMA issuer
-        if (lane == 0) {
-            int it = 0, bc = 0, fixes = 0;
+        if (elect_one()) {
+            int it = 0, bc = 0;
             RingPos at;
             bool ok = true;
             const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
@@ -336,12 +333,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 const int steps = (q.rank + 15) / 16;
                 for (int i = me; i < nn && ok; i += C, ++bc) {
                     const int b = bc & 1;
-                    if (lora_ragged(p, q)) {
-                        ok = gmm_wait_one<1>(b_fixed + (fixes & 1), (uint32_t)((fixes / 2) & 1), &abort_flag);
-                        ++fixes;
-                    } else {
-                        ok = gmm_wait_one<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
-                    }
+                    ok = gmm_wait_one<1>((p.ranks != nullptr ? b_fixed : b_full) + b, (uint32_t)((bc / 2) & 1), &abort_flag);
                     if (ok && bc >= 2) ok = gmm_wait_one<1>(d2_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
                     if (!ok) break;
                     tc_fence_after();
@@ -367,80 +359,71 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         }
         __syncwarp();
     } else if (warp < 2 + kLoraGatherWarps) {
-        // --------------------------------------- rows of x, a warp per chunk
-        const int gw = warp - 2, sub = lane & 7, r4 = lane >> 3;
-        const uint32_t at0 = (uint32_t)r4 * 128u + (uint32_t)((sub ^ r4) << 4);
-        const uint32_t at1 = (uint32_t)(r4 + 4) * 128u + (uint32_t)((sub ^ (r4 + 4)) << 4);
-        const uint32_t pitch = (uint32_t)(p.nb11 >> 4);
-        int turn = 0, bc = 0, fixes = 0;
+        // ------------- rows of x: tile::gather4 copies, up to 32 rows a warp
+        // (a warp without rows in a tile still copies four, as in k_gmm)
+        const int gw = warp - 2;
+        int32_t * rows = reinterpret_cast<int32_t *>(gather_mem + gw * 8);
         RingPos at;
         bool ok = true;
         for (int t = unit; t < tiles && ok; t += units) {
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
-            uint32_t mine[2];
+            const int quads = gather_quads(q.cnt, gw);
+            bool bad = false;
+            const int row = lora_row(p, q.row0 + min(gw * 32 + lane, q.cnt - 1), bad);
+            if (bad) record_error(GX_DEVERR_DOMAIN);
+            __syncwarp();
+            rows[lane] = bad || row < 0 ? 0 : row / p.gather;
+            __syncwarp();
+            if (elect_one()) {
+                int4 of[8];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                mine[i] = 0;
-                if (i * 32 + lane < q.cnt) {
-                    bool bad = false;
-                    const int row = lora_row(p, q.row0 + i * 32 + lane, bad);
-                    if (bad) record_error(GX_DEVERR_DOMAIN);
-                    else if (row >= 0) mine[i] = (uint32_t)(row / p.gather);
-                }
-            }
-            for (int kc = k0; kc < k1; ++kc, at.next(p.stages)) {
-                const bool skip = turn != gw;
-                turn = turn + 1 == kLoraGatherWarps ? 0 : turn + 1;
-                if (skip) continue;
-                if (at.round != 0) {
-                    ok = gmm_wait<1>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
-                    if (!ok) break;
-                }
-                const uint32_t dst = smem_u32(ring) + (uint32_t)at.s * stage_bytes;
-                const uint8_t * col = p.x + (int64_t)kc * 128 + sub * 16;
-                const int left = (p.K - kc * kGmmK) * 2 - sub * 16;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h * 32 >= q.cnt) break;
-                    const uint8_t * src[8];
+                for (int i = 0; i < 8; ++i) of[i] = *reinterpret_cast<const int4 *>(rows + i * 4);
+                RingPos on = at;
+                for (int kc = k0; kc < k1; ++kc, on.next(p.stages)) {
+                    if (on.round != 0) {
+                        ok = gmm_wait_one<1>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
+                        if (!ok) break;
+                    }
+                    uint8_t * to = ring + (uint32_t)on.s * stage_bytes + (uint32_t)gw * 4096u;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        src[i] = col + ((uint64_t)__shfl_sync(0xffffffffu, mine[h], i * 4 + r4) * pitch << 4);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t to = dst + ((i & 1) ? at1 : at0) + (uint32_t)(h * 4 + (i >> 1)) * 1024u;
-                        if (h * 32 + i * 4 + r4 < q.cnt) {
-                            if (left >= 16) cp_async16(to, src[i]);
-                            else cp_async16_part(to, left > 0 ? src[i] : p.x, (uint32_t)max(0, left));
-                        }
-                    }
+                        if (i < quads)
+                            gmm_gather4<1>(to + i * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
                 }
-                cp_async_commit();
-                cp_async_wait<0>();
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) gmm_arrive<1>(full + at.s);
             }
-            // where the rank ends inside a step of 16, B's columns behind it are
-            // cleared in shared memory: a zero in h does not silence a NaN
+            ok = __all_sync(0xffffffffu, ok);
+            at.skip(k1 - k0, p.stages);
+        }
+    } else if (warp < 2 + kLoraGatherWarps + kLoraFixWarps) {
+        // -------- where the rank ends inside a step of 16, B's columns behind
+        // it are cleared in shared memory: a zero in h does not silence a NaN
+        const int fw = warp - 2 - kLoraGatherWarps;
+        int bc = 0;
+        bool ok = p.ranks != nullptr;
+        for (int t = unit; t < tiles && ok; t += units) {
+            const LoraTile q = lora_tile(p, pre, t);
+            if (q.rank == 0) continue;
+            const int behind = q.rank < p.rank ? (q.rank + 15) & ~15 : q.rank;     // (behind the pool's rank TMA fills in zeros)
             for (int i = me; i < nn && ok; i += C, ++bc) {
-                if (!lora_ragged(p, q)) continue;
-                const int b = bc & 1, row = gw * 32 + lane;
+                const int b = bc & 1;
                 ok = gmm_wait<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
                 if (!ok) break;
-                uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * kLoraBTile + (uint32_t)row * 128u;
-                for (int r = q.rank; r < ((q.rank + 15) & ~15); ++r)
-                    *reinterpret_cast<uint16_t *>(tile + ((((r & 63) >> 3) ^ (row & 7)) << 4) + (r & 7) * 2) = 0;
-                fence_async_smem();
+                if (q.rank < behind) {
+                    uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * kLoraBTile;
+                    for (int row = fw * 32 + lane; row < 128; row += 32 * kLoraFixWarps)
+                        for (int r = q.rank; r < behind; ++r)
+                            *reinterpret_cast<uint16_t *>(tile + (uint32_t)row * 128u + ((((r & 63) >> 3) ^ (row & 7)) << 4) +
+                                                          (r & 7) * 2) = 0;
+                    fence_async_smem();
+                }
                 __syncwarp();
-                if (lane == 0) gmm_arrive<1>(b_fixed + (fixes & 1));
-                ++fixes;
+                if (lane == 0) gmm_arrive<1>(b_fixed + b);
             }
         }
     } else {
         // ------------------------------------------------- h and results
-        const int quad = warp & 3, ew = warp - 2 - kLoraGatherWarps;
+        const int quad = warp & 3, ew = warp - 2 - kLoraGatherWarps - kLoraFixWarps;
         float * stage = staging + quad * (16 * 32);
         const int esz = p.out == GMM_F32 ? 4 : 2;
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.nbd |

@@ -184,6 +184,28 @@ def test_gather_scatter_and_foreign_rows(gxlib, dev, T, k, E, gather, scatter, g
     assert device_error() == 0
 
 
+@pytest.mark.parametrize("glu", [False, True])
+@pytest.mark.parametrize("K", [64, 1024])
+def test_uneven_groups_gathered(gxlib, dev, K, glu):
+    """Long and tiny groups side by side, many tiles per CTA: copying warps that have no rows in a tile keep step."""
+    from galactus_b200.moe import device_error
+    rng = np.random.default_rng(K)
+    c = [700, 3, 256, 33, 1, 130, 0, 65, 31, 400, 2, 2] * 6
+    E, N, P = len(c), 700, sum(c)
+    order = torch.from_numpy(rng.permutation(P).astype(np.int32)).cuda()
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(c)]), dtype=torch.int32, device="cuda")
+    w, x = make(E, K, N, P, "bf16", K)
+    up, _ = make(E, K, N, 0, "bf16", K + 1)
+    device_error()
+    if glu:
+        got = gxlib.mul_mat_grouped_glu(w, up, x, offsets, order=order, gather=1)
+    else:
+        got = gxlib.mul_mat_grouped(w, x, offsets, order=order, gather=1)
+    assert device_error() == 0
+    want, tol = reference(w, x, c, 0, 1, order, False, P, 0 if glu else None, up if glu else None)
+    compare(got, want, tol, "bf16")
+
+
 def test_first_border_above_zero_and_experts_in_a_record(gxlib, dev):
     """Matrices inside larger records (an arena's slots), rows in front of the first group."""
     K, N, c = 128, 96, [3, 0, 40]

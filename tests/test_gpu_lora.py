@@ -66,6 +66,8 @@ CASES = [
     (300, 8, 32, 4, 16, False, 256, 192, "bf16", "f32"),
     (1000, 1, 1, 3, 32, True, 4096, 640, "f16", "f16"),
     (9, 2, 3, 700, 72, True, 136, 65, "bf16", "f32"),
+    (3000, 1, 1, 40, 40, True, 192, 300, "f16", "f32"),
+    (2500, 4, 30, 5, 64, True, 512, 136, "bf16", "bf16"),
 ]
 
 

@@ -79,7 +79,7 @@ def test_round_rows_refusals(gxlib, args, want):
     (dict(base=None), INVALID), (dict(dst=None), INVALID), (dict(ne11=0), INVALID), (dict(n_rows=-1), INVALID),
     (dict(gather=0), INVALID), (dict(nba1=112), INVALID), (dict(nba2=128), INVALID), (dict(nbb1=16), INVALID),
     (dict(nbb2=64), INVALID), (dict(nb11=112), INVALID), (dict(nbb=188), INVALID), (dict(nbd=188), INVALID),
-    (dict(nb11=1 << 35), INVALID), (dict(nbb=256, dst=65536), INVALID),       # in place with two strides
+    (dict(nb11=1 << 40), INVALID), (dict(nbb=256, dst=65536), INVALID),       # in place with two strides
     (dict(nba1=136), ALIGN), (dict(nbb1=40), ALIGN), (dict(nba2=16 * 128 + 8), ALIGN), (dict(nbb2=48 * 32 + 8), ALIGN),
     (dict(nb11=136), ALIGN), (dict(a=4104), ALIGN), (dict(b=4104), ALIGN), (dict(x=4104), ALIGN), (dict(base=4098), ALIGN),
     (dict(dst=4098), ALIGN), (dict(offsets=4098), ALIGN), (dict(order=4098), ALIGN), (dict(ranks=4098), ALIGN),
