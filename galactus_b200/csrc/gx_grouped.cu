@@ -81,18 +81,22 @@ PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     return fn;
 }
 
-// rows of K 16-bit elements, 128-byte swizzled boxes of 64 elements by `box` rows
+// rows of K 16-bit elements, boxes of `width` (16, 32, 64) elements by `box`
+// rows, swizzled over the width
 bool encode_rows(CUtensorMap * map, bool bf16, const void * base, int64_t K, int64_t rows, int64_t nb1, int64_t mats,
-                 int64_t nb2, uint32_t box) {
+                 int64_t nb2, uint32_t box, uint32_t width = gx::kGmmK) {
     const auto enc = map_encoder();
     if (enc == nullptr) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)mats};
     const cuuint64_t strides[2] = {(cuuint64_t)nb1, (cuuint64_t)nb2};
-    const cuuint32_t boxes[3] = {(cuuint32_t)gx::kGmmK, box, 1u};
+    const cuuint32_t boxes[3] = {width, box, 1u};
     const cuuint32_t elem[3] = {1u, 1u, 1u};
     return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, mats > 0 ? 3 : 2,
                const_cast<void *>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               width == 64u   ? CU_TENSOR_MAP_SWIZZLE_128B
+               : width == 32u ? CU_TENSOR_MAP_SWIZZLE_64B
+                              : CU_TENSOR_MAP_SWIZZLE_32B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -323,7 +327,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     p.copy = base != dst;
     if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
     if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
-        !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u) ||
+        !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u, (uint32_t)std::min(p.ra, 64)) ||
         !encode_rows(&p.xmap, p.bf16, x, K, ne11, nb11, 0, 0, 1u))
         return GX_ERR_ALIGN;
     const int sms = device_sms();

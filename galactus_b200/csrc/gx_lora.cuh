@@ -28,20 +28,20 @@
 
 namespace gx {
 
-constexpr int kLoraRows = 64;                   // rows of a tile (MMA N)
+constexpr int kLoraRows = 32;                   // rows of a tile (MMA N)
 constexpr int kLoraMaxRank = 128;
-constexpr int kLoraMaxStages = 8;
+constexpr int kLoraMaxStages = 12;
 constexpr int kLoraGatherWarps = kLoraRows / 32;
 constexpr int kLoraFixWarps = 2;
 constexpr int kLoraEpiWarps = 4;
 constexpr int kLoraThreads = 32 * (2 + kLoraGatherWarps + kLoraFixWarps + kLoraEpiWarps);
+constexpr uint32_t kLoraTmem = 128;             // columns: h, two result tiles (of 32)
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
-constexpr uint32_t kLoraBTile = 128u * 128u;    // 128 rows of B, 64 ranks
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
 
 struct LoraParams {
     CUtensorMap amap;         // A: [K, rank, G], boxes 64 x ra
-    CUtensorMap bmap;         // B: [rank, N, G], boxes 64 x 128
+    CUtensorMap bmap;         // B: [rank, N, G], boxes min(ra, 64) x 128
     CUtensorMap xmap;         // x: [K, rows], boxes 64 x 1, gathered
     const int32_t * offsets;  // [G + 1]
     const int32_t * order;    // [n_rows] or NULL: rows in place
@@ -59,11 +59,27 @@ struct LoraParams {
 };
 
 __host__ __device__ constexpr uint32_t lora_stage_bytes(int ra) { return kLoraXTile + (uint32_t)ra * 128u; }
-__host__ __device__ constexpr uint32_t lora_blocks(int ra) { return ra > 64 ? 2u : 1u; }    // of 64 ranks
-__host__ __device__ constexpr uint32_t lora_h_bytes(int ra) { return 3u * lora_blocks(ra) * kLoraXTile; }
+// B and h lie in blocks of up to 64 ranks, their rows swizzled over 32, 64 or
+// 128 bytes: as many as the ranks fill
+__host__ __device__ constexpr uint32_t lora_blocks(int ra) { return ra > 64 ? 2u : 1u; }
+__host__ __device__ constexpr uint32_t lora_row(int ra) { return ra >= 64 ? 128u : (uint32_t)ra * 2u; }
+__host__ __device__ constexpr uint32_t lora_b_block(int ra) { return 128u * lora_row(ra); }
+__host__ __device__ constexpr uint32_t lora_h_block(int ra) { return (uint32_t)kLoraRows * lora_row(ra); }
 __host__ __device__ constexpr uint32_t lora_fixed_bytes(int ra, int groups) {
-    return lora_h_bytes(ra) + 2u * lora_blocks(ra) * kLoraBTile + (uint32_t)kLoraRows * ra * 4u + kLoraStaging +
+    return lora_blocks(ra) * (2u * lora_b_block(ra) + 3u * lora_h_block(ra)) + (uint32_t)kLoraRows * ra * 4u + kLoraStaging +
            kLoraRows * 4u + ((uint32_t)groups + 2u) * 4u;
+}
+// byte of 16-byte piece c of row r in such a block: the piece's number is
+// XOR-ed with the address bits from 7 up
+__device__ __forceinline__ uint32_t lora_swizzle(uint32_t row_bytes, int r, int c) {
+    const uint32_t off = (uint32_t)r * row_bytes + (uint32_t)c * 16u;
+    return off ^ (((off >> 7) & (row_bytes / 16u - 1u)) << 4);
+}
+// shared-memory descriptor of such a block, K-major (layout types 2, 4, 6: 128-, 64- and 32-byte swizzle)
+__device__ __forceinline__ uint64_t lora_desc(const void * smem, uint32_t row_bytes) {
+    const uint64_t layout = row_bytes == 128u ? 2u : row_bytes == 64u ? 4u : 6u;
+    return (uint64_t)((smem_u32(smem) >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)((row_bytes * 8u) >> 4) << 32) |
+           (1ull << 46) | (layout << 61);
 }
 
 // arrive on the same barrier of every CTA of the cluster (lane c of the warp: CTA c)
@@ -129,43 +145,49 @@ __device__ __forceinline__ int lora_row(const LoraParams & p, int j, bool & bad_
     return -1;
 }
 
-// 16 staged columns of f32 deltas ([column][32 rows of B]) plus base, rounded, to the result rows
+// The base of a warp's 32 x 32 tile of results, loaded ahead of the deltas:
+// lane's 16-byte pieces, rows of the 32 columns by `my` (lane i: column i).
 template <typename T>
-__device__ __forceinline__ void lora_add(const LoraParams & p, const float * stage, int my, int n0, bool vec) {
-    constexpr int kPer = 16 / (int)sizeof(T), kLanes = 32 / kPer, kCols = 32 / kLanes;
-    const int lane = threadIdx.x & 31, sub = lane % kLanes;
-    const int n = n0 + sub * kPer;
-    uint4 old[16 / kCols];
-    int rows[16 / kCols];
-    const bool whole = vec && n + kPer <= p.N;
+struct LoraBase {
+    static constexpr int kPer = 16 / (int)sizeof(T), kLanes = 32 / kPer, kCols = 32 / kLanes, kPieces = 32 / kCols;
+    uint4 old[kPieces];
+    __device__ __forceinline__ void load(const LoraParams & p, int my, int n0, bool vec) {
+        const int lane = threadIdx.x & 31, n = n0 + lane % kLanes * kPer;
 #pragma unroll
-    for (int i = 0; i < 16 / kCols; ++i) {
-        rows[i] = __shfl_sync(0xffffffffu, my, i * kCols + lane / kLanes);
-        if (whole && rows[i] >= 0)
-            old[i] = *reinterpret_cast<const uint4 *>(p.base + (int64_t)rows[i] * p.nbb + (int64_t)n * (int)sizeof(T));
-    }
-#pragma unroll
-    for (int i = 0; i < 16 / kCols; ++i) {
-        if (rows[i] < 0) continue;
-        float d[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; e += 4)
-            *reinterpret_cast<float4 *>(d + e) =
-                *reinterpret_cast<const float4 *>(stage + (i * kCols + lane / kLanes) * 32 + sub * kPer + e);
-        T * out = reinterpret_cast<T *>(p.dst + (int64_t)rows[i] * p.nbd) + n;
-        const T * was = reinterpret_cast<const T *>(p.base + (int64_t)rows[i] * p.nbb) + n;
-        if (whole) {
-            T * v = reinterpret_cast<T *>(&old[i]);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) v[e] = round_to<T>((float)v[e] + d[e]);
-            *reinterpret_cast<uint4 *>(out) = old[i];
-        } else {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (n + e < p.N) out[e] = round_to<T>((float)was[e] + d[e]);
+        for (int i = 0; i < kPieces; ++i) {
+            const int row = __shfl_sync(0xffffffffu, my, i * kCols + lane / kLanes);
+            if (vec && n + kPer <= p.N && row >= 0)
+                old[i] = *reinterpret_cast<const uint4 *>(p.base + (int64_t)row * p.nbb + (int64_t)n * (int)sizeof(T));
         }
     }
-}
+    // plus 16 staged columns of f32 deltas ([column][32 rows of B], columns 16 * half ..), rounded, to the result rows
+    __device__ __forceinline__ void add(const LoraParams & p, const float * stage, int half, int my, int n0, bool vec) {
+        const int lane = threadIdx.x & 31, sub = lane % kLanes, n = n0 + sub * kPer;
+#pragma unroll
+        for (int i = 0; i < kPieces / 2; ++i) {
+            const int col = i * kCols + lane / kLanes;
+            const int row = __shfl_sync(0xffffffffu, my, 16 * half + col);
+            if (row < 0) continue;
+            float d[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; e += 4)
+                *reinterpret_cast<float4 *>(d + e) = *reinterpret_cast<const float4 *>(stage + col * 32 + sub * kPer + e);
+            T * out = reinterpret_cast<T *>(p.dst + (int64_t)row * p.nbd) + n;
+            if (vec && n + kPer <= p.N) {
+                uint4 v = half ? old[kPieces / 2 + i] : old[i];
+                T * t = reinterpret_cast<T *>(&v);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) t[e] = round_to<T>((float)t[e] + d[e]);
+                *reinterpret_cast<uint4 *>(out) = v;
+            } else {
+                const T * was = reinterpret_cast<const T *>(p.base + (int64_t)row * p.nbb) + n;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (n + e < p.N) out[e] = round_to<T>((float)was[e] + d[e]);
+            }
+        }
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void lora_copy_row(const LoraParams & p, int row, int first, int step) {
@@ -219,13 +241,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank_of));
     const int C = (int)ctas, me = (int)rank_of;
     const int unit = (int)blockIdx.x / C, units = (int)gridDim.x / C;
-    const uint32_t blocks = lora_blocks(p.ra), stage_bytes = lora_stage_bytes(p.ra), b_bytes = blocks * kLoraBTile;
+    const uint32_t blocks = lora_blocks(p.ra), stage_bytes = lora_stage_bytes(p.ra), b_block = lora_b_block(p.ra);
+    const uint32_t b_bytes = blocks * b_block, h_block = lora_h_block(p.ra), row_bytes = lora_row(p.ra);
     // the ring comes first: an MMA over 128 rows of A reads past the last
     // stage's rows into what follows (lanes that nobody looks at)
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t * bring = ring + (uint32_t)p.stages * stage_bytes;
     uint8_t * hbuf = bring + 2u * b_bytes;
-    float * part = reinterpret_cast<float *>(hbuf + lora_h_bytes(p.ra));       // [row][ra]
+    float * part = reinterpret_cast<float *>(hbuf + 3u * blocks * h_block);    // [row][ra]
     float * staging = part + kLoraRows * p.ra;
     float * esc = staging + kLoraStaging / 4;                                  // [row] power of two of its h
     int32_t * pre = reinterpret_cast<int32_t *>(esc + kLoraRows);
@@ -252,13 +275,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 1) gmm_tmem_alloc<1>(&tslot, 256);
+    if (warp == 1) gmm_tmem_alloc<1>(&tslot, kLoraTmem);
     tile_prefix(pre, wsum, p.G + 1, kLoraRows, [&](int g) { return lora_rows(p, g); });
     tc_fence_before();
     if (C > 1) cluster_sync_all(); else __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
-    const uint32_t d1 = tbase, d2 = tbase + 64u;
+    const uint32_t d1 = tbase, d2 = tbase + (uint32_t)kLoraRows;
     const int tiles = pre[p.G + 1];
     const int nk = (p.K + kGmmK - 1) / kGmmK;
     const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
@@ -289,10 +312,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     if (bc >= 2) ok = gmm_wait_one<1>(b_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
                     if (!ok) break;
                     const int nb = q.rank > 64 ? 2 : 1;
-                    mbar_arrive_expect_tx(b_full + b, (uint32_t)nb * kLoraBTile);
+                    mbar_arrive_expect_tx(b_full + b, (uint32_t)nb * b_block);
                     for (int j = 0; j < nb; ++j)
-                        tma_load_3d(bring + (uint32_t)b * b_bytes + (uint32_t)j * kLoraBTile, &p.bmap, j * 64, i * 128, q.g,
-                                    b_full + b);
+                        tma_load_3d(bring + (uint32_t)b * b_bytes + (uint32_t)j * b_block, &p.bmap, j * 64, i * 128, q.g, b_full + b);
                 }
             }
             if (!ok) {
@@ -310,7 +332,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             RingPos at;
             bool ok = true;
             const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
-            const uint64_t b0 = umma_desc_sw128(bring, 1024u), h0 = umma_desc_sw128(hbuf, 1024u);
+            const uint64_t b0 = lora_desc(bring, row_bytes), h0 = lora_desc(hbuf, row_bytes);
             const int parts = p.bf16 ? 3 : 2;
             for (int t = unit; t < tiles && ok; t += units) {
                 const LoraTile q = lora_tile(p, pre, t);
@@ -339,10 +361,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     tc_fence_after();
                     for (int st = 0; st < steps; ++st) {
                         const uint64_t blk = (uint64_t)(st >> 2), in = (uint64_t)(2 * (st & 3));
-                        const uint64_t bd = b0 + (uint64_t)((uint32_t)b * b_bytes >> 4) + blk * (kLoraBTile >> 4) + in;
+                        const uint64_t bd = b0 + (uint64_t)((uint32_t)b * b_bytes >> 4) + blk * (b_block >> 4) + in;
                         for (int part_i = 0; part_i < parts; ++part_i)
-                            mma_f16<1>(d2 + (uint32_t)b * 64u, bd,
-                                       h0 + ((uint64_t)part_i * blocks + blk) * (kLoraXTile >> 4) + in, idesc,
+                            mma_f16<1>(d2 + (uint32_t)b * (uint32_t)kLoraRows, bd,
+                                       h0 + ((uint64_t)part_i * blocks + blk) * (h_block >> 4) + in, idesc,
                                        (uint32_t)(st | part_i));
                     }
                     gmm_commit<1>(b_empty + b);
@@ -410,11 +432,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 ok = gmm_wait<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
                 if (!ok) break;
                 if (q.rank < behind) {
-                    uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * kLoraBTile;
+                    uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * b_block;
                     for (int row = fw * 32 + lane; row < 128; row += 32 * kLoraFixWarps)
                         for (int r = q.rank; r < behind; ++r)
-                            *reinterpret_cast<uint16_t *>(tile + (uint32_t)row * 128u + ((((r & 63) >> 3) ^ (row & 7)) << 4) +
-                                                          (r & 7) * 2) = 0;
+                            *reinterpret_cast<uint16_t *>(tile + lora_swizzle(row_bytes, row, (r & 63) >> 3) + (r & 7) * 2) = 0;
                     fence_async_smem();
                 }
                 __syncwarp();
@@ -503,10 +524,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     }
                     uint4 v[3];
                     split_h(h, p.bf16 != 0, v);
-                    uint8_t * to = hbuf + (uint32_t)(r0 >> 6) * kLoraXTile + (uint32_t)row * 128u +
-                                   (uint32_t)((((r0 & 63) >> 3) ^ (row & 7)) << 4);
+                    uint8_t * to = hbuf + (uint32_t)(r0 >> 6) * h_block + lora_swizzle(row_bytes, row, (r0 & 63) >> 3);
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(to + (uint32_t)k * blocks * kLoraXTile) = v[k];
+                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(to + (uint32_t)k * blocks * h_block) = v[k];
                 }
             }
             fence_async_smem();
@@ -514,42 +534,41 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             if (lane == 0) gmm_arrive<1>(&h_full);
             arrive_all(&part_free, C);
             ok = gmm_wait<1>(&h_full, (uint32_t)(it & 1), &abort_flag);       // (every row's power of two)
-            int my[2];
-            unsigned nans[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                bool bad = false;
-                my[i] = i * 32 + lane < q.cnt ? lora_row(p, q.row0 + i * 32 + lane, bad) : -1;
-                nans[i] = __ballot_sync(0xffffffffu, bad);
-            }
-            for (int nt = me; nt < nn && ok; nt += C, ++bc) {
-                const int b = bc & 1;
-                ok = gmm_wait<1>(d2_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                const int n0 = nt * 128 + quad * 32;
-                for (int c0 = 0; c0 < q.cnt; c0 += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(d2 + (uint32_t)b * 64u + (uint32_t)c0 + ((uint32_t)quad << 21), v);
-                    tmem_wait_ld();
+            bool bad = false;
+            const int my = lane < q.cnt ? lora_row(p, q.row0 + lane, bad) : -1;
+            const unsigned nans = __ballot_sync(0xffffffffu, bad);
+            auto results = [&](auto base) {
+                base.load(p, my, me * 128 + quad * 32, vec);
+                for (int nt = me; nt < nn && ok; nt += C, ++bc) {
+                    const int b = bc & 1, n0 = nt * 128 + quad * 32;
+                    ok = gmm_wait<1>(d2_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t v[32];
+                    tmem_ld32(d2 + (uint32_t)(b * kLoraRows) + ((uint32_t)quad << 21), v);
+                    tc_fence_before();
                     __syncwarp();
+                    if (lane == 0) gmm_arrive<1>(d2_empty + b);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float f = __uint_as_float(v[i]);
-                        if (!p.bf16) f = __fmul_rn(f, esc[c0 + i]);
-                        if ((nans[c0 >> 5] >> ((c0 & 31) + i)) & 1u) f = kNan;
-                        stage[i * 32 + lane] = f;
+                    for (int half = 0; half < 2; ++half) {
+                        if (half * 16 >= q.cnt) break;
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float f = __uint_as_float(v[half * 16 + i]);
+                            if (!p.bf16) f = __fmul_rn(f, esc[half * 16 + i]);
+                            if ((nans >> (half * 16 + i)) & 1u) f = kNan;
+                            stage[i * 32 + lane] = f;
+                        }
+                        __syncwarp();
+                        base.add(p, stage, half, my, n0, vec);
                     }
-                    __syncwarp();
-                    const int rows = __shfl_sync(0xffffffffu, my[c0 >> 5], (c0 & 16) + (lane & 15));
-                    if (p.out == GMM_F32) lora_add<float>(p, stage, rows, n0, vec);
-                    else if (p.out == GMM_BF16) lora_add<__nv_bfloat16>(p, stage, rows, n0, vec);
-                    else lora_add<__half>(p, stage, rows, n0, vec);
+                    if (nt + C < nn) base.load(p, my, n0 + C * 128, vec);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) gmm_arrive<1>(d2_empty + b);
-            }
+            };
+            if (p.out == GMM_F32) results(LoraBase<float>{});
+            else if (p.out == GMM_BF16) results(LoraBase<__nv_bfloat16>{});
+            else results(LoraBase<__half>{});
             ++it;
         }
     }
@@ -557,7 +576,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     if (C > 1) cluster_sync_all(); else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        gmm_tmem_free<1>(tbase, 256);
+        gmm_tmem_free<1>(tbase, kLoraTmem);
     }
 }
 
