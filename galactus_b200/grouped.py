@@ -16,11 +16,14 @@ import torch
 from . import _lib as L
 
 _TYPE = {torch.float32: L.TYPE_F32, torch.float16: L.TYPE_F16, torch.bfloat16: L.TYPE_BF16}
+_INT = torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_LIB = L.lib()
 
 
-def _raw_stream(stream, dev: int) -> int:
+def _stream(stream, dev: int) -> int:
     if stream is None:
-        return torch._C._cuda_getCurrentRawStream(dev)
+        return _raw_stream(dev)
     return stream if isinstance(stream, int) else int(stream.cuda_stream)
 
 
@@ -33,27 +36,44 @@ def _device(*tensors) -> int:
     return dev
 
 
-def _matrix(t, name: str, dims: int) -> None:
-    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{name}: {dims} dimensions with consecutive elements in the last one, not shape {tuple(t.shape)} "
-                         f"strides {t.stride()}")
+def _rows(t, name: str) -> tuple[int, int, int]:
+    """(rows, columns, bytes between rows) of a matrix with consecutive elements in its rows."""
+    try:
+        n, m = t.shape
+        s, e = t.stride()
+    except ValueError:
+        raise ValueError(f"{name}: two dimensions expected, not {tuple(t.shape)}") from None
+    if e != 1 and m > 1:
+        raise ValueError(f"{name}: consecutive elements in the last dimension expected, not strides {t.stride()}")
+    if n <= 1:                                # no second row to reach
+        s = (m + 7) & ~7
+    return n, m, s * t.element_size()
 
 
-def _index(t, name: str, n: int | None = None) -> None:
+def _matrices(t, name: str) -> tuple[int, int, int, int, int]:
+    """(matrices, rows, columns, bytes between rows, bytes between matrices)."""
+    try:
+        g, n, m = t.shape
+        s0, s1, e = t.stride()
+    except ValueError:
+        raise ValueError(f"{name}: three dimensions expected, not {tuple(t.shape)}") from None
+    if e != 1 and m > 1:
+        raise ValueError(f"{name}: consecutive elements in the last dimension expected, not strides {t.stride()}")
+    if n <= 1:
+        s1 = (m + 7) & ~7
+    if g <= 1:
+        s0 = n * s1
+    size = t.element_size()
+    return g, n, m, s1 * size, s0 * size
+
+
+def _index(t, name: str, n: int | None = None) -> int:
+    """Address of an int32 vector (0 for None)."""
     if t is None:
-        return
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        return 0
+    if t.dtype is not _INT or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
         raise ValueError(f"{name}: contiguous int32 vector{'' if n is None else f' of {n}'} expected")
-
-
-def _row_stride(t, dim: int) -> int:
-    """Bytes between consecutive entries of a dimension; of no consequence, and so the packed value, where there is one."""
-    if t.shape[dim] > 1:
-        return t.stride(dim) * t.element_size()
-    n = t.element_size()
-    for s in t.shape[dim + 1:]:
-        n *= s
-    return (n + 15) // 16 * 16
+    return t.data_ptr()
 
 
 def group_rows(ids, n_as: int = 1, *, adapter=None, n_adapters: int = 0, order=None, offsets=None, stream=None):
@@ -61,73 +81,74 @@ def group_rows(ids, n_as: int = 1, *, adapter=None, n_adapters: int = 0, order=N
     and adapter i32 [T] (or None) -> (order i32 [T*k], offsets i32 [G + 1]),
     G = n_as * max(1, n_adapters). Negative entries take a pair out of every
     group."""
-    if ids is None and adapter is None:
-        raise ValueError("group_rows: ids or adapter")
-    dev = _device(ids, adapter, order, offsets)
-    _index(adapter, "adapter", None if ids is None else ids.shape[0])
     if ids is not None:
-        _matrix(ids, "ids", 2)
-        if ids.dtype != torch.int32:
+        T, k, nbi1 = _rows(ids, "ids")
+        if ids.dtype is not _INT:
             raise ValueError("ids: int32 expected")
-        T, k = ids.shape
-        ids_ptr, nbi1 = ids.data_ptr(), _row_stride(ids, 0) if T > 1 else 4 * k
-    else:
+        ids_ptr, like = ids.data_ptr(), ids
+        adapter_ptr = _index(adapter, "adapter", T)
+    elif adapter is not None:
+        adapter_ptr, like = _index(adapter, "adapter"), adapter
         T, k, ids_ptr, nbi1 = adapter.shape[0], 1, 0, 0
+    else:
+        raise ValueError("group_rows: ids or adapter")
     G = n_as * max(1, n_adapters)
-    where = adapter.device if ids is None else ids.device
+    dev = _device(ids, adapter, order, offsets)
     if order is None:
-        order = torch.empty(T * k, dtype=torch.int32, device=where)
+        order = like.new_empty(T * k)
+        order_ptr = order.data_ptr()
+    else:
+        order_ptr = _index(order, "order", T * k)
     if offsets is None:
-        offsets = torch.empty(G + 1, dtype=torch.int32, device=where)
-    _index(order, "order", T * k)
-    _index(offsets, "offsets", G + 1)
-    rc = L.lib().gx_group_rows(ids_ptr, k, T, nbi1, 0 if adapter is None else adapter.data_ptr(), n_as, n_adapters,
-                               order.data_ptr(), offsets.data_ptr(), _raw_stream(stream, dev))
-    L.check(rc, "gx_group_rows")
+        offsets = like.new_empty(G + 1)
+        offsets_ptr = offsets.data_ptr()
+    else:
+        offsets_ptr = _index(offsets, "offsets", G + 1)
+    rc = _LIB.gx_group_rows(ids_ptr, k, T, nbi1, adapter_ptr, n_as, n_adapters, order_ptr, offsets_ptr, _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_group_rows")
     return order, offsets
 
 
 def round_rows(x, dtype, out=None, stream=None):
     """gx_quantize_rows for unquantised weights: f32 rows [rows, n] rounded to float16 or bfloat16."""
-    dev = _device(x, out)
-    _matrix(x, "x", 2)
+    n, m, nb1 = _rows(x, "x")
     if x.dtype != torch.float32 or dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("round_rows: float32 rows to float16 or bfloat16")
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype, device=x.device)
-    _matrix(out, "out", 2)
-    if out.shape != x.shape or out.dtype != dtype:
+        out = torch.empty((n, m), dtype=dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != dtype:
         raise ValueError("out: the rows' shape and the given type expected")
-    if x.numel():
-        L.check(L.lib().gx_quantize_rows(_TYPE[dtype], x.data_ptr(), x.shape[1], x.shape[0], _row_stride(x, 0),
-                                         out.data_ptr(), _row_stride(out, 0), _raw_stream(stream, dev)),
-                "gx_quantize_rows")
+    dev = _device(x, out)
+    if n and m:
+        L.check(_LIB.gx_quantize_rows(_TYPE[dtype], x.data_ptr(), m, n, nb1, out.data_ptr(), _rows(out, "out")[2],
+                                      _stream(stream, dev)), "gx_quantize_rows")
     return out
 
 
 def _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype):
-    """Common checks and defaults; the arguments the two products share."""
-    _matrix(w, "weights", 3)
-    _matrix(x, "x", 2)
-    if x.dtype != w.dtype or x.shape[1] != w.shape[2]:
-        raise ValueError(f"x: rows of {w.shape[2]} {w.dtype} elements expected, not {x.shape[1]} of {x.dtype}")
-    _index(offsets, "offsets", w.shape[0] + 1)
-    _index(order, "order")
+    """Common checks and defaults: (result, its type and row stride, the arguments the two products share)."""
+    G, N, K, nb01, nb02 = _matrices(w, "weights")
+    rows, m, nb11 = _rows(x, "x")
+    kind = w.dtype
+    if x.dtype is not kind or m != K:
+        raise ValueError(f"x: rows of {K} {kind} elements expected, not {m} of {x.dtype}")
+    offsets_ptr, order_ptr = _index(offsets, "offsets", G + 1), _index(order, "order")
     if n_rows is None:
-        n_rows = x.shape[0] if order is None else order.shape[0]
+        n_rows = rows if order is None else order.shape[0]
     elif order is not None and n_rows > order.shape[0]:
         raise ValueError("n_rows: more than order holds")
     if out is None:
-        out = torch.empty((n_rows, w.shape[1]), dtype=out_dtype or w.dtype, device=w.device)
+        out = torch.empty((n_rows, N), dtype=out_dtype or kind, device=w.device)
+        nbd1 = N * out.element_size()
     else:
-        _matrix(out, "out", 2)
-        if out.shape[1] != w.shape[1] or out.shape[0] < n_rows or (out_dtype is not None and out.dtype != out_dtype):
-            raise ValueError(f"out: at least {n_rows} rows of {w.shape[1]} elements of the result type expected")
-    if out.dtype not in _TYPE:
+        have, cols, nbd1 = _rows(out, "out")
+        if cols != N or have < n_rows or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out: at least {n_rows} rows of {N} elements of the result type expected")
+    kind_out = _TYPE.get(out.dtype)
+    if kind_out is None:
         raise ValueError(f"results of {out.dtype}")
-    tail = (w.shape[2], w.shape[1], _row_stride(w, 1), _row_stride(w, 0), w.shape[0], x.data_ptr(), x.shape[0],
-            _row_stride(x, 0), offsets.data_ptr(), 0 if order is None else order.data_ptr(), n_rows, gather, int(scatter))
-    return out, tail
+    return out, kind_out, nbd1, (K, N, nb01, nb02, G, x.data_ptr(), rows, nb11, offsets_ptr, order_ptr, n_rows, gather, scatter)
 
 
 def mul_mat_grouped(w, x, offsets, *, order=None, n_rows: int | None = None, gather: int = 0, scatter: bool = False,
@@ -138,10 +159,10 @@ def mul_mat_grouped(w, x, offsets, *, order=None, n_rows: int | None = None, gat
     order[j] with scatter. Rows of no group are left as they were
     (uninitialised in a result allocated here)."""
     dev = _device(w, x, offsets, order, out)
-    out, tail = _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
-    rc = L.lib().gx_mul_mat_grouped(_TYPE.get(w.dtype, -1), w.data_ptr(), *tail, _TYPE[out.dtype], out.data_ptr(),
-                                    _row_stride(out, 0), _raw_stream(stream, dev))
-    L.check(rc, "gx_mul_mat_grouped")
+    out, kind, nbd1, args = _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
+    rc = _LIB.gx_mul_mat_grouped(_TYPE.get(w.dtype, -1), w.data_ptr(), *args, kind, out.data_ptr(), nbd1, _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_mul_mat_grouped")
     return out
 
 
@@ -151,15 +172,14 @@ def mul_mat_grouped_glu(gate, up, x, offsets, *, order=None, n_rows: int | None 
     """gx_mul_mat_grouped_glu: as mul_mat_grouped with act(gate product, up
     product) in place of the product (ACT_SWIGLU, or ACT_SWIGLU_OAI with alpha
     and limit)."""
-    dev = _device(gate, up, x, offsets, order, out)
-    _matrix(up, "up", 3)
-    if up.shape != gate.shape or up.dtype != gate.dtype or \
-            (_row_stride(up, 0), _row_stride(up, 1)) != (_row_stride(gate, 0), _row_stride(gate, 1)):
+    if up.shape != gate.shape or up.dtype != gate.dtype or up.stride() != gate.stride():
         raise ValueError("gate and up: one shape, type and layout expected")
-    out, tail = _product(gate, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
-    rc = L.lib().gx_mul_mat_grouped_glu(_TYPE.get(gate.dtype, -1), gate.data_ptr(), up.data_ptr(), *tail, act, alpha, limit,
-                                        _TYPE[out.dtype], out.data_ptr(), _row_stride(out, 0), _raw_stream(stream, dev))
-    L.check(rc, "gx_mul_mat_grouped_glu")
+    dev = _device(gate, up, x, offsets, order, out)
+    out, kind, nbd1, args = _product(gate, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
+    rc = _LIB.gx_mul_mat_grouped_glu(_TYPE.get(gate.dtype, -1), gate.data_ptr(), up.data_ptr(), *args, act, alpha, limit, kind,
+                                     out.data_ptr(), nbd1, _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_mul_mat_grouped_glu")
     return out
 
 
@@ -171,11 +191,11 @@ def lora_mul_mat(a, b, x, offsets, *, order=None, gather: int = 1, n_as: int | N
     input of their type, base [n_rows, N] its output; ranks i32 and scale f32
     [adapters] (n_as defaults to G // len(ranks or scale), else 1). order and
     offsets as group_rows gives them; row r of base belongs to x[r // gather]."""
-    dev = _device(a, b, x, offsets, order, ranks, scale, base, out)
-    for t, name, dims in ((a, "a", 3), (b, "b", 3), (x, "x", 2), (base, "base", 2)):
-        _matrix(t, name, dims)
-    G, rank, K = a.shape
-    if b.shape[0] != G or b.shape[2] != rank or not a.dtype == b.dtype == x.dtype or x.shape[1] != K:
+    G, rank, K, nba1, nba2 = _matrices(a, "a")
+    gb, N, rb, nbb1, nbb2 = _matrices(b, "b")
+    rows, m, nb11 = _rows(x, "x")
+    n_rows, cols, nbb = _rows(base, "base")
+    if gb != G or rb != rank or m != K or not a.dtype is b.dtype is x.dtype:
         raise ValueError("a [G, rank, K], b [G, N, rank] and x [rows, K] of one type expected")
     if n_as is None:
         per = ranks if ranks is not None else scale
@@ -183,22 +203,24 @@ def lora_mul_mat(a, b, x, offsets, *, order=None, gather: int = 1, n_as: int | N
     if n_as <= 0 or G % n_as:
         raise ValueError("n_as: a divisor of the number of matrices")
     adapters = G // n_as
-    _index(offsets, "offsets", G + 1)
-    _index(order, "order", base.shape[0])
-    _index(ranks, "ranks", adapters)
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous()):
         raise ValueError(f"scale: contiguous float32 vector of {adapters} expected")
     if out is None:
-        out = torch.empty(base.shape, dtype=base.dtype, device=base.device)
-    _matrix(out, "out", 2)
-    if base.shape[1] != b.shape[1] or out.shape != base.shape or out.dtype != base.dtype or base.dtype not in _TYPE:
-        raise ValueError(f"base and out: rows of {b.shape[1]} elements of one result type expected")
-    desc = L.gx_lora_desc(_TYPE.get(a.dtype, -1), rank, K, b.shape[1], n_as, adapters, a.data_ptr(), _row_stride(a, 1),
-                          _row_stride(a, 0), b.data_ptr(), _row_stride(b, 1), _row_stride(b, 0),
-                          None if ranks is None else ranks.data_ptr(), None if scale is None else scale.data_ptr())
-    rc = L.lib().gx_lora_mul_mat(C.byref(desc), x.data_ptr(), x.shape[0], _row_stride(x, 0), offsets.data_ptr(),
-                                 0 if order is None else order.data_ptr(), base.shape[0], gather, _TYPE[base.dtype],
-                                 base.data_ptr(), _row_stride(base, 0), out.data_ptr(), _row_stride(out, 0),
-                                 _raw_stream(stream, dev))
-    L.check(rc, "gx_lora_mul_mat")
+        out = torch.empty((n_rows, cols), dtype=base.dtype, device=base.device)
+        nbd = cols * out.element_size()
+    else:
+        if out.shape != base.shape or out.dtype is not base.dtype:
+            raise ValueError("out: base's shape and type expected")
+        nbd = _rows(out, "out")[2]
+    kind = _TYPE.get(base.dtype)
+    if cols != N or kind is None:
+        raise ValueError(f"base: rows of {N} elements of a result type expected")
+    dev = _device(a, b, x, offsets, order, ranks, scale, base, out)
+    desc = L.gx_lora_desc(_TYPE.get(a.dtype, -1), rank, K, N, n_as, adapters, a.data_ptr(), nba1, nba2, b.data_ptr(), nbb1, nbb2,
+                          _index(ranks, "ranks", adapters), 0 if scale is None else scale.data_ptr())
+    rc = _LIB.gx_lora_mul_mat(C.byref(desc), x.data_ptr(), rows, nb11, _index(offsets, "offsets", G + 1),
+                              _index(order, "order", n_rows), n_rows, gather, kind, base.data_ptr(), nbb, out.data_ptr(), nbd,
+                              _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_lora_mul_mat")
     return out
