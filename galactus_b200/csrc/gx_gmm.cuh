@@ -49,6 +49,9 @@ struct GmmParams {
     int32_t stages;
     int32_t box;              // rows of one TMA box of x in place (divides nt / CTAs)
     int32_t mt;               // tiles of the matrix rows
+    int32_t split;            // CTAs of a cluster that share K (single CTAs with nt = 32 only)
+    int32_t seg;              // chunks that one accumulator sums (0: all)
+    int32_t acc;              // TMEM columns of an accumulator
 };
 
 // ------------------------------------------------------------ PTX helpers
@@ -132,6 +135,48 @@ __device__ __forceinline__ void gmm_tma_2d(void * dst, const CUtensorMap * map, 
             "[%4];" ::"r"(smem_u32(dst)),
             "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar) & kLeaderMask)
             : "memory");
+}
+
+// arrive on the same barrier of every CTA of the cluster (lane c of the warp: CTA c)
+__device__ __forceinline__ void arrive_all(uint64_t * bar, int ctas) {
+    const int lane = threadIdx.x & 31;
+    if (lane < ctas)
+        asm volatile(
+            "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar)),
+            "r"(lane)
+            : "memory");
+}
+// arrive on the barrier of CTA `cta`, and a value of its shared memory
+__device__ __forceinline__ void arrive_at(uint64_t * bar, int cta) {
+    asm volatile(
+        "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(cta)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void * p, int cta) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(cta));
+    return r;
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// 32 consecutive columns of this thread's TMEM lane, written
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+    tmem_wait_st();
 }
 
 // four rows of a map with boxes of one row (no multicast: this GPU's own memory)
@@ -292,14 +337,18 @@ struct GmmTile {
 // tile t of the launch: the tiles of the matrix run fastest, so that CTAs at
 // work together read the same rows and one expert's weights (m0: its first
 // matrix row, `rows` per tile)
+template <int ROUND>
 __device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t * pre, int t, int rows) {
     GmmTile r;
     const int tt = t / p.mt;
     r.m0 = (t - tt * p.mt) * rows;
     r.g = tile_group(pre, p.G, tt);
     const int lo = p.offsets[r.g], hi = p.offsets[r.g + 1];
-    r.row0 = lo + (tt - pre[r.g]) * p.nt;
-    r.cnt = min(p.nt, hi - r.row0);
+    // a group's tiles are of one size, rather than full ones and a rest
+    const int n = pre[r.g + 1] - pre[r.g];
+    const int size = ((hi - lo + n - 1) / n + ROUND - 1) / ROUND * ROUND;
+    r.row0 = lo + (tt - pre[r.g]) * size;
+    r.cnt = min(size, hi - r.row0);
     return r;
 }
 
@@ -428,7 +477,7 @@ __device__ __forceinline__ void put_rows_as(const GmmParams & p, uint8_t * stage
 template <int CTAS, bool GLU>
 __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ GmmParams p) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], drained;
+    __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], part_full, part_free[2], drained;
     __shared__ uint32_t tslot;
     __shared__ int4 gather_mem[kGmmGatherWarps * 8];
     __shared__ int32_t wsum[kGmmThreads / 32];
@@ -436,12 +485,15 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     int32_t * gather_rows = reinterpret_cast<int32_t *>(gather_mem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);              // CTA of the pair; 0 leads
-    const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
+    const int split = CTAS == 1 ? p.split : 1;
+    const int me = CTAS == 1 ? (int)blockIdx.x % split : 0;             // share of K
+    const int unit = (int)blockIdx.x / (CTAS * split), units = (int)gridDim.x / (CTAS * split);
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t stage_bytes = gmm_stage_bytes(CTAS, p.nt);
     uint8_t * staging = ring + (uint32_t)p.stages * stage_bytes;
     float * xchg = reinterpret_cast<float *>(staging + kGmmStaging);
-    int32_t * pre = reinterpret_cast<int32_t *>(staging + kGmmStaging + (GLU ? kGmmXchg : 0u));
+    float * part = xchg + (GLU ? kGmmXchg / 4 : 0u);                     // [2][nt][128] partial sums of a shared tile
+    int32_t * pre = reinterpret_cast<int32_t *>(part + (split > 1 ? 2 * p.nt * kGmmRows : 0));
     constexpr int kOut = GLU ? kGmmRows / 2 : kGmmRows;                  // result rows of a CTA's tile
     constexpr int kRound = 16 * CTAS;                                    // MMA N: a multiple of this
 
@@ -454,6 +506,8 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             mbar_init(acc_full + i, 1);
             mbar_init(acc_empty + i, kGmmEpiWarps * CTAS);
         }
+        mbar_init(&part_full, (uint32_t)(kGmmEpiWarps * split));
+        for (int i = 0; i < 2; ++i) mbar_init(part_free + i, kGmmEpiWarps);
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
@@ -461,11 +515,12 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     if (warp == 1) gmm_tmem_alloc<CTAS>(&tslot, 512);
     tile_prefix(pre, wsum, p.G, p.nt, [&](int g) { return group_rows_of(p.offsets, g, p.n_rows); });
     tc_fence_before();
-    if constexpr (CTAS == 1) __syncthreads(); else cluster_sync_all();
+    if (CTAS * split == 1) __syncthreads(); else cluster_sync_all();
     tc_fence_after();
     const uint32_t tbase = tslot;
     const int tiles = pre[p.G] * p.mt;
     const int nk = (p.K + kGmmK - 1) / kGmmK;
+    const int k0 = nk * me / split, k1 = nk * (me + 1) / split;          // this CTA's chunks of K
     const int gathering = p.gather ? (p.nt / CTAS + 31) / 32 : 0;        // warps that gather
 
     if (warp == 0) {
@@ -475,7 +530,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             RingPos at;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
-                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
                 const int m0 = q.m0 + rank * kOut;
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
                 const int r0 = q.row0 + rank * half;
@@ -491,7 +546,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                         if (r == rank) boxes = b;
                     }
                 }
-                for (int kc = 0; kc < nk; ++kc, ++c, at.next(p.stages)) {
+                for (int kc = k0; kc < k1; ++kc, ++c, at.next(p.stages)) {
                     uint64_t * bar = full + at.s;
                     if (at.round != 0) {
                         ok = gmm_wait_one<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
@@ -520,25 +575,30 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             RingPos at;
             bool ok = true;
             const uint64_t da0 = umma_desc_sw128(ring, 1024u), db0 = umma_desc_sw128(ring + kGmmATile, 1024u);
-            for (int t = unit; t < tiles && ok; t += units, ++it) {
-                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+            for (int t = unit; t < tiles && ok; t += units) {
+                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
                 const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
                 const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
-                const int b = it & 1;
-                if (it >= 2) ok = gmm_wait_one<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
-                const uint32_t d = tbase + (uint32_t)b * 256u;
-                for (int kc = 0; kc < nk && ok; ++kc, at.next(p.stages)) {
-                    ok = gmm_wait_one<CTAS>(full + at.s, at.round & 1u, &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    // (a stage's address only touches the low word: 14 bits of 16 bytes)
-                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
+                for (int kc = k0; kc < k1 && ok; ++it) {
+                    const int b = it & 1, end = p.seg ? min(kc + p.seg, k1) : k1;
+                    if (it >= 2) ok = gmm_wait_one<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
+                    const uint32_t d = tbase + (uint32_t)(b * p.acc);
+                    uint32_t more = 0;                                   // the first MMA overwrites the accumulator
+                    for (; kc < end && ok; ++kc, at.next(p.stages)) {
+                        ok = gmm_wait_one<CTAS>(full + at.s, at.round & 1u, &abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        // (a stage's address only touches the low word: 14 bits of 16 bytes)
+                        const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
 #pragma unroll
-                    for (int i = 0; i < kGmmK / 16; ++i)
-                        mma_f16<CTAS>(d, da0 + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i), idesc, kc | i);
-                    gmm_commit<CTAS>(empty + at.s);
+                        for (int i = 0; i < kGmmK / 16; ++i) {
+                            mma_f16<CTAS>(d, da0 + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i), idesc, more);
+                            more = 1;
+                        }
+                        gmm_commit<CTAS>(empty + at.s);
+                    }
+                    if (ok) gmm_commit<CTAS>(acc_full + b);
                 }
-                if (ok) gmm_commit<CTAS>(acc_full + b);
             }
             if (!ok) {
                 volatile int none = 0;
@@ -560,7 +620,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             RingPos at;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
-                const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
+                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
                 const int quads = gather_quads(n, gw);
@@ -579,7 +639,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 8; ++i) of[i] = *reinterpret_cast<const int4 *>(rows + i * 4);
                     RingPos on = at;
-                    for (int kc = 0; kc < nk; ++kc, on.next(p.stages)) {
+                    for (int kc = k0; kc < k1; ++kc, on.next(p.stages)) {
                         if (on.round != 0) {
                             ok = gmm_wait_one<CTAS>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
                             if (!ok) break;
@@ -592,7 +652,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
-                at.skip(nk, p.stages);
+                at.skip(k1 - k0, p.stages);
             }
         }
     } else {
@@ -600,20 +660,91 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
         const int quad = warp & 3;             // TMEM lanes 32 * quad ..
         uint8_t * stage = staging + (uint32_t)quad * (kGmmStaging / kGmmEpiWarps);
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | (uintptr_t)p.nbd1) & 15u) == 0;
-        int it = 0, xb = 0;
+        const uint32_t lanes = (uint32_t)quad << 21, dsum = tbase + lanes + 2u * (uint32_t)p.acc;
+        int it = 0, xb = 0, i_tile = 0;
         bool ok = true;
-        for (int t = unit; t < tiles && ok; t += units, ++it) {
-            const GmmTile q = gmm_tile(p, pre, t, kOut * CTAS);
-            const int b = it & 1;
-            ok = gmm_wait<CTAS>(acc_full + b, (uint32_t)((it / 2) & 1), &abort_flag);
+        for (int t = unit; t < tiles && ok; t += units, ++i_tile) {
+            const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
+            const int nseg = p.seg ? (k1 - k0 + p.seg - 1) / p.seg : 1;
+            uint32_t d = 0;
+            for (int sg = 0; sg < nseg && ok; ++sg, ++it) {
+                const int b = it & 1;
+                ok = gmm_wait<CTAS>(acc_full + b, (uint32_t)((it / 2) & 1), &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                d = tbase + lanes + (uint32_t)(b * p.acc);
+                if (sg + 1 == nseg) break;
+                // an earlier segment of K: onto the running sums in TMEM, rounded to nearest
+                for (int c0 = 0; c0 < q.cnt; c0 += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(d + (uint32_t)c0, v);
+                    if (sg > 0) {
+                        uint32_t w[32];
+                        tmem_ld32(dsum + (uint32_t)c0, w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(w[i]), __uint_as_float(v[i])));
+                    }
+                    tmem_st32(dsum + (uint32_t)c0, v);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<CTAS>(acc_empty + b);
+            }
             if constexpr (GLU) ok = pair_agrees(1 + (quad & 1), ok);
             if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = tbase + (uint32_t)b * 256u + ((uint32_t)quad << 21);
+            // the tile's f32 sums of columns c0 .. c0 + 31
+            auto sums = [&](int c0, uint32_t (&v)[32]) {
+                tmem_ld32(d + (uint32_t)c0, v);
+                if (nseg > 1) {
+                    uint32_t w[32];
+                    tmem_ld32(dsum + (uint32_t)c0, w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(w[i]), __uint_as_float(v[i])));
+                }
+            };
+            const int leader = i_tile % split, pb = i_tile & 1;
+            if (split > 1) {
+                // K is shared: the partial sums go to shared memory, and the
+                // tile's leader (in turn) adds them up in CTA order
+                if (i_tile >= 2) ok = gmm_wait<2>(part_free + pb, (uint32_t)((i_tile / 2 - 1) & 1), &abort_flag);
+                if (ok) {
+                    uint32_t v[32];
+                    sums(0, v);
+                    float * to = part + (pb * p.nt) * kGmmRows + quad * 32 + lane;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (i < q.cnt) to[i * kGmmRows] = __uint_as_float(v[i]);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        gmm_arrive<CTAS>(acc_empty + (it & 1));
+                        arrive_at(&part_full, leader);
+                    }
+                    if (me == leader) ok = gmm_wait<2>(&part_full, (uint32_t)((i_tile / split) & 1), &abort_flag);
+                }
+                if constexpr (GLU) ok = pair_agrees(1 + (quad & 1), ok);
+                if (!ok) break;
+                if (me != leader) {
+                    ++it;
+                    continue;
+                }
+            }
             const int n0 = q.m0 + rank * kOut + (GLU ? quad & 1 : quad) * 32;
             for (int c0 = 0; c0 < q.cnt; c0 += 32) {
                 uint32_t v[32];
-                tmem_ld32(d + (uint32_t)c0, v);
+                if (split > 1) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0u;
+                    for (int c = 0; c < split; ++c) {
+                        const uint32_t from = peer_addr(part + (pb * p.nt) * kGmmRows + quad * 32 + lane, c);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < q.cnt)
+                                v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), ld_peer(from + (uint32_t)i * (kGmmRows * 4u))));
+                    }
+                } else {
+                    sums(c0, v);
+                }
                 bool nan = false;
                 int my = c0 + lane < q.cnt ? gmm_dst_row(p, q.row0 + c0 + lane, nan) : -1;
                 const unsigned nans = __ballot_sync(0xffffffffu, nan);
@@ -646,13 +777,19 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     put_rows_as<32>(p, stage, own, my, n0, vec);
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) gmm_arrive<CTAS>(acc_empty + b);
+            if (split > 1) {
+                __syncwarp();
+                arrive_all(part_free + pb, split);
+            } else {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<CTAS>(acc_empty + (it & 1));
+            }
+            ++it;
         }
     }
     tc_fence_before();
-    if constexpr (CTAS == 1) __syncthreads(); else cluster_sync_all();
+    if (CTAS * split == 1) __syncthreads(); else cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
         gmm_tmem_free<CTAS>(tbase, 512);

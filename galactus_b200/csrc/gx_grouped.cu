@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 
 #include "../../include/galactus_b200.h"
@@ -67,6 +68,32 @@ int device_sms() {
         sms[dev] = n;
     }
     return sms[dev];
+}
+
+// Clusters of a kernel that run at once (SMs are grouped in GPCs of unequal
+// size, so clusters of 4 or 8 leave some out), one CTA per SM; `slot` names
+// the kernel in the table of what was asked before.
+int resident_clusters(const void * fn, int cluster, int threads, uint32_t smem, int slot) {
+    static std::atomic<int> known[kMaxDevices][3][4];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+    std::atomic<int> & k = known[dev][slot][cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3];
+    int n = k.load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) return 0;
+    k.store(n, std::memory_order_relaxed);
+    return n;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
@@ -159,14 +186,45 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const int64_t touched = std::min(n_rows, n_as);
     const int64_t avg = (n_rows + touched - 1) / touched;
     const int ctas = avg >= 96 ? 2 : 1;
+    const int64_t nk = (ne00 + gx::kGmmK - 1) / gx::kGmmK;
+    // The tensor cores' f32 accumulators drop what does not fit instead of
+    // rounding, about 1e-9 of the sum per element of K. Results of 16 bits do
+    // not see that; for f32 results an accumulator takes 512 elements and the
+    // sums of the accumulators are rounded adds. A third of TMEM holds them.
+    p.seg = out == gx::GMM_F32 && nk > 12 ? 8 : 0;
     p.nt = 32;
-    if (ctas == 2) p.nt = 256;
+    if (ctas == 2) p.nt = p.seg ? 160 : 256;
     else
         while (p.nt < 128 && p.nt < 2 * avg) p.nt *= 2;
+    p.acc = p.seg ? p.nt : 256;
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
     p.box = std::min(128, p.nt / ctas);
     const int out_rows = (glu ? gx::kGmmRows / 2 : gx::kGmmRows) * ctas;
     p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
-    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (glu ? gx::kGmmXchg : 0u);
+    const void * fn = ctas == 2 ? (glu ? (const void *)gx::k_gmm<2, true> : (const void *)gx::k_gmm<2, false>)
+                                : (glu ? (const void *)gx::k_gmm<1, true> : (const void *)gx::k_gmm<1, false>);
+    // Few tiles: 2, 4 or 8 CTAs share a tile's K, whichever leaves the fewest
+    // chunks (and about three more per shared tile for the exchange) to the
+    // busiest CTA.
+    p.split = 1;
+    int64_t clusters = sms / ctas;
+    if (ctas == 1 && p.nt == 32) {
+        const int64_t tiles = (int64_t)p.mt * touched;
+        int64_t best = 0;
+        for (int c = 1; c <= 8 && c <= nk; c *= 2) {
+            const int64_t n = c == 1 ? sms : resident_clusters(fn, c, gx::kGmmThreads, gx::kMaxSmem - 2048u, glu ? 1 : 0);
+            if (n == 0) return GX_ERR_CUDA;
+            const int64_t cost = (tiles + n - 1) / n * ((nk + c - 1) / c + (c > 1 ? 3 : 1));
+            if (c == 1 || cost < best) {
+                best = cost;
+                p.split = c;
+                clusters = n;
+            }
+        }
+    }
+    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (glu ? gx::kGmmXchg : 0u) +
+                           (p.split > 1 ? 2u * (uint32_t)p.nt * gx::kGmmRows * 4u : 0u);
     const uint32_t stage = gx::gmm_stage_bytes(ctas, p.nt);
     p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, (gx::kMaxSmem - 2048u - fixed) / stage);
     const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
@@ -174,22 +232,19 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
         (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows / 2)) ||
         !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)p.box))
         return GX_ERR_ALIGN;
-    const int sms = device_sms();
-    if (sms == 0) return GX_ERR_CUDA;
     const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
     if (most > kMaxIndex) return GX_ERR_INVALID;
-    const void * fn = ctas == 2 ? (glu ? (const void *)gx::k_gmm<2, true> : (const void *)gx::k_gmm<2, false>)
-                                : (glu ? (const void *)gx::k_gmm<1, true> : (const void *)gx::k_gmm<1, false>);
     cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(sms / ctas, most)));
+    const int cluster = ctas * p.split;
+    cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(clusters, most)));
     cfg.blockDim = dim3(gx::kGmmThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)ctas;
+    at.val.clusterDim.x = (unsigned)cluster;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
@@ -334,20 +389,32 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (sms == 0) return GX_ERR_CUDA;
     // small ranks leave room for two CTAs per SM, whose phases overlap
     const uint32_t fixed = gx::lora_fixed_bytes(p.ra, p.G), stage = gx::lora_stage_bytes(p.ra);
-    const int per_sm = fixed + 1024u + 4u * stage <= 113u * 1024u ? 2 : 1;
-    const uint32_t room = (per_sm == 2 ? 113u * 1024u : gx::kMaxSmem - 2048u) - 1024u - fixed;
-    p.stages = (int32_t)std::min<uint32_t>(gx::kLoraMaxStages, room / stage);
+    const int per_sm = fixed + 1024u + 4u * stage <= gx::kLoraHalfSm ? 2 : 1;
+    const uint32_t room = (per_sm == 2 ? gx::kLoraHalfSm : gx::kMaxSmem - 2048u) - 1024u - fixed;
+    p.stages = (int32_t)std::min<uint32_t>(gx::kLoraMaxStages, room / stage) & ~1;      // (even: two copying warps in turn)
     const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
     const int64_t most = n_rows / gx::kLoraRows + std::min(n_rows, G);
-    // a cluster per tile of rows, of as many CTAs as still give every tile one
-    // at once (whether or not base is dst: the split of K sets the result's bits)
-    const int64_t slots = (int64_t)sms * per_sm;
-    int ctas = 8;
-    while (ctas > 1 && (most * ctas > slots || ctas > std::max((K + 63) / 64, (N + 127) / 128))) ctas /= 2;
+    // A cluster per tile of rows, of the size whose rounds of tiles cost least:
+    // a tile's work is shared by its CTAs, but for about a sixteenth that each
+    // repeats. (Whether or not base is dst: the split of K sets the result's
+    // bits.)
+    int ctas = 1;
+    int64_t clusters = (int64_t)sms * per_sm, best = 0;
+    for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 63) / 64, (N + 127) / 128)); c *= 2) {
+        const int64_t n = c == 1 ? clusters
+                                 : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kMaxSmem - 2048u, 2) * per_sm;
+        if (n == 0) return GX_ERR_CUDA;
+        const int64_t cost = (most + n - 1) / n * (16 / c + 1);
+        if (c == 1 || cost < best) {
+            best = cost;
+            ctas = c;
+            clusters = n;
+        }
+    }
     cudaError_t e = cudaFuncSetAttribute(gx::k_lora, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(slots / ctas, most + (p.copy ? n_rows / gx::kLoraRows + 1 : 0))));
+    cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(clusters, most + (p.copy ? n_rows / gx::kLoraRows + 1 : 0))));
     cfg.blockDim = dim3(gx::kLoraThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);

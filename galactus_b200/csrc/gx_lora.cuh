@@ -31,11 +31,10 @@ namespace gx {
 constexpr int kLoraRows = 32;                   // rows of a tile (MMA N)
 constexpr int kLoraMaxRank = 128;
 constexpr int kLoraMaxStages = 12;
-constexpr int kLoraGatherWarps = kLoraRows / 32;
-constexpr int kLoraFixWarps = 2;
 constexpr int kLoraEpiWarps = 4;
-constexpr int kLoraThreads = 32 * (2 + kLoraGatherWarps + kLoraFixWarps + kLoraEpiWarps);
-constexpr uint32_t kLoraTmem = 128;             // columns: h, two result tiles (of 32)
+constexpr int kLoraThreads = 32 * (4 + kLoraEpiWarps);           // 8 warps: two CTAs of 128 registers a thread fit an SM
+constexpr uint32_t kLoraHalfSm = 112u * 1024u;  // dynamic shared memory that leaves room for a second CTA
+constexpr uint32_t kLoraTmem = 128;             // columns: two tiles of h, two of results (32 each)
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
 
@@ -80,17 +79,6 @@ __device__ __forceinline__ uint64_t lora_desc(const void * smem, uint32_t row_by
     const uint64_t layout = row_bytes == 128u ? 2u : row_bytes == 64u ? 4u : 6u;
     return (uint64_t)((smem_u32(smem) >> 4) & 0x3FFFu) | ((uint64_t)1u << 16) | ((uint64_t)((row_bytes * 8u) >> 4) << 32) |
            (1ull << 46) | (layout << 61);
-}
-
-// arrive on the same barrier of every CTA of the cluster (lane c of the warp: CTA c)
-__device__ __forceinline__ void arrive_all(uint64_t * bar, int ctas) {
-    const int lane = threadIdx.x & 31;
-    if (lane < ctas)
-        asm volatile(
-            "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\t"
-            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar)),
-            "r"(lane)
-            : "memory");
 }
 
 __device__ __forceinline__ float4 ld_peer4(const float * p, int cta) {
@@ -230,8 +218,8 @@ __device__ __forceinline__ void split_h(const float (&h)[8], bool bf16, uint4 (&
 __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant__ LoraParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kLoraMaxStages], empty[kLoraMaxStages], b_full[2], b_empty[2], b_fixed[2], d2_full[2], d2_empty[2];
-    __shared__ uint64_t d1_full, d1_empty, part_full, part_free, h_full, h_empty, drained;
-    __shared__ int4 gather_mem[kLoraRows / 4];
+    __shared__ uint64_t d1_full[2], d1_empty[2], part_full, part_free, h_full, h_empty, drained;
+    __shared__ int4 gather_mem[2 * kLoraRows / 4];
     __shared__ uint32_t tslot;
     __shared__ int32_t wsum[kLoraThreads / 32];
     __shared__ int abort_flag;
@@ -261,12 +249,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         for (int i = 0; i < 2; ++i) {
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
-            mbar_init(b_fixed + i, kLoraFixWarps);
+            mbar_init(b_fixed + i, 1);
+            mbar_init(d1_full + i, 1);
+            mbar_init(d1_empty + i, kLoraEpiWarps);
             mbar_init(d2_full + i, 1);
             mbar_init(d2_empty + i, kLoraEpiWarps);
         }
-        mbar_init(&d1_full, 1);
-        mbar_init(&d1_empty, kLoraEpiWarps);
         mbar_init(&part_full, (uint32_t)(kLoraEpiWarps * C));
         mbar_init(&part_free, (uint32_t)(kLoraEpiWarps * C));
         mbar_init(&h_full, kLoraEpiWarps);
@@ -281,118 +269,28 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     if (C > 1) cluster_sync_all(); else __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
-    const uint32_t d1 = tbase, d2 = tbase + (uint32_t)kLoraRows;
+    const uint32_t d1 = tbase, d2 = tbase + 2u * (uint32_t)kLoraRows;
     const int tiles = pre[p.G + 1];
     const int nk = (p.K + kGmmK - 1) / kGmmK;
     const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
     const int nn = (p.N + 127) / 128;                                          // result tiles; this CTA's: me, me + C, ..
 
-    if (warp == 0) {
-        // ------------------------------------------------ A and B by TMA
-        if (elect_one()) {
-            int c = 0, done = 0, bc = 0;
-            RingPos at;
-            bool ok = true;
-            for (int t = unit; t < tiles && ok; t += units) {
-                const LoraTile q = lora_tile(p, pre, t);
-                if (q.rank == 0) continue;
-                uint32_t bytes = (uint32_t)p.ra * 128u;
-                for (int w = 0; w < kLoraGatherWarps; ++w) bytes += (uint32_t)gather_quads(q.cnt, w) * 512u;
-                for (int kc = k0; kc < k1; ++kc, ++c, at.next(p.stages)) {
-                    if (at.round != 0) {
-                        ok = gmm_wait_one<1>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
-                        if (!ok) break;
-                        ++done;
-                    }
-                    mbar_arrive_expect_tx(full + at.s, bytes);
-                    tma_load_3d(ring + (uint32_t)at.s * stage_bytes + kLoraXTile, &p.amap, kc * kGmmK, 0, q.g, full + at.s);
-                }
-                for (int i = me; i < nn && ok; i += C, ++bc) {
-                    const int b = bc & 1;
-                    if (bc >= 2) ok = gmm_wait_one<1>(b_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
-                    if (!ok) break;
-                    const int nb = q.rank > 64 ? 2 : 1;
-                    mbar_arrive_expect_tx(b_full + b, (uint32_t)nb * b_block);
-                    for (int j = 0; j < nb; ++j)
-                        tma_load_3d(bring + (uint32_t)b * b_bytes + (uint32_t)j * b_block, &p.bmap, j * 64, i * 128, q.g, b_full + b);
-                }
-            }
-            if (!ok) {
-                // copies in flight land before the CTA leaves
-                volatile int none = 0;
-                for (int i = done; i < c; ++i) gmm_wait_one<1>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
-                for (int i = max(0, bc - 2); i < bc; ++i) gmm_wait_one<1>(b_full + (i & 1), (uint32_t)((i / 2) & 1), &none);
-            }
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ----------------------------------------------------- MMA issuer
-        if (elect_one()) {
-            int it = 0, bc = 0;
-            RingPos at;
-            bool ok = true;
-            const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
-            const uint64_t b0 = lora_desc(bring, row_bytes), h0 = lora_desc(hbuf, row_bytes);
-            const int parts = p.bf16 ? 3 : 2;
-            for (int t = unit; t < tiles && ok; t += units) {
-                const LoraTile q = lora_tile(p, pre, t);
-                if (q.rank == 0) continue;
-                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, 128, (uint32_t)((q.cnt + 15) & ~15));
-                if (it > 0) ok = gmm_wait_one<1>(&d1_empty, (uint32_t)((it - 1) & 1), &abort_flag);
-                for (int kc = k0; kc < k1 && ok; ++kc, at.next(p.stages)) {
-                    ok = gmm_wait_one<1>(full + at.s, at.round & 1u, &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
-#pragma unroll
-                    for (int i = 0; i < kGmmK / 16; ++i)
-                        mma_f16<1>(d1, a0 + off + (uint64_t)(2 * i), x0 + off + (uint64_t)(2 * i), idesc, (uint32_t)((kc - k0) | i));
-                    gmm_commit<1>(empty + at.s);
-                }
-                if (!ok) break;
-                gmm_commit<1>(&d1_full);
-                ok = gmm_wait_one<1>(&h_full, (uint32_t)(it & 1), &abort_flag);
-                const int steps = (q.rank + 15) / 16;
-                for (int i = me; i < nn && ok; i += C, ++bc) {
-                    const int b = bc & 1;
-                    ok = gmm_wait_one<1>((p.ranks != nullptr ? b_fixed : b_full) + b, (uint32_t)((bc / 2) & 1), &abort_flag);
-                    if (ok && bc >= 2) ok = gmm_wait_one<1>(d2_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    for (int st = 0; st < steps; ++st) {
-                        const uint64_t blk = (uint64_t)(st >> 2), in = (uint64_t)(2 * (st & 3));
-                        const uint64_t bd = b0 + (uint64_t)((uint32_t)b * b_bytes >> 4) + blk * (b_block >> 4) + in;
-                        for (int part_i = 0; part_i < parts; ++part_i)
-                            mma_f16<1>(d2 + (uint32_t)b * (uint32_t)kLoraRows, bd,
-                                       h0 + ((uint64_t)part_i * blocks + blk) * (h_block >> 4) + in, idesc,
-                                       (uint32_t)(st | part_i));
-                    }
-                    gmm_commit<1>(b_empty + b);
-                    gmm_commit<1>(d2_full + b);
-                }
-                if (ok) gmm_commit<1>(&h_empty);
-                ++it;
-            }
-            if (!ok) {
-                volatile int none = 0;
-                gmm_commit<1>(&drained);
-                gmm_wait_one<1>(&drained, 0, &none);
-            }
-        }
-        __syncwarp();
-    } else if (warp < 2 + kLoraGatherWarps) {
-        // ------------- rows of x: tile::gather4 copies, up to 32 rows a warp
-        // (a warp without rows in a tile still copies four, as in k_gmm)
-        const int gw = warp - 2;
+    if (warp == 0 || warp == 2) {
+        // ------ A by TMA tiles and the rows of x by tile::gather4: two warps,
+        // chunk by chunk in turn (one thread's issue rate would set the pace;
+        // the stage count is even, so a stage stays with one of them)
+        const int gw = warp >> 1;
         int32_t * rows = reinterpret_cast<int32_t *>(gather_mem + gw * 8);
+        int c0 = 0;                    // chunks of the CTA so far
         RingPos at;
         bool ok = true;
         for (int t = unit; t < tiles && ok; t += units) {
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
-            const int quads = gather_quads(q.cnt, gw);
+            const int quads = (q.cnt + 3) >> 2;                          // rows in fours; those behind the last repeat it
+            const uint32_t bytes = (uint32_t)p.ra * 128u + (uint32_t)quads * 512u;
             bool bad = false;
-            const int row = lora_row(p, q.row0 + min(gw * 32 + lane, q.cnt - 1), bad);
+            const int row = lora_row(p, q.row0 + min(lane, q.cnt - 1), bad);
             if (bad) record_error(GX_DEVERR_DOMAIN);
             __syncwarp();
             rows[lane] = bad || row < 0 ? 0 : row / p.gather;
@@ -402,49 +300,161 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 8; ++i) of[i] = *reinterpret_cast<const int4 *>(rows + i * 4);
                 RingPos on = at;
-                for (int kc = k0; kc < k1; ++kc, on.next(p.stages)) {
+                int c = c0;
+                for (int kc = k0; kc < k1; ++kc, ++c, on.next(p.stages)) {
+                    if ((c & 1) != gw) continue;
                     if (on.round != 0) {
                         ok = gmm_wait_one<1>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
                         if (!ok) break;
                     }
-                    uint8_t * to = ring + (uint32_t)on.s * stage_bytes + (uint32_t)gw * 4096u;
+                    uint8_t * st = ring + (uint32_t)on.s * stage_bytes;
+                    mbar_arrive_expect_tx(full + on.s, bytes);
+                    tma_load_3d(st + kLoraXTile, &p.amap, kc * kGmmK, 0, q.g, full + on.s);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (i < quads)
-                            gmm_gather4<1>(to + i * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
+                            gmm_gather4<1>(st + i * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
+                }
+                if (!ok) {
+                    // copies in flight land before the CTA leaves
+                    volatile int none = 0;
+                    for (int i = max(0, c - p.stages); i < c; ++i)
+                        if ((i & 1) == gw) gmm_wait_one<1>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
+            c0 += k1 - k0;
             at.skip(k1 - k0, p.stages);
         }
-    } else if (warp < 2 + kLoraGatherWarps + kLoraFixWarps) {
-        // -------- where the rank ends inside a step of 16, B's columns behind
-        // it are cleared in shared memory: a zero in h does not silence a NaN
-        const int fw = warp - 2 - kLoraGatherWarps;
-        int bc = 0;
-        bool ok = p.ranks != nullptr;
+    } else if (warp == 1) {
+        // ----------------------------------------------------- MMA issuer
+        if (elect_one()) {
+            int it = 0, bc = 0;
+            RingPos at;
+            bool ok = true;
+            const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
+            const uint64_t b0 = lora_desc(bring, row_bytes), h0 = lora_desc(hbuf, row_bytes);
+            const int parts = p.bf16 ? 3 : 2;
+            // The results of a tile are issued between the chunks of the next
+            // tile's h, as its own h and the tiles of B become ready: neither
+            // the exchange over the cluster nor the copies of x hold the other up.
+            LoraTile last{};
+            int next = 0;                              // result tile of `last` to issue
+            bool open = false, have_h = false;
+            auto ready = [&](uint64_t * bar, uint32_t parity, bool wait) {
+                if (!wait) return mbar_test_wait(bar, parity);
+                ok = ok && gmm_wait_one<1>(bar, parity, &abort_flag);
+                return ok;
+            };
+            auto results = [&](bool wait) {            // (j of `last`: it - 1)
+                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, 128, (uint32_t)((last.cnt + 15) & ~15));
+                if (!have_h) have_h = ready(&h_full, (uint32_t)((it - 1) & 1), wait);
+                if (!have_h) return;
+                const int steps = (last.rank + 15) / 16;
+                for (; next < nn; next += C, ++bc) {
+                    const int b = bc & 1;
+                    if (!ready((p.ranks != nullptr ? b_fixed : b_full) + b, (uint32_t)((bc / 2) & 1), wait)) return;
+                    if (bc >= 2 && !ready(d2_empty + b, (uint32_t)((bc / 2 - 1) & 1), wait)) return;
+                    tc_fence_after();
+                    for (int st = 0; st < steps; ++st) {
+                        const uint64_t blk = (uint64_t)(st >> 2), in = (uint64_t)(2 * (st & 3));
+                        const uint64_t bd = b0 + (uint64_t)((uint32_t)b * b_bytes >> 4) + blk * (b_block >> 4) + in;
+                        for (int part_i = 0; part_i < parts; ++part_i)
+                            mma_f16<1>(d2 + (uint32_t)(b * kLoraRows), bd,
+                                       h0 + ((uint64_t)part_i * blocks + blk) * (h_block >> 4) + in, idesc,
+                                       (uint32_t)(st | part_i));
+                    }
+                    gmm_commit<1>(b_empty + b);
+                    gmm_commit<1>(d2_full + b);
+                }
+                gmm_commit<1>(&h_empty);
+                open = false;
+            };
+            for (int t = unit; t < tiles && ok; t += units) {
+                const LoraTile q = lora_tile(p, pre, t);
+                if (q.rank == 0) continue;
+                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, 128, (uint32_t)((q.cnt + 15) & ~15));
+                const int b = it & 1;
+                if (it >= 2) ok = gmm_wait_one<1>(d1_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
+                for (int kc = k0; kc < k1 && ok; ++kc, at.next(p.stages)) {
+                    for (uint32_t i = 0; open && i < (1u << 20) && !mbar_test_wait(full + at.s, at.round & 1u); ++i) results(false);
+                    ok = gmm_wait_one<1>(full + at.s, at.round & 1u, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
+#pragma unroll
+                    for (int i = 0; i < kGmmK / 16; ++i)
+                        mma_f16<1>(d1 + (uint32_t)(b * kLoraRows), a0 + off + (uint64_t)(2 * i), x0 + off + (uint64_t)(2 * i), idesc,
+                                   (uint32_t)((kc - k0) | i));
+                    gmm_commit<1>(empty + at.s);
+                }
+                if (!ok) break;
+                gmm_commit<1>(d1_full + b);
+                if (open) results(true);
+                if (!ok) break;
+                last = q;
+                next = me;
+                open = true;
+                have_h = false;
+                ++it;
+            }
+            if (ok && open) results(true);
+            if (!ok) {
+                volatile int none = 0;
+                gmm_commit<1>(&drained);
+                gmm_wait_one<1>(&drained, 0, &none);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        // ------------------------------------------------------- B by TMA
+        // and, where an adapter's rank ends inside a step of 16, B's columns
+        // behind it cleared in shared memory: a zero in h does not silence a NaN
+        int bc = 0, seen = 0, rank_was = 0;
+        bool ok = true;
+        auto fix = [&](int rank) {
+            const int b = seen & 1;
+            if (!gmm_wait<1>(b_full + b, (uint32_t)((seen / 2) & 1), &abort_flag)) return false;
+            const int behind = rank < p.rank ? (rank + 15) & ~15 : rank;     // (behind the pool's rank TMA fills in zeros)
+            if (rank < behind) {
+                uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(rank >> 6) * b_block;
+                for (int row = lane; row < 128; row += 32)
+                    for (int r = rank; r < behind; ++r)
+                        *reinterpret_cast<uint16_t *>(tile + lora_swizzle(row_bytes, row, (r & 63) >> 3) + (r & 7) * 2) = 0;
+                fence_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) gmm_arrive<1>(b_fixed + b);
+            ++seen;
+            return true;
+        };
         for (int t = unit; t < tiles && ok; t += units) {
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
-            const int behind = q.rank < p.rank ? (q.rank + 15) & ~15 : q.rank;     // (behind the pool's rank TMA fills in zeros)
             for (int i = me; i < nn && ok; i += C, ++bc) {
                 const int b = bc & 1;
-                ok = gmm_wait<1>(b_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
+                if (bc >= 2) ok = gmm_wait<1>(b_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
                 if (!ok) break;
-                if (q.rank < behind) {
-                    uint8_t * tile = bring + (uint32_t)b * b_bytes + (uint32_t)(q.rank >> 6) * b_block;
-                    for (int row = fw * 32 + lane; row < 128; row += 32 * kLoraFixWarps)
-                        for (int r = q.rank; r < behind; ++r)
-                            *reinterpret_cast<uint16_t *>(tile + lora_swizzle(row_bytes, row, (r & 63) >> 3) + (r & 7) * 2) = 0;
-                    fence_async_smem();
+                if (elect_one()) {
+                    const int nb = q.rank > 64 ? 2 : 1;
+                    mbar_arrive_expect_tx(b_full + b, (uint32_t)nb * b_block);
+                    for (int j = 0; j < nb; ++j)
+                        tma_load_3d(bring + (uint32_t)b * b_bytes + (uint32_t)j * b_block, &p.bmap, j * 64, i * 128, q.g, b_full + b);
                 }
                 __syncwarp();
-                if (lane == 0) gmm_arrive<1>(b_fixed + b);
+                // the tile before this one has had the time of a copy to land
+                if (p.ranks != nullptr && bc > 0) ok = fix(rank_was);
+                rank_was = q.rank;
             }
+        }
+        if (p.ranks != nullptr && ok && bc > 0) ok = fix(rank_was);
+        if (!ok) {
+            volatile int none = 0;
+            for (int i = max(0, bc - 2); i < bc; ++i) gmm_wait<1>(b_full + (i & 1), (uint32_t)((i / 2) & 1), &none);
         }
     } else {
         // ------------------------------------------------- h and results
-        const int quad = warp & 3, ew = warp - 2 - kLoraGatherWarps - kLoraFixWarps;
+        const int quad = warp & 3, ew = warp - 4;
         float * stage = staging + quad * (16 * 32);
         const int esz = p.out == GMM_F32 ? 4 : 2;
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.nbd |
@@ -465,8 +475,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 }
                 continue;
             }
+            // what does not depend on h is on its way before h is
+            bool bad = false;
+            const int my = lane < q.cnt ? lora_row(p, q.row0 + lane, bad) : -1;
+            const unsigned nans = __ballot_sync(0xffffffffu, bad);
+            const float scale = p.scale != nullptr ? p.scale[q.g / p.n_as] : 1.0f;
             // the partial h of this CTA's share of K: lanes are ranks, columns rows
-            ok = gmm_wait<1>(&d1_full, (uint32_t)(it & 1), &abort_flag);
+            const uint32_t d1_now = d1 + (uint32_t)((it & 1) * kLoraRows);
+            ok = gmm_wait<1>(d1_full + (it & 1), (uint32_t)((it / 2) & 1), &abort_flag);
             if (ok && it > 0) ok = gmm_wait<2>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) break;
             tc_fence_after();
@@ -474,7 +490,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 const int r = quad * 32 + lane;
                 for (int c0 = 0; c0 < q.cnt; c0 += 16) {
                     uint32_t v[16];
-                    tmem_ld16(d1 + (uint32_t)c0 + ((uint32_t)quad << 21), v);
+                    tmem_ld16(d1_now + (uint32_t)c0 + ((uint32_t)quad << 21), v);
                     tmem_wait_ld();
                     if (r < p.ra) {
 #pragma unroll
@@ -484,15 +500,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) gmm_arrive<1>(&d1_empty);
+            if (lane == 0) gmm_arrive<1>(d1_empty + (it & 1));
             arrive_all(&part_full, C);
             ok = gmm_wait<2>(&part_full, (uint32_t)(it & 1), &abort_flag);
             if (ok && it > 0) ok = gmm_wait<1>(&h_empty, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) break;
             // sum over the cluster in CTA order, scale, split, store as an MMA operand
             {
-                const int a = q.g / p.n_as;
-                const float s = p.scale != nullptr ? p.scale[a] : 1.0f;
                 const int per = p.ra / 8;                              // eight ranks per thread; a power of two <= 16
                 const int rows16 = (q.cnt + 15) & ~15;
                 const int items = rows16 * per;                        // a multiple of 32
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     float big = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        h[e] = r0 + e < q.rank && row < q.cnt ? __fmul_rn(h[e], s) : 0.0f;
+                        h[e] = r0 + e < q.rank && row < q.cnt ? __fmul_rn(h[e], scale) : 0.0f;
                         big = fmaxf(big, fabsf(h[e]));
                     }
                     if (!p.bf16) {
@@ -534,9 +548,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             if (lane == 0) gmm_arrive<1>(&h_full);
             arrive_all(&part_free, C);
             ok = gmm_wait<1>(&h_full, (uint32_t)(it & 1), &abort_flag);       // (every row's power of two)
-            bool bad = false;
-            const int my = lane < q.cnt ? lora_row(p, q.row0 + lane, bad) : -1;
-            const unsigned nans = __ballot_sync(0xffffffffu, bad);
             auto results = [&](auto base) {
                 base.load(p, my, me * 128 + quad * 32, vec);
                 for (int nt = me; nt < nn && ok; nt += C, ++bc) {
