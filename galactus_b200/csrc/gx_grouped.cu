@@ -383,13 +383,14 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
     if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
         !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u, (uint32_t)std::min(p.ra, 64)) ||
-        !encode_rows(&p.xmap, p.bf16, x, K, ne11, nb11, 0, 0, 1u))
+        !encode_rows(&p.xmap, p.bf16, x, K, ne11, nb11, 0, 0, 1u) ||
+        !encode_rows(&p.rmap, p.bf16, x, K, ne11, nb11, 0, 0, (uint32_t)gx::kLoraRows))
         return GX_ERR_ALIGN;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
     // small ranks leave room for two CTAs per SM, whose phases overlap
     const uint32_t fixed = gx::lora_fixed_bytes(p.ra, p.G), stage = gx::lora_stage_bytes(p.ra);
-    const int per_sm = fixed + 1024u + 4u * stage <= gx::kLoraHalfSm ? 2 : 1;
+    const int per_sm = fixed + 1024u + 2u * stage <= gx::kLoraHalfSm ? 2 : 1;
     const uint32_t room = (per_sm == 2 ? gx::kLoraHalfSm : gx::kMaxSmem - 2048u) - 1024u - fixed;
     p.stages = (int32_t)std::min<uint32_t>(gx::kLoraMaxStages, room / stage) & ~1;      // (even: two copying warps in turn)
     const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
@@ -400,7 +401,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     // bits.)
     int ctas = 1;
     int64_t clusters = (int64_t)sms * per_sm, best = 0;
-    for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 63) / 64, (N + 127) / 128)); c *= 2) {
+    for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 127) / 128, (N + 127) / 128)); c *= 2) {
         const int64_t n = c == 1 ? clusters
                                  : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kMaxSmem - 2048u, 2) * per_sm;
         if (n == 0) return GX_ERR_CUDA;

@@ -35,6 +35,7 @@ constexpr int kLoraEpiWarps = 4;
 constexpr int kLoraThreads = 32 * (4 + kLoraEpiWarps);           // 8 warps: two CTAs of 128 registers a thread fit an SM
 constexpr uint32_t kLoraHalfSm = 112u * 1024u;  // dynamic shared memory that leaves room for a second CTA
 constexpr uint32_t kLoraTmem = 128;             // columns: two tiles of h, two of results (32 each)
+constexpr int kLoraK = 128;                     // elements of K per stage: two swizzled rows of 64
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
 
@@ -42,6 +43,7 @@ struct LoraParams {
     CUtensorMap amap;         // A: [K, rank, G], boxes 64 x ra
     CUtensorMap bmap;         // B: [rank, N, G], boxes min(ra, 64) x 128
     CUtensorMap xmap;         // x: [K, rows], boxes 64 x 1, gathered
+    CUtensorMap rmap;         // x: boxes 64 x 32
     const int32_t * offsets;  // [G + 1]
     const int32_t * order;    // [n_rows] or NULL: rows in place
     const int32_t * ranks;    // [G / n_as] or NULL: all `rank`
@@ -57,7 +59,7 @@ struct LoraParams {
     int32_t stages;
 };
 
-__host__ __device__ constexpr uint32_t lora_stage_bytes(int ra) { return kLoraXTile + (uint32_t)ra * 128u; }
+__host__ __device__ constexpr uint32_t lora_stage_bytes(int ra) { return 2u * (kLoraXTile + (uint32_t)ra * 128u); }
 // B and h lie in blocks of up to 64 ranks, their rows swizzled over 32, 64 or
 // 128 bytes: as many as the ranks fill
 __host__ __device__ constexpr uint32_t lora_blocks(int ra) { return ra > 64 ? 2u : 1u; }
@@ -133,6 +135,8 @@ __device__ __forceinline__ int lora_row(const LoraParams & p, int j, bool & bad_
     return -1;
 }
 
+__device__ const uint4 g_no_piece = {0u, 0u, 0u, 0u};
+
 // The base of a warp's 32 x 32 tile of results, loaded ahead of the deltas:
 // lane's 16-byte pieces, rows of the 32 columns by `my` (lane i: column i).
 template <typename T>
@@ -144,8 +148,10 @@ struct LoraBase {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int row = __shfl_sync(0xffffffffu, my, i * kCols + lane / kLanes);
-            if (vec && n + kPer <= p.N && row >= 0)
-                old[i] = *reinterpret_cast<const uint4 *>(p.base + (int64_t)row * p.nbb + (int64_t)n * (int)sizeof(T));
+            // (always a load: one under a condition is waited for where its branches meet)
+            const bool have = vec && n + kPer <= p.N && row >= 0;
+            old[i] = *reinterpret_cast<const uint4 *>(have ? p.base + (int64_t)row * p.nbb + (int64_t)n * (int)sizeof(T)
+                                                           : reinterpret_cast<const uint8_t *>(&g_no_piece));
         }
     }
     // plus 16 staged columns of f32 deltas ([column][32 rows of B], columns 16 * half ..), rounded, to the result rows
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     const uint32_t blocks = lora_blocks(p.ra), stage_bytes = lora_stage_bytes(p.ra), b_block = lora_b_block(p.ra);
     const uint32_t b_bytes = blocks * b_block, h_block = lora_h_block(p.ra), row_bytes = lora_row(p.ra);
     // the ring comes first: an MMA over 128 rows of A reads past the last
-    // stage's rows into what follows (lanes that nobody looks at)
+    // stage's rows into what follows (16 KB at most; lanes that nobody looks at)
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t * bring = ring + (uint32_t)p.stages * stage_bytes;
     uint8_t * hbuf = bring + 2u * b_bytes;
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     const uint32_t tbase = tslot;
     const uint32_t d1 = tbase, d2 = tbase + 2u * (uint32_t)kLoraRows;
     const int tiles = pre[p.G + 1];
-    const int nk = (p.K + kGmmK - 1) / kGmmK;
+    const int nk = (p.K + kLoraK - 1) / kLoraK;
     const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
     const int nn = (p.N + 127) / 128;                                          // result tiles; this CTA's: me, me + C, ..
 
@@ -288,13 +294,18 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
             const int quads = (q.cnt + 3) >> 2;                          // rows in fours; those behind the last repeat it
-            const uint32_t bytes = (uint32_t)p.ra * 128u + (uint32_t)quads * 512u;
+            
             bool bad = false;
             const int row = lora_row(p, q.row0 + min(lane, q.cnt - 1), bad);
             if (bad) record_error(GX_DEVERR_DOMAIN);
+            const int from = bad || row < 0 ? 0 : row / p.gather;
             __syncwarp();
-            rows[lane] = bad || row < 0 ? 0 : row / p.gather;
+            rows[lane] = from;
             __syncwarp();
+            // rows that follow one another (a request's chunk of a prefill) are one box
+            const int first = __shfl_sync(0xffffffffu, from, 0);
+            const bool run = __all_sync(0xffffffffu, lane >= q.cnt || from == first + lane) && q.cnt > 4;
+            const uint32_t bytes = 2u * ((uint32_t)p.ra * 128u + (run ? kLoraXTile : (uint32_t)quads * 512u));
             if (elect_one()) {
                 int4 of[8];
 #pragma unroll
@@ -309,11 +320,19 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     }
                     uint8_t * st = ring + (uint32_t)on.s * stage_bytes;
                     mbar_arrive_expect_tx(full + on.s, bytes);
-                    tma_load_3d(st + kLoraXTile, &p.amap, kc * kGmmK, 0, q.g, full + on.s);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i < quads)
-                            gmm_gather4<1>(st + i * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
+                    for (int half = 0; half < 2; ++half) {
+                        // (past the end of K, TMA fills in zeros)
+                        const int x = kc * kLoraK + half * kGmmK;
+                        tma_load_3d(st + 2u * kLoraXTile + (uint32_t)half * (uint32_t)p.ra * 128u, &p.amap, x, 0, q.g, full + on.s);
+                        uint8_t * xt = st + (uint32_t)half * kLoraXTile;
+                        if (run) gmm_tma_2d<1>(xt, &p.rmap, x, first, full + on.s);
+                        else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (i < quads) gmm_gather4<1>(xt + i * 512, &p.xmap, x, of[i].x, of[i].y, of[i].z, of[i].w, full + on.s);
+                        }
+                    }
                 }
                 if (!ok) {
                     // copies in flight land before the CTA leaves
@@ -332,7 +351,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             int it = 0, bc = 0;
             RingPos at;
             bool ok = true;
-            const uint64_t a0 = umma_desc_sw128(ring + kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
+            const uint64_t a0 = umma_desc_sw128(ring + 2u * kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
             const uint64_t b0 = lora_desc(bring, row_bytes), h0 = lora_desc(hbuf, row_bytes);
             const int parts = p.bf16 ? 3 : 2;
             // The results of a tile are issued between the chunks of the next
@@ -373,19 +392,27 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             for (int t = unit; t < tiles && ok; t += units) {
                 const LoraTile q = lora_tile(p, pre, t);
                 if (q.rank == 0) continue;
-                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, 128, (uint32_t)((q.cnt + 15) & ~15));
+                // (16 ranks sit in the first lanes of a 64-row MMA too, at half the shared memory reads)
+                const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, p.ra == 16 ? 64 : 128, (uint32_t)((q.cnt + 15) & ~15));
                 const int b = it & 1;
                 if (it >= 2) ok = gmm_wait_one<1>(d1_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
                 for (int kc = k0; kc < k1 && ok; ++kc, at.next(p.stages)) {
-                    for (uint32_t i = 0; open && i < (1u << 20) && !mbar_test_wait(full + at.s, at.round & 1u); ++i) results(false);
+                    uint32_t polls = 0;
+                    while (open) {
+                        results(false);
+                        if (mbar_test_wait(full + at.s, at.round & 1u) || ++polls == (1u << 20)) break;
+                    }
                     ok = gmm_wait_one<1>(full + at.s, at.round & 1u, &abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
 #pragma unroll
-                    for (int i = 0; i < kGmmK / 16; ++i)
-                        mma_f16<1>(d1 + (uint32_t)(b * kLoraRows), a0 + off + (uint64_t)(2 * i), x0 + off + (uint64_t)(2 * i), idesc,
-                                   (uint32_t)((kc - k0) | i));
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int i = 0; i < kGmmK / 16; ++i)
+                            mma_f16<1>(d1 + (uint32_t)(b * kLoraRows), a0 + off + (uint64_t)(half * p.ra * 8 + 2 * i),
+                                       x0 + off + (uint64_t)(half * (int)(kLoraXTile >> 4) + 2 * i), idesc,
+                                       (uint32_t)((kc - k0) | half | i));
                     gmm_commit<1>(empty + at.s);
                 }
                 if (!ok) break;
@@ -459,6 +486,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         const int esz = p.out == GMM_F32 ? 4 : 2;
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | reinterpret_cast<uintptr_t>(p.base) | (uintptr_t)p.nbd |
                            (uintptr_t)p.nbb) & 15u) == 0;
+        const bool row_pieces = (p.N * esz) % 16 == 0;         // whole 16-byte pieces
         int it = 0, bc = 0;
         bool ok = true;
         for (int t = unit; t < tiles && ok; t += units) {
@@ -480,6 +508,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             const int my = lane < q.cnt ? lora_row(p, q.row0 + lane, bad) : -1;
             const unsigned nans = __ballot_sync(0xffffffffu, bad);
             const float scale = p.scale != nullptr ? p.scale[q.g / p.n_as] : 1.0f;
+            if (vec && row_pieces) {
+                // base on its way into L2: lane's row, the warps' result tiles in turn
+                for (int nt = me + ew * C; nt < nn && my >= 0; nt += kLoraEpiWarps * C) {
+                    const uint32_t bytes = (uint32_t)min(128, p.N - nt * 128) * (uint32_t)esz;
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.base + (int64_t)my * p.nbb + (int64_t)nt * 128 * esz),
+                                 "r"(bytes)
+                                 : "memory");
+                }
+            }
             // the partial h of this CTA's share of K: lanes are ranks, columns rows
             const uint32_t d1_now = d1 + (uint32_t)((it & 1) * kLoraRows);
             ok = gmm_wait<1>(d1_full + (it & 1), (uint32_t)((it / 2) & 1), &abort_flag);
