@@ -22,9 +22,17 @@ constexpr int kGmmK = 64;                      // elements of K per stage: one 1
 constexpr uint32_t kGmmATile = kGmmRows * 128u;
 constexpr int kGmmMaxStages = 12;
 constexpr int kGmmGatherWarps = 4;             // 32 rows each
-constexpr int kGmmEpiWarps = 4;
-constexpr int kGmmThreads = 32 * (2 + kGmmGatherWarps + kGmmEpiWarps);
-constexpr uint32_t kGmmStaging = kGmmEpiWarps * 32u * 32u * 4u;   // results of 32 columns per epilogue warp
+// what a kernel makes of its tiles
+enum : int {
+    GMM_PLAIN = 0,   // y = W x: 128 rows of W
+    GMM_GLU = 1,     // gated: 64 gate and 64 up rows, two accumulators in turn
+    GMM_DUAL = 2,    // gated, CTA pairs, 16-bit results: 128 gate and 128 up rows, one accumulator each
+};
+__host__ __device__ constexpr int gmm_epi_warps(int mode) { return mode == GMM_DUAL ? 8 : 4; }
+__host__ __device__ constexpr int gmm_threads(int mode) { return 32 * (2 + kGmmGatherWarps + gmm_epi_warps(mode)); }
+__host__ __device__ constexpr int gmm_out_rows(int mode) { return mode == GMM_GLU ? 64 : 128; }
+__host__ __device__ constexpr uint32_t gmm_a_bytes(int mode) { return mode == GMM_DUAL ? 2u * kGmmATile : kGmmATile; }
+constexpr uint32_t kGmmStaging = 4u * 32u * 32u * 4u;            // results of 32 (dual: 16) columns per epilogue warp
 constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer][warp pair][direction][column][lane] f32
 
 enum : int { GMM_F32 = 0, GMM_F16 = 1, GMM_BF16 = 2 };
@@ -395,15 +403,30 @@ __device__ __forceinline__ float gmm_exp(float x) {
 // The activation on f32 sums. The quotient is CUDA's fast division (2 steps):
 // the sums are not those of the bit-exact formats anyway, and a full division
 // per value kept the epilogue behind the tensor cores.
+template <bool OAI>
 __device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) {
-    if (p.act == 0) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, gmm_exp(-g))), u);
+    if (!OAI) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, gmm_exp(-g))), u);
     const float x = p.limit < g ? p.limit : g;
     const float y = u < -p.limit ? -p.limit : (p.limit < u ? p.limit : u);
     return __fmul_rn(__fdividef(x, __fadd_rn(1.0f, gmm_exp(__fmul_rn(p.alpha, -x)))), __fadd_rn(y, 1.0f));
 }
+// of N values at once: g becomes the result (the choice of the activation
+// stays outside the loop, so that the values' chains of operations overlap)
+template <int N>
+__device__ __forceinline__ void gmm_act_all(const GmmParams & p, float (&g)[N], const float (&u)[N]) {
+    if (p.act == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = gmm_act<false>(p, g[i], u[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = gmm_act<true>(p, g[i], u[i]);
+    }
+}
 
 // bytes of a ring stage: the matrix tile and the CTA's rows
-__host__ __device__ constexpr uint32_t gmm_stage_bytes(int ctas, int nt) { return kGmmATile + (uint32_t)(nt / ctas) * 128u; }
+__host__ __device__ constexpr uint32_t gmm_stage_bytes(int ctas, int nt, int mode) {
+    return gmm_a_bytes(mode) + (uint32_t)(nt / ctas) * 128u;
+}
 
 // position in the ring of stages: stage, and how often the ring was gone round
 struct RingPos {
@@ -474,27 +497,30 @@ __device__ __forceinline__ void put_rows_as(const GmmParams & p, uint8_t * stage
     else put_rows<__half, COLS>(p, stage, v, my, n0, vec);
 }
 
-template <int CTAS, bool GLU>
-__global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ GmmParams p) {
+template <int CTAS, int MODE>
+__global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_constant__ GmmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], part_full, part_free[2], drained;
     __shared__ uint32_t tslot;
     __shared__ int4 gather_mem[kGmmGatherWarps * 8];
-    __shared__ int32_t wsum[kGmmThreads / 32];
+    __shared__ int32_t wsum[gmm_threads(MODE) / 32];
     __shared__ int abort_flag;
     int32_t * gather_rows = reinterpret_cast<int32_t *>(gather_mem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);              // CTA of the pair; 0 leads
     const int split = CTAS == 1 ? p.split : 1;
     const int me = CTAS == 1 ? (int)blockIdx.x % split : 0;             // share of K
-    const int unit = (int)blockIdx.x / (CTAS * split), units = (int)gridDim.x / (CTAS * split);
+    constexpr bool GLU = MODE == GMM_GLU;
+    constexpr int kBufs = MODE == GMM_DUAL ? 1 : 2;                      // accumulators that take turns
+    constexpr int kEpi = gmm_epi_warps(MODE);
+    constexpr uint32_t kABytes = gmm_a_bytes(MODE);
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const uint32_t stage_bytes = gmm_stage_bytes(CTAS, p.nt);
+    const uint32_t stage_bytes = gmm_stage_bytes(CTAS, p.nt, MODE);
     uint8_t * staging = ring + (uint32_t)p.stages * stage_bytes;
     float * xchg = reinterpret_cast<float *>(staging + kGmmStaging);
     float * part = xchg + (GLU ? kGmmXchg / 4 : 0u);                     // [2][nt][128] partial sums of a shared tile
     int32_t * pre = reinterpret_cast<int32_t *>(part + (split > 1 ? 2 * p.nt * kGmmRows : 0));
-    constexpr int kOut = GLU ? kGmmRows / 2 : kGmmRows;                  // result rows of a CTA's tile
+    constexpr int kOut = gmm_out_rows(MODE);                             // result rows of a CTA's tile
     constexpr int kRound = 16 * CTAS;                                    // MMA N: a multiple of this
 
     if (tid == 0) {
@@ -504,10 +530,10 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, kGmmEpiWarps * CTAS);
+            mbar_init(acc_empty + i, kEpi * CTAS);
         }
-        mbar_init(&part_full, (uint32_t)(kGmmEpiWarps * split));
-        for (int i = 0; i < 2; ++i) mbar_init(part_free + i, kGmmEpiWarps);
+        mbar_init(&part_full, (uint32_t)(kEpi * split));
+        for (int i = 0; i < 2; ++i) mbar_init(part_free + i, kEpi);
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
@@ -520,7 +546,27 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     const uint32_t tbase = tslot;
     const int tiles = pre[p.G] * p.mt;
     const int nk = (p.K + kGmmK - 1) / kGmmK;
-    const int k0 = nk * me / split, k1 = nk * (me + 1) / split;          // this CTA's chunks of K
+    // The tiles in turn: whole ones, a CTA (or pair) each, and, when few are
+    // left for the last round, those by all CTAs of a cluster that share K.
+    const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
+    const int cid = (int)blockIdx.x / (CTAS * split), clusters = (int)gridDim.x / (CTAS * split);
+    int whole = tiles;
+    if (split > 1) {
+        const int rest = tiles % units;
+        // (about three chunks of time go into a shared tile's exchange)
+        if ((rest + clusters - 1) / clusters * (nk / split + 3) < nk) whole = tiles - rest;
+    }
+    struct Work {
+        int t;
+        bool shared;
+    };
+    auto start = [&] { return unit < whole ? Work{unit, false} : Work{whole + cid, true}; };
+    auto advance = [&](Work & w) {
+        w.t += w.shared ? clusters : units;
+        if (!w.shared && w.t >= whole) w = Work{whole + cid, true};
+    };
+    auto first_chunk = [&](const Work & w) { return w.shared ? nk * me / split : 0; };
+    auto end_chunk = [&](const Work & w) { return w.shared ? nk * (me + 1) / split : nk; };
     const int gathering = p.gather ? (p.nt / CTAS + 31) / 32 : 0;        // warps that gather
 
     if (warp == 0) {
@@ -529,12 +575,13 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             int c = 0, done = 0;       // chunks started; chunks whose stage was handed back
             RingPos at;
             bool ok = true;
-            for (int t = unit; t < tiles && ok; t += units) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
+            for (Work w = start(); w.t < tiles && ok; advance(w)) {
+                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const int m0 = q.m0 + rank * kOut;
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
                 const int r0 = q.row0 + rank * half;
-                uint32_t bytes = (uint32_t)CTAS * kGmmATile;
+                uint32_t bytes = (uint32_t)CTAS * kABytes;
                 int boxes = 0;
                 for (int r = 0; r < CTAS; ++r) {
                     const int n = max(0, min(half, q.cnt - r * half));
@@ -556,9 +603,9 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     uint8_t * st = ring + (uint32_t)at.s * stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
                     gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
-                    if (GLU) gmm_tma_3d<CTAS>(st + kGmmATile / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
+                    if (MODE != GMM_PLAIN) gmm_tma_3d<CTAS>(st + kABytes / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
                     for (int b = 0; b < boxes; ++b)
-                        gmm_tma_2d<CTAS>(st + kGmmATile + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
+                        gmm_tma_2d<CTAS>(st + kABytes + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
                 }
             }
             if (!ok && rank == 0) {
@@ -574,14 +621,15 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             int it = 0;
             RingPos at;
             bool ok = true;
-            const uint64_t da0 = umma_desc_sw128(ring, 1024u), db0 = umma_desc_sw128(ring + kGmmATile, 1024u);
-            for (int t = unit; t < tiles && ok; t += units) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
+            const uint64_t da0 = umma_desc_sw128(ring, 1024u), db0 = umma_desc_sw128(ring + kABytes, 1024u);
+            for (Work w = start(); w.t < tiles && ok; advance(w)) {
+                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
                 const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
                 for (int kc = k0; kc < k1 && ok; ++it) {
-                    const int b = it & 1, end = p.seg ? min(kc + p.seg, k1) : k1;
-                    if (it >= 2) ok = gmm_wait_one<CTAS>(acc_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
+                    const int b = it % kBufs, end = p.seg ? min(kc + p.seg, k1) : k1;
+                    if (it >= kBufs) ok = gmm_wait_one<CTAS>(acc_empty + b, (uint32_t)((it / kBufs - 1) & 1), &abort_flag);
                     const uint32_t d = tbase + (uint32_t)(b * p.acc);
                     uint32_t more = 0;                                   // the first MMA overwrites the accumulator
                     for (; kc < end && ok; ++kc, at.next(p.stages)) {
@@ -591,10 +639,15 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                         // (a stage's address only touches the low word: 14 bits of 16 bytes)
                         const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
 #pragma unroll
-                        for (int i = 0; i < kGmmK / 16; ++i) {
-                            mma_f16<CTAS>(d, da0 + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i), idesc, more);
-                            more = 1;
+                        for (int i = 0; i < kGmmK / 16; ++i)
+                            mma_f16<CTAS>(d, da0 + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i), idesc, more | (uint32_t)i);
+                        if constexpr (MODE == GMM_DUAL) {
+#pragma unroll
+                            for (int i = 0; i < kGmmK / 16; ++i)
+                                mma_f16<CTAS>(d + 256u, da0 + (kGmmATile >> 4) + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i),
+                                              idesc, more | (uint32_t)i);
                         }
+                        more = 1;
                         gmm_commit<CTAS>(empty + at.s);
                     }
                     if (ok) gmm_commit<CTAS>(acc_full + b);
@@ -619,8 +672,9 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
             int32_t * rows = gather_rows + gw * 32;
             RingPos at;
             bool ok = true;
-            for (int t = unit; t < tiles && ok; t += units) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
+            for (Work w = start(); w.t < tiles && ok; advance(w)) {
+                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
                 const int quads = gather_quads(n, gw);
@@ -644,7 +698,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                             ok = gmm_wait_one<CTAS>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
                             if (!ok) break;
                         }
-                        uint8_t * to = ring + (uint32_t)on.s * stage_bytes + kGmmATile + (uint32_t)gw * 4096u;
+                        uint8_t * to = ring + (uint32_t)on.s * stage_bytes + kABytes + (uint32_t)gw * 4096u;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             if (i < quads)
@@ -658,18 +712,20 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
     } else {
         // -------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lanes 32 * quad ..
-        uint8_t * stage = staging + (uint32_t)quad * (kGmmStaging / kGmmEpiWarps);
+        const int ew = warp - 2 - kGmmGatherWarps;
+        uint8_t * stage = staging + (uint32_t)ew * (kGmmStaging / kEpi);
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | (uintptr_t)p.nbd1) & 15u) == 0;
         const uint32_t lanes = (uint32_t)quad << 21, dsum = tbase + lanes + 2u * (uint32_t)p.acc;
         int it = 0, xb = 0, i_tile = 0;
         bool ok = true;
-        for (int t = unit; t < tiles && ok; t += units, ++i_tile) {
-            const GmmTile q = gmm_tile<kRound>(p, pre, t, kOut * CTAS);
+        for (Work w = start(); w.t < tiles && ok; advance(w)) {
+            const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+            const int k0 = first_chunk(w), k1 = end_chunk(w);
             const int nseg = p.seg ? (k1 - k0 + p.seg - 1) / p.seg : 1;
             uint32_t d = 0;
             for (int sg = 0; sg < nseg && ok; ++sg, ++it) {
-                const int b = it & 1;
-                ok = gmm_wait<CTAS>(acc_full + b, (uint32_t)((it / 2) & 1), &abort_flag);
+                const int b = it % kBufs;
+                ok = gmm_wait<CTAS>(acc_full + b, (uint32_t)((it / kBufs) & 1), &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 d = tbase + lanes + (uint32_t)(b * p.acc);
@@ -703,7 +759,7 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                 }
             };
             const int leader = i_tile % split, pb = i_tile & 1;
-            if (split > 1) {
+            if (w.shared) {
                 // K is shared: the partial sums go to shared memory, and the
                 // tile's leader (in turn) adds them up in CTA order
                 if (i_tile >= 2) ok = gmm_wait<2>(part_free + pb, (uint32_t)((i_tile / 2 - 1) & 1), &abort_flag);
@@ -717,22 +773,24 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        gmm_arrive<CTAS>(acc_empty + (it & 1));
+                        gmm_arrive<CTAS>(acc_empty + it % kBufs);
                         arrive_at(&part_full, leader);
                     }
                     if (me == leader) ok = gmm_wait<2>(&part_full, (uint32_t)((i_tile / split) & 1), &abort_flag);
                 }
                 if constexpr (GLU) ok = pair_agrees(1 + (quad & 1), ok);
                 if (!ok) break;
+                ++i_tile;
                 if (me != leader) {
                     ++it;
                     continue;
                 }
             }
             const int n0 = q.m0 + rank * kOut + (GLU ? quad & 1 : quad) * 32;
-            for (int c0 = 0; c0 < q.cnt; c0 += 32) {
+            constexpr int kStep = 8 * kEpi;              // (dual: two warps of four share the columns)
+            for (int c0 = 32 * (ew / 4); c0 < q.cnt; c0 += kStep) {
                 uint32_t v[32];
-                if (split > 1) {
+                if (w.shared) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
                     for (int c = 0; c < split; ++c) {
@@ -762,14 +820,35 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     }
                     asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
                     my = __shfl_sync(0xffffffffu, my, (lane & 15) + 16 * up);
+                    float gv[16], uv[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float other = recvp[i * 32];
-                        own[i] = gmm_act(p, up ? other : own[i], up ? own[i] : other);
-                        if ((nans >> (i + 16 * up)) & 1u) own[i] = kNan;
+                        gv[i] = up ? other : own[i];
+                        uv[i] = up ? own[i] : other;
                     }
+                    gmm_act_all<16>(p, gv, uv);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) own[i] = (nans >> (i + 16 * up)) & 1u ? kNan : gv[i];
                     xb ^= 1;
                     put_rows_as<16>(p, stage, own, my, n0, vec);
+                } else if constexpr (MODE == GMM_DUAL) {
+                    uint32_t u[32];
+                    tmem_ld32(d + 256u + (uint32_t)c0, u);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float own[16], uv[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            own[i] = __uint_as_float(v[16 * half + i]);
+                            uv[i] = __uint_as_float(u[16 * half + i]);
+                        }
+                        gmm_act_all<16>(p, own, uv);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((nans >> (i + 16 * half)) & 1u) own[i] = kNan;
+                        put_rows_as<16>(p, stage, own, __shfl_sync(0xffffffffu, my, (lane & 15) + 16 * half), n0, vec);
+                    }
                 } else {
                     float own[32];
 #pragma unroll
@@ -777,13 +856,13 @@ __global__ void __launch_bounds__(kGmmThreads, 1) k_gmm(const __grid_constant__ 
                     put_rows_as<32>(p, stage, own, my, n0, vec);
                 }
             }
-            if (split > 1) {
+            if (w.shared) {
                 __syncwarp();
                 arrive_all(part_free + pb, split);
             } else {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) gmm_arrive<CTAS>(acc_empty + (it & 1));
+                if (lane == 0) gmm_arrive<CTAS>(acc_empty + it % kBufs);
             }
             ++it;
         }

@@ -193,6 +193,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     // sums of the accumulators are rounded adds. A third of TMEM holds them.
     p.seg = out == gx::GMM_F32 && nk > 12 ? 8 : 0;
     p.nt = 32;
+    const int mode = !glu ? gx::GMM_PLAIN : ctas == 2 && p.seg == 0 ? gx::GMM_DUAL : gx::GMM_GLU;
     if (ctas == 2) p.nt = p.seg ? 160 : 256;
     else
         while (p.nt < 128 && p.nt < 2 * avg) p.nt *= 2;
@@ -200,36 +201,33 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
     p.box = std::min(128, p.nt / ctas);
-    const int out_rows = (glu ? gx::kGmmRows / 2 : gx::kGmmRows) * ctas;
+    const int out_rows = gx::gmm_out_rows(mode) * ctas;
     p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
-    const void * fn = ctas == 2 ? (glu ? (const void *)gx::k_gmm<2, true> : (const void *)gx::k_gmm<2, false>)
-                                : (glu ? (const void *)gx::k_gmm<1, true> : (const void *)gx::k_gmm<1, false>);
-    // Few tiles: 2, 4 or 8 CTAs share a tile's K, whichever leaves the fewest
-    // chunks (and about three more per shared tile for the exchange) to the
-    // busiest CTA.
+    const void * fn = mode == gx::GMM_DUAL ? (const void *)gx::k_gmm<2, gx::GMM_DUAL>
+                      : ctas == 2          ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU> : (const void *)gx::k_gmm<2, gx::GMM_PLAIN>)
+                                           : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU> : (const void *)gx::k_gmm<1, gx::GMM_PLAIN>);
+    // The last round of tiles, when it leaves most SMs idle, is shared by the
+    // CTAs of clusters that split K: pairs, or four or eight when not even one
+    // round is full.
     p.split = 1;
     int64_t clusters = sms / ctas;
     if (ctas == 1 && p.nt == 32) {
         const int64_t tiles = (int64_t)p.mt * touched;
-        int64_t best = 0;
-        for (int c = 1; c <= 8 && c <= nk; c *= 2) {
-            const int64_t n = c == 1 ? sms : resident_clusters(fn, c, gx::kGmmThreads, gx::kMaxSmem - 2048u, glu ? 1 : 0);
-            if (n == 0) return GX_ERR_CUDA;
-            const int64_t cost = (tiles + n - 1) / n * ((nk + c - 1) / c + (c > 1 ? 3 : 1));
-            if (c == 1 || cost < best) {
-                best = cost;
-                p.split = c;
-                clusters = n;
-            }
+        for (int c = 8; c > 1; c /= 2) {
+            const int64_t n = nk >= 4 * c ? resident_clusters(fn, c, gx::gmm_threads(mode), gx::kMaxSmem - 2048u, glu ? 1 : 0) : 0;
+            if (n == 0 || (c > 2 && tiles > n)) continue;
+            p.split = c;
+            clusters = n;
+            break;
         }
     }
-    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (glu ? gx::kGmmXchg : 0u) +
+    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (mode == gx::GMM_GLU ? gx::kGmmXchg : 0u) +
                            (p.split > 1 ? 2u * (uint32_t)p.nt * gx::kGmmRows * 4u : 0u);
-    const uint32_t stage = gx::gmm_stage_bytes(ctas, p.nt);
+    const uint32_t stage = gx::gmm_stage_bytes(ctas, p.nt, mode);
     p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, (gx::kMaxSmem - 2048u - fixed) / stage);
     const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
-    if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, glu ? gx::kGmmRows / 2 : gx::kGmmRows) ||
-        (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, gx::kGmmRows / 2)) ||
+    if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, (uint32_t)gx::gmm_out_rows(mode)) ||
+        (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, (uint32_t)gx::gmm_out_rows(mode))) ||
         !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)p.box))
         return GX_ERR_ALIGN;
     const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
@@ -239,7 +237,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     cudaLaunchConfig_t cfg{};
     const int cluster = ctas * p.split;
     cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(clusters, most)));
-    cfg.blockDim = dim3(gx::kGmmThreads);
+    cfg.blockDim = dim3((unsigned)gx::gmm_threads(mode));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at{};
