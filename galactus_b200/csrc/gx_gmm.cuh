@@ -174,6 +174,27 @@ __device__ __forceinline__ float ld_peer(uint32_t addr) {
     return v;
 }
 
+// 32 consecutive columns of this thread's TMEM lane, to be waited for (the
+// second call only ties the registers to the wait)
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_end(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                   "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+    asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
+}
+
 // 32 consecutive columns of this thread's TMEM lane, written
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
@@ -364,9 +385,9 @@ __device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t *
 __device__ __forceinline__ int gather_quads(int n, int w) { return max(1, (min(32, n - w * 32) + 3) >> 2); }
 
 // y row of grouped row j, -1 to skip it (no such row); nan: its x row does not exist
-__device__ __forceinline__ int gmm_dst_row(const GmmParams & p, int j, bool & nan) {
+// (o: order[j], where it is read at all)
+__device__ __forceinline__ int gmm_dst_row(const GmmParams & p, int j, int o, bool & nan) {
     if (p.gather == 0 && p.scatter == 0) return j;
-    const int o = p.order[j];
     nan = p.gather != 0 && (o < 0 || o / p.gather >= p.x_rows);
     if (p.scatter == 0) return j;
     if (o >= 0 && o < p.n_rows) return o;
@@ -722,6 +743,10 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
             const int k0 = first_chunk(w), k1 = end_chunk(w);
             const int nseg = p.seg ? (k1 - k0 + p.seg - 1) / p.seg : 1;
+            // the order of the first columns' rows is on its way before the sums are there
+            const bool ordered = p.gather != 0 || p.scatter != 0;
+            const int col0 = 32 * (ew / 4);
+            int o_next = ordered && col0 + lane < q.cnt ? p.order[q.row0 + col0 + lane] : 0;
             uint32_t d = 0;
             for (int sg = 0; sg < nseg && ok; ++sg, ++it) {
                 const int b = it % kBufs;
@@ -788,7 +813,9 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             }
             const int n0 = q.m0 + rank * kOut + (GLU ? quad & 1 : quad) * 32;
             constexpr int kStep = 8 * kEpi;              // (dual: two warps of four share the columns)
-            for (int c0 = 32 * (ew / 4); c0 < q.cnt; c0 += kStep) {
+            for (int c0 = col0; c0 < q.cnt; c0 += kStep) {
+                const int o = o_next;
+                o_next = ordered && c0 + kStep + lane < q.cnt ? p.order[q.row0 + c0 + kStep + lane] : 0;
                 uint32_t v[32];
                 if (w.shared) {
 #pragma unroll
@@ -800,11 +827,13 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                             if (i < q.cnt)
                                 v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), ld_peer(from + (uint32_t)i * (kGmmRows * 4u))));
                     }
+                } else if constexpr (MODE == GMM_DUAL) {
+                    tmem_ld32_start(d + (uint32_t)c0, v);
                 } else {
                     sums(c0, v);
                 }
                 bool nan = false;
-                int my = c0 + lane < q.cnt ? gmm_dst_row(p, q.row0 + c0 + lane, nan) : -1;
+                int my = c0 + lane < q.cnt ? gmm_dst_row(p, q.row0 + c0 + lane, o, nan) : -1;
                 const unsigned nans = __ballot_sync(0xffffffffu, nan);
                 if constexpr (GLU) {
                     // quads 0, 1 hold gate rows, quads 2, 3 the same up rows:
@@ -834,7 +863,9 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                     put_rows_as<16>(p, stage, own, my, n0, vec);
                 } else if constexpr (MODE == GMM_DUAL) {
                     uint32_t u[32];
-                    tmem_ld32(d + 256u + (uint32_t)c0, u);
+                    tmem_ld32_start(d + 256u + (uint32_t)c0, u);
+                    tmem_ld32_end(v);
+                    tmem_ld32_end(u);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float own[16], uv[16];
