@@ -8,12 +8,12 @@
 //
 // ONE launch: the pairs are cut into contiguous segments, one per warp, over
 // a cluster of up to 8 CTAs. Every warp counts its segment's keys into a
-// histogram of its own (match.any finds a step's equal keys, so no atomics
-// and nothing that depends on timing), the counts become starting positions
-// by a prefix over warps, over the CTAs of the cluster (read from their
-// shared memory) and over the groups, and a second pass over the same pairs
-// writes them out. The number of counting warps follows the group count:
-// their histograms must fit in shared memory.
+// histogram of its own, the counts become starting positions by a prefix over
+// warps, over the CTAs of the cluster (read from their shared memory) and
+// over the groups, and a second pass over the same pairs writes them out
+// (match.any ranks a step's equal keys by lane: nothing depends on timing).
+// The number of counting warps follows the group count: their histograms must
+// fit in shared memory.
 //
 // Bound by latency (a 2048-token batch is 131 KB of indices, 20 ns of
 // bandwidth): the design keeps the dependent steps few and the launch single.
@@ -35,6 +35,7 @@ struct GroupParams {
     const int32_t * adapter;  // [T] or NULL
     int32_t k, n_as, n_adapters, G;
     int32_t P;
+    uint32_t div_m, div_l;    // t = q / k as (umulhi(q, div_m) + q) >> div_l
     int32_t warps;            // counting warps per CTA
     int32_t seg;              // pairs per counting warp, a multiple of 32
     int32_t * order;
@@ -43,7 +44,7 @@ struct GroupParams {
 
 // group of pair q, G for none
 __device__ __forceinline__ int group_key(const GroupParams & p, int q) {
-    const int t = q / p.k, s = q - t * p.k;
+    const int t = (int)((__umulhi((uint32_t)q, p.div_m) + (uint32_t)q) >> p.div_l), s = q - t * p.k;
     int key = 0;
     bool bad = false;
     if (p.ids != nullptr) {
@@ -78,12 +79,11 @@ __global__ void __launch_bounds__(1024) k_group_rows(const __grid_constant__ Gro
     const int last = (int)(s0 + p.seg < p.P ? s0 + p.seg : p.P);
     int32_t * mine = hist + warp * G1;
     if (warp < p.warps) {
+        int ahead = first + lane < last ? group_key(p, first + lane) : G1;
         for (int q0 = first; q0 < last; q0 += 32) {
-            const int q = q0 + lane;
-            const int key = q < last ? group_key(p, q) : G1;
-            const unsigned peers = __match_any_sync(0xffffffffu, key);
-            if (key < G1 && lane == __ffs(peers) - 1) mine[key] += __popc(peers);
-            __syncwarp();
+            const int key = ahead;
+            ahead = q0 + 32 + lane < last ? group_key(p, q0 + 32 + lane) : G1;
+            if (key < G1) atomicAdd(mine + key, 1);            // (a count: the order of the adds does not show)
         }
     }
     __syncthreads();
@@ -129,9 +129,10 @@ __global__ void __launch_bounds__(1024) k_group_rows(const __grid_constant__ Gro
     // (the sync also keeps every CTA's totals alive until all have read them)
     if (ncta > 1) cl.sync(); else __syncthreads();
     if (warp < p.warps) {
+        int ahead = first + lane < last ? group_key(p, first + lane) : G1;
         for (int q0 = first; q0 < last; q0 += 32) {
-            const int q = q0 + lane;
-            const int key = q < last ? group_key(p, q) : G1;
+            const int q = q0 + lane, key = ahead;
+            ahead = q + 32 < last ? group_key(p, q + 32) : G1;
             const unsigned peers = __match_any_sync(0xffffffffu, key);
             const int at = __popc(peers & ((1u << lane) - 1u));
             if (key < G1) p.order[base[key] + mine[key] + at] = q;

@@ -276,10 +276,13 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
     p.n_adapters = (int32_t)n_adapters;
     p.G = (int32_t)G;
     p.P = (int32_t)(ne20 * ne21);
+    // exact for dividends below 2^31: l = ceil(log2 k), m = floor(2^32 (2^l - k) / k) + 1
+    while ((1ll << p.div_l) < ne20) ++p.div_l;
+    p.div_m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << p.div_l) - (uint64_t)ne20)) / (uint64_t)ne20 + 1);
     p.order = order;
     p.offsets = offsets;
     const uint32_t bins = (uint32_t)(G + 1) * 4u;
-    const int ncta = p.P <= 2048 ? 1 : gx::kGroupCluster;
+    const int ncta = p.P <= 512 ? 1 : gx::kGroupCluster;      // (at 2048 pairs one CTA takes 6.3 us, eight 4.7)
     const int most = (int)std::min<uint32_t>(32u, (gx::kGroupSmem - 2u * bins) / bins);
     const int64_t steps = ((int64_t)p.P + 31) / 32;
     p.warps = (int)std::max<int64_t>(1, std::min<int64_t>(most, (steps + ncta - 1) / ncta));
