@@ -59,15 +59,14 @@ constexpr int kMaxDevices = 64;
 
 // multiprocessors of the current device
 int device_sms() {
-    static int sms[kMaxDevices];
-    int dev = 0;
+    static std::atomic<int> sms[kMaxDevices];
+    int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-    if (sms[dev] == 0) {
-        int n = 0;
+    if ((n = sms[dev].load(std::memory_order_relaxed)) == 0) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        sms[dev] = n;
+        sms[dev].store(n, std::memory_order_relaxed);
     }
-    return sms[dev];
+    return n;
 }
 
 // Clusters of a kernel that run at once (SMs are grouped in GPCs of unequal

@@ -206,12 +206,10 @@ def lora_mul_mat(a, b, x, offsets, *, order=None, gather: int = 1, n_as: int | N
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous()):
         raise ValueError(f"scale: contiguous float32 vector of {adapters} expected")
     if out is None:
-        out = torch.empty((n_rows, cols), dtype=base.dtype, device=base.device)
-        nbd = cols * out.element_size()
-    else:
-        if out.shape != base.shape or out.dtype is not base.dtype:
-            raise ValueError("out: base's shape and type expected")
-        nbd = _rows(out, "out")[2]
+        out = torch.empty_like(base)
+    elif out.shape != base.shape or out.dtype is not base.dtype:
+        raise ValueError("out: base's shape and type expected")
+    nbd = _rows(out, "out")[2]
     kind = _TYPE.get(base.dtype)
     if cols != N or kind is None:
         raise ValueError(f"base: rows of {N} elements of a result type expected")

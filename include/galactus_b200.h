@@ -302,6 +302,8 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
  * Rows of dst outside every group are left as they were. A group whose borders
  * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped;
  * a row index outside b or dst is reported and its result is NaN or dropped.
+ * With scatter the entries of order in a group must differ from one another and
+ * from those of other groups (each names a row of dst); with gather they need not.
  * Requires 16-byte aligned as, b and strides nb01, nb02, nb11 (so ne00 * 2 may
  * need padded rows), n_as <= 8192. */
 int gx_mul_mat_grouped(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as,
@@ -326,7 +328,7 @@ int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t
  * when order is NULL) and row r / gather of x. base is the projection's output,
  * gx_mul_mat_id's f32 rows for instance; dst may be base (rows without an
  * adapter are then left alone) or lie apart from it (they are copied). dst and
- * base may not overlap in any other way.
+ * base may not overlap in any other way, and order names no row twice.
  *   a      group g's A at a + g*nba2, `rank` rows of ne00 elements, nba1 apart
  *   b      group g's B at b + g*nbb2, ne01 rows of `rank` elements, nbb1 apart
  *   ranks  device i32 [n_adapters], each 0 .. rank (0: no adapter), or NULL:

@@ -114,6 +114,7 @@ def compare(got, want, tol, kind):
 COUNTS = {
     "one": [1], "token": [0, 0, 1, 0, 1, 1, 0, 0, 1], "edges": [15, 16, 17, 0, 31, 32, 33, 0],
     "tiles": [127, 128, 129, 0, 1], "long": [0, 300, 0, 2, 513], "many": [1, 3, 0, 2] * 40, "none": [0, 0, 0],
+    "few": [1, 0, 2, 1, 1], "middle": [40, 90, 0, 20, 64], "wide": [30, 5, 40, 61],
 }
 
 
@@ -130,6 +131,10 @@ def make(G, K, N, rows, kind, seed, sigma=0.05, pad=0):
     ("edges", 72, 129, "bf16", "bf16"), ("edges", 1000, 63, "f16", "f32"), ("tiles", 64, 128, "bf16", "f32"),
     ("tiles", 520, 1001, "f16", "f16"), ("long", 256, 200, "bf16", "bf16"), ("many", 136, 257, "bf16", "f32"),
     ("none", 64, 64, "f16", "f32"), ("long", 4096, 384, "bf16", "f32"),
+    # whole tiles for every SM and a rest that clusters share along K; one round of shared tiles
+    ("few", 2880, 2880, "f16", "f16"), ("few", 2000, 2880, "bf16", "f32"), ("one", 7168, 64, "bf16", "f32"),
+    # 64 and 128 rows a tile in single CTAs, several accumulators for f32 results
+    ("middle", 1544, 500, "bf16", "f32"), ("wide", 328, 260, "f16", "bf16"), ("long", 512, 300, "f16", "f32"),
 ])
 def test_products(gxlib, dev, counts, K, N, kind, out, glu):
     c = COUNTS[counts]
@@ -249,6 +254,62 @@ def test_bad_borders_and_rows_are_reported(gxlib, dev):
     out.fill_(5.0)
     gxlib.mul_mat_grouped(w, x, torch.tensor([0, 10, 10, 10], dtype=torch.int32, device="cuda"), order=order, scatter=True, out=out)
     assert (out == 5.0).all(1).tolist() == [i in (3, 4) for i in range(10)] and device_error() == 1
+
+
+def test_first_call_of_a_process_inside_a_capture(gxlib, dev):
+    """Nothing has to be called before a capture: the first calls of a process may be captured ones."""
+    import subprocess
+    import sys
+    code = """
+import torch, galactus_b200 as gx
+E, K, N, T, k = 6, 256, 200, 20, 2
+g = torch.Generator(device="cuda").manual_seed(1)
+w = torch.randn((E, N, K), device="cuda", generator=g).bfloat16()
+x = torch.randn((T, K), device="cuda", generator=g).bfloat16()
+a = torch.randn((E, 16, K), device="cuda", generator=g).bfloat16()
+b = torch.randn((E, N, 16), device="cuda", generator=g).bfloat16()
+ids = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+def layer():
+    order, offsets = gx.group_rows(ids, E)
+    y = gx.mul_mat_grouped(w, x, offsets, order=order, gather=k, scatter=True, out_dtype=torch.float32)
+    h = gx.mul_mat_grouped_glu(w, w, x, offsets, order=order, gather=k)
+    return gx.lora_mul_mat(a, b, x, offsets, order=order, gather=k, base=y), h
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = layer()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(got, layer()))
+print("captured")
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=str(gxlib._lib.LIB_PATH.parent.parent))
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
+def test_calls_on_two_streams_at_once(gxlib, dev):
+    """Nothing is shared between calls: products, grouping and deltas in flight together give the bits of calls alone."""
+    E, K, N, T, k = 16, 1024, 512, 700, 4
+    w, x = make(E, K, N, T, "bf16", 21)
+    up, _ = make(E, K, N, 0, "bf16", 22)
+    a, b = make(E, K, 16, 0, "bf16", 23)[0], make(E, 16, N, 0, "bf16", 24)[0]
+    ids = torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda")
+
+    def work():
+        order, offsets = gxlib.group_rows(ids, E)
+        y = gxlib.mul_mat_grouped(w, x, offsets, order=order, gather=k, scatter=True, out_dtype=torch.float32)
+        return gxlib.mul_mat_grouped_glu(w, up, x, offsets, order=order, gather=k), \
+            gxlib.lora_mul_mat(a, b, x, offsets, order=order, gather=k, base=y, out=y)
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for g in got:
+        assert torch.equal(g[0], want[0]) and torch.equal(g[1], want[1])
 
 
 def test_capture_streams_and_wrapper_checks(gxlib, dev):
