@@ -253,7 +253,9 @@ __device__ __forceinline__ void gmm_gather4(void * dst, const CUtensorMap * map,
             : "memory");
 }
 
-// arrive on the barrier of the leading CTA
+// arrive on the barrier of the leading CTA: this CTA's reads of TMEM are done
+// (they are ordered by the tcgen05 fences; a release over the cluster would
+// also wait for the results' stores to reach L2)
 template <int CTAS>
 __device__ __forceinline__ void gmm_arrive(uint64_t * bar) {
     if constexpr (CTAS == 1)
@@ -261,7 +263,7 @@ __device__ __forceinline__ void gmm_arrive(uint64_t * bar) {
     else
         asm volatile(
             "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
-            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar))
+            "mbarrier.arrive.release.cta.shared::cluster.b64 _, [r];\n\t}" ::"r"(smem_u32(bar))
             : "memory");
 }
 
@@ -843,7 +845,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             for (int c0 = col0; c0 < q.cnt; c0 += kStep) {
                 const int o = o_next;
                 o_next = ordered && c0 + kStep + lane < q.cnt ? p.order[q.row0 + c0 + kStep + lane] : 0;
-                uint32_t v[32];
+                uint32_t v[32], u[MODE == GMM_DUAL ? 32 : 1];
                 if (w.shared) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
@@ -858,6 +860,17 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                     tmem_ld32_start(d + (uint32_t)c0, v);
                 } else {
                     sums(c0, v);
+                }
+                if constexpr (MODE == GMM_DUAL) {
+                    tmem_ld32_start(d + 256u + (uint32_t)c0, u);
+                    tmem_ld32_end(v);
+                    tmem_ld32_end(u);
+                }
+                // after its last columns are read a warp gives the accumulator back, and then finishes them
+                if (!w.shared && c0 + kStep >= q.cnt) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) gmm_arrive<CTAS>(acc_empty + it % kBufs);
                 }
                 bool nan = false;
                 int my = c0 + lane < q.cnt ? gmm_dst_row(p, q.row0 + c0 + lane, o, nan) : -1;
@@ -889,10 +902,6 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                     xb ^= 1;
                     put_rows_as<16>(p, stage, own, my, n0, vec);
                 } else if constexpr (MODE == GMM_DUAL) {
-                    uint32_t u[32];
-                    tmem_ld32_start(d + 256u + (uint32_t)c0, u);
-                    tmem_ld32_end(v);
-                    tmem_ld32_end(u);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float own[16], uv[16];
@@ -917,7 +926,8 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             if (w.shared) {
                 __syncwarp();
                 arrive_all(part_free + pb, split);
-            } else {
+            } else if (col0 >= q.cnt) {
+                // (a warp without columns in this tile)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) gmm_arrive<CTAS>(acc_empty + it % kBufs);

@@ -531,7 +531,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             // the partial h of this CTA's share of K: lanes are ranks, columns rows
             const uint32_t d1_now = d1 + (uint32_t)((it & 1) * kLoraRows);
             ok = gmm_wait<1>(d1_full + (it & 1), (uint32_t)((it / 2) & 1), &abort_flag);
-            if (ok && it > 0) ok = gmm_wait<2>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag);
+            // (a release or acquire over the cluster also waits for the results' stores: one CTA alone does without)
+            if (ok && it > 0) ok = C > 1 ? gmm_wait<2>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag)
+                                         : gmm_wait<1>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) break;
             tc_fence_after();
             if (quad * 32 < p.ra) {
@@ -549,8 +551,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             tc_fence_before();
             __syncwarp();
             if (lane == 0) gmm_arrive<1>(d1_empty + (it & 1));
-            arrive_all(&part_full, C);
-            ok = gmm_wait<2>(&part_full, (uint32_t)(it & 1), &abort_flag);
+            if (C > 1) {
+                arrive_all(&part_full, C);
+                ok = gmm_wait<2>(&part_full, (uint32_t)(it & 1), &abort_flag);
+            } else {
+                if (lane == 0) gmm_arrive<1>(&part_full);
+                ok = gmm_wait<1>(&part_full, (uint32_t)(it & 1), &abort_flag);
+            }
             if (ok && it > 0) ok = gmm_wait<1>(&h_empty, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) break;
             // sum over the cluster in CTA order, scale, split, store as an MMA operand
@@ -564,7 +571,9 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 8; ++e) h[e] = 0.0f;
                     for (int c = 0; c < C; ++c) {
-                        const float4 lo = ld_peer4(part + row * p.ra + r0, c), hi = ld_peer4(part + row * p.ra + r0 + 4, c);
+                        const float * from = part + row * p.ra + r0;
+                        const float4 lo = C > 1 ? ld_peer4(from, c) : *reinterpret_cast<const float4 *>(from);
+                        const float4 hi = C > 1 ? ld_peer4(from + 4, c) : *reinterpret_cast<const float4 *>(from + 4);
                         h[0] += lo.x; h[1] += lo.y; h[2] += lo.z; h[3] += lo.w;
                         h[4] += hi.x; h[5] += hi.y; h[6] += hi.z; h[7] += hi.w;
                     }
@@ -594,7 +603,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             fence_async_smem();
             __syncwarp();
             if (lane == 0) gmm_arrive<1>(&h_full);
-            arrive_all(&part_free, C);
+            if (C > 1) arrive_all(&part_free, C);
+            else if (lane == 0) gmm_arrive<1>(&part_free);
             ok = gmm_wait<1>(&h_full, (uint32_t)(it & 1), &abort_flag);       // (every row's power of two)
             auto results = [&](auto base) {
                 base.load(p, my, n_lo * 128 + quad * 32, vec);
