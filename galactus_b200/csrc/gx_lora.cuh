@@ -570,12 +570,27 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                     float h[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) h[e] = 0.0f;
-                    for (int c = 0; c < C; ++c) {
-                        const float * from = part + row * p.ra + r0;
-                        const float4 lo = C > 1 ? ld_peer4(from, c) : *reinterpret_cast<const float4 *>(from);
-                        const float4 hi = C > 1 ? ld_peer4(from + 4, c) : *reinterpret_cast<const float4 *>(from + 4);
-                        h[0] += lo.x; h[1] += lo.y; h[2] += lo.z; h[3] += lo.w;
-                        h[4] += hi.x; h[5] += hi.y; h[6] += hi.z; h[7] += hi.w;
+                    const float * from = part + row * p.ra + r0;
+                    if (C == 1) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = from[e];
+                    } else {
+                        // the loads of up to four CTAs together, the sums in CTA order
+                        for (int c0 = 0; c0 < C; c0 += 4) {
+                            float4 lo[4], hi[4];
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const int peer = min(c0 + c, C - 1);
+                                lo[c] = ld_peer4(from, peer);
+                                hi[c] = ld_peer4(from + 4, peer);
+                            }
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                if (c0 + c >= C) break;
+                                h[0] += lo[c].x; h[1] += lo[c].y; h[2] += lo[c].z; h[3] += lo[c].w;
+                                h[4] += hi[c].x; h[5] += hi[c].y; h[6] += hi[c].z; h[7] += hi[c].w;
+                            }
+                        }
                     }
                     float big = 0.0f;
 #pragma unroll
