@@ -299,7 +299,7 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
  * Products and sums are f32; the result is rounded once. order may be NULL
  * when neither gather nor scatter reads it. offsets ascend from >= 0 to <=
  * n_rows (the length of order; without gather b has at least n_rows rows).
- * Rows of dst outside every group are left as they were. A group whose borders
+ * dst may not overlap an input. Rows of dst outside every group are left as they were. A group whose borders
  * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped;
  * a row index outside b or dst is reported and its result is NaN or dropped.
  * With scatter the entries of order in a group must differ from one another and

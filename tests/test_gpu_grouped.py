@@ -256,6 +256,64 @@ def test_bad_borders_and_rows_are_reported(gxlib, dev):
     assert (out == 5.0).all(1).tolist() == [i in (3, 4) for i in range(10)] and device_error() == 1
 
 
+@pytest.mark.parametrize("K,N,kind,out", [(1, 1, "f16", "f32"), (3, 5, "bf16", "bf16"), (65, 130, "bf16", "f32"), (1001, 64, "f16", "f16")])
+@pytest.mark.parametrize("glu", [False, True])
+def test_lengths_that_are_no_multiple_of_anything(gxlib, dev, K, N, kind, out, glu):
+    """Rows padded to 16 bytes; what lies in the padding is not read as numbers."""
+    c = [3, 0, 20, 1]
+    pad = -K % 8
+    w, x = make(4, K, N, 24, kind, K, pad=pad)
+    up, _ = make(4, K, N, 0, kind, K + 1, pad=pad)
+    for t in (w, x, up):
+        if pad:
+            torch.as_strided(t, (*t.shape[:-1], pad), t.stride(), t.storage_offset() + K).fill_(float("nan"))
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(c)]), dtype=torch.int32, device="cuda")
+    order = torch.arange(23, -1, -1, dtype=torch.int32, device="cuda")
+    for gather in (0, 1):
+        kw = dict(order=order, gather=gather, out_dtype=TYPES[out])
+        got = gxlib.mul_mat_grouped_glu(w, up, x, offsets, **kw) if glu else gxlib.mul_mat_grouped(w, x, offsets, **kw)
+        want, tol = reference(w, x, c, 0, gather, order, False, 24, 0 if glu else None, up if glu else None)
+        compare(got, want, tol, out)
+
+
+def test_thousands_of_groups_and_no_rows(gxlib, dev):
+    E, K, N = 8192, 16, 24
+    rng = np.random.default_rng(0)
+    c = rng.integers(0, 3, size=E).tolist()
+    P = sum(c)
+    w, x = make(E, K, N, P, "bf16", 1)
+    offsets = torch.tensor(np.concatenate([[0], np.cumsum(c)]), dtype=torch.int32, device="cuda")
+    got = gxlib.mul_mat_grouped(w, x, offsets, out_dtype=torch.float32)
+    which = torch.repeat_interleave(torch.arange(E, device="cuda"), torch.tensor(c, device="cuda"))
+    want = torch.einsum("pnk,pk->pn", w[which].double(), x.double())
+    tol = torch.einsum("pnk,pk->pn", w[which].double().abs(), x.double().abs()) * acc_bound(K)
+    compare(got, want, tol, "f32")
+    zero = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    assert gxlib.mul_mat_grouped(w, x[:0], zero, order=none, scatter=True).shape == (0, N)
+    assert gxlib.mul_mat_grouped_glu(w, w, x[:0], zero, order=none, gather=2).shape == (0, N)
+    assert gxlib.lora_mul_mat(w, w.transpose(1, 2).contiguous(), x[:0], zero, base=torch.empty((0, K), device="cuda")).shape == (0, K)
+
+
+def test_results_beyond_four_gigabytes(gxlib, dev):
+    """Row 69999 of results that lie 65536 bytes apart, and deltas on such a base."""
+    K, N, rows = 64, 64, 70000
+    w, x = make(2, K, N, rows, "bf16", 2)
+    wide = torch.zeros((rows, 16384), device="cuda")
+    out = wide[:, -N:]
+    offsets = torch.tensor([0, 100, rows], dtype=torch.int32, device="cuda")
+    gxlib.mul_mat_grouped(w, x, offsets, out=out)
+    want, tol = reference(w, x, [100, rows - 100], 0, 0, None, False, rows)
+    compare(out, want, tol, "f32")
+    a, b = make(2, K, 16, 0, "bf16", 3)[0], make(2, 16, N, 0, "bf16", 4)[0]
+    before = out[-200:].clone()
+    small = gxlib.lora_mul_mat(a[1:], b[1:], x[-200:], torch.tensor([0, 200], dtype=torch.int32, device="cuda"), base=before)
+    gxlib.lora_mul_mat(a, b, x, offsets, base=out, out=out)
+    # the sums of K and of the ranks may be split differently: f32 accuracy, not the same bits
+    assert float((out[-200:] - small).abs().max()) <= 1e-5 * float(small.abs().max())
+    assert bool((wide[:, :16384 - N] == 0).all())
+
+
 def test_first_call_of_a_process_inside_a_capture(gxlib, dev):
     """Nothing has to be called before a capture: the first calls of a process may be captured ones."""
     import subprocess
