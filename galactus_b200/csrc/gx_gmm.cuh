@@ -28,8 +28,11 @@
 //   - Gated pairs keep 128 gate and 128 up rows per CTA against the same rows
 //     (both accumulators fill TMEM, nothing takes turns): a copied row is used
 //     twice, which gather4 (24 cycles per four rows) needs. 8192 tokens, 8
-//     experts each, K 4096, N 1536: 1152 us against 1236 with 64 + 64 rows and
-//     two accumulators in turn; 441 against 479 at K 1024.
+//     experts each, K 4096, N 1536: 1128 us against 1244 with 64 + 64 rows and
+//     two accumulators in turn, 384 against 461 at K 1024 (both since a little
+//     faster: 1100 us, 1499 TFLOP/s, and 367). Spreading short groups' tiles
+//     among the long ones' changed nothing (1514 us for 1506 in the case of
+//     128 experts): both then share the board's power.
 //   - The thread that issues copies or MMAs is chosen by elect.sync: with
 //     `lane == 0` a stage took 768 cycles, with it 590, of 512 for its MMAs.
 //   - Gathering by cp.async needs twelve warps (the fence that shows a stage
@@ -452,24 +455,33 @@ __device__ __forceinline__ float gmm_exp(float x) {
 
 // The activation on f32 sums. The quotient is CUDA's fast division (2 steps):
 // the sums are not those of the bit-exact formats anyway, and a full division
-// per value kept the epilogue behind the tensor cores.
-template <bool OAI>
+// per value kept the epilogue behind the tensor cores. FAST: CUDA's fast exp
+// as well, about |x| f32 steps off, for results of 16 bits, whose rounding is
+// hundreds of times that (8192 tokens, 8 experts each, K 1024: 367 us, with
+// gmm_exp 384).
+template <bool OAI, bool FAST>
 __device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) {
-    if (!OAI) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, gmm_exp(-g))), u);
+    if (!OAI) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, FAST ? __expf(-g) : gmm_exp(-g))), u);
     const float x = p.limit < g ? p.limit : g;
     const float y = u < -p.limit ? -p.limit : (p.limit < u ? p.limit : u);
-    return __fmul_rn(__fdividef(x, __fadd_rn(1.0f, gmm_exp(__fmul_rn(p.alpha, -x)))), __fadd_rn(y, 1.0f));
+    const float z = __fmul_rn(p.alpha, -x);
+    return __fmul_rn(__fdividef(x, __fadd_rn(1.0f, FAST ? __expf(z) : gmm_exp(z))), __fadd_rn(y, 1.0f));
 }
-// of N values at once: g becomes the result (the choice of the activation
-// stays outside the loop, so that the values' chains of operations overlap)
+// of N values at once: g becomes the result (the choices stay outside the
+// loop, so that the values' chains of operations overlap)
+template <bool OAI, bool FAST, int N>
+__device__ __forceinline__ void gmm_act_each(const GmmParams & p, float (&g)[N], const float (&u)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = gmm_act<OAI, FAST>(p, g[i], u[i]);
+}
 template <int N>
 __device__ __forceinline__ void gmm_act_all(const GmmParams & p, float (&g)[N], const float (&u)[N]) {
-    if (p.act == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = gmm_act<false>(p, g[i], u[i]);
+    if (p.out == GMM_F32) {
+        if (p.act == 0) gmm_act_each<false, false, N>(p, g, u);
+        else gmm_act_each<true, false, N>(p, g, u);
     } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = gmm_act<true>(p, g[i], u[i]);
+        if (p.act == 0) gmm_act_each<false, true, N>(p, g, u);
+        else gmm_act_each<true, true, N>(p, g, u);
     }
 }
 
