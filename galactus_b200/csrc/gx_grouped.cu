@@ -190,7 +190,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     // rounding, about 1e-9 of the sum per element of K. Results of 16 bits do
     // not see that; for f32 results an accumulator takes 512 elements and the
     // sums of the accumulators are rounded adds. A third of TMEM holds them.
-    p.seg = out == gx::GMM_F32 && nk > 12 ? 8 : 0;
+    p.seg = out == gx::GMM_F32 && nk > 8 ? 8 : 0;
     p.nt = 32;
     const int mode = !glu ? gx::GMM_PLAIN : ctas == 2 && p.seg == 0 ? gx::GMM_DUAL : gx::GMM_GLU;
     if (ctas == 2) p.nt = p.seg ? 160 : 256;
@@ -404,7 +404,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 127) / 128, (N + 127) / 128)); c *= 2) {
         const int64_t n = c == 1 ? clusters
                                  : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kMaxSmem - 2048u, 2) * per_sm;
-        if (n == 0) return GX_ERR_CUDA;
+        if (n == 0) break;
         const int64_t cost = (most + n - 1) / n * (16 / c + 1);
         if (c == 1 || cost < best) {
             best = cost;
