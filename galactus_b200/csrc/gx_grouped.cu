@@ -128,6 +128,11 @@ bool encode_rows(CUtensorMap * map, bool bf16, const void * base, int64_t K, int
 
 bool misaligned(const void * p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+// whether `rows` rows `pitch` bytes apart, `last` bytes of the last one, fit in `stride` bytes
+bool rows_fit(int64_t rows, int64_t pitch, int64_t last, int64_t stride) {
+    return (__int128)(rows - 1) * pitch + last <= stride;
+}
+
 int out_kind(int type) {
     return type == GX_TYPE_F32 ? gx::GMM_F32 : type == GX_TYPE_F16 ? gx::GMM_F16 : type == GX_TYPE_BF16 ? gx::GMM_BF16 : -1;
 }
@@ -161,7 +166,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (nb01 % 16 || nb02 % 16 || nb11 % 16 || misaligned(as, 16) || misaligned(b, 16) || (up && misaligned(up, 16)))
         return GX_ERR_ALIGN;
     if (nbd1 % esz || misaligned(dst, esz) || misaligned(offsets, 4) || (order && misaligned(order, 4))) return GX_ERR_ALIGN;
-    if (nb01 < 2 * ne00 || (n_as > 1 && nb02 < (ne01 - 1) * nb01 + 2 * ne00) || nb11 < 2 * ne00 || nbd1 < esz * ne01)
+    if (nb01 < 2 * ne00 || (n_as > 1 && !rows_fit(ne01, nb01, 2 * ne00, nb02)) || nb11 < 2 * ne00 || nbd1 < esz * ne01)
         return GX_ERR_INVALID;
     const bool glu = up != nullptr;
 
@@ -356,7 +361,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
         misaligned(order, 4) || misaligned(d->ranks, 4) || misaligned(d->scale, 4))
         return GX_ERR_ALIGN;
     if (d->nba1 < 2 * K || d->nbb1 < 2 * d->rank || nb11 < 2 * K || nbb < esz * N || nbd < esz * N) return GX_ERR_INVALID;
-    if (G > 1 && (nba2 < (d->rank - 1) * d->nba1 + 2 * K || nbb2 < (N - 1) * d->nbb1 + 2 * d->rank)) return GX_ERR_INVALID;
+    if (G > 1 && (!rows_fit(d->rank, d->nba1, 2 * K, nba2) || !rows_fit(N, d->nbb1, 2 * d->rank, nbb2))) return GX_ERR_INVALID;
 
     gx::LoraParams p{};
     p.offsets = offsets;

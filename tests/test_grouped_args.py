@@ -34,6 +34,7 @@ COMMON = [
     (dict(nb01=136), ALIGN), (dict(nb11=136), ALIGN), (dict(nb02=48 * 128 + 8), ALIGN), (dict(b=4104), ALIGN),
     (dict(offsets=4098), ALIGN), (dict(order=4097), ALIGN), (dict(dst=4097), ALIGN),
     (dict(n_rows=0, b=None, dst=None, order=None, offsets=None, ne11=0), OK),
+    (dict(ne01=1 << 30, nb01=1 << 39, nb02=1 << 39, nbd1=1 << 33), INVALID),      # a matrix of 2^69 bytes
 ]
 
 
@@ -79,7 +80,7 @@ def test_round_rows_refusals(gxlib, args, want):
     (dict(base=None), INVALID), (dict(dst=None), INVALID), (dict(ne11=0), INVALID), (dict(n_rows=-1), INVALID),
     (dict(gather=0), INVALID), (dict(nba1=112), INVALID), (dict(nba2=128), INVALID), (dict(nbb1=16), INVALID),
     (dict(nbb2=64), INVALID), (dict(nb11=112), INVALID), (dict(nbb=188), INVALID), (dict(nbd=188), INVALID),
-    (dict(nb11=1 << 40), INVALID), (dict(nbb=256, dst=65536), INVALID),       # in place with two strides
+    (dict(nb11=1 << 40), INVALID), (dict(nbb=256, dst=65536), INVALID), (dict(ne01=1 << 30, nbb1=1 << 39, nbb=1 << 33, nbd=1 << 33), INVALID),       # in place with two strides
     (dict(nba1=136), ALIGN), (dict(nbb1=40), ALIGN), (dict(nba2=16 * 128 + 8), ALIGN), (dict(nbb2=48 * 32 + 8), ALIGN),
     (dict(nb11=136), ALIGN), (dict(a=4104), ALIGN), (dict(b=4104), ALIGN), (dict(x=4104), ALIGN), (dict(base=4098), ALIGN),
     (dict(dst=4098), ALIGN), (dict(offsets=4098), ALIGN), (dict(order=4098), ALIGN), (dict(ranks=4098), ALIGN),
