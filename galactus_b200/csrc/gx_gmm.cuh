@@ -670,6 +670,9 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                         gmm_tma_2d<CTAS>(st + kABytes + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
                 }
             }
+            // (the issuer's commits arrive in both CTAs of a pair: the last ones too, before either leaves)
+            for (int i = max(0, c - p.stages); i < c && ok; ++i)
+                ok = gmm_wait_one<CTAS>(empty + i % p.stages, (uint32_t)((i / p.stages) & 1), &abort_flag);
             if (!ok && rank == 0) {
                 // copies in flight land before the CTA leaves
                 volatile int none = 0;
