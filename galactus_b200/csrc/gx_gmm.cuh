@@ -43,27 +43,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "gx_grouped_plan.h"
 #include "gx_tc.cuh"
 
 namespace gx {
-
-constexpr int kGmmRows = 128;                  // matrix rows of an MMA per CTA: TMEM lanes
-constexpr int kGmmK = 64;                      // elements of K per stage: one 128-byte swizzled row
-constexpr uint32_t kGmmATile = kGmmRows * 128u;
-constexpr int kGmmMaxStages = 12;
-constexpr int kGmmGatherWarps = 4;             // 32 rows each
-// what a kernel makes of its tiles
-enum : int {
-    GMM_PLAIN = 0,   // y = W x: 128 rows of W
-    GMM_GLU = 1,     // gated: 64 gate and 64 up rows, two accumulators in turn
-    GMM_DUAL = 2,    // gated, CTA pairs, 16-bit results: 128 gate and 128 up rows, one accumulator each
-};
-__host__ __device__ constexpr int gmm_epi_warps(int mode) { return mode == GMM_DUAL ? 8 : 4; }
-__host__ __device__ constexpr int gmm_threads(int mode) { return 32 * (2 + kGmmGatherWarps + gmm_epi_warps(mode)); }
-__host__ __device__ constexpr int gmm_out_rows(int mode) { return mode == GMM_GLU ? 64 : 128; }
-__host__ __device__ constexpr uint32_t gmm_a_bytes(int mode) { return mode == GMM_DUAL ? 2u * kGmmATile : kGmmATile; }
-constexpr uint32_t kGmmStaging = 4u * 32u * 32u * 4u;            // results of 32 (dual: 16) columns per epilogue warp
-constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer][warp pair][direction][column][lane] f32
 
 enum : int { GMM_F32 = 0, GMM_F16 = 1, GMM_BF16 = 2 };
 
@@ -483,11 +466,6 @@ __device__ __forceinline__ void gmm_act_all(const GmmParams & p, float (&g)[N], 
         if (p.act == 0) gmm_act_each<false, true, N>(p, g, u);
         else gmm_act_each<true, true, N>(p, g, u);
     }
-}
-
-// bytes of a ring stage: the matrix tile and the CTA's rows
-__host__ __device__ constexpr uint32_t gmm_stage_bytes(int ctas, int nt, int mode) {
-    return gmm_a_bytes(mode) + (uint32_t)(nt / ctas) * 128u;
 }
 
 // position in the ring of stages: stage, and how often the ring was gone round

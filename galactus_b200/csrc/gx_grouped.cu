@@ -55,6 +55,8 @@ int cuda_status(cudaError_t e) {
     return e == cudaErrorMemoryAllocation ? GX_ERR_NOMEM : GX_ERR_CUDA;
 }
 
+static_assert(gx::kGroupedSmem == gx::kMaxSmem - 1024u, "the kernels' own shared memory");
+
 constexpr int kMaxDevices = 64;
 
 // multiprocessors of the current device
@@ -218,18 +220,17 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (ctas == 1 && p.nt == 32) {
         const int64_t tiles = (int64_t)p.mt * touched;
         for (int c = 8; c > 1; c /= 2) {
-            const int64_t n = nk >= 4 * c ? resident_clusters(fn, c, gx::gmm_threads(mode), gx::kMaxSmem - 2048u, glu ? 1 : 0) : 0;
+            const int64_t n = nk >= 4 * c ? resident_clusters(fn, c, gx::gmm_threads(mode), gx::kGroupedSmem, glu ? 1 : 0) : 0;
             if (n == 0 || (c > 2 && tiles > n)) continue;
             p.split = c;
             clusters = n;
             break;
         }
     }
-    const uint32_t fixed = (uint32_t)(n_as + 1) * 4u + gx::kGmmStaging + (mode == gx::GMM_GLU ? gx::kGmmXchg : 0u) +
-                           (p.split > 1 ? 2u * (uint32_t)p.nt * gx::kGmmRows * 4u : 0u);
-    const uint32_t stage = gx::gmm_stage_bytes(ctas, p.nt, mode);
-    p.stages = (int32_t)std::min<uint32_t>(gx::kGmmMaxStages, (gx::kMaxSmem - 2048u - fixed) / stage);
-    const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
+    p.stages = gx::gmm_stages(ctas, p.nt, mode, p.G, p.split);
+    if (p.stages < 2) return GX_ERR_INVALID;
+    const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::gmm_stage_bytes(ctas, p.nt, mode) +
+                          gx::gmm_fixed_bytes(p.nt, mode, p.G, p.split);
     if (!encode_rows(&p.wmap, p.bf16, as, ne00, ne01, nb01, n_as, nb02, (uint32_t)gx::gmm_out_rows(mode)) ||
         (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, (uint32_t)gx::gmm_out_rows(mode))) ||
         !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)p.box))
@@ -393,12 +394,10 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
         return GX_ERR_ALIGN;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
-    // small ranks leave room for two CTAs per SM, whose phases overlap
-    const uint32_t fixed = gx::lora_fixed_bytes(p.ra, p.G), stage = gx::lora_stage_bytes(p.ra);
-    const int per_sm = fixed + 1024u + 2u * stage <= gx::kLoraHalfSm ? 2 : 1;
-    const uint32_t room = (per_sm == 2 ? gx::kLoraHalfSm : gx::kMaxSmem - 2048u) - 1024u - fixed;
-    p.stages = (int32_t)std::min<uint32_t>(gx::kLoraMaxStages, room / stage) & ~1;      // (even: two copying warps in turn)
-    const uint32_t smem = 1024u + (uint32_t)p.stages * stage + fixed;
+    const int per_sm = gx::lora_ctas_per_sm(p.ra, p.G);
+    p.stages = gx::lora_stages(p.ra, p.G);
+    if (p.stages < 2) return GX_ERR_INVALID;
+    const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::lora_stage_bytes(p.ra) + gx::lora_fixed_bytes(p.ra, p.G);
     const int64_t most = n_rows / gx::kLoraRows + std::min(n_rows, G);
     // A cluster per tile of rows, of the size whose rounds of tiles cost least:
     // a tile's work is shared by its CTAs, but for about a sixteenth that each
@@ -408,7 +407,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     int64_t clusters = (int64_t)sms * per_sm, best = 0;
     for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 127) / 128, (N + 127) / 128)); c *= 2) {
         const int64_t n = c == 1 ? clusters
-                                 : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kMaxSmem - 2048u, 2) * per_sm;
+                                 : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kGroupedSmem, 2) * per_sm;
         if (n == 0) break;
         const int64_t cost = (most + n - 1) / n * (16 / c + 1);
         if (c == 1 || cost < best) {

@@ -41,17 +41,6 @@
 
 namespace gx {
 
-constexpr int kLoraRows = 32;                   // rows of a tile (MMA N)
-constexpr int kLoraMaxRank = 128;
-constexpr int kLoraMaxStages = 12;
-constexpr int kLoraEpiWarps = 4;
-constexpr int kLoraThreads = 32 * (4 + kLoraEpiWarps);           // 8 warps: two CTAs of 128 registers a thread fit an SM
-constexpr uint32_t kLoraHalfSm = 112u * 1024u;  // dynamic shared memory that leaves room for a second CTA
-constexpr uint32_t kLoraTmem = 128;             // columns: two tiles of h, two of results (32 each)
-constexpr int kLoraK = 128;                     // elements of K per stage: two swizzled rows of 64
-constexpr uint32_t kLoraXTile = kLoraRows * 128u;
-constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
-
 struct LoraParams {
     CUtensorMap amap;         // A: [K, rank, G], boxes 64 x ra
     CUtensorMap bmap;         // B: [rank, N, G], boxes min(ra, 64) x 128
@@ -72,17 +61,6 @@ struct LoraParams {
     int32_t stages;
 };
 
-__host__ __device__ constexpr uint32_t lora_stage_bytes(int ra) { return 2u * (kLoraXTile + (uint32_t)ra * 128u); }
-// B and h lie in blocks of up to 64 ranks, their rows swizzled over 32, 64 or
-// 128 bytes: as many as the ranks fill
-__host__ __device__ constexpr uint32_t lora_blocks(int ra) { return ra > 64 ? 2u : 1u; }
-__host__ __device__ constexpr uint32_t lora_row(int ra) { return ra >= 64 ? 128u : (uint32_t)ra * 2u; }
-__host__ __device__ constexpr uint32_t lora_b_block(int ra) { return 128u * lora_row(ra); }
-__host__ __device__ constexpr uint32_t lora_h_block(int ra) { return (uint32_t)kLoraRows * lora_row(ra); }
-__host__ __device__ constexpr uint32_t lora_fixed_bytes(int ra, int groups) {
-    return lora_blocks(ra) * (2u * lora_b_block(ra) + 3u * lora_h_block(ra)) + (uint32_t)kLoraRows * ra * 4u + kLoraStaging +
-           kLoraRows * 4u + ((uint32_t)groups + 2u) * 4u;
-}
 // byte of 16-byte piece c of row r in such a block: the piece's number is
 // XOR-ed with the address bits from 7 up
 __device__ __forceinline__ uint32_t lora_swizzle(uint32_t row_bytes, int r, int c) {
