@@ -336,6 +336,16 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             c0 += k1 - k0;
             at.skip(k1 - k0, p.stages);
         }
+        // (the issuer's last commits arrive before the CTA leaves: those of the
+        // ring are waited for here, those of B and h by the roles that use them)
+        bool last = ok;
+        for (int i = max(0, c0 - p.stages); i < c0 && last; ++i)
+            if ((i & 1) == gw) last = gmm_wait<1>(empty + i % p.stages, (uint32_t)((i / p.stages) & 1), &abort_flag);
+        if (ok && !last) {
+            volatile int none = 0;
+            for (int i = max(0, c0 - p.stages); i < c0; ++i)
+                if ((i & 1) == gw) gmm_wait<1>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
+        }
     } else if (warp == 1) {
         // ----------------------------------------------------- MMA issuer
         if (elect_one()) {
@@ -417,6 +427,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 ++it;
             }
             if (ok && open) results(true);
+            if (ok && it > 0) ok = gmm_wait_one<1>(&h_empty, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) {
                 volatile int none = 0;
                 gmm_commit<1>(&drained);
@@ -466,6 +477,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             }
         }
         if (p.ranks != nullptr && ok && bc > 0) ok = fix(rank_was);
+        for (int i = max(0, bc - 2); i < bc && ok; ++i) ok = gmm_wait<1>(b_empty + (i & 1), (uint32_t)((i / 2) & 1), &abort_flag);
         if (!ok) {
             volatile int none = 0;
             for (int i = max(0, bc - 2); i < bc; ++i) gmm_wait<1>(b_full + (i & 1), (uint32_t)((i / 2) & 1), &none);

@@ -29,3 +29,19 @@ def test_adapters_at_the_largest_group_counts(gxlib, dev, n_as, adapters, rank, 
                              ranks=torch.from_numpy(ranks).cuda())
     compare(got, want, tol, "f32")
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("T,K,N,rank,adapters", [(1, 4096, 64, 16, 1), (40, 7168, 130, 64, 9), (300, 2048, 1, 16, 40), (5, 64, 1000, 128, 5)])
+def test_adapters_with_ctas_that_have_no_share(gxlib, dev, T, K, N, rank, adapters):
+    """Clusters of more CTAs than result tiles or chunks of K, call after call: each CTA leaves with its barriers at rest."""
+    from galactus_b200.moe import device_error
+    device_error()
+    s = make(T, 1, 1, adapters, rank, K, N, "f16", "f32", T)
+    adapter = np.random.default_rng(T).integers(-1 if T > 2 else 0, adapters, size=T).astype(np.int32)
+    order, offsets = gxlib.group_rows(None, adapter=torch.from_numpy(adapter).cuda(), n_adapters=adapters)
+    want, tol = reference(s, adapter.astype(np.int64), 1, 1, [rank] * adapters, [1.0] * adapters)
+    first = gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, order=order, base=s["base"])
+    compare(first, want, tol, "f32")
+    got = [gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, order=order, base=s["base"]) for _ in range(50)]
+    assert all(torch.equal(g, first) for g in got)
+    assert device_error() == 0
