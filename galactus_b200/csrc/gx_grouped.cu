@@ -71,17 +71,37 @@ int device_sms() {
     return n;
 }
 
+// the kernels that need more dynamic shared memory than a launch has by default
+enum KernelSlot : int { kSlotGroup, kSlotLora, kSlotGmm, kKernelSlots = kSlotGmm + 6 };
+int gmm_slot(int ctas, int mode) { return kSlotGmm + (ctas - 1) * 3 + mode; }
+
+// Lets `fn` have up to `bytes` on the current device: the most that any call
+// asks for, set once. (The limit belongs to the function, not to a call. One
+// set to each call's own size would let another thread's smaller call lower it
+// before the launch.)
+cudaError_t allow_smem(const void * fn, int slot, uint32_t bytes) {
+    static std::atomic<bool> done[kMaxDevices][kKernelSlots];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (done[dev][slot].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done[dev][slot].store(true, std::memory_order_release);
+    return e;
+}
+
 // Clusters of a kernel that run at once (SMs are grouped in GPCs of unequal
-// size, so clusters of 4 or 8 leave some out), one CTA per SM; `slot` names
-// the kernel in the table of what was asked before.
+// size, so clusters of 4 or 8 leave some out), one CTA per SM. The kernel has
+// been given its shared memory (allow_smem); `slot` names it in the table of
+// what was asked before.
 int resident_clusters(const void * fn, int cluster, int threads, uint32_t smem, int slot) {
-    static std::atomic<int> known[kMaxDevices][3][4];
+    static std::atomic<int> known[kMaxDevices][kKernelSlots][4];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
     std::atomic<int> & k = known[dev][slot][cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3];
     int n = k.load(std::memory_order_relaxed);
     if (n > 0) return n;
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)cluster);
     cfg.blockDim = dim3((unsigned)threads);
@@ -212,6 +232,9 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const void * fn = mode == gx::GMM_DUAL ? (const void *)gx::k_gmm<2, gx::GMM_DUAL>
                       : ctas == 2          ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU> : (const void *)gx::k_gmm<2, gx::GMM_PLAIN>)
                                            : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU> : (const void *)gx::k_gmm<1, gx::GMM_PLAIN>);
+    const int slot = gmm_slot(ctas, mode);
+    cudaError_t e = allow_smem(fn, slot, gx::kGroupedSmem);
+    if (e != cudaSuccess) return cuda_status(e);
     // The last round of tiles, when it leaves most SMs idle, is shared by the
     // CTAs of clusters that split K: pairs, or four or eight when not even one
     // round is full.
@@ -220,7 +243,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (ctas == 1 && p.nt == 32) {
         const int64_t tiles = (int64_t)p.mt * touched;
         for (int c = 8; c > 1; c /= 2) {
-            const int64_t n = nk >= 4 * c ? resident_clusters(fn, c, gx::gmm_threads(mode), gx::kGroupedSmem, glu ? 1 : 0) : 0;
+            const int64_t n = nk >= 4 * c ? resident_clusters(fn, c, gx::gmm_threads(mode), gx::kGroupedSmem, slot) : 0;
             if (n == 0 || (c > 2 && tiles > n)) continue;
             p.split = c;
             clusters = n;
@@ -237,8 +260,6 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
         return GX_ERR_ALIGN;
     const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
     if (most > kMaxIndex) return GX_ERR_INVALID;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
     const int cluster = ctas * p.split;
     cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(clusters, most)));
@@ -294,7 +315,7 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
     p.seg = (int)((steps + (int64_t)ncta * p.warps - 1) / ((int64_t)ncta * p.warps) * 32);
     const int threads = std::max(32 * p.warps, G > 1024 ? 1024 : 256);
     const uint32_t smem = (2u + (uint32_t)p.warps) * bins;
-    cudaError_t e = cudaFuncSetAttribute(gx::k_group_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem((const void *)gx::k_group_rows, kSlotGroup, gx::kGroupSmem);
     if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ncta);
@@ -399,6 +420,8 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (p.stages < 2) return GX_ERR_INVALID;
     const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::lora_stage_bytes(p.ra) + gx::lora_fixed_bytes(p.ra, p.G);
     const int64_t most = n_rows / gx::kLoraRows + std::min(n_rows, G);
+    cudaError_t e = allow_smem((const void *)gx::k_lora, kSlotLora, gx::kGroupedSmem);
+    if (e != cudaSuccess) return cuda_status(e);
     // A cluster per tile of rows, of the size whose rounds of tiles cost least:
     // a tile's work is shared by its CTAs, but for about a sixteenth that each
     // repeats. (Whether or not base is dst: the split of K sets the result's
@@ -407,7 +430,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     int64_t clusters = (int64_t)sms * per_sm, best = 0;
     for (int c = 1; c <= 8 && (c == 1 || c <= std::max((K + 127) / 128, (N + 127) / 128)); c *= 2) {
         const int64_t n = c == 1 ? clusters
-                                 : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kGroupedSmem, 2) * per_sm;
+                                 : resident_clusters((const void *)gx::k_lora, c, gx::kLoraThreads, gx::kGroupedSmem, kSlotLora) * per_sm;
         if (n == 0) break;
         const int64_t cost = (most + n - 1) / n * (16 / c + 1);
         if (c == 1 || cost < best) {
@@ -416,8 +439,6 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
             clusters = n;
         }
     }
-    cudaError_t e = cudaFuncSetAttribute(gx::k_lora, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(ctas * std::min<int64_t>(clusters, most + (p.copy ? n_rows / gx::kLoraRows + 1 : 0))));
     cfg.blockDim = dim3(gx::kLoraThreads);

@@ -45,3 +45,68 @@ def test_adapters_with_ctas_that_have_no_share(gxlib, dev, T, K, N, rank, adapte
     got = [gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, order=order, base=s["base"]) for _ in range(50)]
     assert all(torch.equal(g, first) for g in got)
     assert device_error() == 0
+
+
+def test_host_threads_with_calls_of_different_sizes(gxlib, dev):
+    """Every kernel's shared memory differs from call to call; threads that call at once do not get in each other's way."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def job(E, K, N, rank, T):
+        rnd = lambda *s: (torch.randn(s, generator=g, device="cuda") * 0.1).bfloat16()
+        w, up, x, a, b = rnd(E, N, K), rnd(E, N, K), rnd(T, K), rnd(E, rank, K), rnd(E, N, rank)
+        ids = torch.randint(0, E, (T, 1), generator=g, device="cuda", dtype=torch.int32)
+        base = torch.randn((T, N), generator=g, device="cuda")
+
+        def run():
+            order, offsets = gxlib.group_rows(ids, E)
+            return (order, offsets, gxlib.mul_mat_grouped(w, x, offsets, order=order, gather=1, out_dtype=torch.float32),
+                    gxlib.mul_mat_grouped_glu(w, up, x, offsets, order=order, gather=1),
+                    gxlib.lora_mul_mat(a, b, x, offsets, order=order, base=base))
+        return run
+    jobs = [job(*a) for a in ((2, 64, 32, 16, 5), (4096, 64, 32, 128, 40), (300, 512, 64, 64, 9), (1, 256, 130, 32, 700))]
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    failed, gate = [], threading.Barrier(len(jobs))
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                gate.wait()
+                for _ in range(150):
+                    got = jobs[i]()
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                failed.append((i, "other results"))
+        except Exception as e:                                       # noqa: BLE001
+            failed.append((i, repr(e)))
+            gate.abort()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+def test_a_graph_keeps_its_large_call_after_a_small_one(gxlib, dev):
+    """A captured call of many groups and one of few share their kernel; replays and calls in between keep their sizes."""
+    def inputs(E, T):
+        ids = torch.randint(0, E, (T, 1), device="cuda", dtype=torch.int32)
+        return ids, (torch.randn((E, 40, 64), device="cuda") * 0.1).half(), torch.randn((T, 64), device="cuda").half(), E
+
+    def run(ids, w, x, E):
+        order, offsets = gxlib.group_rows(ids, E)
+        return gxlib.mul_mat_grouped(w, x, offsets, order=order, gather=1, out_dtype=torch.float32)
+    large, small = inputs(8192, 100), inputs(3, 7)
+    want = run(*large), run(*small)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*large), run(*small)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        run(*small)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
