@@ -4,8 +4,9 @@ many requests, rows rounded for them.
 
 Every tensor lives on the current CUDA device. The calls run on `stream` (a
 cudaStream_t handle or a torch stream), torch's current stream by default, wait
-for nothing and can be captured into a graph; results they allocate belong to
-torch's current stream.
+for nothing and can be captured into a graph. Results they allocate belong to
+the stream they run on, as if allocated with it current; what is given (inputs,
+`out`, ...) is ordered with it by the caller.
 """
 from __future__ import annotations
 
@@ -25,6 +26,19 @@ def _stream(stream, dev: int) -> int:
     if stream is None:
         return _raw_stream(dev)
     return stream if isinstance(stream, int) else int(stream.cuda_stream)
+
+
+def _new(stream, dev: int, make):
+    """What make() allocates, in memory of the stream that the call runs on: a
+    block of another stream's could still be read there."""
+    if stream is not None:
+        handle = stream if isinstance(stream, int) else int(stream.cuda_stream)
+        if handle != _raw_stream(dev):
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(handle, dev) if handle else torch.cuda.default_stream(dev)
+            with torch.cuda.stream(stream):
+                return make()
+    return make()
 
 
 def _device(*tensors) -> int:
@@ -95,12 +109,12 @@ def group_rows(ids, n_as: int = 1, *, adapter=None, n_adapters: int = 0, order=N
     G = n_as * max(1, n_adapters)
     dev = _device(ids, adapter, order, offsets)
     if order is None:
-        order = like.new_empty(T * k)
+        order = _new(stream, dev, lambda: like.new_empty(T * k))
         order_ptr = order.data_ptr()
     else:
         order_ptr = _index(order, "order", T * k)
     if offsets is None:
-        offsets = like.new_empty(G + 1)
+        offsets = _new(stream, dev, lambda: like.new_empty(G + 1))
         offsets_ptr = offsets.data_ptr()
     else:
         offsets_ptr = _index(offsets, "offsets", G + 1)
@@ -115,18 +129,18 @@ def round_rows(x, dtype, out=None, stream=None):
     n, m, nb1 = _rows(x, "x")
     if x.dtype != torch.float32 or dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("round_rows: float32 rows to float16 or bfloat16")
+    dev = _device(x, out)
     if out is None:
-        out = torch.empty((n, m), dtype=dtype, device=x.device)
+        out = _new(stream, dev, lambda: torch.empty((n, m), dtype=dtype, device=x.device))
     elif out.shape != x.shape or out.dtype != dtype:
         raise ValueError("out: the rows' shape and the given type expected")
-    dev = _device(x, out)
     if n and m:
         L.check(_LIB.gx_quantize_rows(_TYPE[dtype], x.data_ptr(), m, n, nb1, out.data_ptr(), _rows(out, "out")[2],
                                       _stream(stream, dev)), "gx_quantize_rows")
     return out
 
 
-def _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype):
+def _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype, stream, dev):
     """Common checks and defaults: (result, its type and row stride, the arguments the two products share)."""
     G, N, K, nb01, nb02 = _matrices(w, "weights")
     rows, m, nb11 = _rows(x, "x")
@@ -139,7 +153,7 @@ def _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype):
     elif order is not None and n_rows > order.shape[0]:
         raise ValueError("n_rows: more than order holds")
     if out is None:
-        out = torch.empty((n_rows, N), dtype=out_dtype or kind, device=w.device)
+        out = _new(stream, dev, lambda: torch.empty((n_rows, N), dtype=out_dtype or kind, device=w.device))
         nbd1 = N * out.element_size()
     else:
         have, cols, nbd1 = _rows(out, "out")
@@ -159,7 +173,7 @@ def mul_mat_grouped(w, x, offsets, *, order=None, n_rows: int | None = None, gat
     order[j] with scatter. Rows of no group are left as they were
     (uninitialised in a result allocated here)."""
     dev = _device(w, x, offsets, order, out)
-    out, kind, nbd1, args = _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
+    out, kind, nbd1, args = _product(w, x, offsets, order, n_rows, gather, scatter, out, out_dtype, stream, dev)
     rc = _LIB.gx_mul_mat_grouped(_TYPE.get(w.dtype, -1), w.data_ptr(), *args, kind, out.data_ptr(), nbd1, _stream(stream, dev))
     if rc:
         L.check(rc, "gx_mul_mat_grouped")
@@ -175,7 +189,7 @@ def mul_mat_grouped_glu(gate, up, x, offsets, *, order=None, n_rows: int | None 
     if up.shape != gate.shape or up.dtype != gate.dtype or up.stride() != gate.stride():
         raise ValueError("gate and up: one shape, type and layout expected")
     dev = _device(gate, up, x, offsets, order, out)
-    out, kind, nbd1, args = _product(gate, x, offsets, order, n_rows, gather, scatter, out, out_dtype)
+    out, kind, nbd1, args = _product(gate, x, offsets, order, n_rows, gather, scatter, out, out_dtype, stream, dev)
     rc = _LIB.gx_mul_mat_grouped_glu(_TYPE.get(gate.dtype, -1), gate.data_ptr(), up.data_ptr(), *args, act, alpha, limit, kind,
                                      out.data_ptr(), nbd1, _stream(stream, dev))
     if rc:
@@ -205,15 +219,15 @@ def lora_mul_mat(a, b, x, offsets, *, order=None, gather: int = 1, n_as: int | N
     adapters = G // n_as
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous()):
         raise ValueError(f"scale: contiguous float32 vector of {adapters} expected")
+    dev = _device(a, b, x, offsets, order, ranks, scale, base, out)
     if out is None:
-        out = torch.empty_like(base)
+        out = _new(stream, dev, lambda: torch.empty_like(base))
     elif out.shape != base.shape or out.dtype is not base.dtype:
         raise ValueError("out: base's shape and type expected")
     nbd = _rows(out, "out")[2]
     kind = _TYPE.get(base.dtype)
     if cols != N or kind is None:
         raise ValueError(f"base: rows of {N} elements of a result type expected")
-    dev = _device(a, b, x, offsets, order, ranks, scale, base, out)
     desc = L.gx_lora_desc(_TYPE.get(a.dtype, -1), rank, K, N, n_as, adapters, a.data_ptr(), nba1, nba2, b.data_ptr(), nbb1, nbb2,
                           _index(ranks, "ranks", adapters), 0 if scale is None else scale.data_ptr())
     rc = _LIB.gx_lora_mul_mat(C.byref(desc), x.data_ptr(), rows, nb11, _index(offsets, "offsets", G + 1),

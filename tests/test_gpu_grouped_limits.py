@@ -110,3 +110,41 @@ def test_a_graph_keeps_its_large_call_after_a_small_one(gxlib, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_results_allocated_for_another_stream(gxlib, dev, handle):
+    """A result allocated by a call on `stream` takes no memory that work queued on the current stream still reads."""
+    E, K, N, T = 5, 256, 512, 3000
+    w, up, a, b = ((torch.randn(s, device="cuda") * 0.1).bfloat16() for s in ((E, N, K), (E, N, K), (E, 16, K), (E, N, 16)))
+    x32, base = torch.randn((T, K), device="cuda"), torch.randn((T, N), device="cuda")
+    x = x32.bfloat16()
+    ids = torch.randint(0, E, (200000, 1), device="cuda", dtype=torch.int32)
+    order, offsets = gxlib.group_rows(ids[:T], E)
+    side = torch.cuda.Stream()
+    calls = [
+        lambda s: gxlib.group_rows(ids, E, stream=s)[0],
+        lambda s: gxlib.round_rows(x32, torch.bfloat16, stream=s),
+        lambda s: gxlib.mul_mat_grouped(w, x, offsets, order=order, gather=1, out_dtype=torch.float32, stream=s),
+        lambda s: gxlib.mul_mat_grouped_glu(w, up, x, offsets, order=order, gather=1, stream=s),
+        lambda s: gxlib.lora_mul_mat(a, b, x, offsets, order=order, base=base, stream=s),
+    ]
+    for call in calls:
+        want = call(None)
+        sink = torch.empty_like(want)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        read = torch.full_like(want, 3)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)                              # about 50 ms: `read` is given back with its reader still queued
+        sink.copy_(read)
+        del read
+        got = call(side.cuda_stream if handle else side)
+        side.synchronize()
+        assert torch.equal(got, want)
+        torch.cuda.synchronize()
+        assert bool((sink == 3).all())
+    with torch.cuda.stream(side):                                    # and the default stream while another is current
+        got = calls[2](0 if handle else torch.cuda.default_stream())
+        torch.cuda.synchronize()
+        assert torch.equal(got, calls[2](None))
