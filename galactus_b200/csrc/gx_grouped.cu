@@ -407,6 +407,8 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     p.bf16 = d->type == GX_TYPE_BF16;
     p.out = out;
     p.copy = base != dst;
+    // (what f32 results need; 16-bit ones do not see the truncation of a long sum)
+    p.seg = out == gx::GMM_F32 ? gx::kLoraSeg : 0;
     if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
     if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
         !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u, (uint32_t)std::min(p.ra, 64)) ||

@@ -53,8 +53,11 @@ constexpr int kLoraMaxStages = 12;
 constexpr int kLoraEpiWarps = 4;
 constexpr int kLoraThreads = 32 * (4 + kLoraEpiWarps);           // 8 warps: two CTAs of 128 registers a thread fit an SM
 constexpr uint32_t kLoraHalfSm = 112u * 1024u;  // dynamic shared memory that leaves room for a second CTA
-constexpr uint32_t kLoraTmem = 128;             // columns: two tiles of h, two of results (32 each)
+constexpr int kLoraSums = 6;                    // accumulators of h that take turns
+constexpr uint32_t kLoraTmem = 256;             // columns: the sums of h, two tiles of results (32 each)
 constexpr int kLoraK = 128;                     // elements of K per stage: two swizzled rows of 64
+constexpr int kLoraSeg = 4;                     // stages that one accumulator of h sums when results are f32
+static_assert((kLoraSums + 2) * kLoraRows <= kLoraTmem, "columns of TMEM");
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;
 

@@ -18,7 +18,12 @@
 // bits below the row's largest value, the row scaled by a power of two first
 // so that no h overflows F16), all multiplied with the same B tile in shared
 // memory: the deltas keep f32 accuracy for two extra MMAs per 16 ranks, which
-// the memory-bound kernel has time for.
+// the memory-bound kernel has time for. The tensor cores' accumulators truncate
+// (for sums of one sign 4.8e-5 of the sum at K = 7168, 1.6e-4 at 28672), so
+// for f32 results each takes 512 elements of K and the sums of the accumulators
+// are rounded adds (3.1e-6 and 1.4e-6 then; 8192 routed rows take 43.5 us with
+// it, 41.6 without). Six accumulators let a tile of K = 2048 be multiplied
+// while the one before it is finished (1.3 us more with two).
 //
 // Ranks differ by adapter: rows of A and columns of B behind an adapter's
 // rank may hold anything and do not reach the result.
@@ -59,6 +64,7 @@ struct LoraParams {
     int32_t bf16, out;
     int32_t copy;             // base is not dst: rows without an adapter are copied
     int32_t stages;
+    int32_t seg;              // chunks that one accumulator of h sums (0: all)
 };
 
 // byte of 16-byte piece c of row r in such a block: the piece's number is
@@ -215,7 +221,7 @@ __device__ __forceinline__ void split_h(const float (&h)[8], bool bf16, uint4 (&
 __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant__ LoraParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kLoraMaxStages], empty[kLoraMaxStages], b_full[2], b_empty[2], b_fixed[2], d2_full[2], d2_empty[2];
-    __shared__ uint64_t d1_full[2], d1_empty[2], part_full, part_free, h_full, h_empty, drained;
+    __shared__ uint64_t d1_full[kLoraSums], d1_empty[kLoraSums], part_full, part_free, h_full, h_empty, drained;
     __shared__ int4 gather_mem[2 * kLoraRows / 4];
     __shared__ uint32_t tslot;
     __shared__ int32_t wsum[kLoraThreads / 32];
@@ -247,10 +253,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             mbar_init(b_full + i, 1);
             mbar_init(b_empty + i, 1);
             mbar_init(b_fixed + i, 1);
-            mbar_init(d1_full + i, 1);
-            mbar_init(d1_empty + i, kLoraEpiWarps);
             mbar_init(d2_full + i, 1);
             mbar_init(d2_empty + i, kLoraEpiWarps);
+        }
+        for (int i = 0; i < kLoraSums; ++i) {
+            mbar_init(d1_full + i, 1);
+            mbar_init(d1_empty + i, kLoraEpiWarps);
         }
         mbar_init(&part_full, (uint32_t)(kLoraEpiWarps * C));
         mbar_init(&part_free, (uint32_t)(kLoraEpiWarps * C));
@@ -266,11 +274,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
     if (C > 1) cluster_sync_all(); else __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tslot;
-    const uint32_t d1 = tbase, d2 = tbase + 2u * (uint32_t)kLoraRows;
+    const uint32_t d1 = tbase, d2 = tbase + (uint32_t)(kLoraSums * kLoraRows);
     const int tiles = pre[p.G + 1];
     const int nk = (p.K + kLoraK - 1) / kLoraK;
     const int k0 = nk * me / C, k1 = nk * (me + 1) / C;                        // this CTA's chunks of K
     const int nn = (p.N + 127) / 128, n_lo = nn * me / C, n_hi = nn * (me + 1) / C;        // this CTA's result tiles
+    const int nseg = p.seg && k1 > k0 ? (k1 - k0 + p.seg - 1) / p.seg : 1;                 // sums of h per tile
 
     if (warp == 0 || warp == 2) {
         // ------ A by TMA tiles and the rows of x by tile::gather4: two warps,
@@ -390,34 +399,43 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 gmm_commit<1>(&h_empty);
                 open = false;
             };
+            // a wait during which results are issued as they become ready
+            auto wait_issuing = [&](uint64_t * bar, uint32_t parity) {
+                uint32_t polls = 0;
+                while (open) {
+                    results(false);
+                    if (mbar_test_wait(bar, parity) || ++polls == (1u << 20)) break;
+                }
+                if (polls == (1u << 20) && open) results(true);
+                ok = ok && gmm_wait_one<1>(bar, parity, &abort_flag);
+                return ok;
+            };
+            RingPos sum;                               // the accumulator of h in turn
             for (int t = unit; t < tiles && ok; t += units) {
                 const LoraTile q = lora_tile(p, pre, t);
                 if (q.rank == 0) continue;
                 // (16 ranks sit in the first lanes of a 64-row MMA too, at half the shared memory reads)
                 const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, p.ra == 16 ? 64 : 128, (uint32_t)((q.cnt + 15) & ~15));
-                const int b = it & 1;
-                if (it >= 2) ok = gmm_wait_one<1>(d1_empty + b, (uint32_t)((it / 2 - 1) & 1), &abort_flag);
-                for (int kc = k0; kc < k1 && ok; ++kc, at.next(p.stages)) {
-                    uint32_t polls = 0;
-                    while (open) {
-                        results(false);
-                        if (mbar_test_wait(full + at.s, at.round & 1u) || ++polls == (1u << 20)) break;
+                int kc = k0;
+                for (int sg = 0; sg < nseg && ok; ++sg, sum.next(kLoraSums)) {
+                    const int first = kc, end = p.seg ? min(kc + p.seg, k1) : k1;
+                    if (sum.round != 0) wait_issuing(d1_empty + sum.s, (sum.round - 1u) & 1u);
+                    for (; kc < end && ok; ++kc, at.next(p.stages)) {
+                        if (!wait_issuing(full + at.s, at.round & 1u)) break;
+                        tc_fence_after();
+                        const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int i = 0; i < kGmmK / 16; ++i)
+                                mma_f16<1>(d1 + (uint32_t)(sum.s * kLoraRows), a0 + off + (uint64_t)(half * p.ra * 8 + 2 * i),
+                                           x0 + off + (uint64_t)(half * (int)(kLoraXTile >> 4) + 2 * i), idesc,
+                                           (uint32_t)((kc - first) | half | i));
+                        gmm_commit<1>(empty + at.s);
                     }
-                    ok = gmm_wait_one<1>(full + at.s, at.round & 1u, &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t off = (uint64_t)(((uint32_t)at.s * stage_bytes) >> 4);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-#pragma unroll
-                        for (int i = 0; i < kGmmK / 16; ++i)
-                            mma_f16<1>(d1 + (uint32_t)(b * kLoraRows), a0 + off + (uint64_t)(half * p.ra * 8 + 2 * i),
-                                       x0 + off + (uint64_t)(half * (int)(kLoraXTile >> 4) + 2 * i), idesc,
-                                       (uint32_t)((kc - k0) | half | i));
-                    gmm_commit<1>(empty + at.s);
+                    if (ok) gmm_commit<1>(d1_full + sum.s);
                 }
                 if (!ok) break;
-                gmm_commit<1>(d1_full + b);
                 if (open) results(true);
                 if (!ok) break;
                 last = q;
@@ -491,6 +509,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                            (uintptr_t)p.nbb) & 15u) == 0;
         const bool row_pieces = (p.N * esz) % 16 == 0;         // whole 16-byte pieces
         int it = 0, bc = 0;
+        RingPos sum;
         bool ok = true;
         for (int t = unit; t < tiles && ok; t += units) {
             const LoraTile q = lora_tile(p, pre, t);
@@ -519,28 +538,39 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                              : "memory");
             }
             // the partial h of this CTA's share of K: lanes are ranks, columns rows
-            const uint32_t d1_now = d1 + (uint32_t)((it & 1) * kLoraRows);
-            ok = gmm_wait<1>(d1_full + (it & 1), (uint32_t)((it / 2) & 1), &abort_flag);
+            // (for f32 results in sums of 512 elements, added here with rounding)
+            float own[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) own[i] = 0.0f;
+            for (int sg = 0; sg < nseg && ok; ++sg, sum.next(kLoraSums)) {
+                ok = gmm_wait<1>(d1_full + sum.s, sum.round & 1u, &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                if (quad * 32 < p.ra && k0 < k1) {
+#pragma unroll
+                    for (int c0 = 0; c0 < kLoraRows; c0 += 16) {
+                        if (c0 >= q.cnt) break;
+                        uint32_t v[16];
+                        tmem_ld16(d1 + (uint32_t)(sum.s * kLoraRows + c0) + ((uint32_t)quad << 21), v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) own[c0 + i] = __fadd_rn(own[c0 + i], __uint_as_float(v[i]));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) gmm_arrive<1>(d1_empty + sum.s);
+            }
             // (a release or acquire over the cluster also waits for the results' stores: one CTA alone does without)
             if (ok && it > 0) ok = C > 1 ? gmm_wait<2>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag)
                                          : gmm_wait<1>(&part_free, (uint32_t)((it - 1) & 1), &abort_flag);
             if (!ok) break;
-            tc_fence_after();
-            if (quad * 32 < p.ra) {
-                const int r = quad * 32 + lane;
-                for (int c0 = 0; c0 < q.cnt; c0 += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(d1_now + (uint32_t)c0 + ((uint32_t)quad << 21), v);
-                    tmem_wait_ld();
-                    if (r < p.ra) {
+            if (const int r = quad * 32 + lane; r < p.ra) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) part[(c0 + i) * p.ra + r] = k0 < k1 ? __uint_as_float(v[i]) : 0.0f;
-                    }
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (i < ((q.cnt + 15) & ~15)) part[i * p.ra + r] = own[i];
             }
-            tc_fence_before();
             __syncwarp();
-            if (lane == 0) gmm_arrive<1>(d1_empty + (it & 1));
             if (C > 1) {
                 arrive_all(&part_full, C);
                 ok = gmm_wait<2>(&part_full, (uint32_t)(it & 1), &abort_flag);

@@ -148,3 +148,51 @@ def test_results_allocated_for_another_stream(gxlib, dev, handle):
         got = calls[2](0 if handle else torch.cuda.default_stream())
         torch.cuda.synchronize()
         assert torch.equal(got, calls[2](None))
+
+
+def long_bound(K: int) -> float:
+    """Of an f32 sum of K products of one sign, relative to it, when an accumulator takes 512 of them: a step of an
+    accumulator adds 16 products to a sum that is at most the whole (one step of it, 2^-23, and the alignment of the 16,
+    as much each); then one rounded add per accumulator and per CTA that shares K (at most eight), 2^-24 each."""
+    return (512 / 16 + 16) * 2.0 ** -23 + (K / 512 + 1 + 8) * 2.0 ** -24
+
+
+def positive(shape, sigma, seed, kind="bf16"):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda").abs_() * sigma).to({"bf16": torch.bfloat16, "f16": torch.float16}[kind])
+
+
+@pytest.mark.parametrize("T,K,kind", [(6400, 28672, "bf16"), (6400, 7168, "f16"), (3, 28672, "bf16"), (700, 14336, "f16"), (5000, 3080, "bf16")])
+def test_long_sums_of_adapters(gxlib, dev, T, K, kind):
+    """Products of one sign, where a truncating sum shows as a bias: f32 results keep f32 accuracy however long K is,
+    with one CTA per tile of rows (6400 rows) and with clusters."""
+    N, rank = 64, 16
+    x, a, b = positive((T, K), 1.0, 1, kind), positive((1, rank, K), 1.0 / K, 2, kind), positive((1, N, rank), 0.1, 3, kind)
+    offsets = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    got = gxlib.lora_mul_mat(a, b, x, offsets, base=torch.zeros((T, N), device="cuda")).double()
+    want = torch.cat([(c.double() @ a[0].double().T) @ b[0].double().T for c in x.split(1024)])
+    # h, its parts (2^-22), 48 products of the second sum, the last add
+    bound = long_bound(K) + 2.0 ** -22 + (48 / 16 + 16) * 2.0 ** -23 + 2.0 ** -24
+    off = float(((got - want).abs() / want).max())
+    assert off <= bound, f"{off:.3g} of {bound:.3g}"
+
+
+@pytest.mark.parametrize("rows,N", [(300, 200), (3, 200), (40, 130), (3, 4096)])
+@pytest.mark.parametrize("glu", [False, True])
+def test_long_sums_of_products(gxlib, dev, rows, N, glu):
+    """The same of the products: CTA pairs, single CTAs, and clusters that share K."""
+    K = 28672
+    x, w, up = positive((rows, K), 1.0, 4), positive((2, N, K), 1.0 / K, 5), positive((2, N, K), 2.0 / K, 6)
+    offsets = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device="cuda")
+    g = torch.cat([x[:rows // 3].double() @ w[0].double().T, x[rows // 3:].double() @ w[1].double().T])
+    if glu:
+        got = gxlib.mul_mat_grouped_glu(w, up, x, offsets, out_dtype=torch.float32)
+        u = torch.cat([x[:rows // 3].double() @ up[0].double().T, x[rows // 3:].double() @ up[1].double().T])
+        want = g * torch.sigmoid(g) * u
+        # both sums (d silu(g) / dg * g <= 2 silu(g) for g > 0), eight roundings of the activation
+        bound = 3 * long_bound(K) + 8 * 2.0 ** -23
+    else:
+        got = gxlib.mul_mat_grouped(w, x, offsets, out_dtype=torch.float32)
+        want, bound = g, long_bound(K)
+    off = float(((got.double() - want).abs() / want).max())
+    assert off <= bound, f"{off:.3g} of {bound:.3g}"
