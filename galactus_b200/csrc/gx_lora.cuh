@@ -616,13 +616,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         h[e] = r0 + e < q.rank && row < q.cnt ? __fmul_rn(h[e], scale) : 0.0f;
-                        big = fmaxf(big, fabsf(h[e]));
+                        const float size = fabsf(h[e]);
+                        if (size < __int_as_float(0x7f800000)) big = fmaxf(big, size);
                     }
                     if (!p.bf16) {
-                        // the row's largest |h| to [2^13, 2^14)
+                        // the row's largest finite |h| to [2^13, 2^14) (beside
+                        // an infinity too: a finite h must not become another)
                         for (int m = 1; m < per; m <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
-                        const int e2 = big > 0.0f && big < __int_as_float(0x7f800000)
-                                           ? min(max((int)(__float_as_uint(big) >> 23) - 127 - 13, -100), 114) : 0;
+                        const int e2 = big > 0.0f ? min(max((int)(__float_as_uint(big) >> 23) - 127 - 13, -126), 114) : 0;
                         const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) h[e] = __fmul_rn(h[e], down);

@@ -196,3 +196,34 @@ def test_long_sums_of_products(gxlib, dev, rows, N, glu):
         want, bound = g, long_bound(K)
     off = float(((got.double() - want).abs() / want).max())
     assert off <= bound, f"{off:.3g} of {bound:.3g}"
+
+
+def test_an_infinite_h_beside_large_ones_in_f16(gxlib, dev):
+    """One rank's h is infinite, another's finite but beyond F16: the results are infinite with the first one's sign, not NaN."""
+    T, K, N, rank = 20, 64, 200, 16
+    x = positive((T, K), 1000.0, 1, "f16") + 1
+    a = torch.zeros((1, rank, K), dtype=torch.float16, device="cuda")
+    a[0, 0, 5], a[0, 1] = float("inf"), 1000.0
+    a[0, 0, 6:] = 1.0
+    a[0, 0, :5] = 1.0
+    b = torch.zeros((1, N, rank), dtype=torch.float16, device="cuda") + 0.5
+    b[0, ::2, 0] = -0.5
+    b[0, :, 1] = -b[0, :, 0]
+    offsets = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    # (the remaining ranks' h are zero: 0 * inf does not arise)
+    got = gxlib.lora_mul_mat(a, b, x, offsets, base=torch.zeros((T, N), device="cuda"))
+    want = torch.where(b[0, :, 0] > 0, float("inf"), float("-inf")).expand(T, N)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("size", [1e-34, 1e-30, 1e-20, 1e30])
+def test_h_of_any_size_in_f16(gxlib, dev, size):
+    """F16 adapters at the ends of f32: the row's power of two keeps at least 22 bits of h."""
+    s = make(40, 1, 1, 1, 16, 128, 96, "f16", "f32", 12)
+    s["base"].zero_()
+    offsets = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+    scale = torch.tensor([size], device="cuda")
+    want, tol = reference(s, np.zeros(40, np.int64), 1, 1, [16], [float(scale[0])])
+    got = gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, base=s["base"], scale=scale)
+    # (below 2^-126 of the result, f32 itself ends)
+    assert bool(((got.double() - want).abs() <= tol + 2.0 ** -23 * want.abs() + 2.0 ** -149).all())
