@@ -416,12 +416,12 @@ __device__ __forceinline__ void store_out(uint8_t * row, int n, float v, int out
     else reinterpret_cast<__half *>(row)[n] = __float2half_rn(v);
 }
 
-// e^x without branches: x is clamped to where the result leaves the normal
-// range (n = 128 makes the scale infinite), n = x log2 e to nearest, r = x -
-// n ln 2 with ln 2 in two parts (Cody and Waite, 1980), e^r by its Taylor
-// polynomial; within 2 f32 steps on the normal range
-__device__ __forceinline__ float gmm_exp(float x) {
-    x = fminf(fmaxf(x, -87.0f), 89.0f);
+// e^x / 4 without branches: x is clamped to where the quarter leaves the normal
+// range (n = 130 makes the scale infinite) or is nothing beside 1, n = x log2 e
+// to nearest, r = x - n ln 2 with ln 2 in two parts (Cody and Waite, 1980), e^r
+// by its Taylor polynomial; within 2 f32 steps in between
+__device__ __forceinline__ float gmm_quarter_exp(float x) {
+    x = fminf(fmaxf(x, -85.0f), 90.25f);
     const float t = __fmaf_rn(x, 1.44269502162933349609375f, 12582912.0f);
     const float n = __fsub_rn(t, 12582912.0f);
     float r = __fmaf_rn(-n, 0.693145751953125f, x);
@@ -433,22 +433,27 @@ __device__ __forceinline__ float gmm_exp(float x) {
     q = __fmaf_rn(q, r, 0.5f);
     q = __fmaf_rn(q, r, 1.0f);
     q = __fmaf_rn(q, r, 1.0f);
-    return __fmul_rn(q, __uint_as_float((__float_as_uint(t) + 127u) << 23));
+    return __fmul_rn(q, __uint_as_float((__float_as_uint(t) + 125u) << 23));
 }
 
 // The activation on f32 sums. The quotient is CUDA's fast division (2 steps):
 // the sums are not those of the bit-exact formats anyway, and a full division
-// per value kept the epilogue behind the tensor cores. FAST: CUDA's fast exp
-// as well, about |x| f32 steps off, for results of 16 bits, whose rounding is
-// hundreds of times that (8192 tokens, 8 experts each, K 1024: 367 us, with
-// gmm_exp 384).
+// per value kept the epilogue behind the tensor cores. It gives zero for a
+// divisor above 2^126, hence a quarter of both sides: 1 + e^z then stays below
+// that wherever e^z is finite. FAST: CUDA's fast exp as well, about |x| f32
+// steps off, for results of 16 bits, whose rounding is hundreds of times that
+// (8192 tokens, 8 experts each, K 1024: 367 us, with the polynomial 384).
+template <bool FAST>
+__device__ __forceinline__ float gmm_sigmoid_times(float x, float z) {       // x / (1 + e^z)
+    const float y = FAST ? __fmaf_rn(0.25f, __expf(z), 0.25f) : __fadd_rn(0.25f, gmm_quarter_exp(z));
+    return __fdividef(__fmul_rn(0.25f, x), y);
+}
 template <bool OAI, bool FAST>
 __device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) {
-    if (!OAI) return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, FAST ? __expf(-g) : gmm_exp(-g))), u);
+    if (!OAI) return __fmul_rn(gmm_sigmoid_times<FAST>(g, -g), u);
     const float x = p.limit < g ? p.limit : g;
     const float y = u < -p.limit ? -p.limit : (p.limit < u ? p.limit : u);
-    const float z = __fmul_rn(p.alpha, -x);
-    return __fmul_rn(__fdividef(x, __fadd_rn(1.0f, FAST ? __expf(z) : gmm_exp(z))), __fadd_rn(y, 1.0f));
+    return __fmul_rn(gmm_sigmoid_times<FAST>(x, __fmul_rn(p.alpha, -x)), __fadd_rn(y, 1.0f));
 }
 // of N values at once: g becomes the result (the choices stay outside the
 // loop, so that the values' chains of operations overlap)

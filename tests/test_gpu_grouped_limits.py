@@ -227,3 +227,52 @@ def test_h_of_any_size_in_f16(gxlib, dev, size):
     got = gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, base=s["base"], scale=scale)
     # (below 2^-126 of the result, f32 itself ends)
     assert bool(((got.double() - want).abs() <= tol + 2.0 ** -23 * want.abs() + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("kind,out", [("bf16", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_activation_over_the_whole_range(gxlib, dev, kind, out, act, rows):
+    """The gated activation on exactly known gates and ups: a fine grid, the ends where e^-g leaves f32, infinities and
+    NaN; single CTAs and pairs."""
+    half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[out]
+    dtype = {"bf16": torch.bfloat16, "f16": torch.float16}[kind]
+    alpha, limit = (1.702, 7.0) if act else (1.0, float("inf"))
+    grid = np.concatenate([np.linspace(-95, 95, 1501), -np.linspace(50, 54, 300), -np.linspace(86.5, 89.5, 300),
+                           [0.0, -0.0, 1e-3, -1e-3, 3e4, -3e4, np.inf, -np.inf, np.nan]])
+    ups = np.array([1.0, -3.5, 0.0, 7.0, 2.0 ** 14, 2.0 ** -14] + ([2.0 ** 100] if kind == "bf16" else []) + [np.inf, np.nan])
+    g0, u0 = (torch.from_numpy(v.reshape(-1)).cuda() for v in np.meshgrid(grid, ups))
+    N = g0.numel()
+    hi = g0.to(dtype)
+    lo = torch.where(torch.isfinite(hi), g0 - hi.double(), torch.zeros_like(g0)).to(dtype)
+    gate, up = (torch.zeros((1, N, 8), dtype=dtype, device="cuda") for _ in range(2))
+    gate[0, :, 0], gate[0, :, 1], up[0, :, 2] = hi, lo, u0.to(dtype)
+    x = torch.zeros((rows, 8), dtype=dtype, device="cuda")
+    x[:, :3] = 1.0
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    types = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+    got = gxlib.mul_mat_grouped_glu(gate, up, x, offsets, act=act, alpha=alpha, limit=limit if act else 7.0, out_dtype=types[out])
+    assert torch.equal(got.view(torch.int16 if out != "f32" else torch.int32), got[:1].expand(rows, N).contiguous().view(
+        torch.int16 if out != "f32" else torch.int32))
+    got = got[0].double()
+    g, u = hi.double() + lo.double(), up[0, :, 2].double()
+    if act:
+        g, u = torch.where(g > limit, limit, g), torch.where(u > limit, limit, torch.where(u < -limit, -limit, u)) + 1.0
+    z = -float(np.float32(alpha)) * g
+    e = torch.exp(z)
+    e = torch.where(e >= 2.0 ** 128, float("inf"), e)                # (f32, as gx_swiglu: 1 / (1 + inf) is zero)
+    want = g / (1.0 + e) * u
+    # f32: e^z within 2 steps, 16 bits: CUDA's fast exp, 2 + 1.173 |z| steps; the product alpha * x moves e^z by |z| half
+    # steps; the division 2 steps; the sum and the products (three, with u + 1) half a step each
+    steps = (4.0 if out == "f32" else 4.0 + 2.35 * z.abs()) + (z.abs() if act else 0.0) + 4.0 + 4.0
+    tol = torch.nan_to_num(steps * 2.0 ** -24 * want.abs(), nan=0.0, posinf=0.0)
+    # and half a step of the type's smallest numbers: f16's is 2^-24, bf16's 2^-133, f32's 2^-149 (twice: the quotient's too)
+    tol = tol + half * (want.abs() + tol) + {"f32": 2.0 ** -149, "bf16": 2.0 ** -134, "f16": 2.0 ** -25}[out]
+    top = {"f32": 3e38, "bf16": 3e38, "f16": 65000.0}[out]
+    finite = torch.isfinite(want) & (want.abs() < top)
+    bad = finite & ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), [(float(g[i]), float(u[i]), float(got[i]), float(want[i])) for i in bad.nonzero()[:5, 0].tolist()]
+    wild = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(got[wild]), torch.isnan(want[wild]))
+    keep = wild & ~torch.isnan(want)
+    assert torch.equal(got[keep], want[keep])
