@@ -70,6 +70,7 @@ struct GmmParams {
     int32_t stages;
     int32_t box;              // rows of one TMA box of x in place (divides nt / CTAs)
     int32_t mt;               // tiles of the matrix rows
+    int32_t most;             // tiles of nt rows that groups can have
     int32_t split;            // CTAs of a cluster that share K (single CTAs with nt = 32 only)
     int32_t seg;              // chunks that one accumulator sums (0: all)
     int32_t acc;              // TMEM columns of an accumulator
@@ -338,29 +339,36 @@ __device__ __forceinline__ int2 group_rows_of(const int32_t * offsets, int g, in
 }
 
 // pre[g] = tiles of nt rows in the groups before g (G + 1 values), by the
-// whole block; rows(g) are the rows of group g
+// whole block; rows(g) are the rows of group g. Groups that do not overlap have
+// at most `most` tiles; borders that name more (sums stop there, so none wraps
+// round) are reported, and the launch has no tiles.
 template <typename F>
-__device__ __forceinline__ void tile_prefix(int32_t * pre, int32_t * wsum, int G, int nt, F && rows) {
+__device__ __forceinline__ void tile_prefix(int32_t * pre, int32_t * wsum, int G, int nt, int most, F && rows) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = blockDim.x;
     const int per = (G + n - 1) / n;
     const int g0 = min(tid * per, G), g1 = min(g0 + per, G);
+    const int cap = most + 1;                   // (2^26 + 8194 at most)
     int sum = 0;
     for (int g = g0; g < g1; ++g) {
         const int2 r = rows(g);
         pre[g] = sum;
-        sum += (r.y - r.x + nt - 1) / nt;
+        if (r.y > r.x) sum = min(sum + (r.y - r.x - 1) / nt + 1, cap);
     }
     int inc = sum;
     for (int d = 1; d < 32; d <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += v;
+        if (lane >= d) inc = min(inc + v, cap);
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
     int before = inc - sum;
     for (int w = 0; w < warp; ++w) before += wsum[w];
     for (int g = g0; g < g1; ++g) pre[g] += before;
-    if (tid == n - 1) pre[G] = before + sum;
+    if (tid == n - 1) {
+        const bool over = before + sum > most;
+        if (over) record_error(GX_DEVERR_DOMAIN);
+        pre[G] = over ? 0 : before + sum;
+    }
     __syncthreads();
 }
 
@@ -390,7 +398,7 @@ __device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t *
     const int lo = p.offsets[r.g], hi = p.offsets[r.g + 1];
     // a group's tiles are of one size, rather than full ones and a rest
     const int n = pre[r.g + 1] - pre[r.g];
-    const int size = ((hi - lo + n - 1) / n + ROUND - 1) / ROUND * ROUND;
+    const int size = ((hi - lo - 1) / n + ROUND) / ROUND * ROUND;
     r.row0 = lo + (tt - pre[r.g]) * size;
     r.cnt = min(size, hi - r.row0);
     return r;
@@ -584,7 +592,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
         mbar_fence_init();
     }
     if (warp == 1) gmm_tmem_alloc<CTAS>(&tslot, 512);
-    tile_prefix(pre, wsum, p.G, p.nt, [&](int g) { return group_rows_of(p.offsets, g, p.n_rows); });
+    tile_prefix(pre, wsum, p.G, p.nt, p.most, [&](int g) { return group_rows_of(p.offsets, g, p.n_rows); });
     tc_fence_before();
     if (CTAS * split == 1) __syncthreads(); else cluster_sync_all();
     tc_fence_after();

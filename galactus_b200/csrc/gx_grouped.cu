@@ -258,8 +258,9 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
         (glu && !encode_rows(&p.umap, p.bf16, up, ne00, ne01, nb01, n_as, nb02, (uint32_t)gx::gmm_out_rows(mode))) ||
         !encode_rows(&p.xmap, p.bf16, b, ne00, ne11, nb11, 0, 0, gather ? 1u : (uint32_t)p.box))
         return GX_ERR_ALIGN;
-    const int64_t most = (int64_t)p.mt * (n_rows / p.nt + touched);
-    if (most > kMaxIndex) return GX_ERR_INVALID;
+    p.most = (int32_t)(n_rows / p.nt + touched);
+    const int64_t most = (int64_t)p.mt * p.most;
+    if (most > kMaxIndex - 65536) return GX_ERR_INVALID;        // (a CTA's next tile is an index too)
     cudaLaunchConfig_t cfg{};
     const int cluster = ctas * p.split;
     cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(clusters, most)));
@@ -422,6 +423,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (p.stages < 2) return GX_ERR_INVALID;
     const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::lora_stage_bytes(p.ra) + gx::lora_fixed_bytes(p.ra, p.G);
     const int64_t most = n_rows / gx::kLoraRows + std::min(n_rows, G);
+    p.most = (int32_t)(n_rows / gx::kLoraRows + std::min(n_rows, G + 1));
     cudaError_t e = allow_smem((const void *)gx::k_lora, kSlotLora, gx::kGroupedSmem);
     if (e != cudaSuccess) return cuda_status(e);
     // A cluster per tile of rows, of the size whose rounds of tiles cost least:

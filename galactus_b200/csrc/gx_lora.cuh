@@ -64,6 +64,7 @@ struct LoraParams {
     int32_t bf16, out;
     int32_t copy;             // base is not dst: rows without an adapter are copied
     int32_t stages;
+    int32_t most;             // tiles that the rows can have, those without an adapter among them
     int32_t seg;              // chunks that one accumulator of h sums (0: all)
 };
 
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
         mbar_fence_init();
     }
     if (warp == 1) gmm_tmem_alloc<1>(&tslot, kLoraTmem);
-    tile_prefix(pre, wsum, p.G + 1, kLoraRows, [&](int g) { return lora_rows(p, g); });
+    tile_prefix(pre, wsum, p.G + 1, kLoraRows, p.most, [&](int g) { return lora_rows(p, g); });
     tc_fence_before();
     if (C > 1) cluster_sync_all(); else __syncthreads();
     tc_fence_after();

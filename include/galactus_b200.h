@@ -300,8 +300,9 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
  * when neither gather nor scatter reads it. offsets ascend from >= 0 to <=
  * n_rows (the length of order; without gather b has at least n_rows rows).
  * dst may not overlap an input. Rows of dst outside every group are left as they were. A group whose borders
- * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped;
- * a row index outside b or dst is reported and its result is NaN or dropped.
+ * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped.
+ * Groups do not overlap: borders that together name more rows than there can be
+ * are reported, and nothing is computed. A row index outside b or dst is reported and its result is NaN or dropped.
  * With scatter the entries of order in a group must differ from one another and
  * from those of other groups (each names a row of dst); with gather they need not.
  * Requires 16-byte aligned as, b and strides nb01, nb02, nb11 (so ne00 * 2 may
@@ -339,7 +340,8 @@ int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t
  * second product in parts that keep at least 22 bits), the result is rounded
  * once to type_dst. offsets: [n_as * n_adapters + 1], offsets[0] = 0. Errors
  * found on the device are reported (gx_device_error): borders that do not
- * ascend or leave [0, n_rows] (the group is skipped), a rank above `rank` (as
+ * ascend or leave [0, n_rows] (the group is skipped), borders that together name
+ * more rows than there can be (nothing is computed), a rank above `rank` (as
  * 0), a row outside dst (dropped) or x (NaN). rank <= GX_LORA_MAX_RANK; 16-byte
  * aligned a, b, x and strides nba1, nba2, nbb1, nbb2, nb11. */
 #define GX_LORA_MAX_RANK 128

@@ -276,3 +276,27 @@ def test_activation_over_the_whole_range(gxlib, dev, kind, out, act, rows):
     assert torch.equal(torch.isnan(got[wild]), torch.isnan(want[wild]))
     keep = wild & ~torch.isnan(want)
     assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("groups", [3, 8191])
+def test_borders_that_overlap_many_times(gxlib, dev, groups):
+    """0, n, 0, n, ...: more rows than there are. Every second group descends and is skipped; with many of the others,
+    the tiles could outnumber what an index holds, and the call is dropped as a whole."""
+    from galactus_b200.moe import device_error
+    device_error()
+    n, K, N = 40, 64, 32
+    w = torch.randn((groups, N, K), device="cuda").half()
+    a, b = torch.randn((groups, 16, K), device="cuda").half(), torch.randn((groups, N, 16), device="cuda").half()
+    x = torch.randn((n, K), device="cuda").half()
+    offsets = torch.tensor([0, n] * (groups // 2 + 1), dtype=torch.int32, device="cuda")[:groups + 1].contiguous()
+    out = torch.full((n, N), 5.0, device="cuda")
+    gxlib.mul_mat_grouped(w, x, offsets, out=out)
+    assert device_error() == 1 and (groups == 3 or bool((out == 5.0).all()))
+    out.fill_(5.0)
+    gxlib.mul_mat_grouped_glu(w, w, x, offsets, out=out)
+    assert device_error() == 1 and (groups == 3 or bool((out == 5.0).all()))
+    out.fill_(5.0)
+    gxlib.lora_mul_mat(a, b, x, offsets, base=torch.zeros_like(out), out=out)
+    assert device_error() == 1 and (groups == 3 or bool((out == 5.0).all()))
+    one = torch.tensor([0] + [n] * groups, dtype=torch.int32, device="cuda")     # and good borders work as before
+    assert bool(torch.isfinite(gxlib.mul_mat_grouped(w, x, one, out_dtype=torch.float32)).all()) and device_error() == 0
