@@ -186,7 +186,9 @@ def mul_mat_grouped_glu(gate, up, x, offsets, *, order=None, n_rows: int | None 
     """gx_mul_mat_grouped_glu: as mul_mat_grouped with act(gate product, up
     product) in place of the product (ACT_SWIGLU, or ACT_SWIGLU_OAI with alpha
     and limit)."""
-    if up.shape != gate.shape or up.dtype != gate.dtype or up.stride() != gate.stride():
+    # (strides may differ where no element lies: one expert, one row, one column)
+    if up.shape != gate.shape or up.dtype != gate.dtype or \
+            up.stride() != gate.stride() and _matrices(up, "up") != _matrices(gate, "gate"):
         raise ValueError("gate and up: one shape, type and layout expected")
     dev = _device(gate, up, x, offsets, order, out)
     out, kind, nbd1, args = _product(gate, x, offsets, order, n_rows, gather, scatter, out, out_dtype, stream, dev)

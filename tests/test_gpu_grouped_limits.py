@@ -300,3 +300,20 @@ def test_borders_that_overlap_many_times(gxlib, dev, groups):
     assert device_error() == 1 and (groups == 3 or bool((out == 5.0).all()))
     one = torch.tensor([0] + [n] * groups, dtype=torch.int32, device="cuda")     # and good borders work as before
     assert bool(torch.isfinite(gxlib.mul_mat_grouped(w, x, one, out_dtype=torch.float32)).all()) and device_error() == 0
+
+
+@pytest.mark.parametrize("E,N,K", [(1, 40, 64), (4, 1, 64), (1, 1, 8)])
+def test_gate_and_up_with_strides_that_nothing_uses(gxlib, dev, E, N, K):
+    """One expert, or one row per expert: the strides that lead to no second one may differ."""
+    gate = torch.randn((E, N, K), device="cuda").bfloat16()
+    up = torch.randn((E, N, K), device="cuda").bfloat16()
+    x = torch.randn((9, K), device="cuda").bfloat16()
+    offsets = torch.tensor([0] * E + [9], dtype=torch.int32, device="cuda")
+    wide = torch.zeros((E, N + 3, K), dtype=torch.bfloat16, device="cuda")
+    wide[:, :N] = up
+    other = wide[:, :N] if E == 1 else up.as_strided((E, N, K), (K, 5 * K, 1))
+    assert other.stride() != gate.stride()
+    assert torch.equal(gxlib.mul_mat_grouped_glu(gate, other, x, offsets), gxlib.mul_mat_grouped_glu(gate, up, x, offsets))
+    if E == 1 and N > 1:
+        with pytest.raises(ValueError):
+            gxlib.mul_mat_grouped_glu(gate, torch.zeros((E, N, 2 * K), device="cuda").bfloat16()[:, :, :K], x, offsets)
