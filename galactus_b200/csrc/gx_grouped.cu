@@ -25,13 +25,14 @@ cudaError_t read_and_clear_grouped_error(int * code) {
 
 namespace {
 
-// One CTA per row and 1024 elements, four elements a thread. Bound by HBM.
+// One CTA per row and 1024 elements, four elements a thread (more in rows of
+// over 65535 x 1024).
 __global__ void __launch_bounds__(256) k_round_rows(bool bf16, const float * src, int ne0, int64_t nb1, uint8_t * dst,
                                                     int64_t stride) {
     const float * s = reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(src) + (int64_t)blockIdx.x * nb1);
     uint8_t * d = dst + (int64_t)blockIdx.x * stride;
-    for (int64_t i = (int64_t)blockIdx.y * 1024 + threadIdx.x; i < ne0 && i < (int64_t)(blockIdx.y + 1) * 1024; i += 256)
-        store_out(d, (int)i, s[i], bf16 ? GMM_BF16 : GMM_F16);
+    for (int64_t c = (int64_t)blockIdx.y * 1024; c < ne0; c += (int64_t)gridDim.y * 1024)
+        for (int64_t i = c + threadIdx.x; i < ne0 && i < c + 1024; i += 256) store_out(d, (int)i, s[i], bf16 ? GMM_BF16 : GMM_F16);
 }
 
 }  // namespace
@@ -39,8 +40,7 @@ __global__ void __launch_bounds__(256) k_round_rows(bool bf16, const float * src
 cudaError_t launch_round_rows(bool bf16, const float * src, int64_t ne0, int64_t nrows, int64_t nb1, uint8_t * dst,
                               int64_t stride, cudaStream_t stream) {
     if (nrows == 0) return cudaSuccess;
-    const int64_t cols = (ne0 + 1023) / 1024;
-    if (cols > 65535) return cudaErrorInvalidValue;
+    const int64_t cols = std::min<int64_t>((ne0 + 1023) / 1024, 65535);
     k_round_rows<<<dim3((unsigned)nrows, (unsigned)cols), 256, 0, stream>>>(bf16, src, (int)ne0, nb1, dst, stride);
     return cudaGetLastError();
 }

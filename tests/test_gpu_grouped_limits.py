@@ -317,3 +317,10 @@ def test_gate_and_up_with_strides_that_nothing_uses(gxlib, dev, E, N, K):
     if E == 1 and N > 1:
         with pytest.raises(ValueError):
             gxlib.mul_mat_grouped_glu(gate, torch.zeros((E, N, 2 * K), device="cuda").bfloat16()[:, :, :K], x, offsets)
+
+
+def test_rounding_of_very_long_rows(gxlib, dev):
+    """More columns than one CTA per 1024 of them can cover."""
+    n = 65535 * 1024 + 70001
+    x = torch.randn((2, n), device="cuda")
+    assert torch.equal(gxlib.round_rows(x, torch.bfloat16), x.bfloat16())
