@@ -38,6 +38,9 @@ def row_bytes(t: int, n: int) -> int:
 
 
 def vec_dot_type(t: int) -> int:
+    """The type that ggml's CPU path gives the activations of weights of type t."""
+    if t in (TYPE_F32, TYPE_F16, TYPE_BF16):
+        return t
     return TYPE_Q8_0 if t in (TYPE_Q8_0, TYPE_MXFP4) else TYPE_Q8_K
 
 

@@ -49,3 +49,11 @@ def test_adapters_ring_has_two_stages_for_every_group_count(plan, ra):
 def test_products_ring(plan, mode, ctas, nt, split):
     for g in GROUPS:
         assert plan.gmm_stages(ctas, nt, mode, g, split) >= 2 and plan.gmm_smem(ctas, nt, mode, g, split) <= MOST, g
+
+
+def test_types_that_are_not_quantised(gxlib):
+    """Their activations have their own type (gx_quantize_rows' argument), their rows two or four bytes an element."""
+    for t, size in ((gxlib.TYPE_F32, 4), (gxlib.TYPE_F16, 2), (gxlib.TYPE_BF16, 2)):
+        assert gxlib.vec_dot_type(t) == t and gxlib.row_bytes(t, 129) == 129 * size
+    assert gxlib.vec_dot_type(gxlib.TYPE_Q8_0) == gxlib.vec_dot_type(gxlib.TYPE_MXFP4) == gxlib.TYPE_Q8_0
+    assert gxlib.vec_dot_type(gxlib.TYPE_Q4_K) == gxlib.vec_dot_type(gxlib.TYPE_IQ1_S) == gxlib.TYPE_Q8_K
