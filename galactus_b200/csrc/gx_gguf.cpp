@@ -180,6 +180,8 @@ uint64_t row_bytes_of(uint32_t type, uint64_t ne0) {
         case GX_TYPE_Q6_K: return ne0 / 256 * 210;
         case GX_TYPE_IQ1_S: return ne0 / 256 * 50;
         case GX_TYPE_MXFP4: return ne0 / 32 * 17;
+        case GX_TYPE_F16:
+        case GX_TYPE_BF16: return ne0 * 2;
         default: return 0;
     }
 }

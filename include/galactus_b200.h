@@ -495,7 +495,8 @@ int gx_moe_ffn_noalloc(const gx_layer_desc * desc, const void * slot0_record, ui
  * blk.L.ffn_{down,gate,up}_exps.weight tensors ([ne0, ne1, n_expert], expert
  * e's rows contiguous) give the record of (L, e) as down | gate | up, the
  * layout of the reference's packs and profile (scripts/moe-profile.py:116-211,
- * records padded to 16 KiB). gx_gguf_moe_info reads the geometry;
+ * records padded to 16 KiB), of block-quantised, F16 and BF16 experts (the
+ * latter for the operators on grouped rows). gx_gguf_moe_info reads the geometry;
  * gx_arena_load_gguf copies every record of the arena's layers into its host
  * tier (as gx_load_record). gx_fnv1a64 is the record fingerprint of the
  * reference's paranoia check (scripts/verify-paranoia-trace.py:8-20). */
