@@ -192,32 +192,19 @@ __device__ __forceinline__ void lora_copy_row(const LoraParams & p, int row, int
     for (int i = pieces * kPer + first; i < p.N; i += step) d[i] = s[i];
 }
 
-// eight values of h as `parts` vectors of the operand type that sum to them
-__device__ __forceinline__ void split_h(const float (&h)[8], bool bf16, uint4 (&out)[3]) {
-    float rest[8];
+// eight values of h as vectors of the operand type that sum to them: three of
+// BF16 (24 bits), two of F16 (22)
+template <typename T>
+__device__ __forceinline__ void split_part(float (&rest)[8], uint4 & out) {
+    T * v = reinterpret_cast<T *>(&out);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rest[i] = h[i];
-#pragma unroll
-    for (int part = 0; part < 3; ++part) {
-        if (bf16) {
-            __nv_bfloat16 * v = reinterpret_cast<__nv_bfloat16 *>(&out[part]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = __float2bfloat16_rn(rest[i]);
-                const float d = __fsub_rn(rest[i], __bfloat162float(v[i]));
-                rest[i] = fabsf(d) < __int_as_float(0x7f800000) ? d : 0.0f;      // (an infinity or NaN stays in the first part)
-            }
-        } else {
-            __half * v = reinterpret_cast<__half *>(&out[part]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = __float2half_rn(rest[i]);
-                const float d = __fsub_rn(rest[i], __half2float(v[i]));
-                rest[i] = fabsf(d) < __int_as_float(0x7f800000) ? d : 0.0f;
-            }
-        }
+    for (int i = 0; i < 8; ++i) {
+        v[i] = round_to<T>(rest[i]);
+        const float d = __fsub_rn(rest[i], (float)v[i]);
+        rest[i] = fabsf(d) < __int_as_float(0x7f800000) ? d : 0.0f;          // (an infinity or NaN stays in the first part)
     }
 }
+__host__ __device__ constexpr int lora_parts(bool bf16) { return bf16 ? 3 : 2; }
 
 __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant__ LoraParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -295,7 +282,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             const LoraTile q = lora_tile(p, pre, t);
             if (q.rank == 0) continue;
             const int quads = (q.cnt + 3) >> 2;                          // rows in fours; those behind the last repeat it
-            
             bool bad = false;
             const int row = lora_row(p, q.row0 + min(lane, q.cnt - 1), bad);
             if (bad) record_error(GX_DEVERR_DOMAIN);
@@ -364,7 +350,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             bool ok = true;
             const uint64_t a0 = umma_desc_sw128(ring + 2u * kLoraXTile, 1024u), x0 = umma_desc_sw128(ring, 1024u);
             const uint64_t b0 = lora_desc(bring, row_bytes), h0 = lora_desc(hbuf, row_bytes);
-            const int parts = p.bf16 ? 3 : 2;
+            const int parts = lora_parts(p.bf16 != 0);
             // The results of a tile are issued between the chunks of the next
             // tile's h, as its own h and the tiles of B become ready: neither
             // the exchange over the cluster nor the copies of x hold the other up.
@@ -630,11 +616,14 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                         for (int e = 0; e < 8; ++e) h[e] = __fmul_rn(h[e], down);
                         if (r0 == 0) esc[row] = __uint_as_float((uint32_t)(127 + e2) << 23);
                     }
-                    uint4 v[3];
-                    split_h(h, p.bf16 != 0, v);
                     uint8_t * to = hbuf + (uint32_t)(r0 >> 6) * h_block + lora_swizzle(row_bytes, row, (r0 & 63) >> 3);
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(to + (uint32_t)k * blocks * h_block) = v[k];
+                    for (int k = 0; k < 3; ++k) {
+                        if (k >= lora_parts(p.bf16 != 0)) break;
+                        uint4 v;
+                        if (p.bf16) split_part<__nv_bfloat16>(h, v); else split_part<__half>(h, v);
+                        *reinterpret_cast<uint4 *>(to + (uint32_t)k * blocks * h_block) = v;
+                    }
                 }
             }
             fence_async_smem();
