@@ -160,6 +160,7 @@ int out_kind(int type) {
 }
 
 constexpr int64_t kMaxIndex = 0x7fffffff;
+constexpr int64_t kMaxSize = kMaxIndex - 65536;      // of rows and elements: the kernels look a tile ahead in 32 bits
 constexpr int64_t kMaxStride = 1ll << 40;      // of a tensor map
 
 // The shared checks and the launch of the plain (up == NULL) and gated products.
@@ -173,7 +174,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     if (act != GX_ACT_SWIGLU && act != GX_ACT_SWIGLU_OAI) return GX_ERR_INVALID;
     if (ne00 <= 0 || ne01 <= 0 || n_as <= 0 || ne11 < 0 || n_rows < 0 || gather < 0 || scatter < 0 || scatter > 1)
         return GX_ERR_INVALID;
-    if (n_as > gx::kGroupMaxGroups || ne00 > kMaxIndex || ne01 > kMaxIndex || ne11 > kMaxIndex || n_rows > kMaxIndex ||
+    if (n_as > gx::kGroupMaxGroups || ne00 > kMaxSize || ne01 > kMaxSize || ne11 > kMaxSize || n_rows > kMaxSize ||
         gather > kMaxIndex)
         return GX_ERR_INVALID;
     if (n_rows == 0) return GX_OK;
@@ -260,7 +261,7 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
         return GX_ERR_ALIGN;
     p.most = (int32_t)(n_rows / p.nt + touched);
     const int64_t most = (int64_t)p.mt * p.most;
-    if (most > kMaxIndex - 65536) return GX_ERR_INVALID;        // (a CTA's next tile is an index too)
+    if (most > kMaxSize) return GX_ERR_INVALID;        // (a CTA's next tile is an index too)
     cudaLaunchConfig_t cfg{};
     const int cluster = ctas * p.split;
     cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(clusters, most)));
@@ -292,7 +293,7 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
     if (ids != nullptr && (nbi1 < 4 * ne20 || nbi1 % 4)) return GX_ERR_INVALID;
     if (n_as > gx::kGroupMaxGroups || n_adapters > gx::kGroupMaxGroups) return GX_ERR_INVALID;
     const int64_t G = n_as * std::max<int64_t>(1, n_adapters);
-    if (G > gx::kGroupMaxGroups || ne20 > kMaxIndex || ne21 > kMaxIndex || ne20 * ne21 > kMaxIndex - 65536) return GX_ERR_INVALID;
+    if (G > gx::kGroupMaxGroups || ne20 > kMaxIndex || ne21 > kMaxIndex || ne20 * ne21 > kMaxSize) return GX_ERR_INVALID;
     if (misaligned(order, 4) || misaligned(offsets, 4) || misaligned(ids, 4) || misaligned(adapter, 4)) return GX_ERR_ALIGN;
     gx::GroupParams p{};
     p.ids = ids;
@@ -361,8 +362,8 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     if (K <= 0 || N <= 0 || d->rank <= 0 || d->rank > GX_LORA_MAX_RANK || d->n_as <= 0 || d->n_adapters <= 0 || ne11 < 0 ||
         n_rows < 0 || gather <= 0)
         return GX_ERR_INVALID;
-    if (d->n_as > gx::kGroupMaxGroups || d->n_adapters > gx::kGroupMaxGroups || K > kMaxIndex || N > kMaxIndex ||
-        ne11 > kMaxIndex || n_rows > kMaxIndex || gather > kMaxIndex)
+    if (d->n_as > gx::kGroupMaxGroups || d->n_adapters > gx::kGroupMaxGroups || K > kMaxSize || N > kMaxSize ||
+        ne11 > kMaxSize || n_rows > kMaxSize || gather > kMaxIndex)
         return GX_ERR_INVALID;
     const int64_t G = d->n_as * d->n_adapters;
     if (G > gx::kGroupMaxGroups) return GX_ERR_INVALID;

@@ -518,8 +518,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
             const unsigned nans = __ballot_sync(0xffffffffu, bad);
             const float scale = p.scale != nullptr ? p.scale[q.g / p.n_as] : 1.0f;
             if (vec && row_pieces && ew == 0 && my >= 0 && n_lo < n_hi) {
-                // base on its way into L2: lane's row, this CTA's columns
-                const uint32_t bytes = (uint32_t)(min(n_hi * 128, p.N) - n_lo * 128) * (uint32_t)esz;
+                // base on its way into L2: lane's row, this CTA's columns (a megabyte at most)
+                const uint32_t bytes = (uint32_t)min(min(n_hi * 128, p.N) - n_lo * 128, 1 << 18) * (uint32_t)esz;
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.base + (int64_t)my * p.nbb + (int64_t)n_lo * 128 * esz),
                              "r"(bytes)
                              : "memory");

@@ -264,6 +264,7 @@ int gx_expf(const float * x, float * y, int64_t n, void * stream);
  * be captured into a graph and follow gx_router_forward or gx_remap_serve's
  * slots on one stream. All pointers belong to the current device; no call
  * allocates or keeps anything, so calls on different streams are independent.
+ * Rows and their elements are counted in 32 bits: every size below 2^31 - 2^16.
  * One layer:
  *   gx_router_forward(logits)                      -> ids, weights
  *   gx_group_rows(ids)                             -> order, offsets

@@ -324,3 +324,14 @@ def test_rounding_of_very_long_rows(gxlib, dev):
     n = 65535 * 1024 + 70001
     x = torch.randn((2, n), device="cuda")
     assert torch.equal(gxlib.round_rows(x, torch.bfloat16), x.bfloat16())
+
+
+def test_adapters_of_a_very_wide_projection(gxlib, dev):
+    """Rows of base of more than a megabyte (an output head's)."""
+    s = make(3, 1, 1, 1, 8, 64, 300001, "bf16", "f32", 2)
+    want, tol = reference(s, np.zeros(3, np.int64), 1, 1, [8], [1.0])
+    offsets = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    compare(gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, base=s["base"]), want, tol, "f32")
+    wide = make(3, 1, 1, 1, 8, 64, 300032, "bf16", "f32", 3)
+    want, tol = reference(wide, np.zeros(3, np.int64), 1, 1, [8], [1.0])
+    compare(gxlib.lora_mul_mat(wide["a"], wide["b"], wide["x"], offsets, base=wide["base"]), want, tol, "f32")
