@@ -159,6 +159,13 @@ int out_kind(int type) {
     return type == GX_TYPE_F32 ? gx::GMM_F32 : type == GX_TYPE_F16 ? gx::GMM_F16 : type == GX_TYPE_BF16 ? gx::GMM_BF16 : -1;
 }
 
+// Whether one accumulator is too short for sums of K elements. The tensor
+// cores' f32 accumulators drop what does not fit instead of rounding: for
+// products of random signs about 1e-9 of the magnitudes' sum per element, for
+// products of one sign 6e-9 (measured: 4.8e-5 at K = 7168, 1.6e-4 at 28672).
+// Results of 16 bits do not see that while it is a fifth of half a step.
+bool long_sum(int out, int64_t K) { return K > (out == gx::GMM_F32 ? 512 : out == gx::GMM_F16 ? 16384 : 131072); }
+
 constexpr int64_t kMaxIndex = 0x7fffffff;
 constexpr int64_t kMaxSize = kMaxIndex - 65536;      // of rows and elements: the kernels look a tile ahead in 32 bits
 constexpr int64_t kMaxStride = 1ll << 40;      // of a tensor map
@@ -214,11 +221,10 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const int64_t avg = (n_rows + touched - 1) / touched;
     const int ctas = avg >= 96 ? 2 : 1;
     const int64_t nk = (ne00 + gx::kGmmK - 1) / gx::kGmmK;
-    // The tensor cores' f32 accumulators drop what does not fit instead of
-    // rounding, about 1e-9 of the sum per element of K. Results of 16 bits do
-    // not see that; for f32 results an accumulator takes 512 elements and the
-    // sums of the accumulators are rounded adds. A third of TMEM holds them.
-    p.seg = out == gx::GMM_F32 && nk > 8 ? 8 : 0;
+    // Where sums are long for the result's type, an accumulator takes 512
+    // elements and the sums of the accumulators are rounded adds. A third of
+    // TMEM holds them.
+    p.seg = long_sum(out, ne00) ? 8 : 0;
     p.nt = 32;
     const int mode = !glu ? gx::GMM_PLAIN : ctas == 2 && p.seg == 0 ? gx::GMM_DUAL : gx::GMM_GLU;
     if (ctas == 2) p.nt = p.seg ? 160 : 256;
@@ -409,8 +415,7 @@ int gx_lora_mul_mat(const gx_lora_desc * d, const void * x, int64_t ne11, int64_
     p.bf16 = d->type == GX_TYPE_BF16;
     p.out = out;
     p.copy = base != dst;
-    // (what f32 results need; 16-bit ones do not see the truncation of a long sum)
-    p.seg = out == gx::GMM_F32 ? gx::kLoraSeg : 0;
+    p.seg = long_sum(out, K) ? gx::kLoraSeg : 0;
     if (p.copy == 0 && nbb != nbd) return GX_ERR_INVALID;
     if (!encode_rows(&p.amap, p.bf16, d->a, K, d->rank, d->nba1, G, nba2, (uint32_t)p.ra) ||
         !encode_rows(&p.bmap, p.bf16, d->b, d->rank, N, d->nbb1, G, nbb2, 128u, (uint32_t)std::min(p.ra, 64)) ||

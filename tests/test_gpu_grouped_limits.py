@@ -335,3 +335,26 @@ def test_adapters_of_a_very_wide_projection(gxlib, dev):
     wide = make(3, 1, 1, 1, 8, 64, 300032, "bf16", "f32", 3)
     want, tol = reference(wide, np.zeros(3, np.int64), 1, 1, [8], [1.0])
     compare(gxlib.lora_mul_mat(wide["a"], wide["b"], wide["x"], offsets, base=wide["base"]), want, tol, "f32")
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_very_long_sums_with_f16_results(gxlib, dev, rows):
+    """Where a truncating sum would show beside the rounding of a 16-bit result, it is cut as well."""
+    K, N = 1 << 17, 70
+    x, w = positive((rows, K), 1.0, 1, "f16"), positive((1, N, K), 1.0 / 64, 2, "f16")
+    scale = 2.0 ** -4                                                # (sums near 1000 in f16)
+    w.mul_(scale)
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    got = gxlib.mul_mat_grouped(w, x, offsets, out_dtype=torch.float16).double()
+    want = x.double() @ w[0].double().T
+    bound = long_bound(K) + 2.0 ** -11 * (1 + long_bound(K))
+    off = float(((got - want).abs() / want).max())
+    assert off <= bound, f"{off:.3g} of {bound:.3g}"
+    a, b = positive((1, 16, K), 1.0 / K, 3, "f16"), positive((1, N, 16), 0.1, 4, "f16")
+    a = torch.where(a > 2.0 ** -16, a, a + 2.0 ** -16)               # (normal and subnormal f16 alike, all of one sign)
+    got = gxlib.lora_mul_mat(a, b, x, offsets, base=torch.zeros((rows, N), dtype=torch.float16, device="cuda")).double()
+    want = (x.double() @ a[0].double().T) @ b[0].double().T
+    bound = long_bound(K) + 2.0 ** -22 + (48 / 16 + 16) * 2.0 ** -23 + 2.0 ** -24
+    bound += 2.0 ** -11 * (1 + bound)
+    off = float(((got - want).abs() / want).max())
+    assert off <= bound, f"{off:.3g} of {bound:.3g}"
