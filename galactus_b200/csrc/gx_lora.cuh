@@ -21,8 +21,8 @@
 // the memory-bound kernel has time for. The tensor cores' accumulators truncate
 // (for sums of one sign 4.8e-5 of the sum at K = 7168, 1.6e-4 at 28672), so
 // for f32 results each takes 512 elements of K and the sums of the accumulators
-// are rounded adds (3.1e-6 and 1.4e-6 then; 8192 routed rows take 43.5 us with
-// it, 41.6 without). Six accumulators let a tile of K = 2048 be multiplied
+// are rounded adds (3.1e-6 and 1.4e-6 then; 8192 routed rows take 41 us with
+// it, 40 without). Six accumulators let a tile of K = 2048 be multiplied
 // while the one before it is finished (1.3 us more with two).
 //
 // Ranks differ by adapter: rows of A and columns of B behind an adapter's
@@ -534,15 +534,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) k_lora(const __grid_constant_
                 if (!ok) break;
                 tc_fence_after();
                 if (quad * 32 < p.ra && k0 < k1) {
+                    uint32_t v[32];
+                    tmem_ld32(d1 + (uint32_t)(sum.s * kLoraRows) + ((uint32_t)quad << 21), v);
 #pragma unroll
-                    for (int c0 = 0; c0 < kLoraRows; c0 += 16) {
-                        if (c0 >= q.cnt) break;
-                        uint32_t v[16];
-                        tmem_ld16(d1 + (uint32_t)(sum.s * kLoraRows + c0) + ((uint32_t)quad << 21), v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) own[c0 + i] = __fadd_rn(own[c0 + i], __uint_as_float(v[i]));
-                    }
+                    for (int i = 0; i < 32; ++i) own[i] = __fadd_rn(own[i], __uint_as_float(v[i]));
                 }
                 tc_fence_before();
                 __syncwarp();
