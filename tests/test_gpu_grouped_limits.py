@@ -358,3 +358,73 @@ def test_very_long_sums_with_f16_results(gxlib, dev, rows):
     bound += 2.0 ** -11 * (1 + bound)
     off = float(((got - want).abs() / want).max())
     assert off <= bound, f"{off:.3g} of {bound:.3g}"
+
+
+@pytest.mark.parametrize("K,N,rank,kind,out", [(1, 1, 1, "f16", "f32"), (5, 3, 3, "bf16", "bf16"), (65, 130, 17, "bf16", "f32"), (131, 127, 33, "f16", "f16")])
+def test_adapters_with_lengths_that_are_no_multiple(gxlib, dev, K, N, rank, kind, out):
+    """Rows padded to 16 bytes, NaN in the padding; no order and two rows of base per row of x, then an order."""
+    T, k = 21, 2
+    s = make(T, k, 1, 3, rank, K, N, kind, out, K)
+
+    def padded(t):
+        wide = torch.full((*t.shape[:-1], (t.shape[-1] + 7) // 8 * 8 + 8), float("nan"), dtype=t.dtype, device="cuda")
+        wide[..., :t.shape[-1]] = t
+        return wide[..., :t.shape[-1]]
+    a, b, x = padded(s["a"]), padded(s["b"]), padded(s["x"])
+    offsets = torch.tensor([0, 5, 5, 39], dtype=torch.int32, device="cuda")
+    keys = np.array([0] * 5 + [2] * 34 + [-1] * 3)
+    want, tol = reference(s, keys, k, 1, [rank] * 3, [1.0] * 3)
+    compare(gxlib.lora_mul_mat(a, b, x, offsets, gather=k, base=s["base"]), want, tol, out)
+    order = torch.randperm(T * k, device="cuda").int()
+    back = np.empty(T * k, np.int64)
+    back[order.cpu().numpy()] = keys
+    want, tol = reference(s, back, k, 1, [rank] * 3, [1.0] * 3)
+    compare(gxlib.lora_mul_mat(a, b, x, offsets, order=order, gather=k, base=s["base"]), want, tol, out)
+
+
+@pytest.mark.parametrize("rows", [1, 70, 5000])
+def test_no_row_has_an_adapter(gxlib, dev, rows):
+    """Every row is copied, bit for bit (NaN payloads too), or left alone in place; so with adapters of rank 0."""
+    from galactus_b200.moe import device_error
+    device_error()
+    s = make(rows, 1, 1, 4, 16, 64, 100, "bf16", "f32", rows)
+    s["base"].view(torch.int32)[:, 3] = 0x7fc12345
+    none = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    some = torch.arange(rows, device="cuda").int() % 4
+    for adapter, ranks in ((none, None), (some, torch.zeros(4, dtype=torch.int32, device="cuda"))):
+        order, offsets = gxlib.group_rows(None, adapter=adapter, n_adapters=4)
+        got = gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, order=order, ranks=ranks, base=s["base"])
+        assert torch.equal(got.view(torch.int32), s["base"].view(torch.int32))
+        here = s["base"].clone()
+        gxlib.lora_mul_mat(s["a"], s["b"], s["x"], offsets, order=order, ranks=ranks, base=here, out=here)
+        assert torch.equal(here.view(torch.int32), s["base"].view(torch.int32))
+    assert device_error() == 0
+
+
+def test_group_rows_of_millions_of_pairs_into_given_buffers(gxlib, dev):
+    T, k, E = (1 << 20) + 13, 8, 200
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device="cuda")
+    order = torch.full((T * k,), -7, dtype=torch.int32, device="cuda")
+    offsets = torch.full((E + 1,), -7, dtype=torch.int32, device="cuda")
+    got = gxlib.group_rows(ids, E, order=order, offsets=offsets)
+    assert got[0] is order and got[1] is offsets
+    key, want = torch.sort(torch.where(ids < 0, E, ids).reshape(-1), stable=True)
+    assert torch.equal(order, want.int())
+    assert torch.equal(offsets, torch.searchsorted(key, torch.arange(E + 1, device="cuda", dtype=torch.int32)).int())
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+def test_fewer_rows_than_the_order_holds(gxlib, dev, rows):
+    """n_rows: the groups end before the order does; a result with more rows than that keeps the others."""
+    K, N = 72, 40
+    w, x = (torch.randn((3, N, K), device="cuda") * 0.1).bfloat16(), torch.randn((rows + 9, K), device="cuda").bfloat16()
+    order = torch.randperm(rows + 9, device="cuda").int()
+    offsets = torch.tensor([0, rows // 2, rows // 2, rows], dtype=torch.int32, device="cuda")
+    out = torch.full((rows + 4, N), 7.0, device="cuda")
+    got = gxlib.mul_mat_grouped(w, x, offsets, order=order, n_rows=rows, gather=1, out=out)
+    assert got is out and bool((out[rows:] == 7.0).all())
+    g = torch.cat([torch.zeros(rows // 2, dtype=torch.long), torch.full((rows - rows // 2,), 2)]).cuda()
+    xs = x[order[:rows].long()].double()
+    want = torch.einsum("jnk,jk->jn", w[g].double(), xs)
+    tol = torch.einsum("jnk,jk->jn", w[g].double().abs(), xs.abs()) * (K / 16 + 16) * 2.0 ** -23
+    compare(out[:rows], want, tol, "f32")
