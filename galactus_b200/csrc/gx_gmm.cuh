@@ -14,30 +14,34 @@
 // place) by TMA, up to four warps gather other rows by tile::gather4, one
 // thread issues the MMAs, four or eight warps read the accumulators, apply
 // the activation and write 16-byte pieces by way of shared memory. Bounds and
-// choices, as measured on a B200 (1617 TFLOP/s, 6552 GB/s measured peaks):
+// choices, as measured on a B200 (1617 TFLOP/s, 6552 GB/s measured peaks; calls
+// in a row on one set of inputs, a few percent faster than on changing ones):
 //   - Few rows per expert: HBM. Gated, 19 tokens over 64 experts (hidden 2048,
-//     intermediate 1024): 49 us, 5.6 TB/s. Tiles of 32 rows leave room for a
+//     intermediate 1024): 50 us, 5.5 TB/s. Tiles of 32 rows leave room for a
 //     ring of ten stages. A last round of tiles that would leave most SMs idle
 //     is shared by clusters that split K (gated, 2880 x 2880, 4 experts: 180
-//     tiles on 148 SMs, 37 us without, 35 with).
-//   - Long groups: the tensor cores, and the board's power limit above
-//     1.2 PFLOP/s. CTA pairs (256 x 256 tiles): 32768 rows, K 4096, N 1536
-//     take 291 us in place (1415 TFLOP/s) and 341 us gathered. A single CTA's
-//     128 x 256 tile would need 96 bytes a cycle of L2, a pair's needs 64; the
-//     same shape took 495 us on single CTAs.
+//     tiles on 148 SMs, 33 us without, 29 with).
+//   - Long groups: the tensor cores. CTA pairs (256 x 256 tiles): 32768 rows,
+//     K 4096, N 1536 take 300 us in place (1371 TFLOP/s) and 334 us gathered. A
+//     single CTA's 128 x 256 tile would need 96 bytes a cycle of L2, a pair's
+//     needs 64; the same shape took 495 us on single CTAs. With f32 results it
+//     takes 400 us: four warps add the accumulators up (512 elements of K each)
+//     and stage twice the bytes.
 //   - Gated pairs keep 128 gate and 128 up rows per CTA against the same rows
 //     (both accumulators fill TMEM, nothing takes turns): a copied row is used
 //     twice, which gather4 (24 cycles per four rows) needs. 8192 tokens, 8
 //     experts each, K 4096, N 1536: 1128 us against 1244 with 64 + 64 rows and
 //     two accumulators in turn, 384 against 461 at K 1024 (both since a little
-//     faster: 1100 us, 1499 TFLOP/s, and 367). Spreading short groups' tiles
-//     among the long ones' changed nothing (1514 us for 1506 in the case of
-//     128 experts): both then share the board's power.
+//     faster: 1110 us, 1485 TFLOP/s, and 368). At 128 registers a thread 20
+//     bytes of it spill. In the case of 128 experts (1.65 PFLOP) a pass takes
+//     1470 us at 1965 MHz; back to back the board's power limit holds the SMs at
+//     1365 MHz (990 W) and a pass takes 1630. Spreading short groups' tiles
+//     among the long ones' changed nothing (1514 us for 1506).
 //   - The thread that issues copies or MMAs is chosen by elect.sync: with
 //     `lane == 0` a stage took 768 cycles, with it 590, of 512 for its MMAs.
 //   - Gathering by cp.async needs twelve warps (the fence that shows a stage
 //     to the tensor cores waits for all of a warp's copies) and reached 1043
-//     TFLOP/s where gather4 reaches 1208.
+//     TFLOP/s where gather4 reaches 1234.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -606,7 +610,9 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
     int whole = tiles;
     if (split > 1) {
         const int rest = tiles % units;
-        // (about three chunks of time go into a shared tile's exchange)
+        // (about three chunks of time go into a shared tile's exchange; shared
+        // and whole, gated: 180 tiles of 45 chunks 28.5 and 32.9 us, 128 of 32
+        // chunks 19.1 and 16.3, 320 of 112 chunks 87.5 and 100.6)
         if ((rest + clusters - 1) / clusters * (nk / split + 3) < nk) whole = tiles - rest;
     }
     struct Work {

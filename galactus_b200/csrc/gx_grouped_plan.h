@@ -56,7 +56,7 @@ constexpr uint32_t kLoraHalfSm = 112u * 1024u;  // dynamic shared memory that le
 constexpr int kLoraSums = 6;                    // accumulators of h that take turns
 constexpr uint32_t kLoraTmem = 256;             // columns: the sums of h, two tiles of results (32 each)
 constexpr int kLoraK = 128;                     // elements of K per stage: two swizzled rows of 64
-constexpr int kLoraSeg = 4;                     // stages that one accumulator of h sums when results are f32
+constexpr int kLoraSeg = 4;                     // stages that one accumulator of h sums where sums are long
 static_assert((kLoraSums + 2) * kLoraRows <= kLoraTmem, "columns of TMEM");
 constexpr uint32_t kLoraXTile = kLoraRows * 128u;
 constexpr uint32_t kLoraStaging = kLoraEpiWarps * 16u * 32u * 4u;

@@ -28,18 +28,20 @@
 // Ranks differ by adapter: rows of A and columns of B behind an adapter's
 // rank may hold anything and do not reach the result.
 //
-// Bounds, as measured on a B200: a call of one row takes 11 us, of which 2 are
-// the launch's set-up, 1.5 the first product, 2.5 the exchange and 2 the
-// second; 64 requests on 48 adapters of ranks 8 to 64 (K = N = 4096, 15 MB)
-// 21 us in clusters of four; 8192 routed rows in 250 groups (rank 16, K 2048,
-// N 768, f32, 64 MB) 43 us. There the copies of x bound the first product
-// (gather4 moves four rows of 128 bytes in 24 cycles) and the latency of base
-// the results, hence: rows that follow one another are copied as one box, two
-// CTAs share an SM where the ranks allow, base is fetched into L2 at the start
-// of a tile and into registers a result tile ahead (52 us without), and the
-// results of a tile are issued between the chunks of the next one (52 against
-// 46 us). Tiles of 64 rows took 87 us: fewer fit on an SM, and routed groups
-// are shorter.
+// Bounded by latency. On a B200 (calls in a row on one set of inputs; in
+// brackets on changing ones, called from Python) a call of one row takes 12 us
+// [14], of which 2 are the launch's set-up, 1.5 the first product, 2.5 the
+// exchange and 2 the second; 64 requests on 48 adapters of ranks 8 to 64
+// (K = N = 4096, 15 MB) 22 us [25] in clusters of four; 8192 routed rows in 250
+// groups (rank 16, K 2048, N 768, f32, 64 MB) 41 us [47 to 55]. There a CTA has
+// about two tiles; at gather4's rate (four rows of 128 bytes in 24 cycles) the
+// copies of x account for a third of the time, and the rest is not broken down.
+// What helped: rows that follow one another are copied as one box, two CTAs
+// share an SM where the ranks allow, base is fetched into L2 at the start of a
+// tile and into registers a result tile ahead (52 us without, at the time), and
+// the results of a tile are issued between the chunks of the next one (52 us to
+// 46). Tiles of 64 rows took 87 us: fewer fit on an SM, and routed groups are
+// shorter.
 #pragma once
 
 #include "gx_gmm.cuh"

@@ -289,7 +289,8 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
  *   dst row of j = W_g (b row of j)      for offsets[g] <= j < offsets[g+1]
  *   as       F16 or BF16, row r of expert g at as + g*nb02 + r*nb01, ne00 x ne01
  *            per expert, n_as experts (an arena's slots are experts here:
- *            nb02 = the record)
+ *            nb02 = the record). An expert's rows end within nb02 bytes:
+ *            interleaved experts are refused (GX_ERR_INVALID)
  *   b        ne11 rows of ne00 elements of the same type, nb11 bytes apart: the
  *            caller rounds f32 activations to the weight type as ggml does
  *            (gx_quantize_rows with GX_TYPE_F16 / GX_TYPE_BF16)
@@ -297,13 +298,17 @@ int gx_group_rows(const int32_t * ids, int64_t ne20, int64_t ne21, int64_t nbi1,
  *            per token, 1 when it has one per pair)
  *   scatter  0: row j of dst; 1: row order[j]
  *   dst      rows of ne01 elements of type_dst (F32, F16, BF16), nbd1 bytes apart
- * Products and sums are f32; the result is rounded once. order may be NULL
+ * Products and sums are f32; the result is rounded once. (The tensor cores'
+ * sums truncate: f32 results are cut into sums of 512 elements that are added
+ * with rounding, 16-bit ones where K is long enough to show.) order may be NULL
  * when neither gather nor scatter reads it. offsets ascend from >= 0 to <=
  * n_rows (the length of order; without gather b has at least n_rows rows).
- * dst may not overlap an input. Rows of dst outside every group are left as they were. A group whose borders
- * do not ascend or leave [0, n_rows] is reported (gx_device_error) and skipped.
- * Groups do not overlap: borders that together name more rows than there can be
- * are reported, and nothing is computed. A row index outside b or dst is reported and its result is NaN or dropped.
+ * dst may not overlap an input. Rows of dst outside every group are left as
+ * they were. A group whose borders do not ascend or leave [0, n_rows] is
+ * reported (gx_device_error) and skipped. Groups do not overlap: borders that
+ * together name more rows than there can be are reported, and nothing is
+ * computed. A row index outside b or dst is reported and its result is NaN or
+ * dropped.
  * With scatter the entries of order in a group must differ from one another and
  * from those of other groups (each names a row of dst); with gather they need not.
  * Requires 16-byte aligned as, b and strides nb01, nb02, nb11 (so ne00 * 2 may
@@ -332,6 +337,7 @@ int gx_mul_mat_grouped_glu(int type, const void * gate, const void * up, int64_t
  * adapter are then left alone) or lie apart from it (they are copied). dst and
  * base may not overlap in any other way, and order names no row twice.
  *   a      group g's A at a + g*nba2, `rank` rows of ne00 elements, nba1 apart
+ *          (they end within nba2 bytes, B's rows within nbb2)
  *   b      group g's B at b + g*nbb2, ne01 rows of `rank` elements, nbb1 apart
  *   ranks  device i32 [n_adapters], each 0 .. rank (0: no adapter), or NULL:
  *          all of rank `rank`. Rows of A and columns of B behind an adapter's
