@@ -20,17 +20,20 @@ for _code, _name in STATUS.items():
     globals()[_name] = _code
 
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
+TYPE_Q4_0, TYPE_Q4_1 = 2, 3
 TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K, TYPE_IQ1_S, TYPE_MXFP4 = 8, 12, 14, 15, 19, 39
 POLICY_AUTO, POLICY_UNIFORM, POLICY_PLAN, POLICY_FREQUENCY, POLICY_LRU = range(5)
 ACT_SWIGLU, ACT_SWIGLU_OAI = 0, 1
+GATE_NONE, GATE_SIGMOID = 0, 1
+Q4_MAX_IDS = 256
 
 BLOCK_BYTES = {TYPE_Q8_0: 34, TYPE_Q8_K: 292, TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_MXFP4: 17, TYPE_IQ1_S: 50,
-               TYPE_F32: 4, TYPE_F16: 2, TYPE_BF16: 2}
+               TYPE_F32: 4, TYPE_F16: 2, TYPE_BF16: 2, TYPE_Q4_0: 18, TYPE_Q4_1: 20}
 BLOCK_ELEMS = {TYPE_Q8_0: 32, TYPE_Q8_K: 256, TYPE_Q4_K: 256, TYPE_Q6_K: 256, TYPE_MXFP4: 32, TYPE_IQ1_S: 256,
-               TYPE_F32: 1, TYPE_F16: 1, TYPE_BF16: 1}
+               TYPE_F32: 1, TYPE_F16: 1, TYPE_BF16: 1, TYPE_Q4_0: 32, TYPE_Q4_1: 32}
 TYPE_NAMES = {TYPE_Q8_0: "q8_0", TYPE_Q4_K: "q4_K", TYPE_Q6_K: "q6_K", TYPE_Q8_K: "q8_K",
               TYPE_IQ1_S: "iq1_s", TYPE_MXFP4: "mxfp4",
-              TYPE_F32: "f32", TYPE_F16: "f16", TYPE_BF16: "bf16"}
+              TYPE_F32: "f32", TYPE_F16: "f16", TYPE_BF16: "bf16", TYPE_Q4_0: "q4_0", TYPE_Q4_1: "q4_1"}
 
 
 def row_bytes(t: int, n: int) -> int:
@@ -41,7 +44,9 @@ def vec_dot_type(t: int) -> int:
     """The type that ggml's CPU path gives the activations of weights of type t."""
     if t in (TYPE_F32, TYPE_F16, TYPE_BF16):
         return t
-    return TYPE_Q8_0 if t in (TYPE_Q8_0, TYPE_MXFP4) else TYPE_Q8_K
+    if t == TYPE_Q4_1:
+        return 9                             # (ggml's Q8_1, which nothing here computes on)
+    return TYPE_Q8_0 if t in (TYPE_Q4_0, TYPE_Q8_0, TYPE_MXFP4) else TYPE_Q8_K
 
 
 class gx_profile(C.Structure):
@@ -108,6 +113,16 @@ class gx_lora_desc(C.Structure):
     _fields_ = [("type", C.c_int32), ("rank", C.c_int32), ("ne00", C.c_int64), ("ne01", C.c_int64), ("n_as", C.c_int64),
                 ("n_adapters", C.c_int64), ("a", C.c_void_p), ("nba1", C.c_int64), ("nba2", C.c_int64), ("b", C.c_void_p),
                 ("nbb1", C.c_int64), ("nbb2", C.c_int64), ("ranks", C.c_void_p), ("scale", C.c_void_p)]
+
+
+class gx_block_desc(C.Structure):
+    _fields_ = [("ne0", C.c_int64), ("ne1", C.c_int64), ("k", C.c_int32), ("type_y", C.c_int32), ("type_shared", C.c_int32),
+                ("type_residual", C.c_int32), ("type_dst", C.c_int32), ("type_next", C.c_int32), ("y", C.c_void_p),
+                ("nby1", C.c_int64), ("nby2", C.c_int64), ("weights", C.c_void_p), ("ids", C.c_void_p), ("shared", C.c_void_p),
+                ("nbs", C.c_int64), ("shared_gate", C.c_void_p), ("norm", C.c_void_p), ("eps", C.c_float), ("scale", C.c_float),
+                ("gate", C.c_void_p), ("gne0", C.c_int64), ("nbg", C.c_int64), ("gate_act", C.c_int32), ("next_eps", C.c_float),
+                ("residual", C.c_void_p), ("nbr", C.c_int64), ("dst", C.c_void_p), ("nbd", C.c_int64), ("next", C.c_void_p),
+                ("nbn", C.c_int64), ("next_norm", C.c_void_p)]
 
 
 _P = C.c_void_p
@@ -193,6 +208,12 @@ _SIGS = {
                                          _I64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _I64, _P]),
     "gx_lora_mul_mat": (C.c_int, [C.POINTER(gx_lora_desc), _P, _I64, _I64, _P, _P, _I64, _I64, C.c_int, _P, _I64, _P, _I64,
                                   _P]),
+    "gx_mul_mat_q4": (C.c_int, [C.c_int, _P, _I64, _I64, _I64, _I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _I64, _I64,
+                                C.c_int, C.c_int, _P, _I64, _P]),
+    "gx_mul_mat_q4_glu": (C.c_int, [C.c_int, _P, _P, _I64, _I64, _I64, _I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _I64,
+                                    _I64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _I64, _P]),
+    "gx_rms_norm": (C.c_int, [C.c_int, _P, _I64, _I64, _I64, _P, C.c_float, C.c_int, _P, _I64, _P]),
+    "gx_block_out": (C.c_int, [C.POINTER(gx_block_desc), _P]),
     "gx_synth_normal": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
     "gx_synth_weights": (C.c_int, [C.c_int, _P, _I64, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
 }

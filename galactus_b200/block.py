@@ -1,0 +1,175 @@
+"""Products with 4-bit weights and the norms around a block, on torch tensors.
+
+Every tensor lives on the current CUDA device; streams, captures and the memory
+of results are as in the operators on grouped rows.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+from .grouped import _INT, _TYPE, _device, _index, _matrices, _new, _rows, _stream
+
+_LIB = L.lib()
+_F32 = torch.float32
+
+
+def _q4(name, w, up, x, type, ids, offsets, order, n_rows, gather, scatter, act, out, out_dtype, stream):
+    dev = _device(w, up, x, ids, offsets, order, out)
+    G, N, nb, nb01, nb02 = _matrices(w, "weights")
+    if w.dtype is not torch.uint8:
+        raise ValueError(f"weights: uint8 rows of blocks expected, not {w.dtype}")
+    if w.shape[1] <= 1:                      # (one row: no second one to reach)
+        nb01 = (nb + 3) & ~3
+    if G <= 1:
+        nb02 = N * nb01
+    rows, K, nb11 = _rows(x, "x")
+    if type not in (L.TYPE_Q4_0, L.TYPE_Q4_1) or K % 64 or L.row_bytes(type, K) != nb:
+        raise ValueError(f"weights: rows of {K} elements (a multiple of 64) in blocks of TYPE_Q4_0 or TYPE_Q4_1 expected")
+    if ids is not None:
+        if offsets is not None or order is not None:
+            raise ValueError("ids, or offsets and order")
+        if ids.dtype is not _INT or not ids.is_contiguous():
+            raise ValueError("ids: contiguous int32 expected")
+        if n_rows is None:
+            n_rows = ids.numel()
+        elif n_rows > ids.numel():
+            raise ValueError("n_rows: more than ids holds")
+        ids_ptr, offsets_ptr, order_ptr = ids.data_ptr(), 0, 0
+    else:
+        ids_ptr, offsets_ptr, order_ptr = 0, _index(offsets, "offsets", G + 1), _index(order, "order")
+        if n_rows is None:
+            n_rows = rows if order is None else order.shape[0]
+        elif order is not None and n_rows > order.shape[0]:
+            raise ValueError("n_rows: more than order holds")
+    if out is None:
+        out = _new(stream, dev, lambda: torch.empty((n_rows, N), dtype=out_dtype or x.dtype, device=w.device))
+        nbd1 = N * out.element_size()
+    else:
+        have, cols, nbd1 = _rows(out, "out")
+        if cols != N or have < n_rows or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out: at least {n_rows} rows of {N} elements of the result type expected")
+    kind = _TYPE.get(out.dtype)
+    if kind is None:
+        raise ValueError(f"results of {out.dtype}")
+    b_type = _TYPE.get(x.dtype, -1)
+    head = (type, w.data_ptr()) if up is None else (type, w.data_ptr(), up.data_ptr())
+    rc = getattr(_LIB, name)(*head, K, N, nb01, nb02, G, b_type, x.data_ptr(), rows, nb11, ids_ptr, offsets_ptr, order_ptr, n_rows,
+                             gather, scatter, *act, kind, out.data_ptr(), nbd1, _stream(stream, dev))
+    if rc:
+        L.check(rc, name)
+    return out
+
+
+def mul_mat_q4(w, x, *, type: int, ids=None, offsets=None, order=None, n_rows: int | None = None, gather: int = 0,
+               scatter: bool = False, out=None, out_dtype=None, stream=None):
+    """gx_mul_mat_q4: weights uint8 [G, N, bytes] (rows of TYPE_Q4_0 or
+    TYPE_Q4_1 blocks), rows x [rows, K] of float16 or bfloat16 -> [n_rows, N].
+
+    ids (int32, any contiguous shape, at most 256 of them): row j = x[j //
+    gather] times the matrix ids[j], to result row j; rows of negative ids are
+    left as they were (uninitialised in a result allocated here). offsets (and
+    order): the groups of group_rows, as in mul_mat_grouped. Neither: one matrix
+    for all rows."""
+    return _q4("gx_mul_mat_q4", w, None, x, type, ids, offsets, order, n_rows, gather, scatter, (), out, out_dtype, stream)
+
+
+def mul_mat_q4_glu(gate, up, x, *, type: int, ids=None, offsets=None, order=None, n_rows: int | None = None, gather: int = 0,
+                   scatter: bool = False, act: int = L.ACT_SWIGLU, alpha: float = 1.702, limit: float = 7.0, out=None,
+                   out_dtype=None, stream=None):
+    """gx_mul_mat_q4_glu: as mul_mat_q4 with act(gate product, up product) in
+    place of the product (ACT_SWIGLU, or ACT_SWIGLU_OAI with alpha and limit)."""
+    if up.shape != gate.shape or up.dtype != gate.dtype or \
+            up.stride() != gate.stride() and _matrices(up, "up") != _matrices(gate, "gate"):
+        raise ValueError("gate and up: one shape, type and layout expected")
+    return _q4("gx_mul_mat_q4_glu", gate, up, x, type, ids, offsets, order, n_rows, gather, scatter, (act, alpha, limit), out,
+               out_dtype, stream)
+
+
+def _result(t, like, shape, dtype, name, stream, dev):
+    """(tensor, its type, bytes between its rows): t, or a new one."""
+    if t is None:
+        t = _new(stream, dev, lambda: torch.empty(shape, dtype=dtype, device=like.device))
+    elif tuple(t.shape) != tuple(shape) or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name}: {tuple(shape)} of the result type expected")
+    kind = _TYPE.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name}: results of {t.dtype}")
+    return t, kind, _rows(t, name)[2]
+
+
+def _vector(t, name, n):
+    if t is None:
+        return 0
+    if t.dtype is not _F32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous float32 vector of {n} expected")
+    return t.data_ptr()
+
+
+def rms_norm(x, weight=None, *, eps: float = 1e-6, out=None, out_dtype=None, stream=None):
+    """gx_rms_norm: rows x [T, H] / sqrt(mean(x^2) + eps) * weight (float32 [H], or ones)."""
+    T, H, nb1 = _rows(x, "x")
+    dev = _device(x, weight, out)
+    out, kind, nbd = _result(out, x, (T, H), out_dtype or (x.dtype if out is None else None), "out", stream, dev)
+    rc = _LIB.gx_rms_norm(_TYPE.get(x.dtype, -1), x.data_ptr(), H, T, nb1, _vector(weight, "weight", H), eps, kind, out.data_ptr(), nbd,
+                          _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_rms_norm")
+    return out
+
+
+def block_out(y, *, weights=None, ids=None, shared=None, shared_gate=None, norm=None, eps: float = 1e-6, gate=None,
+              gate_sigmoid: bool = False, scale: float = 1.0, residual=None, out=None, out_dtype=None, next_norm=None,
+              next_dtype=None, next_out=None, next_eps: float | None = None, stream=None):
+    """gx_block_out: the end of a block. y [T, k, H] (or [T, H]), weights
+    float32 and ids int32 [T, k], shared [T, H] with shared_gate float32 [T],
+    norm float32 [H], gate float32 [T or 1, H or 1], residual [T, H] ->
+    out [T, H] (of the residual's type, y's without one), and with next_norm
+    (float32 [H]), next_dtype or next_out the pair (out, the next block's normed
+    rows)."""
+    if y.dim() == 2:
+        y = y.unsqueeze(1)
+    if y.dim() != 3 or (y.shape[2] > 1 and y.stride(2) != 1):
+        raise ValueError("y: [T, k, H] with consecutive elements in its rows expected")
+    T, k, H = y.shape
+    dev = _device(y, weights, ids, shared, shared_gate, norm, gate, residual, out, next_norm, next_out)
+    size = y.element_size()
+    d = L.gx_block_desc(ne0=H, ne1=T, k=k, type_y=_TYPE.get(y.dtype, -1), y=y.data_ptr(), eps=eps, scale=scale,
+                        nby1=(y.stride(1) if k > 1 else H) * size, nby2=(y.stride(0) if T > 1 else k * H) * size,
+                        next_eps=eps if next_eps is None else next_eps)
+    d.weights = _vector(weights, "weights", T * k)
+    if ids is not None:
+        if ids.dtype is not _INT or ids.numel() != T * k or not ids.is_contiguous():
+            raise ValueError(f"ids: contiguous int32 [{T}, {k}] expected")
+        d.ids = ids.data_ptr()
+    for name, t in (("shared", shared), ("residual", residual)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (T, H):
+            raise ValueError(f"{name}: [{T}, {H}] expected")
+        setattr(d, name, t.data_ptr())
+        setattr(d, "type_" + name, _TYPE.get(t.dtype, -1))
+        setattr(d, "nbs" if name == "shared" else "nbr", _rows(t, name)[2])
+    d.shared_gate = _vector(shared_gate, "shared_gate", T)
+    d.norm = _vector(norm, "norm", H)
+    if gate is not None:
+        rows, cols, nbg = _rows(gate, "gate")
+        if gate.dtype is not _F32 or rows not in (1, T) or cols not in (1, H):
+            raise ValueError(f"gate: float32 [{T} or 1, {H} or 1] expected")
+        d.gate, d.gne0, d.nbg = gate.data_ptr(), cols, nbg if rows > 1 else 0
+        d.gate_act = L.GATE_SIGMOID if gate_sigmoid else L.GATE_NONE
+    if out_dtype is None and out is None:
+        out_dtype = y.dtype if residual is None else residual.dtype
+    out, d.type_dst, d.nbd = _result(out, y, (T, H), out_dtype, "out", stream, dev)
+    d.dst = out.data_ptr()
+    more = next_norm is not None or next_dtype is not None or next_out is not None
+    if more:
+        next_out, d.type_next, d.nbn = _result(next_out, y, (T, H), next_dtype or (y.dtype if next_out is None else None), "next_out",
+                                               stream, dev)
+        d.next, d.next_norm = next_out.data_ptr(), _vector(next_norm, "next_norm", H)
+    rc = _LIB.gx_block_out(C.byref(d), _stream(stream, dev))
+    if rc:
+        L.check(rc, "gx_block_out")
+    return (out, next_out) if more else out

@@ -252,10 +252,12 @@ int gx_device_init(int device) {
 int gx_device_error(int32_t * code_out) {
     return guarded([&] {
         int code = 0;
-        int grouped = 0;
+        int grouped = 0, q4 = 0;
         ck(gx::read_and_clear_device_error(&code));
         ck(gx::read_and_clear_grouped_error(&grouped));
+        ck(gx::read_and_clear_q4_error(&q4));
         if (code == 0) code = grouped;
+        if (code == 0) code = q4;
         if (code_out) *code_out = code;
         return GX_OK;
     });

@@ -7,6 +7,9 @@
 //   Q6_K   { u8 ql[128]; u8 qh[64]; int8 scales[16]; fp16 d; }     210 B / 256
 //   MXFP4  { u8 e (e8m0); u8 qs[16]; }                             17 B / 32
 //   IQ1_S  { fp16 d; u8 qs[32]; u16 qh[8]; }                       50 B / 256
+// and, for the products with 16-bit rows (gx_q4.cuh):
+//   Q4_0   { fp16 d; u8 qs[16]; }                                  18 B / 32
+//   Q4_1   { fp16 d; fp16 m; u8 qs[16]; }                          20 B / 32
 #pragma once
 
 #include <cstdint>
@@ -20,6 +23,8 @@
 namespace gx {
 
 enum : int {
+    GX_T_Q4_0 = 2,
+    GX_T_Q4_1 = 3,
     GX_T_Q8_0 = 8,
     GX_T_Q4_K = 12,
     GX_T_Q6_K = 14,
@@ -30,6 +35,8 @@ enum : int {
 
 GX_HD int block_bytes(int type) {
     switch (type) {
+        case GX_T_Q4_0: return 18;
+        case GX_T_Q4_1: return 20;
         case GX_T_Q8_0: return 34;
         case GX_T_Q8_K: return 292;
         case GX_T_Q4_K: return 144;
@@ -42,7 +49,7 @@ GX_HD int block_bytes(int type) {
 
 GX_HD int block_elems(int type) {
     switch (type) {
-        case GX_T_Q8_0: case GX_T_MXFP4: return 32;
+        case GX_T_Q4_0: case GX_T_Q4_1: case GX_T_Q8_0: case GX_T_MXFP4: return 32;
         case GX_T_Q8_K: case GX_T_Q4_K: case GX_T_Q6_K: case GX_T_IQ1_S: return 256;
         default: return 0;
     }

@@ -175,6 +175,8 @@ int parse(const char * path, GgufFile & g, std::string & why) {
 
 uint64_t row_bytes_of(uint32_t type, uint64_t ne0) {
     switch (type) {
+        case GX_TYPE_Q4_0: return ne0 / 32 * 18;
+        case GX_TYPE_Q4_1: return ne0 / 32 * 20;
         case GX_TYPE_Q8_0: return ne0 / 32 * 34;
         case GX_TYPE_Q4_K: return ne0 / 256 * 144;
         case GX_TYPE_Q6_K: return ne0 / 256 * 210;

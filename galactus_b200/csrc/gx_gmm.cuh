@@ -413,7 +413,8 @@ __device__ __forceinline__ int gather_quads(int n, int w) { return max(1, (min(3
 
 // y row of grouped row j, -1 to skip it (no such row); nan: its x row does not exist
 // (o: order[j], where it is read at all)
-__device__ __forceinline__ int gmm_dst_row(const GmmParams & p, int j, int o, bool & nan) {
+template <typename P>
+__device__ __forceinline__ int gmm_dst_row(const P & p, int j, int o, bool & nan) {
     if (p.gather == 0 && p.scatter == 0) return j;
     nan = p.gather != 0 && (o < 0 || o / p.gather >= p.x_rows);
     if (p.scatter == 0) return j;
@@ -460,8 +461,8 @@ __device__ __forceinline__ float gmm_sigmoid_times(float x, float z) {       // 
     const float y = FAST ? __fmaf_rn(0.25f, __expf(z), 0.25f) : __fadd_rn(0.25f, gmm_quarter_exp(z));
     return __fdividef(__fmul_rn(0.25f, x), y);
 }
-template <bool OAI, bool FAST>
-__device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) {
+template <bool OAI, bool FAST, typename P>
+__device__ __forceinline__ float gmm_act(const P & p, float g, float u) {
     if (!OAI) return __fmul_rn(gmm_sigmoid_times<FAST>(g, -g), u);
     const float x = p.limit < g ? p.limit : g;
     const float y = u < -p.limit ? -p.limit : (p.limit < u ? p.limit : u);
@@ -469,13 +470,13 @@ __device__ __forceinline__ float gmm_act(const GmmParams & p, float g, float u) 
 }
 // of N values at once: g becomes the result (the choices stay outside the
 // loop, so that the values' chains of operations overlap)
-template <bool OAI, bool FAST, int N>
-__device__ __forceinline__ void gmm_act_each(const GmmParams & p, float (&g)[N], const float (&u)[N]) {
+template <bool OAI, bool FAST, int N, typename P>
+__device__ __forceinline__ void gmm_act_each(const P & p, float (&g)[N], const float (&u)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = gmm_act<OAI, FAST>(p, g[i], u[i]);
 }
-template <int N>
-__device__ __forceinline__ void gmm_act_all(const GmmParams & p, float (&g)[N], const float (&u)[N]) {
+template <int N, typename P>
+__device__ __forceinline__ void gmm_act_all(const P & p, float (&g)[N], const float (&u)[N]) {
     if (p.out == GMM_F32) {
         if (p.act == 0) gmm_act_each<false, false, N>(p, g, u);
         else gmm_act_each<true, false, N>(p, g, u);

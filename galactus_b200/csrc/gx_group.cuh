@@ -27,7 +27,6 @@
 
 namespace gx {
 
-constexpr int kGroupMaxGroups = 8192;
 constexpr int kGroupCluster = 8;
 constexpr uint32_t kGroupSmem = 200u * 1024u;
 

@@ -11,6 +11,7 @@ namespace gx {
 // aligning the ring.
 constexpr uint32_t kGroupedSmem = 226u * 1024u;
 constexpr uint32_t kGroupedAlign = 1024u;
+constexpr int kGroupMaxGroups = 8192;
 
 // ------------------------------------------------------------- products
 

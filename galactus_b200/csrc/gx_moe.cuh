@@ -383,8 +383,6 @@ template <> struct Oct<GX_T_IQ1_S> {
 
 // --------------------------------------------------------- PDL and TMA
 
-__device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------ decode kernels
 

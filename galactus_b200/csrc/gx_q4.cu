@@ -1,0 +1,266 @@
+// Entry points of the products with 4-bit weights and of the norms around a
+// block. No C++ exception crosses this boundary; every entry point returns GX_*.
+#include <algorithm>
+
+#include "gx_block.cuh"
+#include "gx_kernels.h"
+#include "gx_launch.h"
+#include "gx_q4.cuh"
+
+namespace gx {
+
+cudaError_t read_and_clear_q4_error(int * code) {
+    int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_dev_error, sizeof(int));
+    if (e != cudaSuccess) return e;
+    return cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int));
+}
+
+}  // namespace gx
+
+namespace {
+
+// A launch that may begin while the kernel before it on the stream ends: the
+// kernels wait (griddepcontrol.wait) before they read or write anything.
+template <typename P>
+cudaError_t launch_next(const void * fn, dim3 grid, int threads, uint32_t smem, int cluster, void * stream, P & p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    void * args[] = {&p};
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+template <bool BF16, bool Q41, bool GLU>
+const void * q4_kernel(int nt) {
+    return nt == 1 ? (const void *)gx::k_q4<BF16, Q41, GLU, 1> : (const void *)gx::k_q4<BF16, Q41, GLU, 4>;
+}
+const void * q4_kernel(bool bf16, bool q41, bool glu, int nt) {
+    if (bf16) return q41 ? (glu ? q4_kernel<true, true, true>(nt) : q4_kernel<true, true, false>(nt))
+                         : (glu ? q4_kernel<true, false, true>(nt) : q4_kernel<true, false, false>(nt));
+    return q41 ? (glu ? q4_kernel<false, true, true>(nt) : q4_kernel<false, true, false>(nt))
+               : (glu ? q4_kernel<false, false, true>(nt) : q4_kernel<false, false, false>(nt));
+}
+
+// The shared checks and the launch of the plain (up == NULL) and gated products.
+int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as,
+               int type_b, const void * b, int64_t ne11, int64_t nb11, const int32_t * ids, const int32_t * offsets,
+               const int32_t * order, int64_t n_rows, int64_t gather, int scatter, int act, float alpha, float limit, int type_dst,
+               void * dst, int64_t nbd1, void * stream) {
+    if (type != GX_TYPE_Q4_0 && type != GX_TYPE_Q4_1) return GX_ERR_TYPE;
+    if (type_b != GX_TYPE_F16 && type_b != GX_TYPE_BF16) return GX_ERR_TYPE;
+    const int out = out_kind(type_dst);
+    if (out < 0) return GX_ERR_TYPE;
+    if (act != GX_ACT_SWIGLU && act != GX_ACT_SWIGLU_OAI) return GX_ERR_INVALID;
+    if (ne00 <= 0 || ne01 <= 0 || n_as <= 0 || ne11 < 0 || n_rows < 0 || gather < 0 || scatter < 0 || scatter > 1)
+        return GX_ERR_INVALID;
+    if (n_as > gx::kGroupMaxGroups || ne00 > kMaxSize || ne01 > kMaxSize || ne11 > kMaxSize || n_rows > kMaxSize ||
+        gather > kMaxIndex)
+        return GX_ERR_INVALID;
+    if (ids != nullptr && (offsets != nullptr || order != nullptr || n_rows > GX_Q4_MAX_IDS)) return GX_ERR_INVALID;
+    if (n_rows == 0) return GX_OK;
+    if (as == nullptr || b == nullptr || dst == nullptr || ne11 == 0) return GX_ERR_INVALID;
+    if (ids == nullptr && offsets == nullptr && n_as != 1) return GX_ERR_INVALID;
+    if (ids != nullptr) {
+        scatter = 1;
+        gather = std::max<int64_t>(1, gather);
+    } else if (order == nullptr && (gather != 0 || scatter != 0)) {
+        return GX_ERR_INVALID;
+    }
+    if ((gather == 0 || (ids != nullptr && gather == 1)) && ne11 < n_rows) return GX_ERR_INVALID;
+    const int64_t esz = type_dst == GX_TYPE_F32 ? 4 : 2;
+    if (nb01 < 0 || nb02 < 0 || nb11 < 0 || nbd1 < 0 || nb01 >= kMaxStride || nb02 >= kMaxStride || nb11 >= kMaxStride)
+        return GX_ERR_INVALID;
+    if (n_as == 1) nb02 = nb01;                    // (never used to reach a second expert)
+    if (ne00 % 64 || nb01 % 4 || nb02 % 4 || nb11 % 16 || misaligned(as, 16) || misaligned(b, 16) || (up && misaligned(up, 16)))
+        return GX_ERR_ALIGN;
+    if (nbd1 % esz || misaligned(dst, esz) || misaligned(ids, 4) || misaligned(offsets, 4) || misaligned(order, 4))
+        return GX_ERR_ALIGN;
+    const int64_t row = gx::row_bytes(type, ne00);
+    if (nb01 < row || (n_as > 1 && !rows_fit(ne01, nb01, row, nb02)) || nb11 < 2 * ne00 || nbd1 < esz * ne01) return GX_ERR_INVALID;
+    const bool glu = up != nullptr, q41 = type == GX_TYPE_Q4_1, bf16 = type_b == GX_TYPE_BF16;
+
+    gx::Q4Params p{};
+    p.w0 = static_cast<const uint8_t *>(as);
+    p.w1 = static_cast<const uint8_t *>(glu ? up : as);
+    p.nb01 = nb01;
+    p.nb02 = nb02;
+    p.x = static_cast<const uint8_t *>(b);
+    p.nb11 = nb11;
+    p.ids = ids;
+    p.offsets = offsets;
+    p.order = order;
+    p.G = (int32_t)n_as;
+    p.n_rows = (int32_t)n_rows;
+    p.x_rows = (int32_t)ne11;
+    p.N = (int32_t)ne01;
+    p.K = (int32_t)ne00;
+    p.gather = (int32_t)gather;
+    p.scatter = scatter;
+    p.out = out;
+    p.dst = static_cast<uint8_t *>(dst);
+    p.nbd1 = nbd1;
+    p.act = act;
+    p.alpha = alpha;
+    p.limit = limit;
+    const int64_t touched = std::min(n_rows, n_as), avg = (n_rows + touched - 1) / touched;
+    const int nt = avg <= 8 ? 1 : 4;
+    const int rows = (glu ? 8 : 16) * gx::q4_mt(nt);
+    p.rt = (int32_t)((ne01 + rows - 1) / rows);
+    p.most = (int32_t)(n_rows / (8 * nt) + touched);
+    p.entries = ids != nullptr ? gx::kQ4MaxIds : offsets != nullptr ? p.G : 1;
+    const int64_t most = (int64_t)p.rt * p.most;
+    if (most > kMaxSize) return GX_ERR_INVALID;
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
+    const void * fn = q4_kernel(bf16, q41, glu, nt);
+    const int slot = (bf16 ? 8 : 0) + (q41 ? 4 : 0) + (glu ? 2 : 0) + (nt == 1 ? 0 : 1);
+    cudaError_t e = allow_smem(fn, slot, gx::q4_smem(q41, nt, gx::kGroupMaxGroups));
+    if (e != cudaSuccess) return cuda_status(e);
+    return cuda_status(launch_next(fn, dim3((unsigned)std::min<int64_t>(sms, most)), gx::kQ4Threads, gx::q4_smem(q41, nt, p.entries), 1,
+                                   stream, p));
+}
+
+// rows of ne0 elements of a result type: as the kernel takes them; false: a bad type, stride or alignment (in rc)
+bool block_rows(int type, const void * p, int64_t ne0, int64_t nb, int64_t ne1, gx::BlockRows & out, bool & vec, int & rc) {
+    out = gx::BlockRows{nullptr, 0, 0};
+    if (p == nullptr) return true;
+    const int kind = out_kind(type);
+    if (kind < 0) {
+        rc = GX_ERR_TYPE;
+        return false;
+    }
+    const int64_t esz = kind == gx::GMM_F32 ? 4 : 2;
+    if (nb < 0 || nb >= kMaxStride || (ne1 > 1 && nb < esz * ne0)) {
+        rc = GX_ERR_INVALID;
+        return false;
+    }
+    if (nb % esz || misaligned(p, esz)) {
+        rc = GX_ERR_ALIGN;
+        return false;
+    }
+    vec = vec && !misaligned(p, 16) && (ne1 <= 1 || nb % 16 == 0);
+    out = gx::BlockRows{static_cast<uint8_t *>(const_cast<void *>(p)), nb, kind};
+    return true;
+}
+
+int launch_block(gx::BlockParams & p, bool vec, void * stream) {
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
+    vec = vec && p.H % gx::kBlockUnit == 0;
+    const int units = (p.H + gx::kBlockUnit - 1) / gx::kBlockUnit;
+    int cluster = 1;
+    while (cluster < gx::kBlockMaxCluster &&
+           (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads || ((int64_t)p.T * cluster * 2 <= sms && units > cluster * 64)))
+        cluster *= 2;
+    const int per = (units + cluster - 1) / cluster;
+    int threads = 64;
+    while (threads < gx::kBlockMaxThreads && threads * (p.T * cluster > sms ? gx::kBlockUnits : 1) < per) threads *= 2;
+    const void * fn = cluster > 1 ? (vec ? (const void *)gx::k_block<true, true> : (const void *)gx::k_block<false, true>)
+                                  : (vec ? (const void *)gx::k_block<true, false> : (const void *)gx::k_block<false, false>);
+    return cuda_status(launch_next(fn, dim3((unsigned)(p.T * cluster)), threads, 0, cluster, stream, p));
+}
+
+}  // namespace
+
+extern "C" {
+
+int gx_mul_mat_q4(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as, int type_b,
+                  const void * b, int64_t ne11, int64_t nb11, const int32_t * ids, const int32_t * offsets, const int32_t * order,
+                  int64_t n_rows, int64_t gather, int scatter, int type_dst, void * dst, int64_t nbd1, void * stream) {
+    return q4_product(type, as, nullptr, ne00, ne01, nb01, nb02, n_as, type_b, b, ne11, nb11, ids, offsets, order, n_rows, gather,
+                      scatter, GX_ACT_SWIGLU, 0.0f, 0.0f, type_dst, dst, nbd1, stream);
+}
+
+int gx_mul_mat_q4_glu(int type, const void * gate, const void * up, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02,
+                      int64_t n_as, int type_b, const void * b, int64_t ne11, int64_t nb11, const int32_t * ids,
+                      const int32_t * offsets, const int32_t * order, int64_t n_rows, int64_t gather, int scatter, int act,
+                      float alpha, float limit, int type_dst, void * dst, int64_t nbd1, void * stream) {
+    if (up == nullptr && n_rows > 0) return GX_ERR_INVALID;
+    return q4_product(type, gate, up, ne00, ne01, nb01, nb02, n_as, type_b, b, ne11, nb11, ids, offsets, order, n_rows, gather,
+                      scatter, act, alpha, limit, type_dst, dst, nbd1, stream);
+}
+
+int gx_rms_norm(int type_src, const void * src, int64_t ne0, int64_t ne1, int64_t nb1, const float * weight, float eps, int type_dst,
+                void * dst, int64_t nbd1, void * stream) {
+    if (ne0 <= 0 || ne0 > GX_BLOCK_MAX_WIDTH || ne1 < 0 || ne1 > kMaxSize / gx::kBlockMaxCluster || !(eps >= 0.0f)) return GX_ERR_INVALID;
+    if (out_kind(type_src) < 0 || out_kind(type_dst) < 0) return GX_ERR_TYPE;
+    if (ne1 == 0) return GX_OK;
+    if (src == nullptr || dst == nullptr) return GX_ERR_INVALID;
+    gx::BlockParams p{};
+    bool vec = true;
+    int rc = GX_OK;
+    if (!block_rows(type_src, src, ne0, nb1, ne1, p.y, vec, rc) || !block_rows(type_dst, dst, ne0, nbd1, ne1, p.next, vec, rc)) return rc;
+    if (misaligned(weight, 4)) return GX_ERR_ALIGN;
+    p.H = (int32_t)ne0;
+    p.T = (int32_t)ne1;
+    p.k = 1;
+    p.y_nb2 = nb1;
+    p.scale = 1.0f;
+    p.has_next = 1;
+    p.next_eps = eps;
+    p.next_norm = weight;
+    return launch_block(p, vec, stream);
+}
+
+int gx_block_out(const gx_block_desc * d, void * stream) {
+    if (d == nullptr) return GX_ERR_INVALID;
+    if (d->ne0 <= 0 || d->ne0 > GX_BLOCK_MAX_WIDTH || d->ne1 < 0 || d->ne1 > kMaxSize / gx::kBlockMaxCluster || d->k <= 0 ||
+        d->ne1 * (int64_t)d->k > kMaxSize)
+        return GX_ERR_INVALID;
+    if ((d->norm != nullptr && !(d->eps >= 0.0f)) || (d->next != nullptr && !(d->next_eps >= 0.0f))) return GX_ERR_INVALID;
+    if (d->ne1 == 0) return GX_OK;
+    if (d->y == nullptr || (d->dst == nullptr && d->next == nullptr)) return GX_ERR_INVALID;
+    if (d->shared_gate != nullptr && d->shared == nullptr) return GX_ERR_INVALID;
+    gx::BlockParams p{};
+    bool vec = true;
+    int rc = GX_OK;
+    if (!block_rows(d->type_y, d->y, d->ne0, d->nby1, d->k, p.y, vec, rc)) return rc;
+    gx::BlockRows tokens;
+    if (!block_rows(d->type_y, d->y, d->ne0, d->nby2, d->ne1, tokens, vec, rc) ||
+        !block_rows(d->type_shared, d->shared, d->ne0, d->nbs, d->ne1, p.shared, vec, rc) ||
+        !block_rows(d->type_residual, d->residual, d->ne0, d->nbr, d->ne1, p.res, vec, rc) ||
+        !block_rows(d->type_dst, d->dst, d->ne0, d->nbd, d->ne1, p.dst, vec, rc) ||
+        !block_rows(d->type_next, d->next, d->ne0, d->nbn, d->ne1, p.next, vec, rc))
+        return rc;
+    if (misaligned(d->weights, 4) || misaligned(d->ids, 4) || misaligned(d->shared_gate, 4) || misaligned(d->norm, 4) ||
+        misaligned(d->next_norm, 4) || misaligned(d->gate, 4))
+        return GX_ERR_ALIGN;
+    if (d->gate != nullptr) {
+        if ((d->gne0 != 1 && d->gne0 != d->ne0) || d->nbg < 0 || d->nbg >= kMaxStride || (d->nbg != 0 && d->nbg < 4 * d->gne0))
+            return GX_ERR_INVALID;
+        if (d->gate_act != GX_GATE_NONE && d->gate_act != GX_GATE_SIGMOID) return GX_ERR_INVALID;
+        if (d->nbg % 4) return GX_ERR_ALIGN;
+        p.gate = d->gate;
+        p.gate_nb = d->nbg;
+        p.gate_step = d->gne0 == d->ne0 && d->ne0 > 1 ? 1 : 0;
+        p.gate_sigmoid = d->gate_act == GX_GATE_SIGMOID;
+    }
+    p.H = (int32_t)d->ne0;
+    p.T = (int32_t)d->ne1;
+    p.k = d->k;
+    p.y_nb2 = d->nby2;
+    p.w = d->weights;
+    p.ids = d->ids;
+    p.shared_gate = d->shared_gate;
+    p.norm = d->norm;
+    p.has_norm = d->norm != nullptr;
+    p.has_next = d->next != nullptr;
+    p.eps = d->eps;
+    p.next_eps = d->next_eps;
+    p.scale = d->scale;
+    p.next_norm = d->next_norm;
+    return launch_block(p, vec, stream);
+}
+
+}  // extern "C"

@@ -48,6 +48,8 @@ extern "C" {
 #define GX_TYPE_F32    0   /* results of the operators on grouped rows */
 #define GX_TYPE_F16    1   /* unquantised experts and adapters, their rows and results */
 #define GX_TYPE_BF16  30
+#define GX_TYPE_Q4_0   2   /* products with 16-bit rows (gx_mul_mat_q4) */
+#define GX_TYPE_Q4_1   3
 #define GX_TYPE_Q8_0   8
 #define GX_TYPE_Q4_K  12
 #define GX_TYPE_Q6_K  14
@@ -369,6 +371,90 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
                     const int32_t * order, int64_t n_rows, int64_t gather, int type_dst, const void * base, int64_t nbb,
                     void * dst, int64_t nbd, void * stream);
 
+/* ------------------------------------------------------------ 4-bit weights
+ * Products of F16 / BF16 rows with Q4_0 and Q4_1 matrices (GGUF blocks of 32
+ * 4-bit codes and their scales, read in place, so an arena's slots serve as
+ * experts):
+ *   Q4_0  { f16 d; u8 qs[16] }         w = d (q - 8)
+ *   Q4_1  { f16 d; f16 m; u8 qs[16] }  w = d q + m
+ * gx_mul_mat_id refuses these types (it promises ggml's bits, with activations
+ * quantised to 8 bits); here rows keep their 16 bits, products are exact, sums
+ * are f32 and the result is rounded once to type_dst (F32, F16, BF16).
+ *   dst row of j = W_e (b row of j)
+ * The matrix of a row is named in one of three ways:
+ *   ids      device i32 [n_rows], n_rows <= GX_Q4_MAX_IDS: row j's expert (decode:
+ *            the router's ids as they are; j = t*k + s). b row j / gather (gather =
+ *            k where b has a row per token, 1 or 0 where it has one per pair), dst
+ *            row j; order and offsets are NULL, scatter is not read. A negative id
+ *            leaves its row of dst as it was; one >= n_as is reported
+ *            (gx_device_error) and its row left too.
+ *   offsets  device i32 [n_as + 1] and order as gx_group_rows gives them, any
+ *            number of rows, with gather and scatter as in gx_mul_mat_grouped
+ *   neither  n_as = 1: all n_rows rows with the one matrix (a dense projection)
+ * Offsets, row indexes and what is reported: as gx_mul_mat_grouped. A row of b
+ * with an infinity or a NaN makes its own results NaN, and no other.
+ * Requires ne00 % 64 == 0; 16-byte aligned as, b and nb11; nb01 and nb02
+ * multiples of 4; n_as <= 8192. dst may not overlap an input. The calls follow
+ * one another on a stream without a gap (programmatic launches), can be
+ * captured, allocate nothing and keep nothing. */
+#define GX_Q4_MAX_IDS 256
+int gx_mul_mat_q4(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as, int type_b,
+                  const void * b, int64_t ne11, int64_t nb11, const int32_t * ids, const int32_t * offsets, const int32_t * order,
+                  int64_t n_rows, int64_t gather, int scatter, int type_dst, void * dst, int64_t nbd1, void * stream);
+/* The gate and up products and the activation in one pass (gate and up share
+ * their strides), as gx_mul_mat_grouped_glu. */
+int gx_mul_mat_q4_glu(int type, const void * gate, const void * up, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02,
+                      int64_t n_as, int type_b, const void * b, int64_t ne11, int64_t nb11, const int32_t * ids,
+                      const int32_t * offsets, const int32_t * order, int64_t n_rows, int64_t gather, int scatter, int act,
+                      float alpha, float limit, int type_dst, void * dst, int64_t nbd1, void * stream);
+
+/* ------------------------------------------------------- around the block
+ * The norms before and behind a block (the routed FFN, attention, ...), with
+ * what stands between them:
+ *   m    = sum over s of weights[t, s] y[t, s]  +  sigmoid(shared_gate[t]) shared[t]
+ *   out  = residual + scale * gate * norm(m)
+ *   next = norm(out)
+ * norm(v) = v / sqrt(mean(v^2) + eps) * its weight (ggml's rms_norm and mul).
+ * All in f32 (the sum over s in slot order with a rounding per product and per
+ * add, as gx_combine), each result rounded once; next is the norm of the f32
+ * out. Rows have F32, F16 or BF16 elements; sums of their squares must be finite
+ * in f32. Results may lie in place of an input with the same type and strides;
+ * otherwise nothing may overlap a result. */
+#define GX_BLOCK_MAX_WIDTH 65536
+#define GX_GATE_NONE    0
+#define GX_GATE_SIGMOID 1
+/* rows of ne0 elements, nb1 (nbd1) bytes apart: dst = norm(src), weight device f32
+ * [ne0] or NULL (ones) */
+int gx_rms_norm(int type_src, const void * src, int64_t ne0, int64_t ne1, int64_t nb1, const float * weight, float eps, int type_dst,
+                void * dst, int64_t nbd1, void * stream);
+typedef struct gx_block_desc {
+    int64_t ne0, ne1;          /* elements of a row, rows (tokens) */
+    int32_t k;                 /* rows of y per token */
+    int32_t type_y, type_shared, type_residual, type_dst, type_next;
+    const void * y;            /* row (t, s) at y + t*nby2 + s*nby1 */
+    int64_t nby1, nby2;
+    const float * weights;     /* device f32 [ne1, k], or NULL: ones */
+    const int32_t * ids;       /* device i32 [ne1, k], or NULL: a slot with a negative id is left out (its row of y may hold anything) */
+    const void * shared;       /* rows nbs apart, or NULL */
+    int64_t nbs;
+    const float * shared_gate; /* device f32 [ne1], or NULL: 1 in place of the sigmoid */
+    const float * norm;        /* device f32 [ne0], the weight of the norm behind the block, or NULL: no norm */
+    float eps;
+    float scale;
+    const float * gate;        /* device f32, gne0 = 1 or ne0 elements a row, rows nbg apart (0: one for all tokens), or NULL */
+    int64_t gne0, nbg;
+    int32_t gate_act;          /* GX_GATE_*: what is done to the gate first */
+    float next_eps;
+    const void * residual;     /* rows nbr apart, or NULL: zeros */
+    int64_t nbr;
+    void * dst;                /* out, rows nbd apart, or NULL */
+    int64_t nbd;
+    void * next;               /* rows nbn apart, or NULL */
+    int64_t nbn;
+    const float * next_norm;   /* device f32 [ne0], or NULL: ones */
+} gx_block_desc;
+int gx_block_out(const gx_block_desc * desc, void * stream);
+
 /* ------------------------------------------------------------- MoE layer
  * One routed-expert FFN layer, end to end on the device:
  *   remap (policy + miss copies) -> gate/up mul_mat_id + activation
@@ -503,7 +589,7 @@ int gx_moe_ffn_noalloc(const gx_layer_desc * desc, const void * slot0_record, ui
  * e's rows contiguous) give the record of (L, e) as down | gate | up, the
  * layout of the reference's packs and profile (scripts/moe-profile.py:116-211,
  * records padded to 16 KiB), of block-quantised, F16 and BF16 experts (the
- * latter for the operators on grouped rows). gx_gguf_moe_info reads the geometry;
+ * latter for the operators on grouped rows; Q4_0 and Q4_1 for gx_mul_mat_q4). gx_gguf_moe_info reads the geometry;
  * gx_arena_load_gguf copies every record of the arena's layers into its host
  * tier (as gx_load_record). gx_fnv1a64 is the record fingerprint of the
  * reference's paranoia check (scripts/verify-paranoia-trace.py:8-20). */
