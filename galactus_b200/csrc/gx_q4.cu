@@ -41,15 +41,13 @@ cudaError_t launch_next(const void * fn, dim3 grid, int threads, uint32_t smem, 
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
-template <bool BF16, bool Q41, bool GLU>
-const void * q4_kernel(int nt) {
-    return nt == 1 ? (const void *)gx::k_q4<BF16, Q41, GLU, 1> : (const void *)gx::k_q4<BF16, Q41, GLU, 4>;
+template <bool BF16, bool Q41>
+const void * q4_kernel(bool glu) {
+    return glu ? (const void *)gx::k_q4<BF16, Q41, true> : (const void *)gx::k_q4<BF16, Q41, false>;
 }
-const void * q4_kernel(bool bf16, bool q41, bool glu, int nt) {
-    if (bf16) return q41 ? (glu ? q4_kernel<true, true, true>(nt) : q4_kernel<true, true, false>(nt))
-                         : (glu ? q4_kernel<true, false, true>(nt) : q4_kernel<true, false, false>(nt));
-    return q41 ? (glu ? q4_kernel<false, true, true>(nt) : q4_kernel<false, true, false>(nt))
-               : (glu ? q4_kernel<false, false, true>(nt) : q4_kernel<false, false, false>(nt));
+const void * q4_kernel(bool bf16, bool q41, bool glu) {
+    return bf16 ? (q41 ? q4_kernel<true, true>(glu) : q4_kernel<true, false>(glu))
+                : (q41 ? q4_kernel<false, true>(glu) : q4_kernel<false, false>(glu));
 }
 
 // The shared checks and the launch of the plain (up == NULL) and gated products.
@@ -64,7 +62,7 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
     if (act != GX_ACT_SWIGLU && act != GX_ACT_SWIGLU_OAI) return GX_ERR_INVALID;
     if (ne00 <= 0 || ne01 <= 0 || n_as <= 0 || ne11 < 0 || n_rows < 0 || gather < 0 || scatter < 0 || scatter > 1)
         return GX_ERR_INVALID;
-    if (n_as > gx::kGroupMaxGroups || ne00 > kMaxSize || ne01 > kMaxSize || ne11 > kMaxSize || n_rows > kMaxSize ||
+    if (n_as > gx::kGroupMaxGroups || ne00 > GX_Q4_MAX_K || ne01 > kMaxSize || ne11 > kMaxSize || n_rows > kMaxSize ||
         gather > kMaxIndex)
         return GX_ERR_INVALID;
     if (ids != nullptr && (offsets != nullptr || order != nullptr || n_rows > GX_Q4_MAX_IDS)) return GX_ERR_INVALID;
@@ -113,22 +111,37 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
     p.act = act;
     p.alpha = alpha;
     p.limit = limit;
-    const int64_t touched = std::min(n_rows, n_as), avg = (n_rows + touched - 1) / touched;
-    const int nt = avg <= 8 ? 1 : 4;
-    const int rows = (glu ? 8 : 16) * gx::q4_mt(nt);
+    const int64_t touched = std::min(n_rows, n_as);
+    const gx::Q4Shape shape = gx::q4_shape(q41, ne00, n_rows);
+    p.warps = shape.warps;
+    p.cap = shape.cap;
+    p.buffers = shape.buffers;
+    const int rows = (glu ? 8 : 16) * gx::kQ4Mt;
     p.rt = (int32_t)((ne01 + rows - 1) / rows);
-    p.most = (int32_t)(n_rows / (8 * nt) + touched);
-    p.entries = ids != nullptr ? gx::kQ4MaxIds : offsets != nullptr ? p.G : 1;
-    const int64_t most = (int64_t)p.rt * p.most;
-    if (most > kMaxSize) return GX_ERR_INVALID;
+    const int64_t tiles = n_rows / p.cap + touched, most = p.rt * tiles;
+    if (tiles > kMaxSize || most > kMaxSize) return GX_ERR_INVALID;
+    p.most = (int32_t)tiles;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
-    const void * fn = q4_kernel(bf16, q41, glu, nt);
-    const int slot = (bf16 ? 8 : 0) + (q41 ? 4 : 0) + (glu ? 2 : 0) + (nt == 1 ? 0 : 1);
-    cudaError_t e = allow_smem(fn, slot, gx::q4_smem(q41, nt, gx::kGroupMaxGroups));
+    // Warps that share K: as many as make the rounds of jobs cheapest, about four
+    // pairs of blocks being spent on what a job has beside them.
+    const int64_t jobs = p.rt * (touched + (n_rows - touched) / p.cap), pairs = ne00 / 64;
+    int64_t best = 0;
+    for (int c = 1; c <= p.warps; ++c) {
+        if (p.warps % c) continue;
+        const int64_t units = (int64_t)sms * (p.warps / c), cost = (jobs + units - 1) / units * ((pairs + c - 1) / c + (c == 1 ? 4 : 6));
+        if (c == 1 || cost < best) {
+            best = cost;
+            p.share = c;
+        }
+    }
+    const void * fn = q4_kernel(bf16, q41, glu);
+    const int slot = (bf16 ? 4 : 0) + (q41 ? 2 : 0) + (glu ? 1 : 0);
+    cudaError_t e = allow_smem(fn, slot, gx::kQ4Smem);
     if (e != cudaSuccess) return cuda_status(e);
-    return cuda_status(launch_next(fn, dim3((unsigned)std::min<int64_t>(sms, most)), gx::kQ4Threads, gx::q4_smem(q41, nt, p.entries), 1,
-                                   stream, p));
+    const int64_t grid = std::min<int64_t>(sms, (most * p.share + p.warps - 1) / p.warps);
+    return cuda_status(launch_next(fn, dim3((unsigned)grid), 32 * p.warps, gx::q4_smem(q41, ne00, p.warps, p.cap, p.buffers), 1, stream,
+                                   p));
 }
 
 // rows of ne0 elements of a result type: as the kernel takes them; false: a bad type, stride or alignment (in rc)
@@ -154,11 +167,56 @@ bool block_rows(int type, const void * p, int64_t ne0, int64_t nb, int64_t ne1, 
     return true;
 }
 
+constexpr uint32_t kStreamSmem = 220u * 1024u;
+constexpr int kStreamWidth = 512, kStreamRows = 2;     // narrower or fewer rows go a CTA each
+
+template <int YT>
+const void * block_kernel(bool vec, bool cluster) {
+    return vec ? (cluster ? (const void *)gx::k_block<YT, true, true> : (const void *)gx::k_block<YT, true, false>)
+               : (cluster ? (const void *)gx::k_block<YT, false, true> : (const void *)gx::k_block<YT, false, false>);
+}
+
+template <int YT>
+int launch_block_rows(gx::BlockParams & p, int grid, int warps, int slots, int slot_bytes, void * stream) {
+    const void * fn = (const void *)gx::k_block_rows<YT>;
+    const uint32_t smem = (uint32_t)(slots * slot_bytes);
+    cudaError_t e = allow_smem(fn, 8 + YT, kStreamSmem);
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)(32 * (warps + 1)));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    void * args[] = {&p, &slots, &slot_bytes};
+    return cuda_status(cudaLaunchKernelExC(&cfg, fn, args));
+}
+int launch_block_rows(gx::BlockParams & p, int sms, void * stream) {
+    const auto size = [](const gx::BlockRows & r) { return r.p == nullptr ? 0 : r.type == gx::GMM_F32 ? 4 : 2; };
+    const int slot_bytes = (p.H * std::max(size(p.y), std::max(size(p.shared), size(p.res))) + 127) / 128 * 128;
+    const int warps = (p.H + 32 * gx::kBlockUnit * gx::kBlockUnits - 1) / (32 * gx::kBlockUnit * gx::kBlockUnits);
+    const int ctas = warps <= 8 ? 2 : 1;               // per SM
+    const int slots = std::min<int>(gx::kRowsMaxSlots, (int)(kStreamSmem / ctas) / slot_bytes);
+    const int grid = std::min<int64_t>((int64_t)sms * ctas, p.T);
+    switch (p.y.type) {
+        case gx::GMM_F32: return launch_block_rows<gx::GMM_F32>(p, grid, warps, slots, slot_bytes, stream);
+        case gx::GMM_F16: return launch_block_rows<gx::GMM_F16>(p, grid, warps, slots, slot_bytes, stream);
+        default: return launch_block_rows<gx::GMM_BF16>(p, grid, warps, slots, slot_bytes, stream);
+    }
+}
+
 int launch_block(gx::BlockParams & p, bool vec, void * stream) {
+    p.one = 1.0f;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
-    vec = vec && p.H % gx::kBlockUnit == 0;
+    vec = vec && p.H % 8 == 0 && !misaligned(p.norm, 16) && !misaligned(p.next_norm, 16) &&
+          (p.gate_step == 0 || (!misaligned(p.gate, 16) && p.gate_nb % 16 == 0));
     const int units = (p.H + gx::kBlockUnit - 1) / gx::kBlockUnit;
+    if (vec && p.k <= 32 && p.H <= gx::kRowsMaxWidth && p.H >= kStreamWidth && p.T >= kStreamRows * sms) return launch_block_rows(p, sms, stream);
     int cluster = 1;
     while (cluster < gx::kBlockMaxCluster &&
            (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads || ((int64_t)p.T * cluster * 2 <= sms && units > cluster * 64)))
@@ -166,8 +224,10 @@ int launch_block(gx::BlockParams & p, bool vec, void * stream) {
     const int per = (units + cluster - 1) / cluster;
     int threads = 64;
     while (threads < gx::kBlockMaxThreads && threads * (p.T * cluster > sms ? gx::kBlockUnits : 1) < per) threads *= 2;
-    const void * fn = cluster > 1 ? (vec ? (const void *)gx::k_block<true, true> : (const void *)gx::k_block<false, true>)
-                                  : (vec ? (const void *)gx::k_block<true, false> : (const void *)gx::k_block<false, false>);
+    const int kind = p.y.type;
+    const void * fn = kind == gx::GMM_F32   ? block_kernel<gx::GMM_F32>(vec, cluster > 1)
+                      : kind == gx::GMM_F16 ? block_kernel<gx::GMM_F16>(vec, cluster > 1)
+                                            : block_kernel<gx::GMM_BF16>(vec, cluster > 1);
     return cuda_status(launch_next(fn, dim3((unsigned)(p.T * cluster)), threads, 0, cluster, stream, p));
 }
 

@@ -7,6 +7,8 @@
 // plain (y_j = W_e x_j) or gated (act(G_e x_j, U_e x_j)).
 #pragma once
 
+#include <climits>
+
 #include "gx_gmm.cuh"
 #include "gx_q4_plan.h"
 
@@ -31,391 +33,468 @@ struct Q4Params {
     float alpha, limit;
     int32_t rt;               // tiles of a matrix's rows
     int32_t most;             // tiles of rows that the groups can have
-    int32_t entries;          // of the list of groups
+    int32_t warps;            // of a CTA
+    int32_t share;            // warps that share a job's K (a divisor of the CTA's)
+    int32_t cap;              // rows of x per tile
+    int32_t buffers;          // tiles of x in shared memory
 };
 
 // ---------------------------------------------------------------- pieces
 
-__device__ __forceinline__ void q4_copy16(uint32_t dst, const uint8_t * src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void q4_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void q4_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ uint32_t q4_lds(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
 
+__device__ __forceinline__ uint2 q4_lds2(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
+// d = a x b + c
 template <bool BF16>
-__device__ __forceinline__ void q4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                       float c0, float c1, float c2, float c3) {
     if constexpr (BF16)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // The codes of one word of a block (bytes 4t .. 4t+3: elements 4t + i in the
-// low and 16 + 4t + i in the high halves) as pairs of 16-bit floats: (0, 2),
-// (1, 3), (16, 18), (17, 19) from 4t on. A code is put into the upper bits of
-// the mantissa of 16, which gives 16 + q. (F16 codes as they stand, the
-// subnormals q 2^-24, would take one operation less, but the tensor cores add
-// products of subnormals with ten bits less: 4e-5 of the result instead of 1e-7.)
+// low halves, 16 + 4t + i in the high ones) as pairs of 16-bit floats: (0, 1),
+// (2, 3), (16, 17), (18, 19) from 4t on. A code goes into the mantissa of a
+// power of two, all of it into the low byte: 16 + q (BF16) or 64 + q (F16), the
+// high bytes are the same for all. (F16 codes as they stand, the subnormals
+// q 2^-24, would take fewer operations, but the tensor cores add products of
+// subnormals with ten bits less: 4e-5 of the result instead of 1e-7.)
+// (Left shifts are products, which run beside the units for shifts, masks and
+// byte permutations: those are what the kernel needs most.)
+__device__ __forceinline__ uint32_t q4_times(uint32_t w, uint32_t by) {
+    uint32_t v;
+    asm("mul.lo.u32 %0, %1, %2;" : "=r"(v) : "r"(w), "r"(by));
+    return v;
+}
 template <bool BF16>
 __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t (&a)[4]) {
+    uint32_t lo, hi;
     if constexpr (BF16) {
-        a[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-        a[1] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-        a[2] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-        a[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+        lo = (q4_times(w, 8u) & 0x78787878u) | 0x80808080u;
+        hi = ((w >> 1) & 0x78787878u) | 0x80808080u;
     } else {
-        a[0] = ((w << 6) & 0x03C003C0u) | 0x4C004C00u;
-        a[1] = ((w >> 2) & 0x03C003C0u) | 0x4C004C00u;
-        a[2] = ((w << 2) & 0x03C003C0u) | 0x4C004C00u;
-        a[3] = ((w >> 6) & 0x03C003C0u) | 0x4C004C00u;
+        lo = q4_times(w, 16u) & 0xF0F0F0F0u;
+        hi = w & 0xF0F0F0F0u;
     }
+    constexpr uint32_t top = BF16 ? 0x41414141u : 0x54545454u;
+    a[0] = __byte_perm(lo, top, 0x4140);
+    a[1] = __byte_perm(lo, top, 0x4342);
+    a[2] = __byte_perm(hi, top, 0x4140);
+    a[3] = __byte_perm(hi, top, 0x4342);
 }
 // What turns sums of the codes above into the wanted ones, as the A operand of
-// a product with the same x: -24 (Q4_0: sums of q - 8) or -16 (Q4_1: of q)
+// a product with the same x: -24 or -72 (Q4_0: sums of q - 8), -16 or -64 (Q4_1:
+// of q)
 template <bool BF16, bool Q41>
 __device__ __forceinline__ constexpr uint32_t q4_shift() {
-    return BF16 ? (Q41 ? 0xC180C180u : 0xC1C0C1C0u) : (Q41 ? 0xCC00CC00u : 0xCE00CE00u);
+    return BF16 ? (Q41 ? 0xC180C180u : 0xC1C0C1C0u) : (Q41 ? 0xD400D400u : 0xD480D480u);
 }
 
-__device__ __forceinline__ float q4_half(uint32_t bits) {
-    float f;
-    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(f) : "r"(bits));
-    return f;
-}
+// the halves of a word, as f32
+__device__ __forceinline__ float q4_low(uint32_t v) { return __low2float(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ float q4_high(uint32_t v) { return __high2float(*reinterpret_cast<const __half2 *>(&v)); }
 
 // ------------------------------------------------------------- the groups
 
-// The groups of a launch, in shared memory: pre[i], the tiles before group i.
+// The groups of a launch. pre[i]: the tiles of rows before group i * per
 struct Q4Groups {
     const int32_t * pre;
+    int per, n;
     const int32_t * order;    // of the rows (global memory, or shared memory for ids), NULL: as they are
     const int32_t * expert;   // of group i (ids), NULL: i
     const int32_t * start;    // first row of group i (ids), NULL: offsets, or all rows
-    int n;
 };
 
-struct Q4Job {
-    int group, m, tile;       // group, tile of the matrix's rows, tile of the group's rows
-    int e, lo, hi, tiles;     // expert, the group's rows, tiles of them
+// A tile of a group's rows
+struct Q4Tile {
+    int group, before, tiles; // group, tiles of rows before it, and its own
+    int e, row0, rows;        // expert, the tile's rows
 };
 
-__device__ __forceinline__ void q4_enter(const Q4Params & p, const Q4Groups & g, Q4Job & j) {
-    j.tiles = g.pre[j.group + 1] - g.pre[j.group];
-    if (g.start != nullptr) {
-        j.e = g.expert[j.group];
-        j.lo = g.start[j.group];
-        j.hi = g.start[j.group + 1];
-    } else {
-        j.e = j.group;
-        j.lo = p.offsets != nullptr ? p.offsets[j.group] : 0;
-        j.hi = p.offsets != nullptr ? p.offsets[j.group + 1] : p.n_rows;
+// tile `at` of rows
+__device__ __forceinline__ void q4_tile(const Q4Params & p, const Q4Groups & g, int at, Q4Tile & j) {
+    const int i = tile_group(g.pre, (int)blockDim.x, at);
+    j.group = i * g.per;
+    j.before = g.pre[i];
+    int lo, hi;
+    for (;; ++j.group) {
+        if (g.start != nullptr) {
+            lo = g.start[j.group];
+            hi = g.start[j.group + 1];
+        } else {
+            lo = p.offsets != nullptr ? p.offsets[j.group] : 0;
+            hi = p.offsets != nullptr ? p.offsets[j.group + 1] : p.n_rows;
+        }
+        j.tiles = lo < 0 || hi <= lo || hi > p.n_rows ? 0 : (hi - lo - 1) / p.cap + 1;
+        if (at < j.before + j.tiles || j.group + 1 >= g.n) break;
+        j.before += j.tiles;
     }
+    j.e = g.start != nullptr ? g.expert[j.group] : j.group;
+    // (a group's tiles are of one size, rather than full ones and a rest)
+    const int size = (hi - lo - 1) / j.tiles + 1;
+    j.row0 = lo + (at - j.before) * size;
+    j.rows = min(size, hi - j.row0);
 }
-__device__ __forceinline__ void q4_first(const Q4Params & p, const Q4Groups & g, int at, Q4Job & j) {
-    // (the tiles of a group's rows run fastest, then the matrix's, then the groups)
-    j.group = tile_group(g.pre, g.n, at / p.rt);
-    const int tiles = g.pre[j.group + 1] - g.pre[j.group], in = at - g.pre[j.group] * p.rt;
-    j.m = in / tiles;
-    j.tile = in - j.m * tiles;
-    q4_enter(p, g, j);
+// As tile_prefix, for the groups that a thread looks at together: pre[i] is of
+// group i * per, one per thread, and the last is the sum.
+template <typename F>
+__device__ __forceinline__ void q4_prefix(int32_t * pre, int32_t * wsum, int G, int per, int nt, int most, F && rows) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = blockDim.x;
+    const int cap = most + 1;
+    int sum = 0;
+    for (int g = min(tid * per, G); g < min(tid * per + per, G); ++g) {
+        const int2 r = rows(g);
+        if (r.y > r.x) sum = min(sum + (r.y - r.x - 1) / nt + 1, cap);
+    }
+    int inc = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc = min(inc + v, cap);
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int before = inc - sum;
+    for (int w = 0; w < warp; ++w) before += wsum[w];
+    pre[tid] = before;
+    if (tid == n - 1) {
+        const bool over = before + sum > most;
+        if (over) record_error(GX_DEVERR_DOMAIN);
+        pre[n] = over ? 0 : before + sum;
+    }
+    __syncthreads();
 }
-__device__ __forceinline__ void q4_next(const Q4Params & p, const Q4Groups & g, Q4Job & j) {
-    if (++j.tile < j.tiles) return;
-    j.tile = 0;
-    if (++j.m < p.rt) return;
-    j.m = 0;
-    do ++j.group;
-    while (j.group < g.n && g.pre[j.group + 1] == g.pre[j.group]);
-    if (j.group < g.n) q4_enter(p, g, j);
-}
-// rows of a job: a group's tiles are of one size, rather than full ones and a rest
-__device__ __forceinline__ int2 q4_rows(const Q4Job & j) {
-    const int size = ((j.hi - j.lo - 1) / j.tiles + 8) / 8 * 8;
-    const int lo = j.lo + j.tile * size;
-    return make_int2(lo, min(size, j.hi - lo));
-}
-
 // ------------------------------------------------------------- the kernel
 
-template <bool BF16, bool Q41, bool GLU, int NT>
-__global__ void __launch_bounds__(kQ4Threads, 1) k_q4(const __grid_constant__ Q4Params p) {
-    constexpr int MT = q4_mt(NT), CP = q4_pairs(NT), S = kQ4Stages;
-    constexpr int kBlock = Q41 ? 20 : 18, kPair = 2 * kBlock;
-    constexpr int kPitch = q4_pitch(Q41, NT), kStage = 16 * MT * kPitch;
+// the warps that share a job
+__device__ __forceinline__ void q4_sync(int team, int share) {
+    if (share == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * share) : "memory");
+}
+
+template <bool BF16, bool Q41, bool GLU>
+__global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__ Q4Params p) {
+    constexpr int MT = kQ4Mt, CP = kQ4Pairs, S = kQ4Stages;
+    constexpr int kPair = 2 * (Q41 ? 20 : 18);                      // bytes of 64 weights
+    constexpr int kPitch = q4_pitch(Q41), kStage = q4_stage_bytes(Q41);
     constexpr int kRows = GLU ? 8 * MT : 16 * MT;                   // result rows of a job
-    constexpr int kRed = q4_red_pitch(NT);
+    constexpr int kRed = kQ4Cols * kQ4Red;
     extern __shared__ __align__(128) uint8_t q4_smem_raw[];
-    __shared__ int32_t wsum[kQ4Warps];
-    __shared__ int32_t s_order[kQ4MaxIds], s_key[kQ4MaxIds], s_expert[kQ4MaxIds], s_start[kQ4MaxIds + 1];
-    __shared__ int32_t s_groups;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ int32_t wsum[kQ4Warps], pre[32 * kQ4Warps + 1];
+    __shared__ int32_t s_order[kQ4MaxIds], s_key[kQ4MaxIds], s_lead[kQ4MaxIds], s_expert[kQ4MaxIds], s_start[kQ4MaxIds + 1];
+    __shared__ uint64_t full[2], empty[2], ring_full[kQ4Warps][S];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = p.warps;
     const int g = lane >> 2, t = lane & 3;
-    float * red = reinterpret_cast<float *>(q4_smem_raw + kQ4Warps * S * kStage);
-    int32_t * pre = reinterpret_cast<int32_t *>(red + q4_buffers(NT) * kQ4Warps * 8 * NT * kRed);
+    float * red = reinterpret_cast<float *>(q4_smem_raw + W * S * kStage);
+    uint8_t * xbuf = reinterpret_cast<uint8_t *>(red + W * kRed);
+    const int x_pitch = (int)q4_x_pitch(p.K);
 
     griddep_launch_dependents();
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, (uint32_t)W);
+        }
+        for (int i = 0; i < W * S; ++i) mbar_init(&ring_full[0][0] + i, 1);
+        abort_flag = 0;
+        mbar_fence_init();
+    }
     griddep_wait();
 
-    Q4Groups gr{pre, p.order, nullptr, nullptr, p.G};
+    Q4Groups gr{pre, 1, p.G, p.order, nullptr, nullptr};
     if (p.ids != nullptr) {
         // rows by ascending expert, those of one expert in their order
-        int key = -1, at = 0, same = 0;
-        if (tid < p.n_rows) {
-            key = p.ids[tid];
+        for (int r = tid; r < kQ4MaxIds; r += blockDim.x) {
+            int key = r < p.n_rows ? p.ids[r] : -1;
             if (key >= p.G) {
                 record_error(GX_DEVERR_DOMAIN);
                 key = -1;
             }
+            s_key[r] = key < 0 ? INT_MAX : key;
         }
-        if (tid < kQ4MaxIds) s_key[tid] = key;
+        if (tid == 0) wsum[0] = wsum[1] = 0;
         __syncthreads();
-        if (key >= 0) {
+        for (int r = tid; r < p.n_rows; r += blockDim.x) {
+            const int key = s_key[r];
+            int at = 0, same = 0;
             for (int i = 0; i < p.n_rows; ++i) {
-                const int k = s_key[i];
-                at += k >= 0 && k < key;
-                same += k == key && i < tid;
+                at += s_key[i] < key;
+                same += s_key[i] == key && i < r;
             }
-            s_order[at + same] = tid;
+            s_lead[r] = same == 0 ? key : INT_MAX;                  // (the first row of each expert)
+            s_order[at + same] = r;                                 // (rows of no expert come last)
+            if (key == INT_MAX) continue;
+            atomicAdd(&wsum[0], 1);
+            if (same == 0) atomicAdd(&wsum[1], 1);
         }
         __syncthreads();
-        if (same != 0) s_key[tid] = -1;           // only the first of each expert counts now
-        const int rows = __syncthreads_count(key >= 0);
-        const int groups = __syncthreads_count(key >= 0 && same == 0);
-        if (key >= 0 && same == 0) {
-            int i = 0;
-            for (int k = 0; k < p.n_rows; ++k) i += s_key[k] >= 0 && s_key[k] < key;
-            s_expert[i] = key;
-            s_start[i] = at;
+        for (int r = tid; r < p.n_rows; r += blockDim.x) {
+            const int key = s_lead[r];
+            if (key == INT_MAX) continue;
+            int n = 0, at = 0;
+            for (int i = 0; i < p.n_rows; ++i) {
+                n += s_lead[i] < key;
+                at += s_key[i] < key;
+            }
+            s_expert[n] = key;
+            s_start[n] = at;
         }
-        if (tid == 0) {
-            s_start[groups] = rows;
-            s_groups = groups;
-        }
+        gr.n = wsum[1];
+        if (tid == 0) s_start[gr.n] = wsum[0];
         __syncthreads();
-        gr.n = s_groups;
         gr.order = s_order;
         gr.expert = s_expert;
         gr.start = s_start;
-        tile_prefix(pre, wsum, gr.n, 8 * NT, p.most, [&](int i) { return make_int2(s_start[i], s_start[i + 1]); });
+        gr.per = 1 + (gr.n - 1) / (int)blockDim.x;
+        q4_prefix(pre, wsum, gr.n, gr.per, p.cap, p.most, [&](int i) { return make_int2(s_start[i], s_start[i + 1]); });
     } else if (p.offsets != nullptr) {
-        tile_prefix(pre, wsum, p.G, 8 * NT, p.most, [&](int i) { return group_rows_of(p.offsets, i, p.n_rows); });
+        gr.per = (p.G + (int)blockDim.x - 1) / (int)blockDim.x;
+        q4_prefix(pre, wsum, p.G, gr.per, p.cap, p.most, [&](int i) { return group_rows_of(p.offsets, i, p.n_rows); });
     } else {
-        tile_prefix(pre, wsum, 1, 8 * NT, p.most, [&](int) { return make_int2(0, p.n_rows); });
+        q4_prefix(pre, wsum, 1, 1, p.cap, p.most, [&](int) { return make_int2(0, p.n_rows); });
     }
-    const int jobs = pre[gr.n] * p.rt;
+
+    // The CTA's run of jobs: tiles of rows, each with tiles of its matrix. Teams
+    // of warps take the matrix tiles in turn, each warp a share of K.
+    const int jobs = pre[blockDim.x] * p.rt;
     const int j0 = (int)((int64_t)jobs * blockIdx.x / gridDim.x), j1 = (int)((int64_t)jobs * (blockIdx.x + 1) / gridDim.x);
     if (j0 == j1) return;
-
-    // this warp's share of K, in pairs of blocks
+    const int share = p.share, team = warp / share, member = warp - team * share, teams = W / share;
     const int pairs = p.K / 64;
-    const int p0 = (int)((int64_t)pairs * warp / kQ4Warps), p1 = (int)((int64_t)pairs * (warp + 1) / kQ4Warps);
-    const uint32_t ring = smem_u32(q4_smem_raw) + (uint32_t)warp * (S * kStage);
+    const int p0 = pairs * member / share, p1 = pairs * (member + 1) / share;
+    uint8_t * const ring_base = q4_smem_raw + warp * (S * kStage);
+    const uint32_t ring = smem_u32(ring_base);
+    uint64_t * const filled = ring_full[warp];
+    const int t0 = j0 / p.rt, t1 = (j1 - 1) / p.rt;                 // tiles of rows of the run
+    auto m_begin = [&](int tile) { return tile == t0 ? j0 - t0 * p.rt : 0; };
+    auto m_end = [&](int tile) { return tile == t1 ? j1 - t1 * p.rt : p.rt; };
 
     // ------------------------------------------------- the stream of chunks
-    Q4Job ahead;
-    q4_first(p, gr, j0, ahead);
-    int ahead_job = j0, ahead_pair = p0, put = 0;
-    const int sub = lane >> 3, col = lane & 7;
+    Q4Tile ahead;
+    int ahead_tile = t0, ahead_m = m_begin(t0) + team, ahead_pair = p0, put = 0, issued = 0;
+    auto ahead_enter = [&] {                                        // on to the team's next job
+        while (ahead_tile <= t1 && ahead_m >= m_end(ahead_tile)) {
+            ++ahead_tile;
+            ahead_m = team;
+            if (ahead_tile <= t1) q4_tile(p, gr, ahead_tile, ahead);
+        }
+    };
+    q4_tile(p, gr, t0, ahead);
+    Q4Tile job = ahead;
+    ahead_enter();
+    // A lane copies the chunk's piece of one row: rows 16 m + 8 h + g of the tile,
+    // from 16 bytes before their first one on. (The last piece of the last row
+    // ends with the matrix: what is not whole 16 bytes is moved by hand.)
+    const bool second = GLU && (lane & 8);
+    const int lane_row = GLU ? (lane >> 4) * 8 + (lane & 7) : lane;
+    const uint8_t * const w_lane = second ? p.w1 : p.w0;
+    const uint8_t * const w_end = w_lane + (int64_t)(p.G - 1) * p.nb02 + (int64_t)(p.N - 1) * p.nb01 + (int64_t)(p.K / 64) * kPair;
     auto issue = [&] {
-        if (ahead_job < j1 && p0 < p1) {
-            const int n = min(CP, p1 - ahead_pair), bytes = n * kPair;
-            const uint32_t to = ring + (uint32_t)put * kStage;
-            const int64_t base = (int64_t)ahead.e * p.nb02 + (int64_t)ahead_pair * kPair;
-            const int r0 = ahead.m * kRows;
-#pragma unroll
-            for (int i = 0; i < 4 * MT; ++i) {
-                const int s = 4 * i + sub;                         // row of the tile: 16 m + 8 h + g
-                const int row = min(GLU ? r0 + (s >> 4) * 8 + (s & 7) : r0 + s, p.N - 1);
-                const uint8_t * a = (GLU && ((s >> 3) & 1) ? p.w1 : p.w0) + base + (int64_t)row * p.nb01;
-                const int skew = (int)(reinterpret_cast<uintptr_t>(a) & 15u), need = skew + bytes;
-                const uint8_t * from = a - skew;
-                const uint32_t at = to + (uint32_t)(s * kPitch);
-#pragma unroll
-                for (int c = 0; c < (CP * kPair + 12 + 127) / 128; ++c) {
-                    const int off = (c * 8 + col) * 16;
-                    if (off < need) q4_copy16(at + (uint32_t)off, from + off, min(16, need - off));
-                }
+        if (ahead_tile <= t1 && p0 < p1) {
+            const int n = min(CP, p1 - ahead_pair), row = ahead_m * kRows + lane_row;
+            const uint8_t * a = w_lane + (int64_t)ahead.e * p.nb02 + (int64_t)row * p.nb01 + (int64_t)ahead_pair * kPair;
+            const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(a) & 15u;
+            uint32_t bytes = row < p.N ? (skew + (uint32_t)(n * kPair) + 15u) & ~15u : 0u;     // (rows behind the last: nothing)
+            const uint8_t * from = a - skew;
+            uint8_t * to = ring_base + put * kStage + lane * kPitch;
+            if (bytes != 0u && from + bytes > w_end) {
+                bytes -= 16u;
+                for (const uint8_t * b = from + bytes; b < w_end; b += 4)
+                    *reinterpret_cast<uint32_t *>(to + (b - from)) = *reinterpret_cast<const uint32_t *>(b);
             }
+            const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
+            if (lane == 0) mbar_arrive_expect_tx(filled + put, sum);
+            __syncwarp();
+            if (bytes != 0u) bulk_g2s(to, from, bytes, filled + put);
             put = put + 1 == S ? 0 : put + 1;
+            ++issued;
             ahead_pair += n;
             if (ahead_pair >= p1) {
                 ahead_pair = p0;
-                if (++ahead_job < j1) q4_next(p, gr, ahead);
+                ahead_m += teams;
+                ahead_enter();
             }
         }
-        q4_commit();
     };
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) issue();
+    for (int i = 0; i < S; ++i) issue();
+
+    // ------------------------------------------------------ the tiles of x
+    // Warp 0 copies the rows of tile i of the run, a lane a row.
+    auto fetch = [&](const Q4Tile & j, int b) {
+        if (lane == 0) mbar_arrive_expect_tx(full + b, (uint32_t)(j.rows * 2 * p.K));
+        __syncwarp();
+        if (lane < j.rows) {
+            int row = j.row0 + lane;
+            if (p.gather != 0) {
+                const int o = gr.order[row];
+                row = o / p.gather;
+                if (o < 0 || row >= p.x_rows) row = 0;              // (its results are NaN)
+            }
+            bulk_g2s(xbuf + (b * p.cap + lane) * x_pitch, p.x + (int64_t)row * p.nb11, (uint32_t)(2 * p.K), full + b);
+        }
+    };
+    int fetched = 1;
+    if (warp == 0) fetch(job, 0);
 
     // ------------------------------------------------------------ the jobs
-    Q4Job job;
-    q4_first(p, gr, j0, job);
-    int take = 0, last_group = -1, last_tile = -1;
-    const uint8_t * xp[NT];
+    int take = 0;
+    uint32_t round = 0;
+    bool ok = true;
     const uint32_t shift = q4_shift<BF16, Q41>();
-    for (int jb = j0; jb < j1; ++jb, q4_next(p, gr, job)) {
-        const int2 rows = q4_rows(job);
-        const int used = (rows.y + 7) / 8;                          // tiles of eight columns
-        if (job.group != last_group || job.tile != last_tile) {
-            last_group = job.group;
-            last_tile = job.tile;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int j = rows.x + min(n * 8 + g, rows.y - 1);
-                int row = j;
-                if (p.gather != 0) {
-                    const int o = gr.order[j];
-                    row = o / p.gather;
-                    if (o < 0 || row >= p.x_rows) row = 0;          // (its result is NaN)
-                }
-                xp[n] = p.x + (int64_t)row * p.nb11 + t * 8;
-            }
+    for (int tile = t0; tile <= t1; ++tile) {
+        const int i_tile = tile - t0, b = p.buffers == 2 ? i_tile & 1 : 0;
+        Q4Tile next = job;
+        if (tile < t1) q4_tile(p, gr, tile + 1, next);
+        // the next tile of x, once its buffer is no longer read
+        if (p.buffers == 2 && warp == 0 && tile < t1) {
+            if (i_tile >= 1) ok = ok && gmm_wait<1>(empty + (b ^ 1), (uint32_t)(((i_tile - 1) >> 1) & 1), &abort_flag);
+            if (ok) fetch(next, b ^ 1);
+            fetched += ok;
         }
-        // where the rows of the tile start inside their 16 bytes
-        uint32_t low[MT][2];
-        {
-            const uint32_t e = (uint32_t)job.e * (uint32_t)p.nb02;
+        // (a wait that runs out makes all that follows NaN; teams stay together)
+        ok = gmm_wait<1>(full + b, (uint32_t)((p.buffers == 2 ? i_tile >> 1 : i_tile) & 1), &abort_flag) && ok;
+        // (columns behind the last row repeat it)
+        const uint32_t xs = smem_u32(xbuf) + (uint32_t)((b * p.cap + min(g, job.rows - 1)) * x_pitch + t * 8);
+        for (int m = m_begin(tile) + team; m < m_end(tile); m += teams) {
+            // where the lane's rows start inside their 16 bytes (rows 8 apart agree)
+            const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(p.w0) + (uint32_t)job.e * (uint32_t)p.nb02 +
+                                 (uint32_t)(m * kRows + g) * (uint32_t)p.nb01;
+            float acc[MT][2][2];                                   // [tile][half][column]
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = min(job.m * kRows + (GLU ? 8 * m + g : 16 * m + 8 * h + g), p.N - 1);
-                    low[m][h] = (uint32_t)reinterpret_cast<uintptr_t>(GLU && h ? p.w1 : p.w0) + e + (uint32_t)row * (uint32_t)p.nb01;
-                }
-        }
-        uint64_t acc[MT][NT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = 0ull;
+            for (int i = 0; i < MT; ++i) acc[i][0][0] = acc[i][0][1] = acc[i][1][0] = acc[i][1][1] = 0.0f;
 
-        for (int q0 = p0; q0 < p1; q0 += CP) {
-            issue();
-            q4_wait<S - 1>();
-            __syncwarp();
-            const uint32_t st = ring + (uint32_t)take * kStage;
-            uint32_t at[MT][2];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    at[m][h] = st + (uint32_t)((16 * m + 8 * h + g) * kPitch) + ((low[m][h] + (uint32_t)(q0 * kPair)) & 15u);
-            const int n_pairs = min(CP, p1 - q0);
+            for (int q0 = p0; q0 < p1; q0 += CP) {
+                ok = gmm_wait<1>(filled + take, round, &abort_flag) && ok;
+                const uint32_t at = ring + (uint32_t)(take * kStage + g * kPitch) + ((low + (uint32_t)(q0 * kPair)) & 15u);
+                const int n_pairs = min(CP, p1 - q0);
 #pragma unroll 2
-            for (int q = 0; q < n_pairs; ++q) {
-                // codes and scales of two blocks of the tile's rows
-                uint32_t a[MT][2][2][4];                            // [tile][block][half][pair of codes]
-                float d[MT][2][2], mn[MT][2][2];
+                for (int q = 0; q < n_pairs; ++q) {
+                    // x: elements 4t .. and 16 + 4t .. of two blocks
+                    uint2 x[4];
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                    for (int i = 0; i < 4; ++i) x[i] = q4_lds2(xs + (uint32_t)((q0 + q) * 128 + i * 32));
+                    // codes and scales of two blocks of the tile's rows
+                    uint32_t a[MT][2][2][4];                        // [tile][block][half][pair of codes]
+                    float d[MT][2][2], mn[MT][2][2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t b = at[m][h] + (uint32_t)(q * kPair);
-                        if constexpr (Q41) {
-                            const uint32_t s0 = q4_lds(b), s1 = q4_lds(b + 20u);
-                            q4_codes<BF16>(q4_lds(b + 4u + 4u * t), a[m][0][h]);
-                            q4_codes<BF16>(q4_lds(b + 24u + 4u * t), a[m][1][h]);
-                            d[m][0][h] = q4_half(s0 & 0xFFFFu);
-                            mn[m][0][h] = q4_half(s0 >> 16);
-                            d[m][1][h] = q4_half(s1 & 0xFFFFu);
-                            mn[m][1][h] = q4_half(s1 >> 16);
-                            mn[m][0][h] *= -0.0625f;                // (sum x comes as -16 sum x)
-                            mn[m][1][h] *= -0.0625f;
-                        } else {
-                            const uint32_t s0 = q4_lds(b), s1 = q4_lds(b + 16u);
-                            const uint32_t w0 = q4_lds(b + 4u * t), w1 = q4_lds(b + 4u + 4u * t);
-                            q4_codes<BF16>(__byte_perm(w0, w1, 0x5432), a[m][0][h]);
-                            q4_codes<BF16>(q4_lds(b + 20u + 4u * t), a[m][1][h]);
-                            d[m][0][h] = q4_half(s0 & 0xFFFFu);
-                            d[m][1][h] = q4_half(s1 >> 16);
-                        }
-                    }
-                const int64_t xo = (int64_t)(q0 + q) * 128;
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (NT > 1 && n >= used) break;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint2 lo = __ldg(reinterpret_cast<const uint2 *>(xp[n] + xo + b * 64));
-                        const uint2 hi = __ldg(reinterpret_cast<const uint2 *>(xp[n] + xo + b * 64 + 32));
-                        const uint32_t l0 = __byte_perm(lo.x, lo.y, 0x5410), l1 = __byte_perm(lo.x, lo.y, 0x7632);
-                        const uint32_t h0 = __byte_perm(hi.x, hi.y, 0x5410), h1 = __byte_perm(hi.x, hi.y, 0x7632);
-                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        q4_mma<BF16>(s, shift, shift, shift, shift, l0, l1);
-                        q4_mma<BF16>(s, shift, shift, shift, shift, h0, h1);
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            float c[4] = {s[0], s[1], s[2], s[3]};
-                            q4_mma<BF16>(c, a[m][b][0][0], a[m][b][1][0], a[m][b][0][1], a[m][b][1][1], l0, l1);
-                            q4_mma<BF16>(c, a[m][b][0][2], a[m][b][1][2], a[m][b][0][3], a[m][b][1][3], h0, h1);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                acc[m][n][h] = fma_x2(f2pack(d[m][b][h], d[m][b][h]), f2pack(c[2 * h], c[2 * h + 1]), acc[m][n][h]);
-                                if constexpr (Q41)
-                                    acc[m][n][h] = fma_x2(f2pack(mn[m][b][h], mn[m][b][h]), f2pack(s[0], s[1]), acc[m][n][h]);
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t r = at + (uint32_t)((16 * i + 8 * h) * kPitch) + (uint32_t)(q * kPair);
+                            if constexpr (Q41) {
+                                const uint32_t s0 = q4_lds(r), s1 = q4_lds(r + 20u);
+                                q4_codes<BF16>(q4_lds(r + 4u + 4u * t), a[i][0][h]);
+                                q4_codes<BF16>(q4_lds(r + 24u + 4u * t), a[i][1][h]);
+                                constexpr float unit = BF16 ? -0.0625f : -0.015625f;       // (sum x comes as -16 or -64 of it)
+                                d[i][0][h] = q4_low(s0);
+                                mn[i][0][h] = __fmul_rn(unit, q4_high(s0));
+                                d[i][1][h] = q4_low(s1);
+                                mn[i][1][h] = __fmul_rn(unit, q4_high(s1));
+                            } else {
+                                const uint32_t s0 = q4_lds(r), s1 = q4_lds(r + 16u);
+                                const uint32_t w0 = q4_lds(r + 4u * t), w1 = q4_lds(r + 4u + 4u * t);
+                                q4_codes<BF16>(__byte_perm(w0, w1, 0x5432), a[i][0][h]);
+                                q4_codes<BF16>(q4_lds(r + 20u + 4u * t), a[i][1][h]);
+                                d[i][0][h] = q4_low(s0);
+                                d[i][1][h] = q4_high(s1);
                             }
                         }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint2 lo = x[2 * k], hi = x[2 * k + 1];
+                        float s[4];
+                        q4_mma<BF16>(s, shift, shift, shift, shift, lo.x, lo.y, 0.0f, 0.0f, 0.0f, 0.0f);
+                        q4_mma<BF16>(s, shift, shift, shift, shift, hi.x, hi.y, s[0], s[1], s[2], s[3]);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            float c[4];
+                            q4_mma<BF16>(c, a[i][k][0][0], a[i][k][1][0], a[i][k][0][1], a[i][k][1][1], lo.x, lo.y, s[0], s[1], s[2], s[3]);
+                            q4_mma<BF16>(c, a[i][k][0][2], a[i][k][1][2], a[i][k][0][3], a[i][k][1][3], hi.x, hi.y, c[0], c[1], c[2], c[3]);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int v = 0; v < 2; ++v) {
+                                    acc[i][h][v] = __fmaf_rn(d[i][k][h], c[2 * h + v], acc[i][h][v]);
+                                    if constexpr (Q41) acc[i][h][v] = __fmaf_rn(mn[i][k][h], s[v], acc[i][h][v]);
+                                }
+                        }
                     }
                 }
+                if (++take == S) {
+                    take = 0;
+                    round ^= 1u;
+                }
+                __syncwarp();
+                if (ok) issue();
             }
-            take = take + 1 == S ? 0 : take + 1;
-            __syncwarp();
-        }
 
-        // ------------------------------- the warps' sums, added in their order
-        float * part = red + (q4_buffers(NT) == 2 ? jb & 1 : 0) * (kQ4Warps * 8 * NT * kRed);
-        float * mine = part + warp * (8 * NT * kRed);
+            // --------------------------- the warps' sums, added in their order
+            float * part = red + team * share * kRed;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (NT > 1 && n >= used) break;
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float v0, v1;
-                    f2unpack(acc[m][n][h], v0, v1);
-                    float * to = mine + (n * 8 + 2 * t) * kRed + 16 * m + 8 * h + g;
-                    to[0] = v0;
-                    to[kRed] = v1;
+                    float * to = part + member * kRed + 2 * t * kQ4Red + 16 * i + 8 * h + g;
+                    to[0] = acc[i][h][0];
+                    to[kQ4Red] = acc[i][h][1];
                 }
+            q4_sync(team, share);
+            for (int i = member * 32 + lane; i < kRows * job.rows; i += 32 * share) {
+                const int c = i / kRows, r = i - c * kRows;         // (kRows is a power of two)
+                const int row = m * kRows + r;
+                if (row >= p.N) continue;
+                const float * from = part + c * kQ4Red + (GLU ? (r >> 3) * 16 + (r & 7) : r);
+                float v = from[0], u = GLU ? from[8] : 0.0f;
+                for (int w = 1; w < share; ++w) {
+                    v = __fadd_rn(v, from[w * kRed]);
+                    if (GLU) u = __fadd_rn(u, from[w * kRed + 8]);
+                }
+                if (GLU) {
+                    float gv[1] = {v}, uv[1] = {u};
+                    gmm_act_all<1>(p, gv, uv);
+                    v = gv[0];
+                }
+                const int j = job.row0 + c;
+                bool nan = false;
+                const int to = gmm_dst_row(p, j, gr.order != nullptr ? gr.order[j] : j, nan);
+                if (nan && r == 0) record_error(GX_DEVERR_DOMAIN);
+                if (to >= 0) store_out(p.dst + (int64_t)to * p.nbd1, row, nan || !ok ? kNan : v, p.out);
             }
-        __syncthreads();
-        for (int i = tid; i < kRows * rows.y; i += kQ4Threads) {
-            const int c = i / kRows, r = i - c * kRows;             // (kRows is a power of two)
-            const int row = job.m * kRows + r;
-            if (row >= p.N) continue;
-            const float * from = part + c * kRed + (GLU ? (r >> 3) * 16 + (r & 7) : r);
-            float v = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kQ4Warps; ++w) {
-                v = __fadd_rn(v, from[w * (8 * NT * kRed)]);
-                if (GLU) u = __fadd_rn(u, from[w * (8 * NT * kRed) + 8]);
-            }
-            if (GLU) {
-                float gv[1] = {v}, uv[1] = {u};
-                gmm_act_all<1>(p, gv, uv);
-                v = gv[0];
-            }
-            const int j = rows.x + c;
-            bool nan = false;
-            const int to = gmm_dst_row(p, j, gr.order != nullptr ? gr.order[j] : j, nan);
-            if (nan && r == 0) record_error(GX_DEVERR_DOMAIN);
-            if (to >= 0) store_out(p.dst + (int64_t)to * p.nbd1, row, nan ? kNan : v, p.out);
+            q4_sync(team, share);
         }
-        if (q4_buffers(NT) == 1) __syncthreads();
+        // this warp is done with the tile of x
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(empty + b)) : "memory");
+        if (p.buffers == 1 && warp == 0 && tile < t1) {
+            ok = ok && gmm_wait<1>(empty + b, (uint32_t)(i_tile & 1), &abort_flag);
+            if (ok) fetch(next, 0);
+            fetched += ok;
+        }
+        job = next;
+    }
+    // copies in flight land before the CTA leaves
+    volatile int none = 0;
+    for (int i = 0; i < S && !ok; ++i)
+        if (issued > i) gmm_wait<1>(filled + i, (uint32_t)((issued - 1 - i) / S & 1), &none);
+    if (!ok && warp == 0) {
+        const int i = fetched - 1;
+        gmm_wait<1>(full + (p.buffers == 2 ? i & 1 : 0), (uint32_t)((p.buffers == 2 ? i >> 1 : i) & 1), &none);
     }
 }
 

@@ -7,23 +7,48 @@
 namespace gx {
 
 constexpr int kQ4MaxIds = 256;                 // rows of a call that names each row's expert (one thread a row)
-constexpr int kQ4Warps = 8;                    // they share K
-constexpr int kQ4Threads = 32 * kQ4Warps;
-constexpr int kQ4Stages = 3;
 
-// Of NT tiles of eight columns (rows of x): tiles of 16 matrix rows per job,
-// pairs of blocks per stage, bytes between the stage's rows (an odd number of 16
-// bytes: eight rows then lie in different banks; 12 bytes more than the blocks
-// take, as rows start on any 4 bytes)
-GX_HD constexpr int q4_mt(int nt) { return nt == 1 ? 1 : 2; }
-GX_HD constexpr int q4_pairs(int nt) { return nt == 1 ? 8 : 4; }
-GX_HD constexpr int q4_pitch(bool q41, int nt) { return nt == 1 ? (q41 ? 336 : 304) : 176; }
-GX_HD constexpr int q4_red_pitch(int nt) { return 16 * q4_mt(nt) + 4; }
-// partial sums of the warps: two buffers where they are small
-GX_HD constexpr int q4_buffers(int nt) { return nt == 1 ? 2 : 1; }
-GX_HD constexpr uint32_t q4_smem(bool q41, int nt, int entries) {
-    return (uint32_t)(kQ4Warps * kQ4Stages * 16 * q4_mt(nt) * q4_pitch(q41, nt)) +
-           (uint32_t)(q4_buffers(nt) * kQ4Warps * 8 * nt * q4_red_pitch(nt) * 4) + (uint32_t)(entries + 1) * 4u;
+#ifndef GX_Q4_S
+#define GX_Q4_S 2
+#define GX_Q4_P 8
+#define GX_Q4_W 8
+#endif
+
+constexpr int kQ4Warps = GX_Q4_W;              // of a CTA, at most
+constexpr int kQ4Stages = GX_Q4_S;             // of a warp's ring
+constexpr int kQ4Pairs = GX_Q4_P;              // pairs of blocks per stage
+constexpr int kQ4Mt = 2;                       // 16-row tiles of the matrix per job
+constexpr int kQ4Cols = 8;                     // rows of x per job
+
+// Bytes between the rows of a stage: an odd number of 16 bytes (eight rows then
+// lie in different banks), 12 more than the blocks take (rows start on any 4 bytes)
+GX_HD constexpr int q4_pitch(bool q41) { return 16 * (((kQ4Pairs * (q41 ? 40 : 36) + 12 + 15) / 16) | 1); }
+GX_HD constexpr int q4_stage_bytes(bool q41) { return 16 * kQ4Mt * q4_pitch(q41); }
+// A warp's sums: [columns][kQ4Red]
+constexpr int kQ4Red = 16 * kQ4Mt + 4;
+GX_HD constexpr uint32_t q4_warp_bytes(bool q41) { return (uint32_t)(kQ4Stages * q4_stage_bytes(q41) + kQ4Cols * kQ4Red * 4); }
+// a row of x (the 32 bytes more put four rows into different banks)
+GX_HD constexpr int64_t q4_x_pitch(int64_t K) { return 2 * K + 32; }
+// dynamic shared memory; the lists that the kernel declares itself take 8 KB
+constexpr uint32_t kQ4Smem = (227u - 8u) * 1024u;
+
+struct Q4Shape {
+    int warps, cap, buffers;                   // warps of a CTA, rows of x per tile, tiles of x at once
+};
+// As many warps as leave room for two tiles of x (or one; or fewer rows, which
+// only very long rows need)
+inline Q4Shape q4_shape(bool q41, int64_t K, int64_t n_rows) {
+    const int64_t row = q4_x_pitch(K);
+    const int cols = n_rows < kQ4Cols ? (int)n_rows : kQ4Cols;
+    const int step = kQ4Warps / 2;
+    for (int w = kQ4Warps; w >= step; w -= step)
+        for (int b = 2; b >= 1; --b)
+            if (w * (int64_t)q4_warp_bytes(q41) + b * cols * row <= kQ4Smem) return {w, cols, b};
+    const int64_t room = (int64_t)kQ4Smem - step * (int64_t)q4_warp_bytes(q41);
+    return {step, (int)(room / row), 1};
+}
+GX_HD constexpr uint32_t q4_smem(bool q41, int64_t K, int warps, int cap, int buffers) {
+    return (uint32_t)warps * q4_warp_bytes(q41) + (uint32_t)(buffers * cap * q4_x_pitch(K));
 }
 
 }  // namespace gx

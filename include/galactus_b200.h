@@ -393,11 +393,12 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
  *   neither  n_as = 1: all n_rows rows with the one matrix (a dense projection)
  * Offsets, row indexes and what is reported: as gx_mul_mat_grouped. A row of b
  * with an infinity or a NaN makes its own results NaN, and no other.
- * Requires ne00 % 64 == 0; 16-byte aligned as, b and nb11; nb01 and nb02
+ * Requires ne00 % 64 == 0, ne00 <= GX_Q4_MAX_K; 16-byte aligned as, b and nb11; nb01 and nb02
  * multiples of 4; n_as <= 8192. dst may not overlap an input. The calls follow
  * one another on a stream without a gap (programmatic launches), can be
  * captured, allocate nothing and keep nothing. */
 #define GX_Q4_MAX_IDS 256
+#define GX_Q4_MAX_K 65536
 int gx_mul_mat_q4(int type, const void * as, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02, int64_t n_as, int type_b,
                   const void * b, int64_t ne11, int64_t nb11, const int32_t * ids, const int32_t * offsets, const int32_t * order,
                   int64_t n_rows, int64_t gather, int scatter, int type_dst, void * dst, int64_t nbd1, void * stream);
