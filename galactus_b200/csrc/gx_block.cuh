@@ -36,6 +36,7 @@ struct BlockParams {
     int32_t has_norm, has_next;
     float eps, next_eps, scale;
     float one;                // 1 (see block_add)
+    float per;                // 1 / H
     const float * gate;       // or NULL
     int64_t gate_nb;          // 0: one row for all
     int32_t gate_step;        // 1: a value per element; 0: one per row
@@ -153,9 +154,9 @@ __device__ __forceinline__ float block_pair_sum(uint64_t v) {
     f2unpack(v, a, b);
     return __fadd_rn(a, b);
 }
-__device__ __forceinline__ float block_inverse_root(float ss, int H, float eps) {
-    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)H), eps)));
-}
+// 1 / sqrt(ss / H + eps). CUDA's rsqrtf is within 2 steps of f32; a rounded root
+// and quotient take 100 operations more, a quarter of a row's in the norm alone.
+__device__ __forceinline__ float block_inverse_root(float ss, float per, float eps) { return rsqrtf(__fmaf_rn(ss, per, eps)); }
 __device__ __forceinline__ float block_sigmoid(float g) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-g))); }
 // the gate of a row's elements i .. i + 7, times m
 template <bool VEC>
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
         ss = block_squares(m[u], ss);
     }
     float inv = 1.0f;
-    if (p.has_norm) inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[0], ctas[0]), p.H, p.eps);
+    if (p.has_norm) inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[0], ctas[0]), p.per, p.eps);
     ss = 0ull;
 #pragma unroll
     for (int u = 0; u < kBlockUnits; ++u) {
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
         if (p.dst.p != nullptr) block_store<VEC>(p.dst.p + (int64_t)t * p.dst.nb, p.dst.type, i, p.H, m[u]);
     }
     if (!p.has_next) return;
-    inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[1], ctas[1]), p.H, p.next_eps);
+    inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[1], ctas[1]), p.per, p.next_eps);
 #pragma unroll
     for (int u = 0; u < kBlockUnits; ++u) {
         const int i = first + u * step;
@@ -315,11 +316,14 @@ constexpr int kRowsMaxSlots = 32;
 constexpr int kRowsMaxWarps = 16;                 // of them that compute
 constexpr int kRowsMaxWidth = 32 * kRowsMaxWarps * kBlockUnit * kBlockUnits;
 
+// CTAs per SM of up to `warps` computing warps
+GX_HD constexpr int rows_ctas(int warps) { return warps <= 8 ? 3 : 1; }
+
 // The same for many rows: persistent CTAs, one warp copies the rows of the
 // tokens ahead into a ring of slots (one bulk copy a row), the others add them up
 // as they arrive. p.k <= 32, aligned rows.
-template <int YT>
-__global__ void __launch_bounds__(32 * (kRowsMaxWarps + 1)) k_block_rows(const __grid_constant__ BlockParams p, int slots, int slot_bytes) {
+template <int YT, int MAXW>
+__global__ void __launch_bounds__(32 * (MAXW + 1), rows_ctas(MAXW)) k_block_rows(const __grid_constant__ BlockParams p, int slots, int slot_bytes) {
     extern __shared__ __align__(128) uint8_t block_ring[];
     __shared__ uint64_t full[kRowsMaxSlots], empty[kRowsMaxSlots];
     __shared__ float sums[4][kRowsMaxWarps];
@@ -377,12 +381,11 @@ __global__ void __launch_bounds__(32 * (kRowsMaxWarps + 1)) k_block_rows(const _
 
     const int first = tid * kBlockUnit, step = W * 32 * kBlockUnit;
     auto there = [&](int u) { return first + u * step < p.H; };
-    uint64_t nw[kBlockUnits][kBlockPairs], xw[kBlockUnits][kBlockPairs];
+    uint64_t xw[kBlockUnits][kBlockPairs];
 #pragma unroll
     for (int u = 0; u < kBlockUnits; ++u) {
 #pragma unroll
-        for (int j = 0; j < kBlockPairs; ++j) nw[u][j] = xw[u][j] = f2pack(1.0f, 1.0f);
-        if (there(u) && p.norm != nullptr) block_load<true>(reinterpret_cast<const uint8_t *>(p.norm), GMM_F32, first + u * step, p.H, nw[u]);
+        for (int j = 0; j < kBlockPairs; ++j) xw[u][j] = f2pack(1.0f, 1.0f);
         if (there(u) && p.next_norm != nullptr) block_load<true>(reinterpret_cast<const uint8_t *>(p.next_norm), GMM_F32, first + u * step, p.H, xw[u]);
     }
     // the next row of the ring, as f32
@@ -436,11 +439,14 @@ __global__ void __launch_bounds__(32 * (kRowsMaxWarps + 1)) k_block_rows(const _
             uint64_t ss = 0ull;
 #pragma unroll
             for (int u = 0; u < kBlockUnits; ++u) ss = block_squares(m[u], ss);
-            const float inv = block_inverse_root(sum(block_pair_sum(ss), sums[turn]), p.H, p.eps);
+            const float inv = block_inverse_root(sum(block_pair_sum(ss), sums[turn]), p.per, p.eps);
 #pragma unroll
             for (int u = 0; u < kBlockUnits; ++u) {
+                if (!there(u)) continue;
+                uint64_t nw[kBlockPairs];
+                block_load<true>(reinterpret_cast<const uint8_t *>(p.norm), GMM_F32, first + u * step, p.H, nw);
                 block_scale(m[u], inv);
-                block_scale(m[u], nw[u]);
+                block_scale(m[u], nw);
             }
         }
         if (p.gate != nullptr) {
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(32 * (kRowsMaxWarps + 1)) k_block_rows(const _
             if (p.dst.p != nullptr && there(u)) block_store<true>(p.dst.p + (int64_t)t * p.dst.nb, p.dst.type, first + u * step, p.H, m[u]);
         }
         if (!p.has_next) continue;
-        const float inv = block_inverse_root(sum(block_pair_sum(ss), sums[turn + 1]), p.H, p.next_eps);
+        const float inv = block_inverse_root(sum(block_pair_sum(ss), sums[turn + 1]), p.per, p.next_eps);
 #pragma unroll
         for (int u = 0; u < kBlockUnits; ++u) {
             if (!there(u)) continue;

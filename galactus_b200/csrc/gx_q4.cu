@@ -178,9 +178,9 @@ const void * block_kernel(bool vec, bool cluster) {
 
 template <int YT>
 int launch_block_rows(gx::BlockParams & p, int grid, int warps, int slots, int slot_bytes, void * stream) {
-    const void * fn = (const void *)gx::k_block_rows<YT>;
+    const void * fn = warps <= 8 ? (const void *)gx::k_block_rows<YT, 8> : (const void *)gx::k_block_rows<YT, gx::kRowsMaxWarps>;
     const uint32_t smem = (uint32_t)(slots * slot_bytes);
-    cudaError_t e = allow_smem(fn, 8 + YT, kStreamSmem);
+    cudaError_t e = allow_smem(fn, 8 + YT + (warps <= 8 ? 0 : 3), kStreamSmem);
     if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
@@ -199,7 +199,7 @@ int launch_block_rows(gx::BlockParams & p, int sms, void * stream) {
     const auto size = [](const gx::BlockRows & r) { return r.p == nullptr ? 0 : r.type == gx::GMM_F32 ? 4 : 2; };
     const int slot_bytes = (p.H * std::max(size(p.y), std::max(size(p.shared), size(p.res))) + 127) / 128 * 128;
     const int warps = (p.H + 32 * gx::kBlockUnit * gx::kBlockUnits - 1) / (32 * gx::kBlockUnit * gx::kBlockUnits);
-    const int ctas = warps <= 8 ? 2 : 1;               // per SM
+    const int ctas = gx::rows_ctas(warps <= 8 ? 8 : gx::kRowsMaxWarps);
     const int slots = std::min<int>(gx::kRowsMaxSlots, (int)(kStreamSmem / ctas) / slot_bytes);
     const int grid = std::min<int64_t>((int64_t)sms * ctas, p.T);
     switch (p.y.type) {
@@ -211,6 +211,7 @@ int launch_block_rows(gx::BlockParams & p, int sms, void * stream) {
 
 int launch_block(gx::BlockParams & p, bool vec, void * stream) {
     p.one = 1.0f;
+    p.per = 1.0f / (float)p.H;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
     vec = vec && p.H % 8 == 0 && !misaligned(p.norm, 16) && !misaligned(p.next_norm, 16) &&
