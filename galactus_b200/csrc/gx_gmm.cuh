@@ -78,7 +78,16 @@ struct GmmParams {
     int32_t split;            // CTAs of a cluster that share K (single CTAs with nt = 32 only)
     int32_t seg;              // chunks that one accumulator sums (0: all)
     int32_t acc;              // TMEM columns of an accumulator
+    // 4-bit weights (SRC != 0): the matrices in place of the maps
+    const uint8_t * w0;       // W (or G)
+    const uint8_t * w1;       // U
+    int64_t nb01, nb02;
+    int32_t parts;            // 16-bit parts that a weight is made of
 };
+
+// Where the matrix tiles come from: 16-bit weights by TMA, or blocks of 4-bit
+// ones, which warps of their own turn into tiles of the rows' type
+enum : int { GMM_TILES = 0, GMM_Q4_0_F16 = 1, GMM_Q4_0_BF16 = 2, GMM_Q4_1_F16 = 3, GMM_Q4_1_BF16 = 4 };
 
 // ------------------------------------------------------------ PTX helpers
 
@@ -393,13 +402,14 @@ struct GmmTile {
 // tile t of the launch: the tiles of the matrix run fastest, so that CTAs at
 // work together read the same rows and one expert's weights (m0: its first
 // matrix row, `rows` per tile)
-template <int ROUND>
+template <int ROUND, int SRC = GMM_TILES>
 __device__ __forceinline__ GmmTile gmm_tile(const GmmParams & p, const int32_t * pre, int t, int rows) {
     GmmTile r;
     const int tt = t / p.mt;
     r.m0 = (t - tt * p.mt) * rows;
     r.g = tile_group(pre, p.G, tt);
-    const int lo = p.offsets[r.g], hi = p.offsets[r.g + 1];
+    const bool all = SRC != GMM_TILES && p.offsets == nullptr;          // (one matrix for all rows)
+    const int lo = all ? 0 : p.offsets[r.g], hi = all ? p.n_rows : p.offsets[r.g + 1];
     // a group's tiles are of one size, rather than full ones and a rest
     const int n = pre[r.g + 1] - pre[r.g];
     const int size = ((hi - lo - 1) / n + ROUND) / ROUND * ROUND;
@@ -555,13 +565,52 @@ __device__ __forceinline__ void put_rows_as(const GmmParams & p, uint8_t * stage
     else put_rows<__half, COLS>(p, stage, v, my, n0, vec);
 }
 
-template <int CTAS, int MODE>
-__global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_constant__ GmmParams p) {
+// Four bytes of codes as f32: 16 + q, the code in the upper bits of the mantissa
+// (bytes of 0x80 | q << 3 into the third byte of 0x41......)
+__device__ __forceinline__ void q4_spread(uint32_t bytes, float * f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(bytes, 0x41u, 0x4055u + 0x100u * (uint32_t)i));
+}
+
+// Eight weights as `parts` sums of 16-bit values (each the rest rounded): 16
+// bytes of each part's tile
+template <bool BF16>
+__device__ __forceinline__ void q4_put(float (&w)[8], uint32_t to, int parts) {
+    for (int part = 0; part < parts; ++part, to += kGmmATile) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(w[2 * i], w[2 * i + 1]);
+                v[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+                v[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        if (part + 1 == parts) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float2 h;
+            if constexpr (BF16) h = make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xFFFF0000u));
+            else h = __half22float2(*reinterpret_cast<const __half2 *>(&v[i]));
+            w[2 * i] = __fsub_rn(w[2 * i], h.x);
+            w[2 * i + 1] = __fsub_rn(w[2 * i + 1], h.y);
+        }
+    }
+}
+
+template <int CTAS, int MODE, int SRC>
+__global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * kGmmQ4Warps : 0), 1)
+    k_gmm(const __grid_constant__ GmmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], part_full, part_free[2], drained;
     __shared__ uint32_t tslot;
     __shared__ int4 gather_mem[kGmmGatherWarps * 8];
-    __shared__ int32_t wsum[gmm_threads(MODE) / 32];
+    constexpr int kQ4 = SRC != GMM_TILES ? kGmmQ4Warps : 0;              // warps that make matrix tiles
+    __shared__ uint64_t raw_full[kQ4 ? 4 : 1][kGmmQ4Stages], raw_empty[kQ4 ? 4 : 1][kGmmQ4Stages];
+    __shared__ int32_t wsum[gmm_threads(MODE) / 32 + kQ4];
     __shared__ int abort_flag;
     int32_t * gather_rows = reinterpret_cast<int32_t *>(gather_mem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -571,10 +620,11 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
     constexpr bool GLU = MODE == GMM_GLU;
     constexpr int kBufs = MODE == GMM_DUAL ? 1 : 2;                      // accumulators that take turns
     constexpr int kEpi = gmm_epi_warps(MODE);
-    constexpr uint32_t kABytes = gmm_a_bytes(MODE);
+    const uint32_t kABytes = SRC != GMM_TILES ? (uint32_t)p.parts * kGmmATile : gmm_a_bytes(MODE);
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const uint32_t stage_bytes = gmm_stage_bytes(CTAS, p.nt, MODE);
-    uint8_t * staging = ring + (uint32_t)p.stages * stage_bytes;
+    const uint32_t stage_bytes = kABytes + (uint32_t)(p.nt / CTAS) * 128u;
+    uint8_t * raw = ring + (uint32_t)p.stages * stage_bytes;             // 4-bit weights: the rings of blocks
+    uint8_t * staging = raw + (SRC != GMM_TILES ? kGmmQ4Raw : 0u);
     float * xchg = reinterpret_cast<float *>(staging + kGmmStaging);
     float * part = xchg + (GLU ? kGmmXchg / 4 : 0u);                     // [2][nt][128] partial sums of a shared tile
     int32_t * pre = reinterpret_cast<int32_t *>(part + (split > 1 ? 2 * p.nt * kGmmRows : 0));
@@ -583,12 +633,16 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1);
+            mbar_init(full + i, 1 + CTAS * kQ4);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
             mbar_init(acc_empty + i, kEpi * CTAS);
+        }
+        for (int i = 0; i < (kQ4 ? 4 * kGmmQ4Stages : 0); ++i) {
+            mbar_init(&raw_full[0][0] + i, 1);
+            mbar_init(&raw_empty[0][0] + i, 2);
         }
         mbar_init(&part_full, (uint32_t)(kEpi * split));
         for (int i = 0; i < 2; ++i) mbar_init(part_free + i, kEpi);
@@ -597,7 +651,13 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
         mbar_fence_init();
     }
     if (warp == 1) gmm_tmem_alloc<CTAS>(&tslot, 512);
-    tile_prefix(pre, wsum, p.G, p.nt, p.most, [&](int g) { return group_rows_of(p.offsets, g, p.n_rows); });
+    if constexpr (SRC != GMM_TILES) {
+        griddep_launch_dependents();
+        griddep_wait();
+    }
+    tile_prefix(pre, wsum, p.G, p.nt, p.most, [&](int g) {
+        return SRC != GMM_TILES && p.offsets == nullptr ? make_int2(0, p.n_rows) : group_rows_of(p.offsets, g, p.n_rows);
+    });
     tc_fence_before();
     if (CTAS * split == 1) __syncthreads(); else cluster_sync_all();
     tc_fence_after();
@@ -636,12 +696,12 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             RingPos at;
             bool ok = true;
             for (Work w = start(); w.t < tiles && ok; advance(w)) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
                 const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const int m0 = q.m0 + rank * kOut;
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
                 const int r0 = q.row0 + rank * half;
-                uint32_t bytes = (uint32_t)CTAS * kABytes;
+                uint32_t bytes = SRC != GMM_TILES ? 0u : (uint32_t)CTAS * kABytes;
                 int boxes = 0;
                 for (int r = 0; r < CTAS; ++r) {
                     const int n = max(0, min(half, q.cnt - r * half));
@@ -662,8 +722,8 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                     }
                     uint8_t * st = ring + (uint32_t)at.s * stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
-                    gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
-                    if (MODE != GMM_PLAIN) gmm_tma_3d<CTAS>(st + kABytes / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
+                    if (SRC == GMM_TILES) gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
+                    if (SRC == GMM_TILES && MODE != GMM_PLAIN) gmm_tma_3d<CTAS>(st + kABytes / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
                     for (int b = 0; b < boxes; ++b)
                         gmm_tma_2d<CTAS>(st + kABytes + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
                 }
@@ -686,7 +746,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             bool ok = true;
             const uint64_t da0 = umma_desc_sw128(ring, 1024u), db0 = umma_desc_sw128(ring + kABytes, 1024u);
             for (Work w = start(); w.t < tiles && ok; advance(w)) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
                 const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const uint32_t n = (uint32_t)((q.cnt + kRound - 1) / kRound * kRound);
                 const uint32_t idesc = umma_idesc_f16(p.bf16 != 0, kGmmRows * CTAS, n);
@@ -709,6 +769,13 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                             for (int i = 0; i < kGmmK / 16; ++i)
                                 mma_f16<CTAS>(d + 256u, da0 + (kGmmATile >> 4) + off + (uint64_t)(2 * i), db0 + off + (uint64_t)(2 * i),
                                               idesc, more | (uint32_t)i);
+                        }
+                        if constexpr (SRC != GMM_TILES) {
+                            for (int part = 1; part < p.parts; ++part)
+#pragma unroll
+                                for (int i = 0; i < kGmmK / 16; ++i)
+                                    mma_f16<CTAS>(d, da0 + (uint64_t)part * (kGmmATile >> 4) + off + (uint64_t)(2 * i),
+                                                  db0 + off + (uint64_t)(2 * i), idesc, 1u);
                         }
                         more = 1;
                         gmm_commit<CTAS>(empty + at.s);
@@ -736,7 +803,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
             RingPos at;
             bool ok = true;
             for (Work w = start(); w.t < tiles && ok; advance(w)) {
-                const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+                const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
                 const int k0 = first_chunk(w), k1 = end_chunk(w);
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;
                 const int n = max(0, min(half, q.cnt - rank * half));             // this CTA's rows
@@ -772,6 +839,135 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
                 at.skip(k1 - k0, p.stages);
             }
         }
+    } else if (SRC != GMM_TILES && warp >= 2 + kGmmGatherWarps + kEpi) {
+        // --------------------------------- tiles of weights from their blocks
+        // Warp (rows of 32, block of the chunk's two): a lane a row's block, 32
+        // weights. The rows' pieces come by bulk copies, a lane a row, into a ring
+        // that the two warps of 32 rows share. (cp.async by these warps would be
+        // waited for by every fence that shows a tile to the tensor cores: 2860
+        // cycles a chunk.)
+        if constexpr (SRC != GMM_TILES) {
+            constexpr bool Q41 = SRC >= GMM_Q4_1_F16, BF = SRC == GMM_Q4_0_BF16 || SRC == GMM_Q4_1_BF16;
+            constexpr int kPair = Q41 ? 40 : 36, kWords = 5;
+            const int qw = warp - (2 + kGmmGatherWarps + kEpi), rg = qw & 3, blk = qw >> 2;
+            uint8_t * my = raw + (uint32_t)rg * (kGmmQ4Stages * 32u * kGmmQ4Pitch) + (uint32_t)lane * kGmmQ4Pitch;
+            const uint8_t * w_of = GLU && rg >= 2 ? p.w1 : p.w0;
+            const uint8_t * const w_end = w_of + (int64_t)(p.G - 1) * p.nb02 + (int64_t)(p.N - 1) * p.nb01 + (int64_t)nk * kPair;
+            const int base_row = (GLU ? (rg & 1) * 32 : rg * 32) + lane;
+            const int steps = (nk + kGmmQ4Chunks - 1) / kGmmQ4Chunks;        // stages of a tile
+            bool ok = true;
+            // the copies run a stage or two ahead (warps of block 0)
+            Work aw = start();
+            GmmTile aq{};
+            int a_step = 0, issued = 0;
+            if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
+            auto fetch = [&] {
+                if (blk != 0 || aw.t >= tiles || !ok) return;
+                const int s = issued % kGmmQ4Stages;
+                if (issued >= kGmmQ4Stages) ok = gmm_wait<1>(&raw_empty[rg][s], (uint32_t)((issued / kGmmQ4Stages - 1) & 1), &abort_flag);
+                if (!ok) return;
+                const int m = aq.m0 + rank * kOut + base_row, n = min(kGmmQ4Chunks, nk - a_step * kGmmQ4Chunks);
+                const uint8_t * a = w_of + (int64_t)aq.g * p.nb02 + (int64_t)m * p.nb01 + (int64_t)a_step * (kGmmQ4Chunks * kPair);
+                const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(a) & 15u;
+                uint32_t bytes = m < p.N ? (skew + (uint32_t)(n * kPair) + 15u) & ~15u : 0u;     // (rows behind the last: nothing)
+                const uint8_t * from = a - skew;
+                uint8_t * to = my + (uint32_t)s * (32u * kGmmQ4Pitch);
+                // (the last row's last piece ends with the matrix: what is not whole 16 bytes is moved by hand)
+                if (bytes != 0u && from + bytes > w_end) {
+                    bytes -= 16u;
+                    for (const uint8_t * b = from + bytes; b < w_end; b += 4)
+                        *reinterpret_cast<uint32_t *>(to + (b - from)) = *reinterpret_cast<const uint32_t *>(b);
+                }
+                const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
+                if (lane == 0) mbar_arrive_expect_tx(&raw_full[rg][s], sum);
+                __syncwarp();
+                if (bytes != 0u) bulk_g2s(to, from, bytes, &raw_full[rg][s]);
+                ++issued;
+                if (++a_step == steps) {
+                    a_step = 0;
+                    advance(aw);
+                    if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
+                }
+            };
+            fetch();
+            const int row = rg * 32 + lane;
+            RingPos at;
+            int taken = 0;
+            for (Work w = start(); w.t < tiles && ok; advance(w)) {
+                const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
+                // where the lane's row starts inside its 16 bytes
+                const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(w_of) + (uint32_t)q.g * (uint32_t)p.nb02 +
+                                     (uint32_t)(q.m0 + rank * kOut + base_row) * (uint32_t)p.nb01;
+                uint32_t src = 0, stage_low = 0;
+                for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
+                    const int in = kc % kGmmQ4Chunks, rs = taken % kGmmQ4Stages;
+                    if (in == 0) {
+                        fetch();
+                        ok = ok && gmm_wait<1>(&raw_full[rg][rs], (uint32_t)((taken / kGmmQ4Stages) & 1), &abort_flag);
+                        if (!ok) break;
+                        stage_low = (low + (uint32_t)(kc * kPair)) & 15u;
+                        src = smem_u32(my + (uint32_t)rs * (32u * kGmmQ4Pitch));
+                    }
+                    // the block's five words, out of two pieces of 16 bytes
+                    uint32_t v[8];
+                    {
+                        const uint32_t o = stage_low + (uint32_t)(in * kPair + blk * (Q41 ? 20 : 16)), a = src + (o & ~15u);
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(a + 16u) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 6; ++i) v[i] = o & 8u ? v[i + 2] : v[i];
+#pragma unroll
+                        for (int i = 0; i < kWords; ++i) v[i] = o & 4u ? v[i + 1] : v[i];
+                    }
+                    if (in + 1 == kGmmQ4Chunks || kc + 1 == nk) {
+                        __syncwarp();
+                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&raw_empty[rg][rs])) : "memory");
+                        ++taken;
+                    }
+                    const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[0]));
+                    float d = head.x, c;
+                    uint32_t qs[4];
+                    if (Q41 || blk == 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) qs[i] = v[i + 1];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) qs[i] = __byte_perm(v[i], v[i + 1], 0x5432);
+                    }
+                    if constexpr (Q41) c = __fmaf_rn(-16.0f, d, head.y);
+                    else {
+                        if (blk == 1) d = head.y;
+                        c = __fmul_rn(-24.0f, d);
+                    }
+                    if (at.round != 0) {
+                        ok = gmm_wait<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
+                        if (!ok) break;
+                    }
+                    const uint32_t tile = smem_u32(ring + (uint32_t)at.s * stage_bytes) + (uint32_t)row * 128u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // elements 8 i .. 8 i + 7 of the block
+                        float f[8];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t q = qs[2 * (i & 1) + j];
+                            q4_spread(((i < 2 ? q << 3 : q >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
+                        q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    // (the fence has put the tile where the tensor cores of both CTAs see it: no release over the cluster)
+                    if (lane == 0) gmm_arrive<CTAS>(full + at.s);
+                }
+            }
+            // copies in flight land before the CTA leaves
+            volatile int none = 0;
+            for (int i = 0; i < kGmmQ4Stages && !ok; ++i)
+                if (issued > i) gmm_wait<1>(&raw_full[rg][i], (uint32_t)((issued - 1 - i) / kGmmQ4Stages & 1), &none);
+        }
     } else {
         // -------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lanes 32 * quad ..
@@ -782,7 +978,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE), 1) k_gmm(const __grid_const
         int it = 0, xb = 0, i_tile = 0;
         bool ok = true;
         for (Work w = start(); w.t < tiles && ok; advance(w)) {
-            const GmmTile q = gmm_tile<kRound>(p, pre, w.t, kOut * CTAS);
+            const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
             const int k0 = first_chunk(w), k1 = end_chunk(w);
             const int nseg = p.seg ? (k1 - k0 + p.seg - 1) / p.seg : 1;
             // the order of the first columns' rows is on its way before the sums are there

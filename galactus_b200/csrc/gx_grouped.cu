@@ -50,13 +50,6 @@ enum KernelSlot : int { kSlotGroup, kSlotLora, kSlotGmm, kSlotEnd = kSlotGmm + 6
 static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
 int gmm_slot(int ctas, int mode) { return kSlotGmm + (ctas - 1) * 3 + mode; }
 
-// Whether one accumulator is too short for sums of K elements. The tensor
-// cores' f32 accumulators drop what does not fit instead of rounding: for
-// products of random signs about 1e-9 of the magnitudes' sum per element, for
-// products of one sign 6e-9 (measured: 4.8e-5 at K = 7168, 1.6e-4 at 28672).
-// Results of 16 bits do not see that while it is a fifth of half a step.
-bool long_sum(int out, int64_t K) { return K > (out == gx::GMM_F32 ? 512 : out == gx::GMM_F16 ? 16384 : 131072); }
-
 // The shared checks and the launch of the plain (up == NULL) and gated products.
 int grouped_product(int type, const void * as, const void * up, int64_t ne00, int64_t ne01, int64_t nb01, int64_t nb02,
                     int64_t n_as, const void * b, int64_t ne11, int64_t nb11, const int32_t * offsets,
@@ -128,9 +121,9 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     p.box = std::min(128, p.nt / ctas);
     const int out_rows = gx::gmm_out_rows(mode) * ctas;
     p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
-    const void * fn = mode == gx::GMM_DUAL ? (const void *)gx::k_gmm<2, gx::GMM_DUAL>
-                      : ctas == 2          ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU> : (const void *)gx::k_gmm<2, gx::GMM_PLAIN>)
-                                           : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU> : (const void *)gx::k_gmm<1, gx::GMM_PLAIN>);
+    const void * fn = mode == gx::GMM_DUAL ? (const void *)gx::k_gmm<2, gx::GMM_DUAL, gx::GMM_TILES>
+                      : ctas == 2          ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU, gx::GMM_TILES> : (const void *)gx::k_gmm<2, gx::GMM_PLAIN, gx::GMM_TILES>)
+                                           : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU, gx::GMM_TILES> : (const void *)gx::k_gmm<1, gx::GMM_PLAIN, gx::GMM_TILES>);
     const int slot = gmm_slot(ctas, mode);
     cudaError_t e = allow_smem(fn, slot, gx::kGroupedSmem);
     if (e != cudaSuccess) return cuda_status(e);

@@ -20,6 +20,11 @@ cudaError_t read_and_clear_q4_error(int * code) {
 
 namespace {
 
+enum KernelSlot : int { kSlotQ4 = 0, kSlotRows = 8, kSlotTiles = kSlotRows + 6, kSlotEnd = kSlotTiles + 8 };
+static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
+
+constexpr int64_t kTileRows = 8;       // rows per matrix on average, above which matrix tiles are made for the tensor cores
+
 // A launch that may begin while the kernel before it on the stream ends: the
 // kernels wait (griddepcontrol.wait) before they read or write anything.
 template <typename P>
@@ -48,6 +53,43 @@ const void * q4_kernel(bool glu) {
 const void * q4_kernel(bool bf16, bool q41, bool glu) {
     return bf16 ? (q41 ? q4_kernel<true, true>(glu) : q4_kernel<true, false>(glu))
                 : (q41 ? q4_kernel<false, true>(glu) : q4_kernel<false, false>(glu));
+}
+
+template <int MODE>
+const void * q4_tiles_kernel(bool bf16, bool q41) {
+    if (q41) return bf16 ? (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_1_BF16> : (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_1_F16>;
+    return bf16 ? (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_BF16> : (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_F16>;
+}
+
+// Many rows per matrix: the grouped products' kernel on CTA pairs, its matrix
+// tiles made from the blocks.
+int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11, int64_t touched, void * stream) {
+    const int mode = glu ? gx::GMM_GLU : gx::GMM_PLAIN;
+    // Parts of 16 bits that a weight is made of. One for results of 16 bits: the
+    // weight is then rounded as the result is, by half a step of their type. f32
+    // results take the weight whole, or to 22 bits (d q + m in F16) or 24 (BF16).
+    p.parts = p.out != gx::GMM_F32 ? 1 : q41 && p.bf16 ? 3 : 2;
+    p.seg = long_sum(p.out, p.K) ? 8 : 0;
+    p.nt = p.seg ? 160 : 256;
+    while (gx::gmm_q4_stages(p.nt, mode, p.G, p.parts) < 2) p.nt -= 32;       // (thousands of matrices, f32 results)
+    p.acc = p.seg ? p.nt : 256;
+    p.box = p.nt / 2;
+    if (!encode_rows(&p.xmap, p.bf16 != 0, b, p.K, p.x_rows, nb11, 0, 0, p.gather ? 1u : (uint32_t)p.box)) return GX_ERR_ALIGN;
+    p.split = 1;
+    const int out_rows = gx::gmm_out_rows(mode) * 2;
+    p.mt = (int32_t)((p.N + out_rows - 1) / out_rows);
+    p.most = (int32_t)(p.n_rows / p.nt + touched);
+    const int64_t most = (int64_t)p.mt * p.most;
+    if (most > kMaxSize) return GX_ERR_INVALID;
+    const int sms = device_sms();
+    if (sms == 0) return GX_ERR_CUDA;
+    const void * fn = glu ? q4_tiles_kernel<gx::GMM_GLU>(p.bf16 != 0, q41) : q4_tiles_kernel<gx::GMM_PLAIN>(p.bf16 != 0, q41);
+    cudaError_t e = allow_smem(fn, kSlotTiles + (glu ? 4 : 0) + (q41 ? 2 : 0) + (p.bf16 ? 1 : 0), gx::kGroupedSmem);
+    if (e != cudaSuccess) return cuda_status(e);
+    p.stages = gx::gmm_q4_stages(p.nt, mode, p.G, p.parts);
+    const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::gmm_q4_stage_bytes(p.nt, p.parts) + gx::gmm_q4_fixed_bytes(p.nt, mode, p.G);
+    return cuda_status(launch_next(fn, dim3((unsigned)(2 * std::min<int64_t>(sms / 2, most))), gx::gmm_threads(mode) + 32 * gx::kGmmQ4Warps, smem,
+                                   2, stream, p));
 }
 
 // The shared checks and the launch of the plain (up == NULL) and gated products.
@@ -112,6 +154,30 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
     p.alpha = alpha;
     p.limit = limit;
     const int64_t touched = std::min(n_rows, n_as);
+    if (ids == nullptr && n_rows > kTileRows * touched) {
+        gx::GmmParams t{};
+        t.bf16 = bf16;
+        t.offsets = offsets;
+        t.order = order;
+        t.G = p.G;
+        t.n_rows = p.n_rows;
+        t.x_rows = p.x_rows;
+        t.N = p.N;
+        t.K = p.K;
+        t.gather = p.gather;
+        t.scatter = p.scatter;
+        t.out = out;
+        t.dst = p.dst;
+        t.nbd1 = nbd1;
+        t.act = act;
+        t.alpha = alpha;
+        t.limit = limit;
+        t.w0 = p.w0;
+        t.w1 = p.w1;
+        t.nb01 = nb01;
+        t.nb02 = nb02;
+        return q4_tiles(t, q41, glu, b, nb11, touched, stream);
+    }
     const gx::Q4Shape shape = gx::q4_shape(q41, ne00, n_rows);
     p.warps = shape.warps;
     p.cap = shape.cap;
@@ -136,7 +202,7 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
         }
     }
     const void * fn = q4_kernel(bf16, q41, glu);
-    const int slot = (bf16 ? 4 : 0) + (q41 ? 2 : 0) + (glu ? 1 : 0);
+    const int slot = kSlotQ4 + (bf16 ? 4 : 0) + (q41 ? 2 : 0) + (glu ? 1 : 0);
     cudaError_t e = allow_smem(fn, slot, gx::kQ4Smem);
     if (e != cudaSuccess) return cuda_status(e);
     const int64_t grid = std::min<int64_t>(sms, (most * p.share + p.warps - 1) / p.warps);
@@ -180,7 +246,7 @@ template <int YT>
 int launch_block_rows(gx::BlockParams & p, int grid, int warps, int slots, int slot_bytes, void * stream) {
     const void * fn = warps <= 8 ? (const void *)gx::k_block_rows<YT, 8> : (const void *)gx::k_block_rows<YT, gx::kRowsMaxWarps>;
     const uint32_t smem = (uint32_t)(slots * slot_bytes);
-    cudaError_t e = allow_smem(fn, 8 + YT + (warps <= 8 ? 0 : 3), kStreamSmem);
+    cudaError_t e = allow_smem(fn, kSlotRows + YT + (warps <= 8 ? 0 : 3), kStreamSmem);
     if (e != cudaSuccess) return cuda_status(e);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);

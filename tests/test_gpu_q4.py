@@ -36,10 +36,11 @@ def parts(w, kind):
     return tuple(torch.from_numpy(t.reshape(*w.shape[:-1], -1)).cuda() for t in (v, a))
 
 
-def want(w, x, kind, e):
+def want(w, x, kind, e, rounded=False):
     """Row j of x times matrix e[j] (-1: none) in 64 bits, and how far f32 sums may be off: the tensor cores add a block's
     64 products of codes (at most 31 |d x|, and 24 |d x| taken off) within 6e-9 of their magnitudes each, then the
-    block's sums are added in f32, K / 32 roundings of half a step."""
+    block's sums are added in f32, K / 32 roundings of half a step. rounded: many rows and results of 16 bits, where a weight is rounded
+    to x's type first, by half a step of its own."""
     n = w.shape[1]
     y = torch.zeros((len(e), n), dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(y)
@@ -50,12 +51,19 @@ def want(w, x, kind, e):
         xs = x[rows].double()
         y[rows] = xs @ v.T
         tol[rows] = (xs.abs() @ a.T) * 64 * 6e-9 + (xs.abs() @ v.abs().T) * (K // 32 + 8) * 2.0 ** -24
+        if rounded:
+            tol[rows] += (xs.abs() @ v.abs().T) * torch.finfo(x.dtype).eps / 2
     return y, tol
 
 
-def want_glu(gate, up, x, kind, e, act):
-    g, eg = want(gate, x, kind, e)
-    u, eu = want(up, x, kind, e)
+def many(rows, groups, out):
+    """Whether a call without ids makes matrix tiles of rounded weights."""
+    return rows > 8 * min(rows, groups) and out != F32
+
+
+def want_glu(gate, up, x, kind, e, act, rounded=False):
+    g, eg = want(gate, x, kind, e, rounded)
+    u, eu = want(up, x, kind, e, rounded)
     if act:
         ok = g < LIMIT
         g, eg = g.clamp(max=LIMIT), torch.where(ok | ((g - LIMIT).abs() < eg), eg, 0.0)
@@ -104,7 +112,7 @@ def test_dense(gxlib, dev, kind, dtype, out, K, N):
     for rows in (1, 2, 8, 9, 17, 31, 32, 33, 70):
         x = torch.from_numpy(rng.standard_normal((rows, K))).cuda().to(dtype)
         got = gxlib.mul_mat_q4(w, x, type=kind, out_dtype=out)
-        check(got, *want(w, x, kind, [0] * rows))
+        check(got, *want(w, x, kind, [0] * rows, many(rows, 1, out)))
     assert error_code(gxlib) == 0
 
 
@@ -150,7 +158,7 @@ def test_groups(gxlib, dev, kind, dtype, out, T, k, E, K, N):
     none = torch.tensor([j for j, v in enumerate(flat) if v < 0], dtype=torch.long, device="cuda")
     keep = torch.full((T * k, N), 7.0, dtype=out, device="cuda")
     got = gxlib.mul_mat_q4(w, x, type=kind, offsets=offsets, order=order, gather=k, scatter=True, out=keep)
-    y, tol = want(w, x.repeat_interleave(k, 0), kind, flat)
+    y, tol = want(w, x.repeat_interleave(k, 0), kind, flat, many(T * k, E, out))
     check(got, y, tol, none)
     assert bool((got[none] == 7.0).all())
     # into expert order, and from expert order
@@ -180,6 +188,8 @@ def test_glu(gxlib, dev, kind, act, dtype, out, T, k, E, K, N):
     if T * k <= 256:
         check(gxlib.mul_mat_q4_glu(gate, up, x, type=kind, ids=dids, gather=k, act=act, out_dtype=out), y, tol)
     order, offsets = gxlib.group_rows(dids, E)
+    if many(T * k, E, out):
+        y, tol = want_glu(gate, up, x.repeat_interleave(k, 0), kind, flat, act, True)
     check(gxlib.mul_mat_q4_glu(gate, up, x, type=kind, offsets=offsets, order=order, gather=k, scatter=True, act=act, out_dtype=out), y, tol)
     assert error_code(gxlib) == 0
 
