@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
     uint8_t * ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t stage_bytes = kABytes + (uint32_t)(p.nt / CTAS) * 128u;
     uint8_t * raw = ring + (uint32_t)p.stages * stage_bytes;             // 4-bit weights: the rings of blocks
-    uint8_t * staging = raw + (SRC != GMM_TILES ? kGmmQ4Raw : 0u);
+    uint8_t * staging = raw + (SRC != GMM_TILES ? gmm_q4_raw(SRC >= GMM_Q4_1_F16) : 0u);
     float * xchg = reinterpret_cast<float *>(staging + kGmmStaging);
     float * part = xchg + (GLU ? kGmmXchg / 4 : 0u);                     // [2][nt][128] partial sums of a shared tile
     int32_t * pre = reinterpret_cast<int32_t *>(part + (split > 1 ? 2 * p.nt * kGmmRows : 0));
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1 + CTAS * kQ4);
+            mbar_init(full + i, 1 + CTAS * (kQ4 / 2));
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -841,28 +841,30 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
         }
     } else if (SRC != GMM_TILES && warp >= 2 + kGmmGatherWarps + kEpi) {
         // --------------------------------- tiles of weights from their blocks
-        // Warp (rows of 32, block of the chunk's two): a lane a row's block, 32
-        // weights. The rows' pieces come by bulk copies, a lane a row, into a ring
-        // that the two warps of 32 rows share. (cp.async by these warps would be
-        // waited for by every fence that shows a tile to the tensor cores: 2860
-        // cycles a chunk.)
+        // Four warps a tile of 128 rows, a lane a row, the two fours taking the
+        // chunks of 64 elements in turn (a stage's barrier is at most one phase
+        // behind what they wait for: they have waited for the chunk two before, in
+        // another stage, and stages come free in order). The rows' pieces come by
+        // bulk copies, a lane a row, into a ring that two warps share. (cp.async
+        // would be waited for by every fence that shows a tile to the tensor cores.)
         if constexpr (SRC != GMM_TILES) {
             constexpr bool Q41 = SRC >= GMM_Q4_1_F16, BF = SRC == GMM_Q4_0_BF16 || SRC == GMM_Q4_1_BF16;
-            constexpr int kPair = Q41 ? 40 : 36, kWords = 5;
-            const int qw = warp - (2 + kGmmGatherWarps + kEpi), rg = qw & 3, blk = qw >> 2;
-            uint8_t * my = raw + (uint32_t)rg * (kGmmQ4Stages * 32u * kGmmQ4Pitch) + (uint32_t)lane * kGmmQ4Pitch;
+            constexpr int kPair = Q41 ? 40 : 36, kWords = kPair / 4;
+            constexpr uint32_t kPitch = gmm_q4_pitch(Q41);
+            const int qw = warp - (2 + kGmmGatherWarps + kEpi), rg = qw & 3, odd = qw >> 2;
+            uint8_t * my = raw + (uint32_t)rg * (kGmmQ4Stages * 32u * kPitch) + (uint32_t)lane * kPitch;
             const uint8_t * w_of = GLU && rg >= 2 ? p.w1 : p.w0;
             const uint8_t * const w_end = w_of + (int64_t)(p.G - 1) * p.nb02 + (int64_t)(p.N - 1) * p.nb01 + (int64_t)nk * kPair;
             const int base_row = (GLU ? (rg & 1) * 32 : rg * 32) + lane;
             const int steps = (nk + kGmmQ4Chunks - 1) / kGmmQ4Chunks;        // stages of a tile
             bool ok = true;
-            // the copies run a stage or two ahead (warps of block 0)
+            // the copies run a stage or two ahead (the first four's)
             Work aw = start();
             GmmTile aq{};
             int a_step = 0, issued = 0;
             if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
             auto fetch = [&] {
-                if (blk != 0 || aw.t >= tiles || !ok) return;
+                if (odd != 0 || aw.t >= tiles || !ok) return;
                 const int s = issued % kGmmQ4Stages;
                 if (issued >= kGmmQ4Stages) ok = gmm_wait<1>(&raw_empty[rg][s], (uint32_t)((issued / kGmmQ4Stages - 1) & 1), &abort_flag);
                 if (!ok) return;
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                 const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(a) & 15u;
                 uint32_t bytes = m < p.N ? (skew + (uint32_t)(n * kPair) + 15u) & ~15u : 0u;     // (rows behind the last: nothing)
                 const uint8_t * from = a - skew;
-                uint8_t * to = my + (uint32_t)s * (32u * kGmmQ4Pitch);
+                uint8_t * to = my + (uint32_t)s * (32u * kPitch);
                 // (the last row's last piece ends with the matrix: what is not whole 16 bytes is moved by hand)
                 if (bytes != 0u && from + bytes > w_end) {
                     bytes -= 16u;
@@ -892,30 +894,37 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
             fetch();
             const int row = rg * 32 + lane;
             RingPos at;
-            int taken = 0;
+            int taken = 0, turn = 0;
             for (Work w = start(); w.t < tiles && ok; advance(w)) {
                 const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
                 // where the lane's row starts inside its 16 bytes
                 const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(w_of) + (uint32_t)q.g * (uint32_t)p.nb02 +
                                      (uint32_t)(q.m0 + rank * kOut + base_row) * (uint32_t)p.nb01;
-                uint32_t src = 0, stage_low = 0;
+                uint32_t src = 0, skew = 0;
                 for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
                     const int in = kc % kGmmQ4Chunks, rs = taken % kGmmQ4Stages;
                     if (in == 0) {
                         fetch();
                         ok = ok && gmm_wait<1>(&raw_full[rg][rs], (uint32_t)((taken / kGmmQ4Stages) & 1), &abort_flag);
                         if (!ok) break;
-                        stage_low = (low + (uint32_t)(kc * kPair)) & 15u;
-                        src = smem_u32(my + (uint32_t)rs * (32u * kGmmQ4Pitch));
+                        skew = (low + (uint32_t)(kc * kPair)) & 15u;
+                        src = smem_u32(my + (uint32_t)rs * (32u * kPitch));
                     }
-                    // the block's five words, out of two pieces of 16 bytes
-                    uint32_t v[8];
-                    {
-                        const uint32_t o = stage_low + (uint32_t)(in * kPair + blk * (Q41 ? 20 : 16)), a = src + (o & ~15u);
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(a + 16u) : "memory");
+                    const bool mine = turn == odd;
+                    turn ^= 1;
+                    // the chunk's words, out of three or four pieces of 16 bytes
+                    constexpr int kPieces = (kPair + 12 + 15) / 16;
+                    uint32_t v[4 * kPieces];
+                    if (mine) {
+                        const uint32_t o = skew + (uint32_t)(in * kPair), a = src + (o & ~15u);
 #pragma unroll
-                        for (int i = 0; i < 6; ++i) v[i] = o & 8u ? v[i + 2] : v[i];
+                        for (int i = 0; i < kPieces; ++i)
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v[4 * i]), "=r"(v[4 * i + 1]), "=r"(v[4 * i + 2]), "=r"(v[4 * i + 3])
+                                         : "r"(a + 16u * (uint32_t)i)
+                                         : "memory");
+#pragma unroll
+                        for (int i = 0; i + 2 < 4 * kPieces && i < kWords + 1; ++i) v[i] = o & 8u ? v[i + 2] : v[i];
 #pragma unroll
                         for (int i = 0; i < kWords; ++i) v[i] = o & 4u ? v[i + 1] : v[i];
                     }
@@ -924,38 +933,43 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&raw_empty[rg][rs])) : "memory");
                         ++taken;
                     }
-                    const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[0]));
-                    float d = head.x, c;
-                    uint32_t qs[4];
-                    if (Q41 || blk == 1) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) qs[i] = v[i + 1];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) qs[i] = __byte_perm(v[i], v[i + 1], 0x5432);
-                    }
-                    if constexpr (Q41) c = __fmaf_rn(-16.0f, d, head.y);
-                    else {
-                        if (blk == 1) d = head.y;
-                        c = __fmul_rn(-24.0f, d);
-                    }
+                    if (!mine) continue;
                     if (at.round != 0) {
                         ok = gmm_wait<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
                         if (!ok) break;
                     }
                     const uint32_t tile = smem_u32(ring + (uint32_t)at.s * stage_bytes) + (uint32_t)row * 128u;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // elements 8 i .. 8 i + 7 of the block
-                        float f[8];
+                    for (int blk = 0; blk < 2; ++blk) {
+                        // Q4_0: words 0 .. 4 and 4 .. 8 (codes from the middle of a word on in the first block); Q4_1: five each
+                        uint32_t qs[4];
+                        float d, c;
+                        if constexpr (Q41) {
+                            const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[5 * blk]));
+                            d = head.x;
+                            c = __fmaf_rn(-16.0f, d, head.y);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const uint32_t q = qs[2 * (i & 1) + j];
-                            q4_spread(((i < 2 ? q << 3 : q >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                            for (int i = 0; i < 4; ++i) qs[i] = v[5 * blk + 1 + i];
+                        } else {
+                            const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[4 * blk]));
+                            d = blk == 0 ? head.x : head.y;
+                            c = __fmul_rn(-24.0f, d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) qs[i] = blk == 0 ? __byte_perm(v[i], v[i + 1], 0x5432) : v[5 + i];
                         }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
-                        q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
+                        for (int i = 0; i < 4; ++i) {
+                            // elements 8 i .. 8 i + 7 of the block
+                            float f[8];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const uint32_t b = qs[2 * (i & 1) + j];
+                                q4_spread(((i < 2 ? b << 3 : b >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
+                            q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
+                        }
                     }
                     fence_async_smem();
                     __syncwarp();

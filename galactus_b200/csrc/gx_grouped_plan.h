@@ -33,16 +33,15 @@ GX_HD constexpr uint32_t gmm_a_bytes(int mode) { return mode == GMM_DUAL ? 2u * 
 constexpr uint32_t kGmmStaging = 4u * 32u * 32u * 4u;            // results of 32 (dual: 16) columns per epilogue warp
 constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer][warp pair][direction][column][lane] f32
 
-// 4-bit weights: warps that make the matrix tiles (two to 32 rows), chunks of 64
-// elements per stage of their rings of blocks, bytes between a stage's rows (an
-// odd number of 16 bytes: eight rows then lie in different banks; 12 bytes more
-// than the blocks take, as rows start on any 4 bytes)
+// 4-bit weights: warps that make the matrix tiles (four a tile of 128 rows, in
+// turn), chunks of 64 elements per stage of their rings of blocks, bytes between a
+// stage's rows (an odd number of 16 bytes: eight rows then lie in different
+// banks; 12 bytes more than the blocks take, as rows start on any 4 bytes)
 constexpr int kGmmQ4Warps = 8;
-constexpr int kGmmQ4Chunks = 4;
+constexpr int kGmmQ4Chunks = 8;
 constexpr int kGmmQ4Stages = 2;
-constexpr uint32_t kGmmQ4Pitch = 176;
-static_assert(kGmmQ4Chunks * 40 + 12 <= (int)kGmmQ4Pitch && kGmmQ4Pitch % 32 == 16, "rows of a stage");
-constexpr uint32_t kGmmQ4Raw = 4u * kGmmQ4Stages * 32u * kGmmQ4Pitch;
+GX_HD constexpr uint32_t gmm_q4_pitch(bool q41) { return 16u * (((uint32_t)kGmmQ4Chunks * (q41 ? 40u : 36u) + 12u + 15u) / 16u | 1u); }
+GX_HD constexpr uint32_t gmm_q4_raw(bool q41) { return 4u * kGmmQ4Stages * 32u * gmm_q4_pitch(q41); }
 
 // bytes of a ring stage: the matrix tile and the CTA's rows
 GX_HD constexpr uint32_t gmm_stage_bytes(int ctas, int nt, int mode) {
@@ -60,9 +59,11 @@ GX_HD constexpr int gmm_stages(int ctas, int nt, int mode, int groups, int split
 
 // the same with 4-bit weights, made of `parts` tiles (CTA pairs)
 GX_HD constexpr uint32_t gmm_q4_stage_bytes(int nt, int parts) { return (uint32_t)parts * kGmmATile + (uint32_t)(nt / 2) * 128u; }
-GX_HD constexpr uint32_t gmm_q4_fixed_bytes(int nt, int mode, int groups) { return gmm_fixed_bytes(nt, mode, groups, 1) + kGmmQ4Raw; }
-GX_HD constexpr int gmm_q4_stages(int nt, int mode, int groups, int parts) {
-    const uint32_t n = (kGroupedSmem - kGroupedAlign - gmm_q4_fixed_bytes(nt, mode, groups)) / gmm_q4_stage_bytes(nt, parts);
+GX_HD constexpr uint32_t gmm_q4_fixed_bytes(bool q41, int nt, int mode, int groups) {
+    return gmm_fixed_bytes(nt, mode, groups, 1) + gmm_q4_raw(q41);
+}
+GX_HD constexpr int gmm_q4_stages(bool q41, int nt, int mode, int groups, int parts) {
+    const uint32_t n = (kGroupedSmem - kGroupedAlign - gmm_q4_fixed_bytes(q41, nt, mode, groups)) / gmm_q4_stage_bytes(nt, parts);
     return n < (uint32_t)kGmmMaxStages ? (int)n : kGmmMaxStages;
 }
 

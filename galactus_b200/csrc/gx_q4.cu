@@ -71,7 +71,7 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     p.parts = p.out != gx::GMM_F32 ? 1 : q41 && p.bf16 ? 3 : 2;
     p.seg = long_sum(p.out, p.K) ? 8 : 0;
     p.nt = p.seg ? 160 : 256;
-    while (gx::gmm_q4_stages(p.nt, mode, p.G, p.parts) < 2) p.nt -= 32;       // (thousands of matrices, f32 results)
+    while (gx::gmm_q4_stages(q41, p.nt, mode, p.G, p.parts) < 2) p.nt -= 32;       // (thousands of matrices, f32 results)
     p.acc = p.seg ? p.nt : 256;
     p.box = p.nt / 2;
     if (!encode_rows(&p.xmap, p.bf16 != 0, b, p.K, p.x_rows, nb11, 0, 0, p.gather ? 1u : (uint32_t)p.box)) return GX_ERR_ALIGN;
@@ -86,8 +86,8 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     const void * fn = glu ? q4_tiles_kernel<gx::GMM_GLU>(p.bf16 != 0, q41) : q4_tiles_kernel<gx::GMM_PLAIN>(p.bf16 != 0, q41);
     cudaError_t e = allow_smem(fn, kSlotTiles + (glu ? 4 : 0) + (q41 ? 2 : 0) + (p.bf16 ? 1 : 0), gx::kGroupedSmem);
     if (e != cudaSuccess) return cuda_status(e);
-    p.stages = gx::gmm_q4_stages(p.nt, mode, p.G, p.parts);
-    const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::gmm_q4_stage_bytes(p.nt, p.parts) + gx::gmm_q4_fixed_bytes(p.nt, mode, p.G);
+    p.stages = gx::gmm_q4_stages(q41, p.nt, mode, p.G, p.parts);
+    const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::gmm_q4_stage_bytes(p.nt, p.parts) + gx::gmm_q4_fixed_bytes(q41, p.nt, mode, p.G);
     return cuda_status(launch_next(fn, dim3((unsigned)(2 * std::min<int64_t>(sms / 2, most))), gx::gmm_threads(mode) + 32 * gx::kGmmQ4Warps, smem,
                                    2, stream, p));
 }
