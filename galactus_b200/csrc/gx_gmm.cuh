@@ -83,6 +83,7 @@ struct GmmParams {
     const uint8_t * w1;       // U
     int64_t nb01, nb02;
     int32_t parts;            // 16-bit parts that a weight is made of
+    int32_t boxes;            // rows on 16 bytes: wmap and umap are maps of the blocks, [words of a row, N, G]
 };
 
 // Where the matrix tiles come from: 16-bit weights by TMA, or blocks of 4-bit
@@ -565,15 +566,81 @@ __device__ __forceinline__ void put_rows_as(const GmmParams & p, uint8_t * stage
     else put_rows<__half, COLS>(p, stage, v, my, n0, vec);
 }
 
+// Eight weights as `parts` sums of 16-bit values: 16 bytes of each part's tile
+__device__ __forceinline__ void q4_store(uint32_t to, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t q4_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+// `one`: 1 in both halves (a sum as a product with 1)
+template <bool BF16>
+__host__ __device__ constexpr uint32_t q4_one() {
+    return BF16 ? 0x3F803F80u : 0x3C003C00u;
+}
+
+// d (q - 8) for eight codes in the bytes of two words' low (or high) halves, two
+// 16-bit values at a time. q - 8 has four bits, d eleven: F16 rounds their product
+// once, and the rest is a 16-bit value too. BF16 takes d in two parts of eight and
+// three bits; q - 8 times the second is exact, so a product and a sum round once.
+template <bool BF16>
+struct Q4Scale {
+    uint32_t hi, lo;
+    __device__ __forceinline__ Q4Scale(__half d) {
+        if constexpr (BF16) {
+            const __nv_bfloat16 h = __float2bfloat16_rn(__half2float(d));
+            const __nv_bfloat162 a = __halves2bfloat162(h, h);
+            const __nv_bfloat162 b = __float2bfloat162_rn(__fsub_rn(__half2float(d), __bfloat162float(h)));
+            hi = *reinterpret_cast<const uint32_t *>(&a);
+            lo = *reinterpret_cast<const uint32_t *>(&b);
+        } else {
+            const __half2 a = __halves2half2(d, d);
+            hi = *reinterpret_cast<const uint32_t *>(&a);
+            lo = 0u;
+        }
+    }
+};
+template <bool BF16>
+__device__ __forceinline__ void q4_put_pairs(const uint32_t (&codes)[4], const Q4Scale<BF16> & d, uint32_t to, int parts) {
+    uint32_t v[4], q[4], t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // 16 + q - 24 (BF16), 64 + q - 72 (F16)
+        q[i] = q4_fma<BF16>(codes[i], q4_one<BF16>(), BF16 ? 0xC1C0C1C0u : 0xD480D480u);
+        t[i] = BF16 ? q4_fma<BF16>(q[i], d.lo, 0x80008000u) : 0x80008000u;
+        v[i] = q4_fma<BF16>(q[i], d.hi, t[i]);
+    }
+    q4_store(to, v);
+    if (parts == 1) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = q4_fma<BF16>(q[i], d.hi, v[i] ^ 0x80008000u);
+        if (BF16) v[i] = q4_fma<BF16>(t[i], q4_one<BF16>(), v[i]);
+    }
+    q4_store(to + kGmmATile, v);
+}
+// bytes of codes (q << 3 | 0x80, or q << 4) as pairs of 16 + q (BF16) or 64 + q (F16)
+template <bool BF16>
+__device__ __forceinline__ void q4_pairs(uint32_t word, bool high, uint32_t & a, uint32_t & b) {
+    uint32_t v;
+    if constexpr (BF16) v = ((high ? word >> 1 : word << 3) & 0x78787878u) | 0x80808080u;
+    else v = (high ? word : word << 4) & 0xF0F0F0F0u;
+    constexpr uint32_t top = BF16 ? 0x41414141u : 0x54545454u;
+    a = __byte_perm(v, top, 0x4140);
+    b = __byte_perm(v, top, 0x4342);
+}
+
 // Four bytes of codes as f32: 16 + q, the code in the upper bits of the mantissa
 // (bytes of 0x80 | q << 3 into the third byte of 0x41......)
 __device__ __forceinline__ void q4_spread(uint32_t bytes, float * f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(bytes, 0x41u, 0x4055u + 0x100u * (uint32_t)i));
 }
-
-// Eight weights as `parts` sums of 16-bit values (each the rest rounded): 16
-// bytes of each part's tile
+// Eight weights from f32, each part the rest rounded
 template <bool BF16>
 __device__ __forceinline__ void q4_put(float (&w)[8], uint32_t to, int parts) {
     for (int part = 0; part < parts; ++part, to += kGmmATile) {
@@ -588,7 +655,7 @@ __device__ __forceinline__ void q4_put(float (&w)[8], uint32_t to, int parts) {
                 v[i] = *reinterpret_cast<const uint32_t *>(&h);
             }
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        q4_store(to, v);
         if (part + 1 == parts) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -844,9 +911,11 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
         // Four warps a tile of 128 rows, a lane a row, the two fours taking the
         // chunks of 64 elements in turn (a stage's barrier is at most one phase
         // behind what they wait for: they have waited for the chunk two before, in
-        // another stage, and stages come free in order). The rows' pieces come by
-        // bulk copies, a lane a row, into a ring that two warps share. (cp.async
-        // would be waited for by every fence that shows a tile to the tensor cores.)
+        // another stage, and stages come free in order). The rows' pieces come into a
+        // ring that two warps share: by TMA boxes, or, where rows do not start on
+        // 16 bytes, by bulk copies, a lane a row (32 of those keep a warp for 2800
+        // cycles; cp.async would be waited for by every fence that shows a tile to
+        // the tensor cores).
         if constexpr (SRC != GMM_TILES) {
             constexpr bool Q41 = SRC >= GMM_Q4_1_F16, BF = SRC == GMM_Q4_0_BF16 || SRC == GMM_Q4_1_BF16;
             constexpr int kPair = Q41 ? 40 : 36, kWords = kPair / 4;
@@ -863,11 +932,30 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
             GmmTile aq{};
             int a_step = 0, issued = 0;
             if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
+            auto step_on = [&] {
+                ++issued;
+                if (++a_step == steps) {
+                    a_step = 0;
+                    advance(aw);
+                    if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
+                }
+            };
             auto fetch = [&] {
                 if (odd != 0 || aw.t >= tiles || !ok) return;
                 const int s = issued % kGmmQ4Stages;
                 if (issued >= kGmmQ4Stages) ok = gmm_wait<1>(&raw_empty[rg][s], (uint32_t)((issued / kGmmQ4Stages - 1) & 1), &abort_flag);
                 if (!ok) return;
+                if (p.boxes) {
+                    // (one copy; words behind the row's and rows behind the last are zeros)
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(&raw_full[rg][s], 32u * kPitch);
+                        tma_load_3d(raw + (uint32_t)(rg * kGmmQ4Stages + s) * (32u * kPitch), GLU && rg >= 2 ? &p.umap : &p.wmap,
+                                    a_step * (kGmmQ4Chunks * kWords), aq.m0 + rank * kOut + base_row - lane, aq.g, &raw_full[rg][s]);
+                    }
+                    __syncwarp();
+                    step_on();
+                    return;
+                }
                 const int m = aq.m0 + rank * kOut + base_row, n = min(kGmmQ4Chunks, nk - a_step * kGmmQ4Chunks);
                 const uint8_t * a = w_of + (int64_t)aq.g * p.nb02 + (int64_t)m * p.nb01 + (int64_t)a_step * (kGmmQ4Chunks * kPair);
                 const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(a) & 15u;
@@ -884,12 +972,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                 if (lane == 0) mbar_arrive_expect_tx(&raw_full[rg][s], sum);
                 __syncwarp();
                 if (bytes != 0u) bulk_g2s(to, from, bytes, &raw_full[rg][s]);
-                ++issued;
-                if (++a_step == steps) {
-                    a_step = 0;
-                    advance(aw);
-                    if (aw.t < tiles) aq = gmm_tile<kRound, SRC>(p, pre, aw.t, kOut * CTAS);
-                }
+                step_on();
             };
             fetch();
             const int row = rg * 32 + lane;
@@ -942,33 +1025,35 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
 #pragma unroll
                     for (int blk = 0; blk < 2; ++blk) {
                         // Q4_0: words 0 .. 4 and 4 .. 8 (codes from the middle of a word on in the first block); Q4_1: five each
-                        uint32_t qs[4];
-                        float d, c;
                         if constexpr (Q41) {
                             const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[5 * blk]));
-                            d = head.x;
-                            c = __fmaf_rn(-16.0f, d, head.y);
+                            const float d = head.x, c = __fmaf_rn(-16.0f, d, head.y);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) qs[i] = v[5 * blk + 1 + i];
+                            for (int i = 0; i < 4; ++i) {
+                                // elements 8 i .. 8 i + 7 of the block: d q + m
+                                float f[8];
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const uint32_t b = v[5 * blk + 1 + 2 * (i & 1) + j];
+                                    q4_spread(((i < 2 ? b << 3 : b >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
+                                q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
+                            }
                         } else {
-                            const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[4 * blk]));
-                            d = blk == 0 ? head.x : head.y;
-                            c = __fmul_rn(-24.0f, d);
+                            const __half2 head = *reinterpret_cast<const __half2 *>(&v[4 * blk]);
+                            const Q4Scale<BF> d(blk == 0 ? __low2half(head) : __high2half(head));
+                            uint32_t qs[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) qs[i] = blk == 0 ? __byte_perm(v[i], v[i + 1], 0x5432) : v[5 + i];
-                        }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            // elements 8 i .. 8 i + 7 of the block
-                            float f[8];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const uint32_t b = qs[2 * (i & 1) + j];
-                                q4_spread(((i < 2 ? b << 3 : b >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t codes[4];
+                                q4_pairs<BF>(qs[2 * (i & 1)], i >= 2, codes[0], codes[1]);
+                                q4_pairs<BF>(qs[2 * (i & 1) + 1], i >= 2, codes[2], codes[3]);
+                                q4_put_pairs<BF>(codes, d, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
                             }
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
-                            q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
                         }
                     }
                     fence_async_smem();

@@ -61,6 +61,18 @@ const void * q4_tiles_kernel(bool bf16, bool q41) {
     return bf16 ? (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_BF16> : (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_F16>;
 }
 
+// rows of blocks as 32-bit words, boxes of a stage's words (rounded up to an odd number of 16 bytes) by 32 rows
+bool encode_blocks(CUtensorMap * map, const void * base, bool q41, int64_t K, int64_t rows, int64_t nb1, int64_t mats, int64_t nb2) {
+    const auto enc = map_encoder();
+    if (enc == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)(K / 64 * (q41 ? 10 : 9)), (cuuint64_t)rows, (cuuint64_t)mats};
+    const cuuint64_t strides[2] = {(cuuint64_t)nb1, (cuuint64_t)nb2};
+    const cuuint32_t boxes[3] = {gx::gmm_q4_pitch(q41) / 4u, 32u, 1u};
+    const cuuint32_t elem[3] = {1u, 1u, 1u};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void *>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Many rows per matrix: the grouped products' kernel on CTA pairs, its matrix
 // tiles made from the blocks.
 int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11, int64_t touched, void * stream) {
@@ -75,6 +87,9 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     p.acc = p.seg ? p.nt : 256;
     p.box = p.nt / 2;
     if (!encode_rows(&p.xmap, p.bf16 != 0, b, p.K, p.x_rows, nb11, 0, 0, p.gather ? 1u : (uint32_t)p.box)) return GX_ERR_ALIGN;
+    // rows on 16 bytes come as boxes of 32 rows by a stage's words
+    p.boxes = p.nb01 % 16 == 0 && p.nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, p.K, p.N, p.nb01, p.G, p.nb02) &&
+              encode_blocks(&p.umap, p.w1, q41, p.K, p.N, p.nb01, p.G, p.nb02);
     p.split = 1;
     const int out_rows = gx::gmm_out_rows(mode) * 2;
     p.mt = (int32_t)((p.N + out_rows - 1) / out_rows);
