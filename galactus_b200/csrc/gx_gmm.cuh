@@ -604,24 +604,19 @@ struct Q4Scale {
         }
     }
 };
+// the first part of a pair, q - 8 being left in q and its product with d.lo in t
 template <bool BF16>
-__device__ __forceinline__ void q4_put_pairs(const uint32_t (&codes)[4], const Q4Scale<BF16> & d, uint32_t to, int parts) {
-    uint32_t v[4], q[4], t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // 16 + q - 24 (BF16), 64 + q - 72 (F16)
-        q[i] = q4_fma<BF16>(codes[i], q4_one<BF16>(), BF16 ? 0xC1C0C1C0u : 0xD480D480u);
-        t[i] = BF16 ? q4_fma<BF16>(q[i], d.lo, 0x80008000u) : 0x80008000u;
-        v[i] = q4_fma<BF16>(q[i], d.hi, t[i]);
-    }
-    q4_store(to, v);
-    if (parts == 1) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = q4_fma<BF16>(q[i], d.hi, v[i] ^ 0x80008000u);
-        if (BF16) v[i] = q4_fma<BF16>(t[i], q4_one<BF16>(), v[i]);
-    }
-    q4_store(to + kGmmATile, v);
+__device__ __forceinline__ uint32_t q4_first_part(uint32_t & q, uint32_t & t, const Q4Scale<BF16> & d) {
+    // 16 + q - 24 (BF16), 64 + q - 72 (F16)
+    q = q4_fma<BF16>(q, q4_one<BF16>(), BF16 ? 0xC1C0C1C0u : 0xD480D480u);
+    t = BF16 ? q4_fma<BF16>(q, d.lo, 0x80008000u) : 0x80008000u;
+    return q4_fma<BF16>(q, d.hi, t);
+}
+// and what is left of it
+template <bool BF16>
+__device__ __forceinline__ uint32_t q4_second_part(uint32_t v, uint32_t q, uint32_t t, const Q4Scale<BF16> & d) {
+    v = q4_fma<BF16>(q, d.hi, v ^ 0x80008000u);
+    return BF16 ? q4_fma<BF16>(t, q4_one<BF16>(), v) : v;
 }
 // bytes of codes (q << 3 | 0x80, or q << 4) as pairs of 16 + q (BF16) or 64 + q (F16)
 template <bool BF16>
@@ -983,22 +978,18 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                 // where the lane's row starts inside its 16 bytes
                 const uint32_t low = (uint32_t)reinterpret_cast<uintptr_t>(w_of) + (uint32_t)q.g * (uint32_t)p.nb02 +
                                      (uint32_t)(q.m0 + rank * kOut + base_row) * (uint32_t)p.nb01;
-                uint32_t src = 0, skew = 0;
-                for (int kc = 0; kc < nk; ++kc, at.next(p.stages)) {
-                    const int in = kc % kGmmQ4Chunks, rs = taken % kGmmQ4Stages;
-                    if (in == 0) {
-                        fetch();
-                        ok = ok && gmm_wait<1>(&raw_full[rg][rs], (uint32_t)((taken / kGmmQ4Stages) & 1), &abort_flag);
-                        if (!ok) break;
-                        skew = (low + (uint32_t)(kc * kPair)) & 15u;
-                        src = smem_u32(my + (uint32_t)rs * (32u * kPitch));
-                    }
-                    const bool mine = turn == odd;
-                    turn ^= 1;
-                    // the chunk's words, out of three or four pieces of 16 bytes
-                    constexpr int kPieces = (kPair + 12 + 15) / 16;
-                    uint32_t v[4 * kPieces];
-                    if (mine) {
+                for (int kc = 0; kc < nk && ok; kc += kGmmQ4Chunks) {
+                    const int rs = taken % kGmmQ4Stages, n = min(kGmmQ4Chunks, nk - kc);
+                    fetch();
+                    ok = ok && gmm_wait<1>(&raw_full[rg][rs], (uint32_t)((taken / kGmmQ4Stages) & 1), &abort_flag);
+                    if (!ok) break;
+                    const uint32_t skew = (low + (uint32_t)(kc * kPair)) & 15u;
+                    const uint32_t src = smem_u32(my + (uint32_t)rs * (32u * kPitch));
+                    for (int in = 0; in < n; ++in, turn ^= 1, at.next(p.stages)) {
+                        if (turn != odd) continue;
+                        // the chunk's words, out of three or four pieces of 16 bytes
+                        constexpr int kPieces = (kPair + 12 + 15) / 16;
+                        uint32_t v[4 * kPieces];
                         const uint32_t o = skew + (uint32_t)(in * kPair), a = src + (o & ~15u);
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i)
@@ -1010,56 +1001,71 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                         for (int i = 0; i + 2 < 4 * kPieces && i < kWords + 1; ++i) v[i] = o & 8u ? v[i + 2] : v[i];
 #pragma unroll
                         for (int i = 0; i < kWords; ++i) v[i] = o & 4u ? v[i + 1] : v[i];
-                    }
-                    if (in + 1 == kGmmQ4Chunks || kc + 1 == nk) {
-                        __syncwarp();
-                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&raw_empty[rg][rs])) : "memory");
-                        ++taken;
-                    }
-                    if (!mine) continue;
-                    if (at.round != 0) {
-                        ok = gmm_wait<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag);
-                        if (!ok) break;
-                    }
-                    const uint32_t tile = smem_u32(ring + (uint32_t)at.s * stage_bytes) + (uint32_t)row * 128u;
-#pragma unroll
-                    for (int blk = 0; blk < 2; ++blk) {
-                        // Q4_0: words 0 .. 4 and 4 .. 8 (codes from the middle of a word on in the first block); Q4_1: five each
+                        const uint32_t tile = smem_u32(ring + (uint32_t)at.s * stage_bytes) + (uint32_t)row * 128u;
+                        auto place = [&](int blk, int i) { return tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4); };
+                        auto mine = [&] { return at.round == 0 || gmm_wait<CTAS>(empty + at.s, (at.round - 1u) & 1u, &abort_flag); };
                         if constexpr (Q41) {
-                            const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[5 * blk]));
-                            const float d = head.x, c = __fmaf_rn(-16.0f, d, head.y);
+                            ok = mine();
+                            if (!ok) break;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // elements 8 i .. 8 i + 7 of the block: d q + m
-                                float f[8];
+                            for (int blk = 0; blk < 2; ++blk) {
+                                const float2 head = __half22float2(*reinterpret_cast<const __half2 *>(&v[5 * blk]));
+                                const float d = head.x, c = __fmaf_rn(-16.0f, d, head.y);
 #pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    const uint32_t b = v[5 * blk + 1 + 2 * (i & 1) + j];
-                                    q4_spread(((i < 2 ? b << 3 : b >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                                for (int i = 0; i < 4; ++i) {
+                                    // elements 8 i .. 8 i + 7 of the block: d q + m
+                                    float f[8];
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+                                        const uint32_t b = v[5 * blk + 1 + 2 * (i & 1) + j];
+                                        q4_spread(((i < 2 ? b << 3 : b >> 1) & 0x78787878u) | 0x80808080u, f + 4 * j);
+                                    }
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
+                                    q4_put<BF>(f, place(blk, i), p.parts);
                                 }
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) f[j] = __fmaf_rn(f[j], d, c);
-                                q4_put<BF>(f, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
                             }
                         } else {
-                            const __half2 head = *reinterpret_cast<const __half2 *>(&v[4 * blk]);
-                            const Q4Scale<BF> d(blk == 0 ? __low2half(head) : __high2half(head));
-                            uint32_t qs[4];
+                            // words 0 .. 4 and 4 .. 8: the first block's codes begin in the middle of a word
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) qs[i] = blk == 0 ? __byte_perm(v[i], v[i + 1], 0x5432) : v[5 + i];
+                            for (int blk = 0; blk < 2; ++blk) {
+                                const __half2 head = *reinterpret_cast<const __half2 *>(&v[4 * blk]);
+                                const Q4Scale<BF> d(blk == 0 ? __low2half(head) : __high2half(head));
+                                uint32_t qs[4], q[4][4], t[4][4], w[4][4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t codes[4];
-                                q4_pairs<BF>(qs[2 * (i & 1)], i >= 2, codes[0], codes[1]);
-                                q4_pairs<BF>(qs[2 * (i & 1) + 1], i >= 2, codes[2], codes[3]);
-                                q4_put_pairs<BF>(codes, d, tile + (uint32_t)(((4 * blk + i) ^ (row & 7)) << 4), p.parts);
+                                for (int i = 0; i < 4; ++i) qs[i] = blk == 0 ? __byte_perm(v[i], v[i + 1], 0x5432) : v[5 + i];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    // elements 8 i .. 8 i + 7 of the block
+                                    q4_pairs<BF>(qs[2 * (i & 1)], i >= 2, q[i][0], q[i][1]);
+                                    q4_pairs<BF>(qs[2 * (i & 1) + 1], i >= 2, q[i][2], q[i][3]);
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) w[i][j] = q4_first_part<BF>(q[i][j], t[i][j], d);
+                                }
+                                // (the first half is made before the stage is free)
+                                if (blk == 0) ok = mine();
+                                if (!ok) break;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) q4_store(place(blk, i), w[i]);
+                                if (p.parts > 1) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                                        for (int j = 0; j < 4; ++j) w[i][j] = q4_second_part<BF>(w[i][j], q[i][j], t[i][j], d);
+                                        q4_store(place(blk, i) + kGmmATile, w[i]);
+                                    }
+                                }
                             }
+                            if (!ok) break;
                         }
+                        fence_async_smem();
+                        __syncwarp();
+                        // (the fence has put the tile where the tensor cores of both CTAs see it: no release over the cluster)
+                        if (lane == 0) gmm_arrive<CTAS>(full + at.s);
                     }
-                    fence_async_smem();
                     __syncwarp();
-                    // (the fence has put the tile where the tensor cores of both CTAs see it: no release over the cluster)
-                    if (lane == 0) gmm_arrive<CTAS>(full + at.s);
+                    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&raw_empty[rg][rs])) : "memory");
+                    ++taken;
                 }
             }
             // copies in flight land before the CTA leaves

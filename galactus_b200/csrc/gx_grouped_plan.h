@@ -38,7 +38,7 @@ constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer
 // stage's rows (an odd number of 16 bytes: eight rows then lie in different
 // banks; 12 bytes more than the blocks take, as rows start on any 4 bytes)
 constexpr int kGmmQ4Warps = 8;
-constexpr int kGmmQ4Chunks = 8;
+constexpr int kGmmQ4Chunks = 4;
 constexpr int kGmmQ4Stages = 2;
 GX_HD constexpr uint32_t gmm_q4_pitch(bool q41) { return 16u * (((uint32_t)kGmmQ4Chunks * (q41 ? 40u : 36u) + 12u + 15u) / 16u | 1u); }
 GX_HD constexpr uint32_t gmm_q4_raw(bool q41) { return 4u * kGmmQ4Stages * 32u * gmm_q4_pitch(q41); }
