@@ -664,13 +664,14 @@ __device__ __forceinline__ void q4_put(float (&w)[8], uint32_t to, int parts) {
 }
 
 template <int CTAS, int MODE, int SRC>
-__global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * kGmmQ4Warps : 0), 1)
+__global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_threads(MODE), 1)
     k_gmm(const __grid_constant__ GmmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kGmmMaxStages], empty[kGmmMaxStages], acc_full[2], acc_empty[2], part_full, part_free[2], drained;
     __shared__ uint32_t tslot;
-    __shared__ int4 gather_mem[kGmmGatherWarps * 8];
+    __shared__ int4 gather_mem[SRC != GMM_TILES ? 3 * kGmmQ4Quads : kGmmGatherWarps * 8];
     constexpr int kQ4 = SRC != GMM_TILES ? kGmmQ4Warps : 0;              // warps that make matrix tiles
+    constexpr int kGather = SRC != GMM_TILES ? kGmmQ4GatherWarps : kGmmGatherWarps;
     __shared__ uint64_t raw_full[kQ4 ? 4 : 1][kGmmQ4Stages], raw_empty[kQ4 ? 4 : 1][kGmmQ4Stages];
     __shared__ int32_t wsum[gmm_threads(MODE) / 32 + kQ4];
     __shared__ int abort_flag;
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
 
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(full + i, 1 + CTAS * (kQ4 / 2));
+            mbar_init(full + i, SRC != GMM_TILES ? CTAS * ((p.gather ? 1 + kGmmQ4GatherWarps : 1) + kQ4 / 2) : 1);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -751,7 +752,76 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
     auto end_chunk = [&](const Work & w) { return w.shared ? nk * (me + 1) / split : nk; };
     const int gathering = p.gather ? (p.nt / CTAS + 31) / 32 : 0;        // warps that gather
 
-    if (warp == 0) {
+    if (SRC != GMM_TILES && (warp == 0 || (warp >= 2 && warp < 2 + kGmmQ4GatherWarps))) {
+        // --------------------------------------- rows, beside 4-bit weights
+        // Rows in place by one thread, or gathered by three warps, which take the
+        // fours of a CTA's rows in turn. Each arrives at every stage, with rows or
+        // without: a stage that did not wait for it could go round the ring twice
+        // before it looks, and the parity of its barrier would then say the opposite
+        // (this timed out once, with groups of a few rows among long ones).
+        const int gi = warp == 0 ? 0 : warp - 1;
+        if (gi == 0 || p.gather != 0) {
+            int32_t * rows = gather_rows + gi * (4 * kGmmQ4Quads);
+            RingPos at;
+            bool ok = true;
+            int c = 0, done = 0;       // chunks started; chunks whose stage was handed back
+            for (Work w = start(); w.t < tiles && ok; advance(w)) {
+                const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
+                const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
+                auto rows_of = [&](int r) { return max(0, min(half, q.cnt - r * half)); };
+                const int n = rows_of(rank), r0 = q.row0 + rank * half, all_quads = (n + 3) >> 2;
+                const int quads = p.gather ? (all_quads - gi + 2) / 3 : 0, boxes = p.gather ? 0 : (n + p.box - 1) / p.box;
+                uint32_t bytes = 0;
+                for (int r = 0; r < CTAS; ++r)
+                    bytes += p.gather ? (uint32_t)((rows_of(r) + 3) >> 2) * 512u : (uint32_t)((rows_of(r) + p.box - 1) / p.box) * (p.box * 128u);
+                __syncwarp();
+                for (int i = lane; i < 4 * quads; i += 32) {
+                    // (rows behind the last repeat it)
+                    const int o = p.order[r0 + min(4 * (gi + 3 * (i >> 2)) + (i & 3), n - 1)];
+                    int row = o / p.gather;
+                    if (o < 0 || row >= p.x_rows) {
+                        record_error(GX_DEVERR_DOMAIN);
+                        row = 0;
+                    }
+                    rows[i] = row;
+                }
+                __syncwarp();
+                if (elect_one()) {
+                    RingPos on = at;
+                    for (int kc = 0; kc < nk; ++kc, ++c, on.next(p.stages)) {
+                        if (on.round != 0) {
+                            ok = gmm_wait_one<CTAS>(empty + on.s, (on.round - 1u) & 1u, &abort_flag);
+                            if (!ok) break;
+                            ++done;
+                        }
+                        uint64_t * bar = full + on.s;
+                        if (rank == 0 && gi == 0) mbar_arrive_expect_tx(bar, bytes);
+                        else gmm_arrive<CTAS>(bar);
+                        uint8_t * to = ring + (uint32_t)on.s * stage_bytes + kABytes;
+                        for (int b = 0; b < boxes; ++b)
+                            gmm_tma_2d<CTAS>(to + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
+                        for (int i = 0; i < quads; ++i) {
+                            const int4 r = *reinterpret_cast<const int4 *>(rows + 4 * i);
+                            gmm_gather4<CTAS>(to + (gi + 3 * i) * 512, &p.xmap, kc * kGmmK, r.x, r.y, r.z, r.w, bar);
+                        }
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                at.skip(nk, p.stages);
+            }
+            if (gi == 0 && (c = __reduce_max_sync(0xffffffffu, c)) > 0) {
+                done = __reduce_max_sync(0xffffffffu, done);
+                // (the issuer's commits arrive in both CTAs of a pair: the last ones too, before either leaves)
+                for (int i = max(0, c - p.stages); i < c && ok; ++i)
+                    ok = gmm_wait<CTAS>(empty + i % p.stages, (uint32_t)((i / p.stages) & 1), &abort_flag);
+                if (!ok && rank == 0) {
+                    // copies in flight land before the CTA leaves
+                    volatile int none = 0;
+                    for (int i = done; i < c; ++i) gmm_wait<CTAS>(full + i % p.stages, (uint32_t)((i / p.stages) & 1), &none);
+                }
+            }
+        }
+    } else if (warp == 0) {
         // ------------------------------------------- weights, rows in place
         if (elect_one()) {
             int c = 0, done = 0;       // chunks started; chunks whose stage was handed back
@@ -763,7 +833,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                 const int m0 = q.m0 + rank * kOut;
                 const int half = ((q.cnt + kRound - 1) / kRound * kRound) / CTAS;      // rows of x per CTA
                 const int r0 = q.row0 + rank * half;
-                uint32_t bytes = SRC != GMM_TILES ? 0u : (uint32_t)CTAS * kABytes;
+                uint32_t bytes = (uint32_t)CTAS * kABytes;
                 int boxes = 0;
                 for (int r = 0; r < CTAS; ++r) {
                     const int n = max(0, min(half, q.cnt - r * half));
@@ -784,8 +854,8 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                     }
                     uint8_t * st = ring + (uint32_t)at.s * stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
-                    if (SRC == GMM_TILES) gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
-                    if (SRC == GMM_TILES && MODE != GMM_PLAIN) gmm_tma_3d<CTAS>(st + kABytes / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
+                    gmm_tma_3d<CTAS>(st, &p.wmap, kc * kGmmK, m0, q.g, bar);
+                    if (MODE != GMM_PLAIN) gmm_tma_3d<CTAS>(st + kABytes / 2, &p.umap, kc * kGmmK, m0, q.g, bar);
                     for (int b = 0; b < boxes; ++b)
                         gmm_tma_2d<CTAS>(st + kABytes + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
                 }
@@ -852,7 +922,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
             }
         }
         __syncwarp();
-    } else if (warp < 2 + kGmmGatherWarps) {
+    } else if (warp < 2 + kGather) {
         // -------------------------------------------------- gathered rows
         // four rows of 128 bytes per copy (tile::gather4), up to 32 rows per
         // warp: the warp looks its rows up, one thread issues the copies. A
@@ -901,7 +971,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                 at.skip(k1 - k0, p.stages);
             }
         }
-    } else if (SRC != GMM_TILES && warp >= 2 + kGmmGatherWarps + kEpi) {
+    } else if (SRC != GMM_TILES && warp >= 2 + kGather + kEpi) {
         // --------------------------------- tiles of weights from their blocks
         // Four warps a tile of 128 rows, a lane a row, the two fours taking the
         // chunks of 64 elements in turn (a stage's barrier is at most one phase
@@ -915,7 +985,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
             constexpr bool Q41 = SRC >= GMM_Q4_1_F16, BF = SRC == GMM_Q4_0_BF16 || SRC == GMM_Q4_1_BF16;
             constexpr int kPair = Q41 ? 40 : 36, kWords = kPair / 4;
             constexpr uint32_t kPitch = gmm_q4_pitch(Q41);
-            const int qw = warp - (2 + kGmmGatherWarps + kEpi), rg = qw & 3, odd = qw >> 2;
+            const int qw = warp - (2 + kGather + kEpi), rg = qw & 3, odd = qw >> 2;
             uint8_t * my = raw + (uint32_t)rg * (kGmmQ4Stages * 32u * kPitch) + (uint32_t)lane * kPitch;
             const uint8_t * w_of = GLU && rg >= 2 ? p.w1 : p.w0;
             const uint8_t * const w_end = w_of + (int64_t)(p.G - 1) * p.nb02 + (int64_t)(p.N - 1) * p.nb01 + (int64_t)nk * kPair;
@@ -972,7 +1042,8 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
             fetch();
             const int row = rg * 32 + lane;
             RingPos at;
-            int taken = 0, turn = 0;
+            int taken = 0, lead = odd;                  // lead: chunks of others before the next own one
+            if (odd) at.next(p.stages);
             for (Work w = start(); w.t < tiles && ok; advance(w)) {
                 const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
                 // where the lane's row starts inside its 16 bytes
@@ -985,8 +1056,8 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                     if (!ok) break;
                     const uint32_t skew = (low + (uint32_t)(kc * kPair)) & 15u;
                     const uint32_t src = smem_u32(my + (uint32_t)rs * (32u * kPitch));
-                    for (int in = 0; in < n; ++in, turn ^= 1, at.next(p.stages)) {
-                        if (turn != odd) continue;
+                    int in = lead;
+                    for (; in < n; in += 2) {
                         // the chunk's words, out of three or four pieces of 16 bytes
                         constexpr int kPieces = (kPair + 12 + 15) / 16;
                         uint32_t v[4 * kPieces];
@@ -1062,7 +1133,10 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
                         __syncwarp();
                         // (the fence has put the tile where the tensor cores of both CTAs see it: no release over the cluster)
                         if (lane == 0) gmm_arrive<CTAS>(full + at.s);
+                        at.next(p.stages);
+                        at.next(p.stages);
                     }
+                    lead = in - n;
                     __syncwarp();
                     if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&raw_empty[rg][rs])) : "memory");
                     ++taken;
@@ -1076,7 +1150,7 @@ __global__ void __launch_bounds__(gmm_threads(MODE) + (SRC != GMM_TILES ? 32 * k
     } else {
         // -------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lanes 32 * quad ..
-        const int ew = warp - 2 - kGmmGatherWarps;
+        const int ew = warp - 2 - kGather;
         uint8_t * stage = staging + (uint32_t)ew * (kGmmStaging / kEpi);
         const bool vec = ((reinterpret_cast<uintptr_t>(p.dst) | (uintptr_t)p.nbd1) & 15u) == 0;
         const uint32_t lanes = (uint32_t)quad << 21, dsum = tbase + lanes + 2u * (uint32_t)p.acc;

@@ -38,6 +38,12 @@ constexpr uint32_t kGmmXchg = 2u * 2u * 2u * 16u * 32u * 4u;   // gated: [buffer
 // stage's rows (an odd number of 16 bytes: eight rows then lie in different
 // banks; 12 bytes more than the blocks take, as rows start on any 4 bytes)
 constexpr int kGmmQ4Warps = 8;
+// (Rows are gathered by three warps, the one that copies rows in place among
+// them: 16 warps in all have 128 registers a thread, 18 had 96 and kept what the
+// loops count in local memory. Two were too few: 72 cycles per four rows and warp.)
+constexpr int kGmmQ4GatherWarps = 2;           // beside the first
+constexpr int kGmmQ4Quads = 11;                // fours of rows of each, at most
+GX_HD constexpr int gmm_q4_threads(int mode) { return 32 * (2 + kGmmQ4GatherWarps + gmm_epi_warps(mode) + kGmmQ4Warps); }
 constexpr int kGmmQ4Chunks = 4;
 constexpr int kGmmQ4Stages = 2;
 GX_HD constexpr uint32_t gmm_q4_pitch(bool q41) { return 16u * (((uint32_t)kGmmQ4Chunks * (q41 ? 40u : 36u) + 12u + 15u) / 16u | 1u); }

@@ -103,7 +103,7 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     if (e != cudaSuccess) return cuda_status(e);
     p.stages = gx::gmm_q4_stages(q41, p.nt, mode, p.G, p.parts);
     const uint32_t smem = gx::kGroupedAlign + (uint32_t)p.stages * gx::gmm_q4_stage_bytes(p.nt, p.parts) + gx::gmm_q4_fixed_bytes(q41, p.nt, mode, p.G);
-    return cuda_status(launch_next(fn, dim3((unsigned)(2 * std::min<int64_t>(sms / 2, most))), gx::gmm_threads(mode) + 32 * gx::kGmmQ4Warps, smem,
+    return cuda_status(launch_next(fn, dim3((unsigned)(2 * std::min<int64_t>(sms / 2, most))), gx::gmm_q4_threads(mode), smem,
                                    2, stream, p));
 }
 
