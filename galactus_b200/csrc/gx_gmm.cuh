@@ -787,6 +787,10 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
                 }
                 __syncwarp();
                 if (elect_one()) {
+                    // (the rows in registers, the copies one behind the other: read in a loop they took 85 cycles each)
+                    int4 of[kGmmQ4Quads];
+#pragma unroll
+                    for (int i = 0; i < kGmmQ4Quads; ++i) of[i] = *reinterpret_cast<const int4 *>(rows + 4 * i);
                     RingPos on = at;
                     for (int kc = 0; kc < nk; ++kc, ++c, on.next(p.stages)) {
                         if (on.round != 0) {
@@ -798,12 +802,11 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
                         if (rank == 0 && gi == 0) mbar_arrive_expect_tx(bar, bytes);
                         else gmm_arrive<CTAS>(bar);
                         uint8_t * to = ring + (uint32_t)on.s * stage_bytes + kABytes;
-                        for (int b = 0; b < boxes; ++b)
-                            gmm_tma_2d<CTAS>(to + (uint32_t)b * (p.box * 128u), &p.xmap, kc * kGmmK, r0 + b * p.box, bar);
-                        for (int i = 0; i < quads; ++i) {
-                            const int4 r = *reinterpret_cast<const int4 *>(rows + 4 * i);
-                            gmm_gather4<CTAS>(to + (gi + 3 * i) * 512, &p.xmap, kc * kGmmK, r.x, r.y, r.z, r.w, bar);
-                        }
+                        if (boxes) gmm_tma_2d<CTAS>(to, &p.xmap, kc * kGmmK, r0, bar);      // (half a tile's rows: one box)
+#pragma unroll
+                        for (int i = 0; i < kGmmQ4Quads; ++i)
+                            if (i < quads)
+                                gmm_gather4<CTAS>(to + (gi + 3 * i) * 512, &p.xmap, kc * kGmmK, of[i].x, of[i].y, of[i].z, of[i].w, bar);
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
