@@ -83,6 +83,7 @@ struct GmmParams {
     const uint8_t * w1;       // U
     int64_t nb01, nb02;
     int32_t parts;            // 16-bit parts that a weight is made of
+    int32_t lo;               // rows of the shortest group that the launch is for
     int32_t boxes;            // rows on 16 bytes: wmap and umap are maps of the blocks, [words of a row, N, G]
 };
 
@@ -719,7 +720,9 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
         griddep_wait();
     }
     tile_prefix(pre, wsum, p.G, p.nt, p.most, [&](int g) {
-        return SRC != GMM_TILES && p.offsets == nullptr ? make_int2(0, p.n_rows) : group_rows_of(p.offsets, g, p.n_rows);
+        if (SRC != GMM_TILES && p.offsets == nullptr) return make_int2(0, p.n_rows);
+        const int2 r = group_rows_of(p.offsets, g, p.n_rows);
+        return SRC != GMM_TILES && r.y - r.x < p.lo ? make_int2(0, 0) : r;
     });
     tc_fence_before();
     if (CTAS * split == 1) __syncthreads(); else cluster_sync_all();

@@ -23,7 +23,9 @@ namespace {
 enum KernelSlot : int { kSlotQ4 = 0, kSlotRows = 8, kSlotTiles = kSlotRows + 6, kSlotEnd = kSlotTiles + 8 };
 static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
 
-constexpr int64_t kTileRows = 8;       // rows per matrix on average, above which matrix tiles are made for the tensor cores
+// Rows of a group above which matrix tiles are made for the tensor cores. (Two
+// passes of eight rows cost 700 cycles per 8192 weights and SM, a tile 900.)
+constexpr int64_t kTileRows = 16;
 
 // A launch that may begin while the kernel before it on the stream ends: the
 // kernels wait (griddepcontrol.wait) before they read or write anything.
@@ -61,13 +63,14 @@ const void * q4_tiles_kernel(bool bf16, bool q41) {
     return bf16 ? (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_BF16> : (const void *)gx::k_gmm<2, MODE, gx::GMM_Q4_0_F16>;
 }
 
-// rows of blocks as 32-bit words, boxes of a stage's words (rounded up to an odd number of 16 bytes) by 32 rows
-bool encode_blocks(CUtensorMap * map, const void * base, bool q41, int64_t K, int64_t rows, int64_t nb1, int64_t mats, int64_t nb2) {
+// rows of blocks as 32-bit words, boxes of `words` by `rows`
+bool encode_blocks(CUtensorMap * map, const void * base, bool q41, int64_t K, int64_t N, int64_t nb1, int64_t mats, int64_t nb2, uint32_t words,
+                   uint32_t rows) {
     const auto enc = map_encoder();
     if (enc == nullptr) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)(K / 64 * (q41 ? 10 : 9)), (cuuint64_t)rows, (cuuint64_t)mats};
+    const cuuint64_t dims[3] = {(cuuint64_t)(K / 64 * (q41 ? 10 : 9)), (cuuint64_t)N, (cuuint64_t)mats};
     const cuuint64_t strides[2] = {(cuuint64_t)nb1, (cuuint64_t)nb2};
-    const cuuint32_t boxes[3] = {gx::gmm_q4_pitch(q41) / 4u, 32u, 1u};
+    const cuuint32_t boxes[3] = {words, rows, 1u};
     const cuuint32_t elem[3] = {1u, 1u, 1u};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void *>(base), dims, strides, boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -88,8 +91,8 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     p.box = p.nt / 2;
     if (!encode_rows(&p.xmap, p.bf16 != 0, b, p.K, p.x_rows, nb11, 0, 0, p.gather ? 1u : (uint32_t)p.box)) return GX_ERR_ALIGN;
     // rows on 16 bytes come as boxes of 32 rows by a stage's words
-    p.boxes = p.nb01 % 16 == 0 && p.nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, p.K, p.N, p.nb01, p.G, p.nb02) &&
-              encode_blocks(&p.umap, p.w1, q41, p.K, p.N, p.nb01, p.G, p.nb02);
+    p.boxes = p.nb01 % 16 == 0 && p.nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, p.K, p.N, p.nb01, p.G, p.nb02, gx::gmm_q4_pitch(q41) / 4u, 32u) &&
+              encode_blocks(&p.umap, p.w1, q41, p.K, p.N, p.nb01, p.G, p.nb02, gx::gmm_q4_pitch(q41) / 4u, 32u);
     p.split = 1;
     const int out_rows = gx::gmm_out_rows(mode) * 2;
     p.mt = (int32_t)((p.N + out_rows - 1) / out_rows);
@@ -169,7 +172,9 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
     p.alpha = alpha;
     p.limit = limit;
     const int64_t touched = std::min(n_rows, n_as);
-    if (ids == nullptr && n_rows > kTileRows * touched) {
+    // Groups of more than kTileRows rows go to the tensor cores' tiles, shorter ones
+    // (which only the device tells apart) stream their matrices past a few rows.
+    if (ids == nullptr && n_rows > kTileRows) {
         gx::GmmParams t{};
         t.bf16 = bf16;
         t.offsets = offsets;
@@ -191,12 +196,16 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
         t.w1 = p.w1;
         t.nb01 = nb01;
         t.nb02 = nb02;
-        return q4_tiles(t, q41, glu, b, nb11, touched, stream);
+        t.lo = offsets != nullptr ? (int32_t)kTileRows + 1 : 1;
+        const int rc = q4_tiles(t, q41, glu, b, nb11, touched, stream);
+        if (rc != GX_OK || offsets == nullptr) return rc;
     }
     const gx::Q4Shape shape = gx::q4_shape(q41, ne00, n_rows);
     p.warps = shape.warps;
     p.cap = shape.cap;
     p.buffers = shape.buffers;
+    p.lo = 1;
+    p.hi = ids == nullptr ? (int32_t)kTileRows : (int32_t)kMaxIndex;
     const int rows = (glu ? 8 : 16) * gx::kQ4Mt;
     p.rt = (int32_t)((ne01 + rows - 1) / rows);
     const int64_t tiles = n_rows / p.cap + touched, most = p.rt * tiles;
@@ -204,18 +213,17 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
     p.most = (int32_t)tiles;
     const int sms = device_sms();
     if (sms == 0) return GX_ERR_CUDA;
-    // Warps that share K: as many as make the rounds of jobs cheapest, about four
-    // pairs of blocks being spent on what a job has beside them.
-    const int64_t jobs = p.rt * (touched + (n_rows - touched) / p.cap), pairs = ne00 / 64;
-    int64_t best = 0;
-    for (int c = 1; c <= p.warps; ++c) {
-        if (p.warps % c) continue;
-        const int64_t units = (int64_t)sms * (p.warps / c), cost = (jobs + units - 1) / units * ((pairs + c - 1) / c + (c == 1 ? 4 : 6));
-        if (c == 1 || cost < best) {
-            best = cost;
-            p.share = c;
-        }
-    }
+    // Warps that share K: as many as leave four fifths of the jobs a team each. In
+    // us with 2, 4, 8 and 16 of 16 warps, one row, the choice marked: 512 jobs of 12
+    // pairs of blocks 10.9, 9.4*, 11.0, 12.7; 720 of 45: 30, 23*, 24, 26; 448 of 64:
+    // 19.1, 17.8*, 18.5, 20.3; 128 of 64: 16.9, 11.2, 8.5, 8.3*.
+    const int64_t jobs = p.rt * (touched + (n_rows - touched) / p.cap);
+    p.share = 2;
+    for (int c = 4; c <= p.warps; c += 2)
+        if (p.warps % c == 0 && (int64_t)sms * (p.warps / c) * 5 >= jobs * 4) p.share = c;
+    const uint32_t words = (uint32_t)gx::q4_pitch(q41) / 4u, box = glu ? 16u : 32u;
+    p.boxes = nb01 % 16 == 0 && nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, ne00, ne01, nb01, n_as, nb02, words, box) &&
+              encode_blocks(&p.umap, p.w1, q41, ne00, ne01, nb01, n_as, nb02, words, box);
     const void * fn = q4_kernel(bf16, q41, glu);
     const int slot = kSlotQ4 + (bf16 ? 4 : 0) + (q41 ? 2 : 0) + (glu ? 1 : 0);
     cudaError_t e = allow_smem(fn, slot, gx::kQ4Smem);

@@ -15,6 +15,7 @@
 namespace gx {
 
 struct Q4Params {
+    CUtensorMap wmap, umap;   // their blocks as [words of a row, N, G], where rows lie on 16 bytes (boxes)
     const uint8_t * w0;       // W, or the gate matrices
     const uint8_t * w1;       // the up matrices
     int64_t nb01, nb02;
@@ -37,10 +38,16 @@ struct Q4Params {
     int32_t share;            // warps that share a job's K (a divisor of the CTA's)
     int32_t cap;              // rows of x per tile
     int32_t buffers;          // tiles of x in shared memory
+    int32_t boxes;
+    int32_t lo, hi;           // rows of the groups that this launch is for
 };
 
 // ---------------------------------------------------------------- pieces
 
+// (the first `bytes` of 16, zeros behind them)
+__device__ __forceinline__ void q4_copy16(uint32_t dst, const uint8_t * src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ uint32_t q4_lds(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -140,7 +147,7 @@ __device__ __forceinline__ void q4_tile(const Q4Params & p, const Q4Groups & g, 
             lo = p.offsets != nullptr ? p.offsets[j.group] : 0;
             hi = p.offsets != nullptr ? p.offsets[j.group + 1] : p.n_rows;
         }
-        j.tiles = lo < 0 || hi <= lo || hi > p.n_rows ? 0 : (hi - lo - 1) / p.cap + 1;
+        j.tiles = lo < 0 || hi - lo < p.lo || hi - lo > p.hi || hi > p.n_rows ? 0 : (hi - lo - 1) / p.cap + 1;
         if (at < j.before + j.tiles || j.group + 1 >= g.n) break;
         j.before += j.tiles;
     }
@@ -196,11 +203,11 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     extern __shared__ __align__(128) uint8_t q4_smem_raw[];
     __shared__ int32_t wsum[kQ4Warps], pre[32 * kQ4Warps + 1];
     __shared__ int32_t s_order[kQ4MaxIds], s_key[kQ4MaxIds], s_lead[kQ4MaxIds], s_expert[kQ4MaxIds], s_start[kQ4MaxIds + 1];
-    __shared__ uint64_t full[2], empty[2], ring_full[kQ4Warps][S];
+    __shared__ uint64_t full[2], empty[2], ring_full[kQ4Warps / 2][S], ring_free[kQ4Warps / 2][S];
     __shared__ int abort_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, W = p.warps;
     const int g = lane >> 2, t = lane & 3;
-    float * red = reinterpret_cast<float *>(q4_smem_raw + W * S * kStage);
+    float * red = reinterpret_cast<float *>(q4_smem_raw + W / 2 * S * kStage);
     uint8_t * xbuf = reinterpret_cast<uint8_t *>(red + W * kRed);
     const int x_pitch = (int)q4_x_pitch(p.K);
 
@@ -210,7 +217,10 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
             mbar_init(full + i, 1);
             mbar_init(empty + i, (uint32_t)W);
         }
-        for (int i = 0; i < W * S; ++i) mbar_init(&ring_full[0][0] + i, 1);
+        for (int i = 0; i < W / 2 * S; ++i) {
+            mbar_init(&ring_full[0][0] + i, p.boxes ? 1 : 64);
+            mbar_init(&ring_free[0][0] + i, 2);
+        }
         abort_flag = 0;
         mbar_fence_init();
     }
@@ -264,7 +274,10 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
         q4_prefix(pre, wsum, gr.n, gr.per, p.cap, p.most, [&](int i) { return make_int2(s_start[i], s_start[i + 1]); });
     } else if (p.offsets != nullptr) {
         gr.per = (p.G + (int)blockDim.x - 1) / (int)blockDim.x;
-        q4_prefix(pre, wsum, p.G, gr.per, p.cap, p.most, [&](int i) { return group_rows_of(p.offsets, i, p.n_rows); });
+        q4_prefix(pre, wsum, p.G, gr.per, p.cap, p.most, [&](int i) {
+            const int2 r = group_rows_of(p.offsets, i, p.n_rows);
+            return r.y - r.x < p.lo || r.y - r.x > p.hi ? make_int2(0, 0) : r;
+        });
     } else {
         q4_prefix(pre, wsum, 1, 1, p.cap, p.most, [&](int) { return make_int2(0, p.n_rows); });
     }
@@ -276,10 +289,13 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     if (j0 == j1) return;
     const int share = p.share, team = warp / share, member = warp - team * share, teams = W / share;
     const int pairs = p.K / 64;
-    const int p0 = pairs * member / share, p1 = pairs * (member + 1) / share;
-    uint8_t * const ring_base = q4_smem_raw + warp * (S * kStage);
+    // A ring per two warps, which take its chunks' pairs of blocks in turn: a share
+    // of K is theirs together. (Boxes start on 16 bytes: every fourth pair.)
+    const int unit = p.boxes ? 4 : 1, parts = (pairs + unit - 1) / unit, of = share / 2, part2 = member >> 1, odd = member & 1;
+    const int p0 = min(pairs, unit * (parts * part2 / of)), p1 = min(pairs, unit * (parts * (part2 + 1) / of));
+    uint8_t * const ring_base = q4_smem_raw + (warp >> 1) * (S * kStage);
     const uint32_t ring = smem_u32(ring_base);
-    uint64_t * const filled = ring_full[warp];
+    uint64_t * const filled = ring_full[warp >> 1], * const freed = ring_free[warp >> 1];
     const int t0 = j0 / p.rt, t1 = (j1 - 1) / p.rt;                 // tiles of rows of the run
     auto m_begin = [&](int tile) { return tile == t0 ? j0 - t0 * p.rt : 0; };
     auto m_end = [&](int tile) { return tile == t1 ? j1 - t1 * p.rt : p.rt; };
@@ -297,38 +313,52 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     q4_tile(p, gr, t0, ahead);
     Q4Tile job = ahead;
     ahead_enter();
-    // A lane copies the chunk's piece of one row: rows 16 m + 8 h + g of the tile,
-    // from 16 bytes before their first one on. (The last piece of the last row
-    // ends with the matrix: what is not whole 16 bytes is moved by hand.)
-    const bool second = GLU && (lane & 8);
-    const int lane_row = GLU ? (lane >> 4) * 8 + (lane & 7) : lane;
-    const uint8_t * const w_lane = second ? p.w1 : p.w0;
-    const uint8_t * const w_end = w_lane + (int64_t)(p.G - 1) * p.nb02 + (int64_t)(p.N - 1) * p.nb01 + (int64_t)(p.K / 64) * kPair;
+    // Rows of a stage: 16 m + 8 h + g, or (gated) 16 h + 8 m + g: the gate's, the
+    // up's. Where rows lie on 16 bytes they come as TMA boxes; elsewhere both warps
+    // copy, eight lanes a row, pieces of 16 bytes from 16 bytes before its first one on.
+    const int sub = lane >> 3, col = lane & 7;
+    const int64_t up = p.w1 - p.w0;
+    bool ok = true;
     auto issue = [&] {
-        if (ahead_tile <= t1 && p0 < p1) {
-            const int n = min(CP, p1 - ahead_pair), row = ahead_m * kRows + lane_row;
-            const uint8_t * a = w_lane + (int64_t)ahead.e * p.nb02 + (int64_t)row * p.nb01 + (int64_t)ahead_pair * kPair;
-            const uint32_t skew = (uint32_t)reinterpret_cast<uintptr_t>(a) & 15u;
-            uint32_t bytes = row < p.N ? (skew + (uint32_t)(n * kPair) + 15u) & ~15u : 0u;     // (rows behind the last: nothing)
-            const uint8_t * from = a - skew;
-            uint8_t * to = ring_base + put * kStage + lane * kPitch;
-            if (bytes != 0u && from + bytes > w_end) {
-                bytes -= 16u;
-                for (const uint8_t * b = from + bytes; b < w_end; b += 4)
-                    *reinterpret_cast<uint32_t *>(to + (b - from)) = *reinterpret_cast<const uint32_t *>(b);
+        if ((odd && p.boxes) || ahead_tile > t1 || p0 >= p1) return;
+        if (issued >= S) ok = ok && gmm_wait<1>(freed + put, (uint32_t)((issued / S - 1) & 1), &abort_flag);
+        if (!ok) return;
+        const int n = min(CP, p1 - ahead_pair);
+        uint8_t * const stage = ring_base + put * kStage;
+        if (p.boxes) {
+            if (elect_one()) {
+                mbar_arrive_expect_tx(filled + put, (uint32_t)kStage);
+                tma_load_3d(stage, &p.wmap, ahead_pair * (kPair / 4), ahead_m * kRows, ahead.e, filled + put);
+                if (GLU) tma_load_3d(stage + kStage / 2, &p.umap, ahead_pair * (kPair / 4), ahead_m * kRows, ahead.e, filled + put);
             }
-            const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
-            if (lane == 0) mbar_arrive_expect_tx(filled + put, sum);
             __syncwarp();
-            if (bytes != 0u) bulk_g2s(to, from, bytes, filled + put);
-            put = put + 1 == S ? 0 : put + 1;
-            ++issued;
-            ahead_pair += n;
-            if (ahead_pair >= p1) {
-                ahead_pair = p0;
-                ahead_m += teams;
-                ahead_enter();
+        } else {
+            const int r0 = ahead_m * kRows + sub;
+            const uint8_t * a = p.w0 + (int64_t)ahead.e * p.nb02 + (int64_t)r0 * p.nb01 + (int64_t)ahead_pair * kPair;
+            const int skew = (int)(reinterpret_cast<uintptr_t>(a) & 15u), need = skew + n * kPair - col * 16;
+            a += col * 16 - skew;
+            const uint32_t to = smem_u32(stage) + (uint32_t)((16 * odd + sub) * kPitch + col * 16);
+            const int half = GLU ? 0 : 16 * odd;                    // (each warp half of the stage's rows)
+            if (GLU && odd) a += up;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                           // row 4 i + sub of the half
+                const int row = half + 4 * i;
+                const uint8_t * from = a + (int64_t)row * p.nb01;
+                if (r0 + row < p.N) {                               // (what lies in rows behind the last is not used)
+#pragma unroll
+                    for (int c = 0; c < (CP * kPair + 12 + 127) / 128; ++c)
+                        if (c * 128 < need) q4_copy16(to + (uint32_t)(4 * i * kPitch + c * 128), from + c * 128, min(16, need - c * 128));
+                }
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(filled + put)) : "memory");
+        }
+        put = put + 1 == S ? 0 : put + 1;
+        ++issued;
+        ahead_pair += n;
+        if (ahead_pair >= p1) {
+            ahead_pair = p0;
+            ahead_m += teams;
+            ahead_enter();
         }
     };
 #pragma unroll
@@ -355,7 +385,6 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     // ------------------------------------------------------------ the jobs
     int take = 0;
     uint32_t round = 0;
-    bool ok = true;
     const uint32_t shift = q4_shift<BF16, Q41>();
     for (int tile = t0; tile <= t1; ++tile) {
         const int i_tile = tile - t0, b = p.buffers == 2 ? i_tile & 1 : 0;
@@ -384,7 +413,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                 const uint32_t at = ring + (uint32_t)(take * kStage + g * kPitch) + ((low + (uint32_t)(q0 * kPair)) & 15u);
                 const int n_pairs = min(CP, p1 - q0);
 #pragma unroll 2
-                for (int q = 0; q < n_pairs; ++q) {
+                for (int q = odd; q < n_pairs; q += 2) {
                     // x: elements 4t .. and 16 + 4t .. of two blocks
                     uint2 x[4];
 #pragma unroll
@@ -396,7 +425,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t r = at + (uint32_t)((16 * i + 8 * h) * kPitch) + (uint32_t)(q * kPair);
+                            const uint32_t r = at + (uint32_t)((GLU ? 16 * h + 8 * i : 16 * i + 8 * h) * kPitch) + (uint32_t)(q * kPair);
                             if constexpr (Q41) {
                                 const uint32_t s0 = q4_lds(r), s1 = q4_lds(r + 20u);
                                 q4_codes<BF16>(q4_lds(r + 4u + 4u * t), a[i][0][h]);
@@ -436,12 +465,13 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                         }
                     }
                 }
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(freed + take)) : "memory");
                 if (++take == S) {
                     take = 0;
                     round ^= 1u;
                 }
-                __syncwarp();
-                if (ok) issue();
+                issue();
             }
 
             // --------------------------- the warps' sums, added in their order
@@ -489,6 +519,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
         job = next;
     }
     // copies in flight land before the CTA leaves
+    if (!ok) asm volatile("cp.async.wait_all;" ::: "memory");
     volatile int none = 0;
     for (int i = 0; i < S && !ok; ++i)
         if (issued > i) gmm_wait<1>(filled + i, (uint32_t)((issued - 1 - i) / S & 1), &none);

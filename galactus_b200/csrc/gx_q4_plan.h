@@ -8,25 +8,19 @@ namespace gx {
 
 constexpr int kQ4MaxIds = 256;                 // rows of a call that names each row's expert (one thread a row)
 
-#ifndef GX_Q4_S
-#define GX_Q4_S 2
-#define GX_Q4_P 8
-#define GX_Q4_W 8
-#endif
-
-constexpr int kQ4Warps = GX_Q4_W;              // of a CTA, at most
-constexpr int kQ4Stages = GX_Q4_S;             // of a warp's ring
-constexpr int kQ4Pairs = GX_Q4_P;              // pairs of blocks per stage
+constexpr int kQ4Warps = 16;                   // of a CTA, at most
+constexpr int kQ4Stages = 2;                   // of the ring that two warps share
+constexpr int kQ4Pairs = 8;                    // pairs of blocks per stage
 constexpr int kQ4Mt = 2;                       // 16-row tiles of the matrix per job
 constexpr int kQ4Cols = 8;                     // rows of x per job
-
 // Bytes between the rows of a stage: an odd number of 16 bytes (eight rows then
 // lie in different banks), 12 more than the blocks take (rows start on any 4 bytes)
 GX_HD constexpr int q4_pitch(bool q41) { return 16 * (((kQ4Pairs * (q41 ? 40 : 36) + 12 + 15) / 16) | 1); }
 GX_HD constexpr int q4_stage_bytes(bool q41) { return 16 * kQ4Mt * q4_pitch(q41); }
 // A warp's sums: [columns][kQ4Red]
 constexpr int kQ4Red = 16 * kQ4Mt + 4;
-GX_HD constexpr uint32_t q4_warp_bytes(bool q41) { return (uint32_t)(kQ4Stages * q4_stage_bytes(q41) + kQ4Cols * kQ4Red * 4); }
+// two warps: their ring and their sums
+GX_HD constexpr uint32_t q4_pair_bytes(bool q41) { return (uint32_t)(kQ4Stages * q4_stage_bytes(q41) + 2 * kQ4Cols * kQ4Red * 4); }
 // a row of x (the 32 bytes more put four rows into different banks)
 GX_HD constexpr int64_t q4_x_pitch(int64_t K) { return 2 * K + 32; }
 // dynamic shared memory; the lists that the kernel declares itself take 8 KB
@@ -40,15 +34,14 @@ struct Q4Shape {
 inline Q4Shape q4_shape(bool q41, int64_t K, int64_t n_rows) {
     const int64_t row = q4_x_pitch(K);
     const int cols = n_rows < kQ4Cols ? (int)n_rows : kQ4Cols;
-    const int step = kQ4Warps / 2;
-    for (int w = kQ4Warps; w >= step; w -= step)
+    for (int w = kQ4Warps; w >= 4; w -= 4)
         for (int b = 2; b >= 1; --b)
-            if (w * (int64_t)q4_warp_bytes(q41) + b * cols * row <= kQ4Smem) return {w, cols, b};
-    const int64_t room = (int64_t)kQ4Smem - step * (int64_t)q4_warp_bytes(q41);
-    return {step, (int)(room / row), 1};
+            if (w / 2 * (int64_t)q4_pair_bytes(q41) + b * cols * row <= kQ4Smem) return {w, cols, b};
+    const int64_t room = (int64_t)kQ4Smem - 2 * (int64_t)q4_pair_bytes(q41);
+    return {4, (int)(room / row), 1};
 }
 GX_HD constexpr uint32_t q4_smem(bool q41, int64_t K, int warps, int cap, int buffers) {
-    return (uint32_t)warps * q4_warp_bytes(q41) + (uint32_t)(buffers * cap * q4_x_pitch(K));
+    return (uint32_t)(warps / 2) * q4_pair_bytes(q41) + (uint32_t)(buffers * cap * q4_x_pitch(K));
 }
 
 }  // namespace gx

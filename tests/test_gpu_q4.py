@@ -57,8 +57,8 @@ def want(w, x, kind, e, rounded=False):
 
 
 def many(rows, groups, out):
-    """Whether a call without ids makes matrix tiles of rounded weights."""
-    return rows > 8 * min(rows, groups) and out != F32
+    """Whether a call without ids may make matrix tiles of rounded weights."""
+    return rows > 16 and out != F32
 
 
 def want_glu(gate, up, x, kind, e, act, rounded=False):
