@@ -213,7 +213,7 @@ _SIGS = {
     "gx_mul_mat_q4_glu": (C.c_int, [C.c_int, _P, _P, _I64, _I64, _I64, _I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _I64,
                                     _I64, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _I64, _P]),
     "gx_rms_norm": (C.c_int, [C.c_int, _P, _I64, _I64, _I64, _P, C.c_float, C.c_int, _P, _I64, _P]),
-    "gx_block_out": (C.c_int, [C.POINTER(gx_block_desc), _P]),
+    "gx_block_out": (C.c_int, [_P, _P]),
     "gx_synth_normal": (C.c_int, [_P, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
     "gx_synth_weights": (C.c_int, [C.c_int, _P, _I64, _I64, C.c_uint64, C.c_uint64, C.c_float, _P]),
 }

@@ -5,7 +5,7 @@ of results are as in the operators on grouped rows.
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import torch
 
@@ -14,6 +14,7 @@ from .grouped import _INT, _TYPE, _device, _index, _matrices, _new, _rows, _stre
 
 _LIB = L.lib()
 _F32 = torch.float32
+_CALLS = {"gx_mul_mat_q4": _LIB.gx_mul_mat_q4, "gx_mul_mat_q4_glu": _LIB.gx_mul_mat_q4_glu}
 
 
 def _q4(name, w, up, x, type, ids, offsets, order, n_rows, gather, scatter, act, out, out_dtype, stream):
@@ -45,7 +46,8 @@ def _q4(name, w, up, x, type, ids, offsets, order, n_rows, gather, scatter, act,
         elif order is not None and n_rows > order.shape[0]:
             raise ValueError("n_rows: more than order holds")
     if out is None:
-        out = _new(stream, dev, lambda: torch.empty((n_rows, N), dtype=out_dtype or x.dtype, device=w.device))
+        kind = out_dtype or x.dtype
+        out = x.new_empty((n_rows, N), dtype=kind) if stream is None else _new(stream, dev, lambda: x.new_empty((n_rows, N), dtype=kind))
         nbd1 = N * out.element_size()
     else:
         have, cols, nbd1 = _rows(out, "out")
@@ -56,7 +58,7 @@ def _q4(name, w, up, x, type, ids, offsets, order, n_rows, gather, scatter, act,
         raise ValueError(f"results of {out.dtype}")
     b_type = _TYPE.get(x.dtype, -1)
     head = (type, w.data_ptr()) if up is None else (type, w.data_ptr(), up.data_ptr())
-    rc = getattr(_LIB, name)(*head, K, N, nb01, nb02, G, b_type, x.data_ptr(), rows, nb11, ids_ptr, offsets_ptr, order_ptr, n_rows,
+    rc = _CALLS[name](*head, K, N, nb01, nb02, G, b_type, x.data_ptr(), rows, nb11, ids_ptr, offsets_ptr, order_ptr, n_rows,
                              gather, scatter, *act, kind, out.data_ptr(), nbd1, _stream(stream, dev))
     if rc:
         L.check(rc, name)
@@ -88,12 +90,24 @@ def mul_mat_q4_glu(gate, up, x, *, type: int, ids=None, offsets=None, order=None
                out_dtype, stream)
 
 
-def _result(t, like, shape, dtype, name, stream, dev):
+# gx_block_desc, field by field (a structure's attributes, set one by one, took 5 us)
+_DESC = struct.Struct("@2q6i P2q2P P q 2P 2f P2q i f P q P q P q P")
+assert _DESC.size == L.C.sizeof(L.gx_block_desc)
+
+
+def _result(t, like, rows, cols, dtype, name, stream, dev):
     """(tensor, its type, bytes between its rows): t, or a new one."""
     if t is None:
-        t = _new(stream, dev, lambda: torch.empty(shape, dtype=dtype, device=like.device))
-    elif tuple(t.shape) != tuple(shape) or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name}: {tuple(shape)} of the result type expected")
+        if stream is None:
+            t = like.new_empty((rows, cols), dtype=dtype)
+        else:
+            t = _new(stream, dev, lambda: like.new_empty((rows, cols), dtype=dtype))
+        kind = _TYPE.get(dtype)
+        if kind is None:
+            raise ValueError(f"{name}: results of {dtype}")
+        return t, kind, cols * t.element_size()
+    if tuple(t.shape) != (rows, cols) or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name}: {(rows, cols)} of the result type expected")
     kind = _TYPE.get(t.dtype)
     if kind is None:
         raise ValueError(f"{name}: results of {t.dtype}")
@@ -108,11 +122,21 @@ def _vector(t, name, n):
     return t.data_ptr()
 
 
+def _given(t, name, rows, cols):
+    """(type, address, bytes between rows) of rows that may be absent."""
+    if t is None:
+        return 0, 0, 0
+    n, m, nb = _rows(t, name)
+    if n != rows or m != cols:
+        raise ValueError(f"{name}: [{rows}, {cols}] expected")
+    return _TYPE.get(t.dtype, -1), t.data_ptr(), nb
+
+
 def rms_norm(x, weight=None, *, eps: float = 1e-6, out=None, out_dtype=None, stream=None):
     """gx_rms_norm: rows x [T, H] / sqrt(mean(x^2) + eps) * weight (float32 [H], or ones)."""
     T, H, nb1 = _rows(x, "x")
     dev = _device(x, weight, out)
-    out, kind, nbd = _result(out, x, (T, H), out_dtype or (x.dtype if out is None else None), "out", stream, dev)
+    out, kind, nbd = _result(out, x, T, H, out_dtype or (x.dtype if out is None else None), "out", stream, dev)
     rc = _LIB.gx_rms_norm(_TYPE.get(x.dtype, -1), x.data_ptr(), H, T, nb1, _vector(weight, "weight", H), eps, kind, out.data_ptr(), nbd,
                           _stream(stream, dev))
     if rc:
@@ -129,47 +153,44 @@ def block_out(y, *, weights=None, ids=None, shared=None, shared_gate=None, norm=
     out [T, H] (of the residual's type, y's without one), and with next_norm
     (float32 [H]), next_dtype or next_out the pair (out, the next block's normed
     rows)."""
-    if y.dim() == 2:
-        y = y.unsqueeze(1)
-    if y.dim() != 3 or (y.shape[2] > 1 and y.stride(2) != 1):
+    shape, strides = y.shape, y.stride()
+    if len(shape) == 2:
+        shape, strides = (shape[0], 1, shape[1]), (strides[0], 0, strides[1])
+    if len(shape) != 3 or (shape[2] > 1 and strides[2] != 1):
         raise ValueError("y: [T, k, H] with consecutive elements in its rows expected")
-    T, k, H = y.shape
+    T, k, H = shape
     dev = _device(y, weights, ids, shared, shared_gate, norm, gate, residual, out, next_norm, next_out)
     size = y.element_size()
-    d = L.gx_block_desc(ne0=H, ne1=T, k=k, type_y=_TYPE.get(y.dtype, -1), y=y.data_ptr(), eps=eps, scale=scale,
-                        nby1=(y.stride(1) if k > 1 else H) * size, nby2=(y.stride(0) if T > 1 else k * H) * size,
-                        next_eps=eps if next_eps is None else next_eps)
-    d.weights = _vector(weights, "weights", T * k)
+    ids_ptr = 0
     if ids is not None:
         if ids.dtype is not _INT or ids.numel() != T * k or not ids.is_contiguous():
             raise ValueError(f"ids: contiguous int32 [{T}, {k}] expected")
-        d.ids = ids.data_ptr()
-    for name, t in (("shared", shared), ("residual", residual)):
-        if t is None:
-            continue
-        if tuple(t.shape) != (T, H):
-            raise ValueError(f"{name}: [{T}, {H}] expected")
-        setattr(d, name, t.data_ptr())
-        setattr(d, "type_" + name, _TYPE.get(t.dtype, -1))
-        setattr(d, "nbs" if name == "shared" else "nbr", _rows(t, name)[2])
-    d.shared_gate = _vector(shared_gate, "shared_gate", T)
-    d.norm = _vector(norm, "norm", H)
+        ids_ptr = ids.data_ptr()
+    type_shared, shared_ptr, nbs = _given(shared, "shared", T, H)
+    type_residual, residual_ptr, nbr = _given(residual, "residual", T, H)
+    gate_ptr = gne0 = nbg = 0
     if gate is not None:
-        rows, cols, nbg = _rows(gate, "gate")
-        if gate.dtype is not _F32 or rows not in (1, T) or cols not in (1, H):
+        rows, gne0, nbg = _rows(gate, "gate")
+        if gate.dtype is not _F32 or rows not in (1, T) or gne0 not in (1, H):
             raise ValueError(f"gate: float32 [{T} or 1, {H} or 1] expected")
-        d.gate, d.gne0, d.nbg = gate.data_ptr(), cols, nbg if rows > 1 else 0
-        d.gate_act = L.GATE_SIGMOID if gate_sigmoid else L.GATE_NONE
+        gate_ptr = gate.data_ptr()
+        if rows == 1:
+            nbg = 0
     if out_dtype is None and out is None:
         out_dtype = y.dtype if residual is None else residual.dtype
-    out, d.type_dst, d.nbd = _result(out, y, (T, H), out_dtype, "out", stream, dev)
-    d.dst = out.data_ptr()
+    out, type_dst, nbd = _result(out, y, T, H, out_dtype, "out", stream, dev)
     more = next_norm is not None or next_dtype is not None or next_out is not None
+    type_next = next_ptr = nbn = 0
     if more:
-        next_out, d.type_next, d.nbn = _result(next_out, y, (T, H), next_dtype or (y.dtype if next_out is None else None), "next_out",
-                                               stream, dev)
-        d.next, d.next_norm = next_out.data_ptr(), _vector(next_norm, "next_norm", H)
-    rc = _LIB.gx_block_out(C.byref(d), _stream(stream, dev))
+        next_out, type_next, nbn = _result(next_out, y, T, H, next_dtype or (y.dtype if next_out is None else None), "next_out", stream,
+                                           dev)
+        next_ptr = next_out.data_ptr()
+    desc = _DESC.pack(H, T, k, _TYPE.get(y.dtype, -1), type_shared, type_residual, type_dst, type_next, y.data_ptr(),
+                      (strides[1] if k > 1 else H) * size, (strides[0] if T > 1 else k * H) * size, _vector(weights, "weights", T * k),
+                      ids_ptr, shared_ptr, nbs, _vector(shared_gate, "shared_gate", T), _vector(norm, "norm", H), eps, scale, gate_ptr,
+                      gne0, nbg, L.GATE_SIGMOID if gate_sigmoid else L.GATE_NONE, eps if next_eps is None else next_eps, residual_ptr,
+                      nbr, out.data_ptr(), nbd, next_ptr, nbn, _vector(next_norm, "next_norm", H))
+    rc = _LIB.gx_block_out(desc, _stream(stream, dev))
     if rc:
         L.check(rc, "gx_block_out")
     return (out, next_out) if more else out

@@ -23,9 +23,11 @@ namespace {
 enum KernelSlot : int { kSlotQ4 = 0, kSlotRows = 8, kSlotTiles = kSlotRows + 6, kSlotEnd = kSlotTiles + 8 };
 static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
 
-// Rows of a group above which matrix tiles are made for the tensor cores. (Two
-// passes of eight rows cost 700 cycles per 8192 weights and SM, a tile 900.)
-constexpr int64_t kTileRows = 16;
+// Rows of a group above which matrix tiles are made for the tensor cores. In us
+// from 8, 16, 24, 32 and 48 rows on: 64 tokens x 8 of 128 experts 123, 122, 115,
+// 120, 127; 1031 tokens 174, 169, 170, 169, 174; 2048 tokens, gated, 837, 806, 817,
+// 828, 855.
+constexpr int64_t kTileRows = 24;
 
 // A launch that may begin while the kernel before it on the stream ends: the
 // kernels wait (griddepcontrol.wait) before they read or write anything.
@@ -92,7 +94,7 @@ int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11
     if (!encode_rows(&p.xmap, p.bf16 != 0, b, p.K, p.x_rows, nb11, 0, 0, p.gather ? 1u : (uint32_t)p.box)) return GX_ERR_ALIGN;
     // rows on 16 bytes come as boxes of 32 rows by a stage's words
     p.boxes = p.nb01 % 16 == 0 && p.nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, p.K, p.N, p.nb01, p.G, p.nb02, gx::gmm_q4_pitch(q41) / 4u, 32u) &&
-              encode_blocks(&p.umap, p.w1, q41, p.K, p.N, p.nb01, p.G, p.nb02, gx::gmm_q4_pitch(q41) / 4u, 32u);
+              (!glu || encode_blocks(&p.umap, p.w1, q41, p.K, p.N, p.nb01, p.G, p.nb02, gx::gmm_q4_pitch(q41) / 4u, 32u));
     p.split = 1;
     const int out_rows = gx::gmm_out_rows(mode) * 2;
     p.mt = (int32_t)((p.N + out_rows - 1) / out_rows);
@@ -223,7 +225,7 @@ int q4_product(int type, const void * as, const void * up, int64_t ne00, int64_t
         if (p.warps % c == 0 && (int64_t)sms * (p.warps / c) * 5 >= jobs * 4) p.share = c;
     const uint32_t words = (uint32_t)gx::q4_pitch(q41) / 4u, box = glu ? 16u : 32u;
     p.boxes = nb01 % 16 == 0 && nb02 % 16 == 0 && encode_blocks(&p.wmap, p.w0, q41, ne00, ne01, nb01, n_as, nb02, words, box) &&
-              encode_blocks(&p.umap, p.w1, q41, ne00, ne01, nb01, n_as, nb02, words, box);
+              (!glu || encode_blocks(&p.umap, p.w1, q41, ne00, ne01, nb01, n_as, nb02, words, box));
     const void * fn = q4_kernel(bf16, q41, glu);
     const int slot = kSlotQ4 + (bf16 ? 4 : 0) + (q41 ? 2 : 0) + (glu ? 1 : 0);
     cudaError_t e = allow_smem(fn, slot, gx::kQ4Smem);

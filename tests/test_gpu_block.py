@@ -230,24 +230,33 @@ def test_layer(gxlib, dev, T):
     out, after = gxlib.block_out(y.view(T, k, H), weights=probs, ids=ids, shared=s, shared_gate=h.float() @ ws, residual=x,
                                  next_norm=w1, next_dtype=BF16)
 
-    # the formula on the same routes, each rounding to BF16 where the layer has one (off by half a step: 2^-8, or a whole one where
-    # f32 sums stand at the other side of a border)
+    # The formula on the same routes, with a rounding to BF16 where the layer has one. What the layer may be off by is taken as a sum
+    # of independent errors: a rounding is off by half a step, 2^-8 of the value at most, so by a variance of (2^-8)^2 / 3 of its
+    # square. Weights are rounded for the gated products of many rows; an activation that is off is rounded elsewhere, which is two
+    # roundings. |d(x sigmoid(x))/dx| <= 1.1. Of 150 thousand results none is six deviations off.
     h64 = unit(x, w0).to(BF16).double()
     e64 = torch.topk(h64 @ wr.double().T, k, dim=1).indices
     assert torch.equal(e64.sort(1).values, ids.long().sort(1).values)
     p64 = torch.softmax(h64 @ wr.double().T, 1).gather(1, ids.long())
     p64 = p64 / p64.sum(1, keepdim=True)
-    want = x.double().clone()
+    step = (2.0 ** -8) ** 2 / 3
+
+    def ffn(rows, gm, um, dm):
+        gm, um, dm = (parts(m, Q4_0)[0] for m in (gm, um, dm))
+        g, u = rows @ gm.T, rows @ um.T
+        act = g * torch.sigmoid(g) * u
+        var = (1.1 * u) ** 2 * step * (rows ** 2 @ (gm ** 2).T) + (g * torch.sigmoid(g)) ** 2 * step * (rows ** 2 @ (um ** 2).T) + 2 * step * act ** 2
+        return act.to(BF16).double() @ dm.T, var @ (dm ** 2).T
+
+    want, var = x.double().clone(), torch.zeros((T, H), dtype=torch.float64, device="cuda")
     for e in range(E):
         t, sl = (ids == e).nonzero(as_tuple=True)
         if len(t):
-            g = h64[t] @ parts(gate[e], Q4_0)[0].T
-            act = (g * torch.sigmoid(g) * (h64[t] @ parts(up[e], Q4_0)[0].T)).to(BF16).double()
-            want.index_add_(0, t, p64[t, sl][:, None] * (act @ parts(down[e], Q4_0)[0].T))
-    g = h64 @ parts(sg[0], Q4_0)[0].T
-    act = (g * torch.sigmoid(g) * (h64 @ parts(su[0], Q4_0)[0].T)).to(BF16).double()
-    want += torch.sigmoid(h64 @ ws.double())[:, None] * (act @ parts(sd[0], Q4_0)[0].T)
-    # a value of h or act on the other side of a border moves by 2^-8 of itself; few do, all would move a sum by that of its terms
-    tol = 2.0 ** -8 * (want - x.double()).square().mean().sqrt() * 4
-    assert float((out.double() - want).abs().max()) < float(tol)
+            y64, v64 = ffn(h64[t], gate[e], up[e], down[e])
+            want.index_add_(0, t, p64[t, sl][:, None] * y64)
+            var.index_add_(0, t, p64[t, sl][:, None] ** 2 * v64)
+    y64, v64 = ffn(h64, sg[0], su[0], sd[0])
+    weight = torch.sigmoid(h64 @ ws.double())[:, None]
+    want, var = want + weight * y64, var + weight ** 2 * v64
+    assert bool(((out.double() - want).abs() <= 6 * var.sqrt() + want.abs() * 2.0 ** -20).all())
     close(after, unit(out, w1), unit(out, w1).abs() * 64 * U)

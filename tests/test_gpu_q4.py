@@ -58,7 +58,7 @@ def want(w, x, kind, e, rounded=False):
 
 def many(rows, groups, out):
     """Whether a call without ids may make matrix tiles of rounded weights."""
-    return rows > 16 and out != F32
+    return rows > 24 and out != F32
 
 
 def want_glu(gate, up, x, kind, e, act, rounded=False):
