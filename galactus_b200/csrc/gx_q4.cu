@@ -82,11 +82,12 @@ bool encode_blocks(CUtensorMap * map, const void * base, bool q41, int64_t K, in
 // tiles made from the blocks.
 int q4_tiles(gx::GmmParams & p, bool q41, bool glu, const void * b, int64_t nb11, int64_t touched, void * stream) {
     const int mode = glu ? gx::GMM_GLU : gx::GMM_PLAIN;
-    // Parts of 16 bits that a weight is made of. One for results of 16 bits: the
-    // weight is then rounded as the result is, by half a step of their type. f32
-    // results take the weight whole, or to 22 bits (d q + m in F16) or 24 (BF16).
-    p.parts = p.out != gx::GMM_F32 ? 1 : q41 && p.bf16 ? 3 : 2;
-    p.seg = long_sum(p.out, p.K) ? 8 : 0;
+    // Parts of 16 bits that a weight is made of: d (q - 8) whole, d q + m to 22 bits
+    // (F16) or to 16, and for f32 results 24 (BF16). One part, a weight rounded to the
+    // rows' type, would leave results of 16 bits 1.7 times as far from 64 bits.
+    p.parts = p.out == gx::GMM_F32 && q41 && p.bf16 ? 3 : 2;
+    // (two MMAs a chunk: sums of 256 elements where grouped products take 512)
+    p.seg = long_sum(p.out, 2 * (int64_t)p.K) ? 4 : 0;
     p.nt = p.seg ? 160 : 256;
     while (gx::gmm_q4_stages(q41, p.nt, mode, p.G, p.parts) < 2) p.nt -= 32;       // (thousands of matrices, f32 results)
     p.acc = p.seg ? p.nt : 256;

@@ -379,7 +379,10 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
  *   Q4_1  { f16 d; f16 m; u8 qs[16] }  w = d q + m
  * gx_mul_mat_id refuses these types (it promises ggml's bits, with activations
  * quantised to 8 bits); here rows keep their 16 bits, products are exact, sums
- * are f32 and the result is rounded once to type_dst (F32, F16, BF16).
+ * are f32 and the result is rounded once to type_dst (F32, F16, BF16). (Calls of
+ * more than 24 rows without ids take a Q4_1 weight, d q + m, to 22 bits with F16
+ * rows, and to 24 or, for 16-bit results, 16 with BF16 rows; a weight must lie in
+ * the range of the rows' type.)
  *   dst row of j = W_e (b row of j)
  * The matrix of a row is named in one of three ways:
  *   ids      device i32 [n_rows], n_rows <= GX_Q4_MAX_IDS: row j's expert (decode:

@@ -36,34 +36,28 @@ def parts(w, kind):
     return tuple(torch.from_numpy(t.reshape(*w.shape[:-1], -1)).cuda() for t in (v, a))
 
 
-def want(w, x, kind, e, rounded=False):
+def want(w, x, kind, e, out=F32):
     """Row j of x times matrix e[j] (-1: none) in 64 bits, and how far f32 sums may be off: the tensor cores add a block's
-    64 products of codes (at most 31 |d x|, and 24 |d x| taken off) within 6e-9 of their magnitudes each, then the
-    block's sums are added in f32, K / 32 roundings of half a step. rounded: many rows and results of 16 bits, where a weight is rounded
-    to x's type first, by half a step of its own."""
+    64 products of codes (at most 31 |d x|, and 24 |d x| taken off; F16 64 + q and 72, of which as much is left) within 6e-9 of
+    their magnitudes each, then the block's sums are added in f32, K / 32 roundings of half a step. In calls of many rows a Q4_1
+    weight is taken to 22 bits (F16 rows), or to 24 or 16 (BF16 rows; f32 results, others): off by half of the last."""
     n = w.shape[1]
     y = torch.zeros((len(e), n), dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(y)
     K = x.shape[1]
+    cut = 0.0 if kind == Q4_0 else 2.0 ** -22 if x.dtype == F16 else 2.0 ** -24 if out == F32 else 2.0 ** -16
     for g in sorted(set(int(v) for v in e if v >= 0)):
         rows = torch.tensor([j for j, v in enumerate(e) if v == g], device="cuda")
         v, a = parts(w[g], kind)
         xs = x[rows].double()
         y[rows] = xs @ v.T
-        tol[rows] = (xs.abs() @ a.T) * 64 * 6e-9 + (xs.abs() @ v.abs().T) * (K // 32 + 8) * 2.0 ** -24
-        if rounded:
-            tol[rows] += (xs.abs() @ v.abs().T) * torch.finfo(x.dtype).eps / 2
+        tol[rows] = (xs.abs() @ a.T) * 64 * 6e-9 + (xs.abs() @ v.abs().T) * ((K // 32 + 8) * 2.0 ** -24 + cut)
     return y, tol
 
 
-def many(rows, groups, out):
-    """Whether a call without ids may make matrix tiles of rounded weights."""
-    return rows > 24 and out != F32
-
-
-def want_glu(gate, up, x, kind, e, act, rounded=False):
-    g, eg = want(gate, x, kind, e, rounded)
-    u, eu = want(up, x, kind, e, rounded)
+def want_glu(gate, up, x, kind, e, act, out=F32):
+    g, eg = want(gate, x, kind, e, out)
+    u, eu = want(up, x, kind, e, out)
     if act:
         ok = g < LIMIT
         g, eg = g.clamp(max=LIMIT), torch.where(ok | ((g - LIMIT).abs() < eg), eg, 0.0)
@@ -112,7 +106,7 @@ def test_dense(gxlib, dev, kind, dtype, out, K, N):
     for rows in (1, 2, 8, 9, 17, 31, 32, 33, 70):
         x = torch.from_numpy(rng.standard_normal((rows, K))).cuda().to(dtype)
         got = gxlib.mul_mat_q4(w, x, type=kind, out_dtype=out)
-        check(got, *want(w, x, kind, [0] * rows, many(rows, 1, out)))
+        check(got, *want(w, x, kind, [0] * rows, out))
     assert error_code(gxlib) == 0
 
 
@@ -158,7 +152,7 @@ def test_groups(gxlib, dev, kind, dtype, out, T, k, E, K, N):
     none = torch.tensor([j for j, v in enumerate(flat) if v < 0], dtype=torch.long, device="cuda")
     keep = torch.full((T * k, N), 7.0, dtype=out, device="cuda")
     got = gxlib.mul_mat_q4(w, x, type=kind, offsets=offsets, order=order, gather=k, scatter=True, out=keep)
-    y, tol = want(w, x.repeat_interleave(k, 0), kind, flat, many(T * k, E, out))
+    y, tol = want(w, x.repeat_interleave(k, 0), kind, flat, out)
     check(got, y, tol, none)
     assert bool((got[none] == 7.0).all())
     # into expert order, and from expert order
@@ -183,13 +177,11 @@ def test_glu(gxlib, dev, kind, act, dtype, out, T, k, E, K, N):
     ids = np.stack([rng.choice(E, k, replace=False) for _ in range(T)]).astype(np.int32)
     x = torch.from_numpy(3.0 * rng.standard_normal((T, K))).cuda().to(dtype)
     flat = ids.reshape(-1).tolist()
-    y, tol = want_glu(gate, up, x.repeat_interleave(k, 0), kind, flat, act)
+    y, tol = want_glu(gate, up, x.repeat_interleave(k, 0), kind, flat, act, out)
     dids = torch.from_numpy(ids).cuda()
     if T * k <= 256:
         check(gxlib.mul_mat_q4_glu(gate, up, x, type=kind, ids=dids, gather=k, act=act, out_dtype=out), y, tol)
     order, offsets = gxlib.group_rows(dids, E)
-    if many(T * k, E, out):
-        y, tol = want_glu(gate, up, x.repeat_interleave(k, 0), kind, flat, act, True)
     check(gxlib.mul_mat_q4_glu(gate, up, x, type=kind, offsets=offsets, order=order, gather=k, scatter=True, act=act, out_dtype=out), y, tol)
     assert error_code(gxlib) == 0
 
@@ -321,6 +313,134 @@ def test_far_weights(gxlib, dev):
     offsets = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
     offsets[E] = 40
     check(gxlib.mul_mat_q4(w, x, type=Q4_0, offsets=offsets, out_dtype=F32), y, tol)
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q4_1])
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("K,N", [(256, 130), (320, 70), (1600, 40)])
+def test_short_groups_among_long_ones(gxlib, dev, kind, dtype, out, K, N):
+    """Groups of none, one, a few and hundreds of rows in one call: which kernel takes a group goes by its length, and tiles of few
+    rows follow full ones (a CTA of a pair may then have no rows at all)."""
+    rng = np.random.default_rng(K)
+    sizes = [1, 0, 300, 2, 24, 25, 16, 17, 513, 3, 0, 8, 9, 70, 26, 1, 257, 33]
+    E, P = len(sizes), sum(sizes)
+    w = weights(rng, E, N, K, kind)
+    offsets = torch.from_numpy(np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)).cuda()
+    order = torch.from_numpy(rng.permutation(P).astype(np.int32)).cuda()
+    e = np.repeat(np.arange(E), sizes).tolist()
+    x = torch.from_numpy(rng.standard_normal((P, K))).cuda().to(dtype)
+    y, tol = want(w, x[order.long()], kind, e, out)
+    for _ in range(3):
+        check(gxlib.mul_mat_q4(w, x, type=kind, offsets=offsets, order=order, gather=1, out_dtype=out), y, tol)
+        got = gxlib.mul_mat_q4(w, x[order.long()].contiguous(), type=kind, offsets=offsets, order=order, scatter=True, out_dtype=out)
+        check(got[order.long()], y, tol)
+    y, tol = want_glu(w, w.flip(0).contiguous(), x[order.long()], kind, e, 0, out)
+    check(gxlib.mul_mat_q4_glu(w, w.flip(0).contiguous(), x, type=kind, offsets=offsets, order=order, gather=1, out_dtype=out), y, tol)
+    assert error_code(gxlib) == 0
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q4_1])
+@pytest.mark.parametrize("pad", [4, 16, 20])
+def test_strides_of_many_rows(gxlib, dev, kind, pad):
+    rng = np.random.default_rng(pad)
+    G, N, K, T = 2, 77, 448, 150
+    w = weights(rng, G, N, K, kind)
+    rb = w.shape[2]
+    wide = torch.zeros(G * (N * (rb + pad) + 4 * pad) + 64, dtype=torch.uint8, device="cuda")
+    view = wide.as_strided((G, N, rb), (N * (rb + pad) + 4 * pad, rb + pad, 1))
+    view.copy_(w)
+    x = torch.from_numpy(rng.standard_normal((T, K + 24))).cuda().to(F16)[:, :K]
+    out = torch.full((T, N + 5), 3.0, dtype=F16, device="cuda")
+    offsets = torch.tensor([0, 60, 150], dtype=torch.int32, device="cuda")
+    gxlib.mul_mat_q4(view, x, type=kind, offsets=offsets, out=out[:, :N])
+    check(out[:, :N], *want(w, x, kind, [0] * 60 + [1] * 90, F16))
+    assert bool((out[:, N:] == 3.0).all())
+
+
+@pytest.mark.parametrize("K,rows,E", [(65536, 2, 1), (65536, 40, 1), (16384, 256, 3), (7168, 256, 2)])
+def test_long_rows(gxlib, dev, K, rows, E):
+    """The longest rows (of which shared memory holds one), and CTAs of fewer threads than ids."""
+    rng = np.random.default_rng(K)
+    w = weights(rng, E, 9, K, Q4_0)
+    x = torch.from_numpy(rng.standard_normal((rows, K))).cuda().to(BF16)
+    e = rng.integers(0, E, rows).astype(np.int32)
+    if rows <= 256:
+        check(gxlib.mul_mat_q4(w, x, type=Q4_0, ids=torch.from_numpy(e).cuda(), out_dtype=F32), *want(w, x, Q4_0, e.tolist()))
+    if E == 1:
+        check(gxlib.mul_mat_q4(w, x, type=Q4_0, out_dtype=F32), *want(w, x, Q4_0, e.tolist()))
+    assert error_code(gxlib) == 0
+
+
+def test_many_rows_captured_and_beside_another_stream(gxlib, dev):
+    rng = np.random.default_rng(12)
+    E, N, K, T, k = 8, 200, 512, 120, 4
+    w = weights(rng, E, N, K, Q4_0)
+    x = torch.zeros((T, K), dtype=BF16, device="cuda")
+    ids = torch.zeros((T, k), dtype=torch.int32, device="cuda")
+
+    def step(stream=None):
+        order, offsets = gxlib.group_rows(ids, E, stream=stream)
+        return gxlib.mul_mat_q4(w, x, type=Q4_0, offsets=offsets, order=order, gather=k, scatter=True, stream=stream)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    for _ in range(3):
+        x.copy_(torch.from_numpy(rng.standard_normal((T, K))).cuda())
+        ids.copy_(torch.from_numpy(rng.integers(0, E, (T, k)).astype(np.int32)).cuda())
+        graph.replay()
+        assert torch.equal(y, step())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = [step(s) for _ in range(10) for s in (None, side)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, y) for t in got)
+
+
+def test_products_on_the_slots_of_an_arena(gxlib, dev, tmp_path):
+    """A checkpoint of Q4_0 and Q4_1 experts, its records in an arena, the slots the products' matrices."""
+    import ctypes as C
+    from gguf import GGMLQuantizationType, GGUFWriter
+    from galactus_b200.models import ModelShape
+    H, I, E = 128, 192, 5
+    rng = np.random.default_rng(13)
+    f = GGUFWriter(str(tmp_path / "m.gguf"), "qwen3moe")
+    f.add_block_count(1)
+    f.add_expert_count(E)
+    f.add_expert_used_count(2)
+    held = {}
+    for role, n, m, kind in (("down", H, I, Q4_1), ("gate", I, H, Q4_0), ("up", I, H, Q4_0)):
+        held[role] = weights(rng, E, n, m, kind)
+        f.add_tensor(f"blk.0.ffn_{role}_exps.weight", held[role].cpu().numpy(), raw_dtype=GGMLQuantizationType(kind))
+    f.write_header_to_file()
+    f.write_kv_data_to_file()
+    f.write_tensors_to_file()
+    f.close()
+    m = ModelShape("q4", 1, H, E, 2, I, Q4_0, Q4_0, Q4_1)
+    arena = gxlib.Arena(m, capacity_bytes=E * m.record, policy=gxlib.POLICY_AUTO, max_tokens=8)
+    try:
+        n = C.c_uint32()
+        gxlib.check(gxlib.lib().gx_arena_load_gguf(arena.h, str(tmp_path / "m.gguf").encode(), C.byref(n)), "gx_arena_load_gguf")
+        assert n.value == E
+        stream = torch.cuda.current_stream()
+        arena.warm_all(stream)
+        base, record, slots = arena.layer_view(0)
+        e = [3, 0, 4, 3, 1]
+        ids = torch.tensor([arena.slot_of(0, v) for v in e], dtype=torch.int32, device="cuda")
+        x = torch.from_numpy(rng.standard_normal((5, H))).cuda().to(BF16)
+        h = torch.empty((5, I), dtype=F16, device="cuda")
+        lib, s = gxlib.lib(), stream.cuda_stream
+        gxlib.check(lib.gx_mul_mat_q4_glu(Q4_0, base + m.off_gate, base + m.off_up, H, I, H // 32 * 18, record, slots, 30, x.data_ptr(), 5,
+                                          2 * H, ids.data_ptr(), None, None, 5, 1, 0, 0, 0.0, 0.0, 1, h.data_ptr(), 2 * I, s))
+        check(h, *want_glu(held["gate"], held["up"], x, Q4_0, e, 0, F16))
+        y = torch.empty((5, H), device="cuda")
+        gxlib.check(lib.gx_mul_mat_q4(Q4_1, base, I, H, I // 32 * 20, record, slots, 1, h.data_ptr(), 5, 2 * I, ids.data_ptr(), None, None, 5, 1,
+                                      0, 0, y.data_ptr(), 4 * H, s))
+        check(y, *want(held["down"], h, Q4_1, e))
+    finally:
+        arena.close()
 
 
 def test_python_refusals(gxlib, dev):
