@@ -6,6 +6,20 @@
 //
 // with norm(v) = v / sqrt(mean(v^2) + eps) * weight. Every part may be absent;
 // the norm before a block is `next` of a single row y.
+//
+// Every row is read once and every result written once; what lies between stays in
+// f32 registers (16 elements a thread). Two kernels:
+//   k_block       a CTA per row, or a cluster of up to eight whose sums of squares
+//                 are exchanged through their shared memories (wide rows, or so few
+//                 wide rows that most SMs would idle): latency bound. One token:
+//                 2.2 us (2880 elements, a norm), 3.4 us (2048 x 8 experts, with
+//                 residual and next norm), of which a launch alone is about 2.
+//   k_block_rows  many rows: HBM bound, as far as the instructions keep up. 8192 rows
+//                 of 4096, f32 to bf16, a norm: 43 us, 4.7 TB/s; the sum over 8 experts,
+//                 norm, gate, residual and next norm, bf16: 151 us, 5.8 TB/s (of 6.55
+//                 measured for a copy); 517 rows of 7168, 37 % of the slots left out:
+//                 32 us, 4.0 TB/s. One CTA per row took 65, 276 and 43 us: few loads
+//                 are in flight, and rows wait for their sums.
 #pragma once
 
 #include "gx_gmm.cuh"
@@ -321,7 +335,8 @@ GX_HD constexpr int rows_ctas(int warps) { return warps <= 8 ? 3 : 1; }
 
 // The same for many rows: persistent CTAs, one warp copies the rows of the
 // tokens ahead into a ring of slots (one bulk copy a row), the others add them up
-// as they arrive. p.k <= 32, aligned rows.
+// as they arrive. p.k <= 32, aligned rows. (Packed f32 pairs halve the arithmetic;
+// 2.6 instructions a cycle are issued in the sum over 8 experts.)
 template <int YT, int MAXW>
 __global__ void __launch_bounds__(32 * (MAXW + 1), rows_ctas(MAXW)) k_block_rows(const __grid_constant__ BlockParams p, int slots, int slot_bytes) {
     extern __shared__ __align__(128) uint8_t block_ring[];

@@ -42,6 +42,21 @@
 //   - Gathering by cp.async needs twelve warps (the fence that shows a stage
 //     to the tensor cores waits for all of a warp's copies) and reached 1043
 //     TFLOP/s where gather4 reaches 1234.
+//
+// With 4-bit weights (SRC; Q4_0 and Q4_1 blocks) eight warps make the matrix
+// tiles instead: w = d (q - 8) or d q + m as two (Q4_1, BF16 rows, f32 results: three)
+// 16-bit values, each the rest rounded, one MMA per part into the same sums.
+//   - Two parts: results are as far from 64 bits as sums of exact products (f32
+//     6e-7, BF16 1.7e-3, which is the rounding of the result). One part, a weight
+//     rounded to 8 or 11 bits, is faster (gated 2048 tokens, 128 experts, 4096 x 1536:
+//     818 us for 956) but leaves 16-bit results 1.7 times as far.
+//   - What bounds it: the warps that make tiles. A chunk of 64 elements takes 900
+//     to 1200 cycles, its MMAs 512 a part; every other role's instructions share their
+//     issue slots (1.5 a cycle in all). 2048 rows, 4096 x 14336: 332 us, 724 TFLOP/s
+//     of products, 1450 with both parts. Short groups pay for whole tiles of weights:
+//     the 1031 tokens x 8 of 64 experts, 1024 x 2048, f32 results, take 172 us.
+//   - Tried, no gain: twelve warps in three fours, a register split by setmaxnreg
+//     (spills), blocks loaded straight into registers (278 us where boxes took 220).
 #pragma once
 
 #include <cuda_bf16.h>

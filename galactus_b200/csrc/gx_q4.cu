@@ -24,9 +24,9 @@ enum KernelSlot : int { kSlotQ4 = 0, kSlotRows = 8, kSlotTiles = kSlotRows + 6, 
 static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
 
 // Rows of a group above which matrix tiles are made for the tensor cores. In us
-// from 8, 16, 24, 32 and 48 rows on: 64 tokens x 8 of 128 experts 123, 122, 115,
-// 120, 127; 1031 tokens 174, 169, 170, 169, 174; 2048 tokens, gated, 837, 806, 817,
-// 828, 855.
+// with 8, 16, 24, 32 and 48 rows: 64 tokens x 8 of 128 experts, 1536 x 4096, 123,
+// 123, 114, 119, 126; 1031 tokens x 8 of 64, 1024 x 2048, 176, 172, 172, 170, 176;
+// one matrix of 4096 x 14336 with 32 rows 45, 44, 45, 56, 55.
 constexpr int64_t kTileRows = 24;
 
 // A launch that may begin while the kernel before it on the stream ends: the
@@ -260,7 +260,13 @@ bool block_rows(int type, const void * p, int64_t ne0, int64_t nb, int64_t ne1, 
 }
 
 constexpr uint32_t kStreamSmem = 220u * 1024u;
-constexpr int kStreamWidth = 512, kStreamRows = 2;     // narrower or fewer rows go a CTA each
+// Rows of fewer elements, or fewer elements in all, go a CTA each (k_block) rather
+// than through rings (k_block_rows). In us a CTA each / rings, sum of k rows of
+// BF16, residual, next norm: 8192 rows of 1024, k = 1, 27 / 34; of 2880, 109 / 52;
+// of 512, k = 8, 42 / 77; of 2048, k = 8, 192 / 88. 296 and 592 rows of 4096, k = 1, 4.7 /
+// 4.9 and 8.9 / 8.5; of 2048, k = 8, 5.6 / 6.3 and 14.2 / 11.0; 148 of 7168, k = 8, 13.0 / 6.6.
+constexpr int kStreamWidth = 2048;
+constexpr int64_t kStreamElements = 1 << 20;
 
 template <int YT>
 const void * block_kernel(bool vec, bool cluster) {
@@ -309,14 +315,20 @@ int launch_block(gx::BlockParams & p, bool vec, void * stream) {
     vec = vec && p.H % 8 == 0 && !misaligned(p.norm, 16) && !misaligned(p.next_norm, 16) &&
           (p.gate_step == 0 || (!misaligned(p.gate, 16) && p.gate_nb % 16 == 0));
     const int units = (p.H + gx::kBlockUnit - 1) / gx::kBlockUnit;
-    if (vec && p.k <= 32 && p.H <= gx::kRowsMaxWidth && p.H >= kStreamWidth && p.T >= kStreamRows * sms) return launch_block_rows(p, sms, stream);
+    if (vec && p.k <= 32 && p.H <= gx::kRowsMaxWidth && p.H >= kStreamWidth && (int64_t)p.T * p.H >= kStreamElements)
+        return launch_block_rows(p, sms, stream);
+    // A cluster per row: where a CTA's registers do not hold the row, or where few rows
+    // leave SMs idle and a CTA's threads would take two steps. One row, us without and
+    // with: 2880 elements 2.7, 2.9; 4096 3.0, 2.9; 5120 3.5, 3.0; 7168, k = 8, 7.5, 4.7.
     int cluster = 1;
     while (cluster < gx::kBlockMaxCluster &&
-           (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads || ((int64_t)p.T * cluster * 2 <= sms && units > cluster * 64)))
+           (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads || ((int64_t)p.T * cluster * 2 <= sms && units > gx::kBlockMaxThreads && units > cluster * 64)))
         cluster *= 2;
     const int per = (units + cluster - 1) / cluster;
+    // Steps of a thread: one, or two where CTAs wait for SMs and there is one row to
+    // load (290 rows of 2880, k = 1: 5.0 us with one, 3.7 with two; of 2048, k = 8: 4.9, 8.1)
     int threads = 64;
-    while (threads < gx::kBlockMaxThreads && threads * (p.T * cluster > sms ? gx::kBlockUnits : 1) < per) threads *= 2;
+    while (threads < gx::kBlockMaxThreads && threads * (p.k == 1 && p.T * cluster > sms ? gx::kBlockUnits : 1) < per) threads *= 2;
     const int kind = p.y.type;
     const void * fn = kind == gx::GMM_F32   ? block_kernel<gx::GMM_F32>(vec, cluster > 1)
                       : kind == gx::GMM_F16 ? block_kernel<gx::GMM_F16>(vec, cluster > 1)

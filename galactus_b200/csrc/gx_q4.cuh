@@ -5,6 +5,31 @@
 //   Q4_1  y = sum over blocks  (d * sum q x + m * sum x)
 //
 // plain (y_j = W_e x_j) or gated (act(G_e x_j, U_e x_j)).
+//
+// A job is 32 rows of a matrix (gated: 16 of each) against up to eight rows of x.
+// A warp's step is 64 elements of K: codes become 16-bit floats without a rounding
+// (16 + q, 64 + q), the tensor cores (mma.sync m16n8k16) add their products with x
+// in f32, one more product with a constant takes 16 + 8 or 64 + 8 times sum x off
+// again, and f32 fmas apply the block's d (and m): the only roundings are f32's.
+// (tcgen05 needs its matrices in shared memory, written and fenced: for a few rows
+// that costs more than the products. With many, gx_gmm.cuh does just that.)
+//
+// Choices, as measured on a B200 (device time, calls in a row in a graph):
+//   - x of the job's rows lies in shared memory, copied ahead by bulk copies: read
+//     through L2 by each warp, 32 rows x 4096 x 14336 took 92 us, now 45.
+//   - A ring per two warps that take the pairs of blocks in turn: TMA boxes of
+//     32 rows x 8 pairs, or pieces of 16 bytes by cp.async where rows do not start on
+//     16 bytes (2880 elements: 1620 bytes). Bulk copies, one a row, cost the issuing
+//     warp 2800 cycles for 32 of them.
+//   - Few jobs: warps share a job's K (p.share) and add their sums in their order, so
+//     the same call gives the same bits.
+// What bounds it: instructions. A step is 178 of them, 87 cycles per SM, 83 of those
+// on the units for shifts, masks, byte permutations and conversions alone (64 lanes
+// a cycle): 3.5 TB/s of weights, 264 MB in 74 us where the copies by themselves take
+// 47. 19 tokens x 8 of 64 experts, gated, 2048 x 1024, Q4_1: 46 us, 1.9 TB/s (two and
+// three tiles of rows for the popular experts); one token, 8 of 128, 768 x 2048: 9.3 us,
+// set-up and one round of jobs; 2880 x 2880, 4 experts, gated: 23 us, of which the
+// copies of 16 bytes take 20.
 #pragma once
 
 #include <climits>
@@ -157,6 +182,7 @@ __device__ __forceinline__ void q4_tile(const Q4Params & p, const Q4Groups & g, 
     j.row0 = lo + (at - j.before) * size;
     j.rows = min(size, hi - j.row0);
 }
+
 // As tile_prefix, for the groups that a thread looks at together: pre[i] is of
 // group i * per, one per thread, and the last is the sum.
 template <typename F>
@@ -185,6 +211,7 @@ __device__ __forceinline__ void q4_prefix(int32_t * pre, int32_t * wsum, int G, 
     }
     __syncthreads();
 }
+
 // ------------------------------------------------------------- the kernel
 
 // the warps that share a job
