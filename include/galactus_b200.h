@@ -394,8 +394,10 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
  *   offsets  device i32 [n_as + 1] and order as gx_group_rows gives them, any
  *            number of rows, with gather and scatter as in gx_mul_mat_grouped
  *   neither  n_as = 1: all n_rows rows with the one matrix (a dense projection)
- * Offsets, row indexes and what is reported: as gx_mul_mat_grouped. A row of b
- * with an infinity or a NaN makes its own results NaN, and no other.
+ * Offsets, row indexes and what is reported: as gx_mul_mat_grouped (borders that
+ * name more rows than n_rows are reported, and groups of one kind, short or long,
+ * may be computed all the same). A row of b with an infinity or a NaN makes its
+ * own results NaN, and no other.
  * Requires ne00 % 64 == 0, ne00 <= GX_Q4_MAX_K; 16-byte aligned as, b and nb11; nb01 and nb02
  * multiples of 4; n_as <= 8192. dst may not overlap an input. The calls follow
  * one another on a stream without a gap (programmatic launches), can be

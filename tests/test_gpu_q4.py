@@ -460,3 +460,35 @@ def test_python_refusals(gxlib, dev):
     with pytest.raises(gxlib.GxError):
         gxlib.mul_mat_q4(w, x.float(), type=Q4_0, ids=ids, out_dtype=F32)
     assert gxlib.mul_mat_q4(w, x[:0], type=Q4_0, ids=ids[:0]).shape == (0, 8)
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q4_1])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,K", [(3, 7168), (40, 1024), (40, 4096)])
+def test_sums_of_one_sign(gxlib, dev, kind, dtype, rows, K):
+    """Positive rows (and, with Q4_1, positive weights): what the sums cut off does not cancel."""
+    rng = np.random.default_rng(K + rows)
+    w = weights(rng, 1, 40, K, kind)
+    if kind == Q4_1:
+        b = w.view(1, 40, K // 32, BLOCK[kind])
+        b[..., 1] &= 127                                       # (the signs of d and m)
+        b[..., 3] &= 127
+    x = torch.from_numpy(0.5 + np.abs(rng.standard_normal((rows, K)))).cuda().to(dtype)
+    got = gxlib.mul_mat_q4(w, x, type=kind, out_dtype=F32)
+    check(got, *want(w, x, kind, [0] * rows), rms=None)
+
+
+@pytest.mark.parametrize("T,k", [(3, 4), (20, 3)])
+@pytest.mark.parametrize("scatter", [False, True])
+def test_one_matrix_in_an_order(gxlib, dev, T, k, scatter):
+    """Neither ids nor offsets, but an order: rows of x by order[j] // gather, results in place or scattered."""
+    rng = np.random.default_rng(T)
+    K, N = 256, 70
+    w = weights(rng, 1, N, K, Q4_0)
+    x = torch.from_numpy(rng.standard_normal((T, K))).cuda().to(BF16)
+    order = rng.permutation(T * k).astype(np.int32)
+    got = gxlib.mul_mat_q4(w, x, type=Q4_0, order=torch.from_numpy(order).cuda(), gather=k, scatter=scatter, out_dtype=F32)
+    if scatter:
+        got = got[torch.from_numpy(order).long().cuda()]
+    check(got, *want(w, x[torch.from_numpy(order // k).long().cuda()], Q4_0, [0] * (T * k)))
+    assert error_code(gxlib) == 0
