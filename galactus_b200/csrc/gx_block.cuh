@@ -9,7 +9,8 @@
 //
 // Every row is read once and every result written once; what lies between stays in
 // f32 registers (16 elements a thread). Two kernels:
-//   k_block       a CTA per row, or a cluster of up to eight whose sums of squares
+//   k_block       narrow rows: a warp each, without a barrier (65536 rows of 128, sum,
+//                 residual and next norm: 45 us, 109 with a CTA each). Others: a CTA per row, or a cluster of up to eight whose sums of squares
 //                 are exchanged through their shared memories (wide rows, or so few
 //                 wide rows that most SMs would idle): latency bound. One token:
 //                 2.2 us (2880 elements, a norm), 3.4 us (2048 x 8 experts, with
@@ -194,18 +195,22 @@ __device__ __forceinline__ void block_gate(const BlockParams & p, int t, int i, 
     block_scale(m, v);
 }
 
-// The sum of v over the row's threads: the warps of a CTA, then the CTAs of
-// the row's cluster, each in their order. `warps`, `ctas`: buffers of this sum alone.
-template <bool CLUSTER>
+// what a row's elements are spread over
+enum : int { ROW_WARP = 0, ROW_CTA = 1, ROW_CLUSTER = 2 };
+
+// The sum of v over the row's threads: a warp, the warps of a CTA, then the CTAs
+// of the row's cluster, each in their order. `warps`, `ctas`: buffers of this sum alone.
+template <int OVER>
 __device__ __forceinline__ float block_sum(float v, float * warps, float * ctas) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
+    if constexpr (OVER == ROW_WARP) return v;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
     if (lane == 0) warps[warp] = v;
     __syncthreads();
     v = 0.0f;
     for (int i = 0; i < n; ++i) v = __fadd_rn(v, warps[i]);
-    if constexpr (CLUSTER) {
+    if constexpr (OVER == ROW_CLUSTER) {
         uint32_t me, size;
         asm("mov.u32 %0, %cluster_ctarank;" : "=r"(me));
         asm("mov.u32 %0, %cluster_nctarank;" : "=r"(size));
@@ -219,26 +224,30 @@ __device__ __forceinline__ float block_sum(float v, float * warps, float * ctas)
 }
 
 constexpr int kBlockBatch = 4;      // rows of y that a thread loads before it adds them
+constexpr int kBlockWarps = 8;      // rows of a CTA whose warps have one each
+GX_HD constexpr int block_threads(int over) { return over == ROW_WARP ? 32 * kBlockWarps : kBlockMaxThreads; }
 
-// A CTA, or a cluster of them, per row of the result.
-template <int YT, bool VEC, bool CLUSTER>
-__global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constant__ BlockParams p) {
+// A warp, a CTA, or a cluster of them, per row of the result.
+template <int YT, bool VEC, int OVER, int kUnits>
+__global__ void __launch_bounds__(block_threads(OVER)) k_block(const __grid_constant__ BlockParams p) {
     __shared__ float warps[2][kBlockMaxThreads / 32], ctas[2][kBlockMaxCluster];
     const int tid = threadIdx.x, lane = tid & 31;
     int rank = 0, size = 1;
-    if constexpr (CLUSTER) {
+    if constexpr (OVER == ROW_CLUSTER) {
         asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
         asm("mov.u32 %0, %cluster_nctarank;" : "=r"(size));
     }
-    const int t = (int)blockIdx.x / size;
-    const int first = (rank * (int)blockDim.x + tid) * kBlockUnit, step = size * (int)blockDim.x * kBlockUnit;
+    const int t = OVER == ROW_WARP ? (int)blockIdx.x * (int)(blockDim.x >> 5) + (tid >> 5) : (int)blockIdx.x / size;
+    const int first = (OVER == ROW_WARP ? lane : rank * (int)blockDim.x + tid) * kBlockUnit;
+    const int step = (OVER == ROW_WARP ? 32 : size * (int)blockDim.x) * kBlockUnit;
     griddep_launch_dependents();
-    if constexpr (CLUSTER) cluster_sync_all();      // (peers are written to once they run)
+    if constexpr (OVER == ROW_CLUSTER) cluster_sync_all();      // (peers are written to once they run)
     griddep_wait();
+    if (OVER == ROW_WARP && t >= p.T) return;
 
-    uint64_t m[kBlockUnits][kBlockPairs], r[kBlockUnits][kBlockPairs];
+    uint64_t m[kUnits][kBlockPairs], r[kUnits][kBlockPairs];
 #pragma unroll
-    for (int u = 0; u < kBlockUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
         const int i = first + u * step;
 #pragma unroll
         for (int j = 0; j < kBlockPairs; ++j) m[u][j] = r[u][j] = 0ull;
@@ -247,7 +256,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
     const uint8_t * row = p.y.p + (int64_t)t * p.y_nb2;
     if (p.w == nullptr && p.ids == nullptr && p.k == 1) {
 #pragma unroll
-        for (int u = 0; u < kBlockUnits; ++u) {
+        for (int u = 0; u < kUnits; ++u) {
             const int i = first + u * step;
             if (i < p.H) block_load<VEC>(row, YT, i, p.H, m[u]);
         }
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
             const int n = min(32, p.k - s0);
             for (int s = 0; s < n; s += kBlockBatch) {
 #pragma unroll
-                for (int u = 0; u < kBlockUnits; ++u) {
+                for (int u = 0; u < kUnits; ++u) {
                     const int i = first + u * step;
                     if (__all_sync(0xffffffffu, i >= p.H)) continue;
                     uint64_t v[kBlockBatch][kBlockPairs];
@@ -280,7 +289,7 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
     }
     uint64_t ss = 0ull;
 #pragma unroll
-    for (int u = 0; u < kBlockUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
         const int i = first + u * step;
         if (i >= p.H) continue;
         if (p.shared.p != nullptr) {
@@ -291,10 +300,10 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
         ss = block_squares(m[u], ss);
     }
     float inv = 1.0f;
-    if (p.has_norm) inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[0], ctas[0]), p.per, p.eps);
+    if (p.has_norm) inv = block_inverse_root(block_sum<OVER>(block_pair_sum(ss), warps[0], ctas[0]), p.per, p.eps);
     ss = 0ull;
 #pragma unroll
-    for (int u = 0; u < kBlockUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
         const int i = first + u * step;
         if (i >= p.H) continue;
         uint64_t v[kBlockPairs];
@@ -309,9 +318,9 @@ __global__ void __launch_bounds__(kBlockMaxThreads) k_block(const __grid_constan
         if (p.dst.p != nullptr) block_store<VEC>(p.dst.p + (int64_t)t * p.dst.nb, p.dst.type, i, p.H, m[u]);
     }
     if (!p.has_next) return;
-    inv = block_inverse_root(block_sum<CLUSTER>(block_pair_sum(ss), warps[1], ctas[1]), p.per, p.next_eps);
+    inv = block_inverse_root(block_sum<OVER>(block_pair_sum(ss), warps[1], ctas[1]), p.per, p.next_eps);
 #pragma unroll
-    for (int u = 0; u < kBlockUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
         const int i = first + u * step;
         if (i >= p.H) continue;
         block_scale(m[u], inv);

@@ -267,11 +267,21 @@ constexpr uint32_t kStreamSmem = 220u * 1024u;
 // 4.9 and 8.9 / 8.5; of 2048, k = 8, 5.6 / 6.3 and 14.2 / 11.0; 148 of 7168, k = 8, 13.0 / 6.6.
 constexpr int kStreamWidth = 2048;
 constexpr int64_t kStreamElements = 1 << 20;
+// Steps of a lane up to which a row has a warp, with any number of rows and with
+// many. In us a CTA each / a warp each, as above: 74 rows of 256, k = 1, 2.4 / 2.2;
+// 8192, 13.0 / 6.3; 74 of 128, k = 8, 4.4 / 3.1; 592, 2368 and 8192 of 512, k = 1, 3.3 /
+// 3.6, 5.6 / 5.1 and 17.1 / 13.7; 8192 of 1024, 27 / 29.
+constexpr int kWarpSteps = 1, kWarpStepsMany = 2, kWarpMany = 2048;
 
 template <int YT>
 const void * block_kernel(bool vec, bool cluster) {
-    return vec ? (cluster ? (const void *)gx::k_block<YT, true, true> : (const void *)gx::k_block<YT, true, false>)
-               : (cluster ? (const void *)gx::k_block<YT, false, true> : (const void *)gx::k_block<YT, false, false>);
+    constexpr int n = gx::kBlockUnits;
+    return vec ? (cluster ? (const void *)gx::k_block<YT, true, gx::ROW_CLUSTER, n> : (const void *)gx::k_block<YT, true, gx::ROW_CTA, n>)
+               : (cluster ? (const void *)gx::k_block<YT, false, gx::ROW_CLUSTER, n> : (const void *)gx::k_block<YT, false, gx::ROW_CTA, n>);
+}
+template <int YT>
+const void * block_warp_kernel(int steps) {
+    return steps == 1 ? (const void *)gx::k_block<YT, true, gx::ROW_WARP, 1> : (const void *)gx::k_block<YT, true, gx::ROW_WARP, kWarpStepsMany>;
 }
 
 template <int YT>
@@ -317,12 +327,21 @@ int launch_block(gx::BlockParams & p, bool vec, void * stream) {
     const int units = (p.H + gx::kBlockUnit - 1) / gx::kBlockUnit;
     if (vec && p.k <= 32 && p.H <= gx::kRowsMaxWidth && p.H >= kStreamWidth && (int64_t)p.T * p.H >= kStreamElements)
         return launch_block_rows(p, sms, stream);
+    const int steps = (units + 31) / 32;
+    if (vec && steps <= (p.T >= kWarpMany ? kWarpStepsMany : kWarpSteps)) {
+        const void * fn = p.y.type == gx::GMM_F32   ? block_warp_kernel<gx::GMM_F32>(steps)
+                          : p.y.type == gx::GMM_F16 ? block_warp_kernel<gx::GMM_F16>(steps)
+                                                    : block_warp_kernel<gx::GMM_BF16>(steps);
+        const int ctas = (p.T - 1) / gx::kBlockWarps + 1;
+        return cuda_status(launch_next(fn, dim3((unsigned)ctas), 32 * gx::kBlockWarps, 0, 1, stream, p));
+    }
     // A cluster per row: where a CTA's registers do not hold the row, or where few rows
     // leave SMs idle and a CTA's threads would take two steps. One row, us without and
     // with: 2880 elements 2.7, 2.9; 4096 3.0, 2.9; 5120 3.5, 3.0; 7168, k = 8, 7.5, 4.7.
     int cluster = 1;
     while (cluster < gx::kBlockMaxCluster &&
-           (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads || ((int64_t)p.T * cluster * 2 <= sms && units > gx::kBlockMaxThreads && units > cluster * 64)))
+           (units > cluster * gx::kBlockUnits * gx::kBlockMaxThreads ||
+            ((int64_t)p.T * cluster * 2 <= sms && units > gx::kBlockMaxThreads && units > cluster * 64)))
         cluster *= 2;
     const int per = (units + cluster - 1) / cluster;
     // Steps of a thread: one, or two where CTAs wait for SMs and there is one row to

@@ -145,6 +145,15 @@ def test_block_out(gxlib, dev, case, kind, res, out, nxt, T, k, H):
     close(got, want, err)
 
 
+@pytest.mark.parametrize("case", [1, 4, 5, 8])
+@pytest.mark.parametrize("kind,res,out,nxt", [(F32, F32, F32, BF16), (BF16, F32, F32, F16), (F16, F16, F16, F16)])
+@pytest.mark.parametrize("T,k,H", [(3, 2, 8), (77, 3, 256), (9, 40, 136), (2048, 2, 512), (2047, 2, 512), (2100, 35, 264), (5000, 1, 64),
+                                   (300, 3, 4096), (512, 8, 2048), (511, 8, 2048), (300, 33, 4096), (20, 2, 4104), (74, 2, 4104), (75, 2, 4104)])
+def test_block_out_beside_the_borders(gxlib, dev, case, kind, res, out, nxt, T, k, H):
+    """On both sides of what chooses a warp, a CTA, a cluster per row, or rings of rows."""
+    test_block_out(gxlib, dev, case, kind, res, out, nxt, T, k, H)
+
+
 def test_equals_combine(gxlib, dev):
     """The weighted sum alone has gx_combine's bits."""
     rng = np.random.default_rng(3)
