@@ -50,11 +50,11 @@
 //     6e-7, BF16 1.7e-3, which is the rounding of the result). One part, a weight
 //     rounded to 8 or 11 bits, is faster (gated 2048 tokens, 128 experts, 4096 x 1536:
 //     818 us for 956) but leaves 16-bit results 1.7 times as far.
-//   - What bounds it: the warps that make tiles. A chunk of 64 elements takes 900
-//     to 1200 cycles, its MMAs 512 a part; every other role's instructions share their
-//     issue slots (1.5 a cycle in all). 2048 rows, 4096 x 14336: 332 us, 724 TFLOP/s
-//     of products, 1450 with both parts. Short groups pay for whole tiles of weights:
-//     the 1031 tokens x 8 of 64 experts, 1024 x 2048, f32 results, take 172 us.
+//   - What bounds it: the MMAs of both parts, 1024 cycles a chunk of 64 elements, and
+//     hardly less the warps that make tiles, 900 to 1200. 2048 rows, 4096 x 14336: 332
+//     us, 724 TFLOP/s of products, 1450 with both parts; 512 rows keep the tensor pipe
+//     72 % busy. Short groups pay for whole tiles of weights: 1031 tokens x 8 of 64
+//     experts, 1024 x 2048, f32 results, 141 us and 36 more for those of up to 24 rows.
 //   - Tried, no gain: twelve warps in three fours, a register split by setmaxnreg
 //     (spills), blocks loaded straight into registers (278 us where boxes took 220).
 #pragma once

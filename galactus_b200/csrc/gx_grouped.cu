@@ -122,8 +122,10 @@ int grouped_product(int type, const void * as, const void * up, int64_t ne00, in
     const int out_rows = gx::gmm_out_rows(mode) * ctas;
     p.mt = (int32_t)((ne01 + out_rows - 1) / out_rows);
     const void * fn = mode == gx::GMM_DUAL ? (const void *)gx::k_gmm<2, gx::GMM_DUAL, gx::GMM_TILES>
-                      : ctas == 2          ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU, gx::GMM_TILES> : (const void *)gx::k_gmm<2, gx::GMM_PLAIN, gx::GMM_TILES>)
-                                           : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU, gx::GMM_TILES> : (const void *)gx::k_gmm<1, gx::GMM_PLAIN, gx::GMM_TILES>);
+                      : ctas == 2 ? (glu ? (const void *)gx::k_gmm<2, gx::GMM_GLU, gx::GMM_TILES>
+                                         : (const void *)gx::k_gmm<2, gx::GMM_PLAIN, gx::GMM_TILES>)
+                                  : (glu ? (const void *)gx::k_gmm<1, gx::GMM_GLU, gx::GMM_TILES>
+                                         : (const void *)gx::k_gmm<1, gx::GMM_PLAIN, gx::GMM_TILES>);
     const int slot = gmm_slot(ctas, mode);
     cudaError_t e = allow_smem(fn, slot, gx::kGroupedSmem);
     if (e != cudaSuccess) return cuda_status(e);

@@ -22,6 +22,7 @@ namespace {
 
 enum KernelSlot : int { kSlotQ4 = 0, kSlotRows = 8, kSlotTiles = kSlotRows + 6, kSlotEnd = kSlotTiles + 8 };
 static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
+static_assert(gx::kQ4MaxIds == GX_Q4_MAX_IDS && gx::kBlockMaxWidth == GX_BLOCK_MAX_WIDTH, "limits of the header");
 
 // Rows of a group above which matrix tiles are made for the tensor cores. In us
 // with 8, 16, 24, 32 and 48 rows: 64 tokens x 8 of 128 experts, 1536 x 4096, 123,
