@@ -7,10 +7,12 @@
 // plain (y_j = W_e x_j) or gated (act(G_e x_j, U_e x_j)).
 //
 // A job is 32 rows of a matrix (gated: 16 of each) against up to eight rows of x.
-// A warp's step is 64 elements of K: codes become 16-bit floats without a rounding
-// (16 + q, 64 + q), the tensor cores (mma.sync m16n8k16) add their products with x
-// in f32, one more product with a constant takes 16 + 8 or 64 + 8 times sum x off
-// again, and f32 fmas apply the block's d (and m): the only roundings are f32's.
+// A warp's step is 64 elements of K: codes become 16-bit floats without a rounding,
+// the tensor cores (mma.sync m16n8k16) add their products with x in f32, and f32 fmas
+// apply the block's d (and m). F16: q - 8, and for Q4_1 sum x from products with 1,
+// which m + 8 d applies to; BF16: 16 + q, of which products with a constant take 24 or
+// 16 times sum x off again. The roundings are those of f32 sums; the tensor cores
+// cut where f32 would round (a step, for a half of one).
 // (tcgen05 needs its matrices in shared memory, written and fenced: for a few rows
 // that costs more than the products. With many, gx_gmm.cuh does just that.)
 //
@@ -106,6 +108,12 @@ __device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 // high bytes are the same for all. (F16 codes as they stand, the subnormals
 // q 2^-24, would take fewer operations, but the tensor cores add products of
 // subnormals with ten bits less: 4e-5 of the result instead of 1e-7.)
+// (F16: 72 comes off here, so that q - 8 enters the sums. With 64 + q in them and 72
+// or 64 sum x taken off behind, what the tensor cores cut off was that of sums up to
+// sixteen times the result: rows of mean 1, 1024 elements, 1.7e-6 of a Q4_0 result and
+// 8.7e-7 of a Q4_1 one where f32 sums leave 1.8e-7. It rounds nothing, and a Q4_0
+// step needs no product for sum x. BF16's 16 + q, and 24 or 16 sum x behind, stays at
+// 1.1e-7 and 1.8e-7.)
 // (Left shifts are products, which run beside the units for shifts, masks and
 // byte permutations: those are what the kernel needs most.)
 __device__ __forceinline__ uint32_t q4_times(uint32_t w, uint32_t by) {
@@ -128,13 +136,17 @@ __device__ __forceinline__ void q4_codes(uint32_t w, uint32_t (&a)[4]) {
     a[1] = __byte_perm(lo, top, 0x4342);
     a[2] = __byte_perm(hi, top, 0x4140);
     a[3] = __byte_perm(hi, top, 0x4342);
+    if constexpr (!BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = q4_fma<false>(a[i], q4_one<false>(), 0xD480D480u);
+    }
 }
-// What turns sums of the codes above into the wanted ones, as the A operand of
-// a product with the same x: -24 or -72 (Q4_0: sums of q - 8), -16 or -64 (Q4_1:
-// of q)
+// The A operand of the products with x that are wanted beside the codes': BF16, what
+// turns sums of 16 + q into those of q - 8 (Q4_0) or q (Q4_1), -24 or -16; F16, Q4_1:
+// 1, for sum x itself
 template <bool BF16, bool Q41>
-__device__ __forceinline__ constexpr uint32_t q4_shift() {
-    return BF16 ? (Q41 ? 0xC180C180u : 0xC1C0C1C0u) : (Q41 ? 0xD400D400u : 0xD480D480u);
+__device__ __forceinline__ constexpr uint32_t q4_beside() {
+    return BF16 ? (Q41 ? 0xC180C180u : 0xC1C0C1C0u) : 0x3C003C00u;
 }
 
 // the halves of a word, as f32
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     // ------------------------------------------------------------ the jobs
     int take = 0;
     uint32_t round = 0;
-    const uint32_t shift = q4_shift<BF16, Q41>();
+    const uint32_t beside = q4_beside<BF16, Q41>();
     for (int tile = t0; tile <= t1; ++tile) {
         const int i_tile = tile - t0, b = p.buffers == 2 ? i_tile & 1 : 0;
         Q4Tile next = job;
@@ -457,11 +469,11 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                                 const uint32_t s0 = q4_lds(r), s1 = q4_lds(r + 20u);
                                 q4_codes<BF16>(q4_lds(r + 4u + 4u * t), a[i][0][h]);
                                 q4_codes<BF16>(q4_lds(r + 24u + 4u * t), a[i][1][h]);
-                                constexpr float unit = BF16 ? -0.0625f : -0.015625f;       // (sum x comes as -16 or -64 of it)
                                 d[i][0][h] = q4_low(s0);
-                                mn[i][0][h] = __fmul_rn(unit, q4_high(s0));
                                 d[i][1][h] = q4_low(s1);
-                                mn[i][1][h] = __fmul_rn(unit, q4_high(s1));
+                                // (BF16: sum x comes as -16 of it; F16: the codes' sums lack 8 d sum x)
+                                mn[i][0][h] = BF16 ? __fmul_rn(-0.0625f, q4_high(s0)) : __fmaf_rn(8.0f, d[i][0][h], q4_high(s0));
+                                mn[i][1][h] = BF16 ? __fmul_rn(-0.0625f, q4_high(s1)) : __fmaf_rn(8.0f, d[i][1][h], q4_high(s1));
                             } else {
                                 const uint32_t s0 = q4_lds(r), s1 = q4_lds(r + 16u);
                                 const uint32_t w0 = q4_lds(r + 4u * t), w1 = q4_lds(r + 4u + 4u * t);
@@ -474,13 +486,16 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const uint2 lo = x[2 * k], hi = x[2 * k + 1];
-                        float s[4];
-                        q4_mma<BF16>(s, shift, shift, shift, shift, lo.x, lo.y, 0.0f, 0.0f, 0.0f, 0.0f);
-                        q4_mma<BF16>(s, shift, shift, shift, shift, hi.x, hi.y, s[0], s[1], s[2], s[3]);
+                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (BF16 || Q41) {
+                            q4_mma<BF16>(s, beside, beside, beside, beside, lo.x, lo.y, 0.0f, 0.0f, 0.0f, 0.0f);
+                            q4_mma<BF16>(s, beside, beside, beside, beside, hi.x, hi.y, s[0], s[1], s[2], s[3]);
+                        }
 #pragma unroll
                         for (int i = 0; i < MT; ++i) {
                             float c[4];
-                            q4_mma<BF16>(c, a[i][k][0][0], a[i][k][1][0], a[i][k][0][1], a[i][k][1][1], lo.x, lo.y, s[0], s[1], s[2], s[3]);
+                            q4_mma<BF16>(c, a[i][k][0][0], a[i][k][1][0], a[i][k][0][1], a[i][k][1][1], lo.x, lo.y, BF16 ? s[0] : 0.0f,
+                                         BF16 ? s[1] : 0.0f, BF16 ? s[2] : 0.0f, BF16 ? s[3] : 0.0f);
                             q4_mma<BF16>(c, a[i][k][0][2], a[i][k][1][2], a[i][k][0][3], a[i][k][1][3], hi.x, hi.y, c[0], c[1], c[2], c[3]);
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
