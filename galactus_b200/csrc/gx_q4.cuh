@@ -184,7 +184,7 @@ __device__ __forceinline__ void q4_tile(const Q4Params & p, const Q4Groups & g, 
             lo = p.offsets != nullptr ? p.offsets[j.group] : 0;
             hi = p.offsets != nullptr ? p.offsets[j.group + 1] : p.n_rows;
         }
-        j.tiles = lo < 0 || hi - lo < p.lo || hi - lo > p.hi || hi > p.n_rows ? 0 : (hi - lo - 1) / p.cap + 1;
+        j.tiles = q4_group_tiles(lo, hi, p.n_rows, p.lo, p.hi, p.cap);
         if (at < j.before + j.tiles || j.group + 1 >= g.n) break;
         j.before += j.tiles;
     }

@@ -44,4 +44,13 @@ GX_HD constexpr uint32_t q4_smem(bool q41, int64_t K, int warps, int cap, int bu
     return (uint32_t)(warps / 2) * q4_pair_bytes(q41) + (uint32_t)(buffers * cap * q4_x_pitch(K));
 }
 
+// Tiles of `cap` rows in the group of rows [lo, hi), if it has from `least` (>= 1) to
+// `most` rows. Borders that do not ascend or leave the rows, whatever they hold (their
+// difference may pass 32 bits), are those of no rows.
+GX_HD int q4_group_tiles(int lo, int hi, int n_rows, int least, int most, int cap) {
+    if (lo < 0 || hi < lo || hi > n_rows) return 0;
+    const int n = hi - lo;
+    return n < least || n > most ? 0 : (n - 1) / cap + 1;
+}
+
 }  // namespace gx
