@@ -1055,6 +1055,7 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
                         *reinterpret_cast<uint32_t *>(to + (b - from)) = *reinterpret_cast<const uint32_t *>(b);
                 }
                 const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
+                __syncwarp();                            // (that lane's stores, before the arrival that shows them to the other four's warp)
                 if (lane == 0) mbar_arrive_expect_tx(&raw_full[rg][s], sum);
                 __syncwarp();
                 if (bytes != 0u) bulk_g2s(to, from, bytes, &raw_full[rg][s]);
