@@ -64,6 +64,7 @@
 
 #include "gx_grouped_plan.h"
 #include "gx_tc.cuh"
+#include "gx_wait.cuh"
 
 namespace gx {
 
@@ -296,55 +297,7 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-
-// one poll of a phase, with what the peer CTA's arrivals released (suspends for a while)
-template <int CTAS>
-__device__ __forceinline__ bool gmm_poll(uint64_t * bar, uint32_t parity) {
-    if constexpr (CTAS == 1) return mbar_try_wait(bar, parity);
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, "
-        "p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Bounded wait of a thread: gives up after two seconds, or once another role of the CTA has.
-template <int CTAS>
-__device__ __noinline__ bool gmm_wait_long(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-        if (gmm_poll<CTAS>(bar, parity)) return true;
-        if ((i & 63u) == 0u) {
-            if (*abort_flag != 0) return false;
-            const uint64_t t = global_ns();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > 2000000000ull) {
-                *abort_flag = 1;
-                record_error(GX_DEVERR_TIMEOUT);
-                return false;
-            }
-        }
-    }
-}
-template <int CTAS>
-__device__ __forceinline__ bool gmm_wait_one(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
-    return gmm_poll<CTAS>(bar, parity) || gmm_wait_long<CTAS>(bar, parity, abort_flag);
-}
-// the same by a whole warp
-template <int CTAS>
-__device__ __forceinline__ bool gmm_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag) {
-    return __all_sync(0xffffffffu, gmm_wait_one<CTAS>(bar, parity, abort_flag));
-}
-
-// and of a value over the two warps that share a named barrier
+// a value's agreement over the two warps that share a named barrier
 __device__ __forceinline__ bool pair_agrees(int id, bool v) {
     uint32_t r;
     asm volatile(

@@ -435,7 +435,9 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
             if (ok) fetch(next, b ^ 1);
             fetched += ok;
         }
-        // (a wait that runs out makes all that follows NaN; teams stay together)
+        // A wait that runs out makes what this warp adds to its team's sums NaN from here
+        // on, and it hands nothing back: others then compute on what they have, and give up
+        // behind it. Teams stay together.
         ok = gmm_wait<1>(full + b, (uint32_t)((p.buffers == 2 ? i_tile >> 1 : i_tile) & 1), &abort_flag) && ok;
         // (columns behind the last row repeat it)
         const uint32_t xs = smem_u32(xbuf) + (uint32_t)((b * p.cap + min(g, job.rows - 1)) * x_pitch + t * 8);
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                     }
                 }
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(freed + take)) : "memory");
+                if (lane == 0 && ok) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(freed + take)) : "memory");
                 if (++take == S) {
                     take = 0;
                     round ^= 1u;
@@ -523,8 +525,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float * to = part + member * kRed + 2 * t * kQ4Red + 16 * i + 8 * h + g;
-                    to[0] = acc[i][h][0];
-                    to[kQ4Red] = acc[i][h][1];
+                    to[0] = ok ? acc[i][h][0] : kNan;
+                    to[kQ4Red] = ok ? acc[i][h][1] : kNan;
                 }
             q4_sync(team, share);
             for (int i = member * 32 + lane; i < kRows * job.rows; i += 32 * share) {
@@ -546,13 +548,13 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
                 bool nan = false;
                 const int to = gmm_dst_row(p, j, gr.order != nullptr ? gr.order[j] : j, nan);
                 if (nan && r == 0) record_error(GX_DEVERR_DOMAIN);
-                if (to >= 0) store_out(p.dst + (int64_t)to * p.nbd1, row, nan || !ok ? kNan : v, p.out);
+                if (to >= 0) store_out(p.dst + (int64_t)to * p.nbd1, row, nan ? kNan : v, p.out);
             }
             q4_sync(team, share);
         }
         // this warp is done with the tile of x
         __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(empty + b)) : "memory");
+        if (lane == 0 && ok) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(empty + b)) : "memory");
         if (p.buffers == 1 && warp == 0 && tile < t1) {
             ok = ok && gmm_wait<1>(empty + b, (uint32_t)(i_tile & 1), &abort_flag);
             if (ok) fetch(next, 0);
