@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(32 * (MAXW + 1), rows_ctas(MAXW)) k_block_rows
         for (int j = 0; j < kBlockPairs; ++j) xw[u][j] = f2pack(1.0f, 1.0f);
         if (there(u) && p.next_norm != nullptr) block_load<true>(reinterpret_cast<const uint8_t *>(p.next_norm), GMM_F32, first + u * step, p.H, xw[u]);
     }
-    // the next row of the ring, as f32
+    // The next row of the ring, as f32. (A warp whose wait ran out hands no slot back: the
+    // others then compute on what they have, and give up behind it.)
     auto take = [&](int type, uint64_t (&v)[kBlockUnits][kBlockPairs]) {
         ok = gmm_wait<1>(full + at.s, at.round & 1u, &abort_flag) && ok;
         const uint8_t * row = block_ring + at.s * slot_bytes;
@@ -420,13 +421,13 @@ __global__ void __launch_bounds__(32 * (MAXW + 1), rows_ctas(MAXW)) k_block_rows
         for (int u = 0; u < kBlockUnits; ++u)
             if (there(u)) block_load<true>(row, type, first + u * step, p.H, v[u]);
         __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(empty + at.s)) : "memory");
+        if (lane == 0 && ok) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(empty + at.s)) : "memory");
         at.next(slots);
     };
     auto sum = [&](float v, float * part) {
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
-        if (lane == 0) part[warp] = v;
+        if (lane == 0) part[warp] = ok ? v : kNan;
         asm volatile("bar.sync 1, %0;" ::"r"(32 * W) : "memory");
         v = part[0];
         for (int i = 1; i < W; ++i) v = __fadd_rn(v, part[i]);

@@ -86,3 +86,31 @@ def test_streamed_products(late, kind, dtype, K, N, E, rows):
     out = torch.empty((rows, N), dtype=F32, device="cuda")
     args = q4_args(w, x, kind, ids, rows, 1, out)
     check(late, lambda: late.gx_mul_mat_q4(*args), out, [0, 1, 2], [0, 1, 2, 5])
+
+
+@pytest.mark.parametrize("parts", ["plain", "norm", "next", "all"])
+@pytest.mark.parametrize("T,k,H", [(700, 2, 4096), (300, 3, 8192)])
+def test_rings_of_rows(gxlib, late, parts, T, k, H):
+    """One warp of eight (or sixteen) that compute, with each of the sums over the row there or not, and the warp that copies."""
+    rng = np.random.default_rng(H)
+    rand = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()      # noqa: E731
+    y, weights_, res, norm, after = rand(T, k, H), rand(T, k), rand(T, H), rand(H), rand(H)
+    both = torch.empty((2, T, H), device="cuda")
+    d = gxlib._lib.gx_block_desc()
+    d.ne0, d.ne1, d.k, d.scale, d.eps, d.next_eps = H, T, k, 1.0, 1e-6, 1e-6
+    d.y, d.nby1, d.nby2, d.weights = y.data_ptr(), 4 * H, 4 * H * k, weights_.data_ptr()
+    d.residual, d.nbr, d.dst, d.nbd = res.data_ptr(), 4 * H, both.data_ptr(), 4 * H
+    if parts in ("norm", "all"):
+        d.norm = norm.data_ptr()
+    if parts in ("next", "all"):
+        d.next, d.nbn, d.next_norm = both.data_ptr() + 4 * T * H, 4 * H, after.data_ptr()
+    else:
+        both = both[:1]
+    out = both.view(-1, H)
+    check(late, lambda: late.gx_block_out(C.byref(d), torch.cuda.current_stream().cuda_stream), out, [0, 17], [0, 3, H // 512])
+    if parts in ("norm", "all"):
+        # the last expert's row of a block's last token: its warp's share of the norm is lost to the whole row
+        _, n = run(late, lambda: late.gx_block_out(C.byref(d), torch.cuda.current_stream().cuda_stream), out, 17, 3, -1)
+        got, _ = run(late, lambda: late.gx_block_out(C.byref(d), torch.cuda.current_stream().cuda_stream), out, 17, 3, n - 2)
+        bad = torch.isnan(got).sum(1)
+        assert set(bad.tolist()) == {0, H} and int((bad == H).sum()) == both.shape[0]
