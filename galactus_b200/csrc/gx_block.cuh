@@ -396,9 +396,9 @@ __global__ void __launch_bounds__(32 * (MAXW + 1), rows_ctas(MAXW)) k_block_rows
             if (p.shared.p != nullptr) copy(p.shared.p + (int64_t)t * p.shared.nb, p.H * (p.shared.type == GMM_F32 ? 4 : 2));
             if (p.res.p != nullptr) copy(p.res.p + (int64_t)t * p.res.nb, p.H * (p.res.type == GMM_F32 ? 4 : 2));
         }
-        // copies in flight land before the CTA leaves
+        // copies in flight land before the CTA leaves (those that compute may have given up on them)
         volatile int no_flag = 0;
-        for (int i = 0; i < slots && !ok; ++i)
+        for (int i = 0; i < slots; ++i)
             if (issued > i) gmm_wait<1>(full + i, (uint32_t)((issued - 1 - i) / slots & 1), &no_flag);
         return;
     }
