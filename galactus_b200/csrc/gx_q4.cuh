@@ -567,10 +567,8 @@ __global__ void __launch_bounds__(32 * kQ4Warps, 1) k_q4(const __grid_constant__
     volatile int none = 0;
     for (int i = 0; i < S && !ok; ++i)
         if (issued > i) gmm_wait<1>(filled + i, (uint32_t)((issued - 1 - i) / S & 1), &none);
-    if (!ok && warp == 0) {
-        const int i = fetched - 1;
+    for (int i = max(0, fetched - p.buffers); i < fetched && !ok && warp == 0; ++i)
         gmm_wait<1>(full + (p.buffers == 2 ? i & 1 : 0), (uint32_t)((p.buffers == 2 ? i >> 1 : i) & 1), &none);
-    }
 }
 
 }  // namespace gx
