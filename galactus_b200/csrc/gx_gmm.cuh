@@ -632,6 +632,20 @@ __device__ __forceinline__ void q4_put(float (&w)[8], uint32_t to, int parts) {
     }
 }
 
+// NaN in place of what a warp gave up: 32 matrix rows from m on of tile t and those behind it
+template <int ROUND, int SRC>
+__device__ __noinline__ void gmm_fill_nan(const GmmParams & p, const int32_t * pre, int t, int units, int tiles, int rows, int m) {
+    for (; t < tiles; t += units) {
+        const GmmTile q = gmm_tile<ROUND, SRC>(p, pre, t, rows);
+        const int n = q.m0 + m + (int)(threadIdx.x & 31);
+        for (int j = q.row0; j < q.row0 + q.cnt && n < p.N; ++j) {
+            bool nan = false;
+            const int to = gmm_dst_row(p, j, p.gather != 0 || p.scatter != 0 ? p.order[j] : 0, nan);
+            if (to >= 0) store_out(p.dst + (int64_t)to * p.nbd1, n, kNan, p.out);
+        }
+    }
+}
+
 template <int CTAS, int MODE, int SRC>
 __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_threads(MODE), 1)
     k_gmm(const __grid_constant__ GmmParams p) {
@@ -1131,7 +1145,8 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
         const uint32_t lanes = (uint32_t)quad << 21, dsum = tbase + lanes + 2u * (uint32_t)p.acc;
         int it = 0, xb = 0, i_tile = 0;
         bool ok = true;
-        for (Work w = start(); w.t < tiles && ok; advance(w)) {
+        Work w = start();
+        for (; w.t < tiles && ok; advance(w)) {
             const GmmTile q = gmm_tile<kRound, SRC>(p, pre, w.t, kOut * CTAS);
             const int k0 = first_chunk(w), k1 = end_chunk(w);
             const int nseg = p.seg ? (k1 - k0 + p.seg - 1) / p.seg : 1;
@@ -1296,6 +1311,9 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
                 if (lane == 0) gmm_arrive<CTAS>(acc_empty + it % kBufs);
             }
             ++it;
+        }
+        if constexpr (SRC != GMM_TILES) {
+            if (!ok) gmm_fill_nan<kRound, SRC>(p, pre, w.t, units, tiles, kOut * CTAS, rank * kOut + (GLU ? quad & 1 : quad) * 32);
         }
     }
     tc_fence_before();

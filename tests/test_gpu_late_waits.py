@@ -114,3 +114,36 @@ def test_rings_of_rows(gxlib, late, parts, T, k, H):
         got, _ = run(late, lambda: late.gx_block_out(C.byref(d), torch.cuda.current_stream().cuda_stream), out, 17, 3, n - 2)
         bad = torch.isnan(got).sum(1)
         assert set(bad.tolist()) == {0, H} and int((bad == H).sum()) == both.shape[0]
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q4_1])
+@pytest.mark.parametrize("glu", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("scatter", [False, True])
+def test_tiles_of_many_rows(late, kind, glu, dtype, scatter):
+    """The warps that read the accumulators, at their last wait (all else has then ended): their share of the last tile is NaN, and
+    nothing keeps what dst held before."""
+    rng = np.random.default_rng(5)
+    E, N, K, P = 3, 300, 512, 700
+    w, up = weights(rng, E, N, K, kind), weights(rng, E, N, K, kind)
+    x = torch.from_numpy(rng.standard_normal((P, K))).cuda().to(F16)
+    offsets = torch.tensor([0, 200, 430, P], dtype=torch.int32, device="cuda")
+    order = torch.from_numpy(rng.permutation(P).astype(np.int32)).cuda()
+    out = torch.empty((P, N), dtype=dtype, device="cuda")
+    head = (kind, w.data_ptr(), up.data_ptr()) if glu else (kind, w.data_ptr())
+    args = head + (K, N, w.shape[2], N * w.shape[2], E, 1, x.data_ptr(), P, 2 * K, None, offsets.data_ptr(), order.data_ptr(), P, 1, int(scatter))
+    args += ((0, 0.0, 0.0) if glu else ()) + (0 if dtype == F32 else 1, out.data_ptr(), N * out.element_size())
+    f = late.gx_mul_mat_q4_glu if glu else late.gx_mul_mat_q4
+    call = lambda: f(*args, torch.cuda.current_stream().cuda_stream)                           # noqa: E731
+    good, _ = run(late, call, out, -1, -1, -1)
+    tried = 0
+    for block in (0, 1, 6):
+        for warp in range(4, 8):
+            same, n = run(late, call, out, block, warp, -1)
+            assert torch.equal(same, good)
+            if n:
+                got, _ = run(late, call, out, block, warp, n - 1)
+                nan = torch.isnan(got)
+                assert bool((nan | (got == good)).all()), (block, warp)
+                tried += int(nan.any())
+    assert tried >= 8
