@@ -903,10 +903,15 @@ __global__ void __launch_bounds__(SRC != GMM_TILES ? gmm_q4_threads(MODE) : gmm_
                     if (ok) gmm_commit<CTAS>(acc_full + b);
                 }
             }
+            // MMAs in flight end before TMEM is freed and the CTA leaves, whoever gave up: where this
+            // thread did not, the last chunk's commit says so
+            volatile int none = 0;
             if (!ok) {
-                volatile int none = 0;
                 gmm_commit<CTAS>(&drained);
                 gmm_wait_one<CTAS>(&drained, 0, &none);
+            } else if (it > 0) {
+                const bool wrap = at.s == 0;
+                gmm_wait_one<CTAS>(empty + (wrap ? p.stages : at.s) - 1, (at.round - (wrap ? 1u : 0u)) & 1u, &none);
             }
         }
         __syncwarp();
