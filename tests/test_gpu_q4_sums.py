@@ -60,3 +60,22 @@ def test_rows_with_a_mean(gxlib, dev, kind, dtype, mean, K):
     adds = (1 if kind == Q4_0 else 2) * (y ** 2).sum(-1)
     bound = (off.sum(-1) * 2.0 ** -46 + adds * 2.0 ** -48).mean().sqrt()
     assert float((got - y[..., -1]).square().mean().sqrt()) <= float(bound)
+
+
+@pytest.mark.parametrize("kind", [Q4_0, Q4_1])
+@pytest.mark.parametrize("rows", [8, 24, 25, 80])
+def test_weights_at_the_border_of_the_rows_type(gxlib, dev, kind, rows):
+    """F16 rows: the largest weights, 65504 and a little less, on both sides of the length from which tiles of weights are made. (d is
+    8188: every weight is a multiple of 4 of at most 15 bits, and so is its product with an element of -1, 0 or 1.)"""
+    rng = np.random.default_rng(rows)
+    N, K = 40, 128
+    w, _, _, q = centred(rng, N, K, kind)
+    b = w.cpu().numpy().reshape(N, K // 32, BLOCK[kind])
+    b[..., 0:2] = np.frombuffer(np.float16(8188.0).tobytes(), np.uint8)
+    if kind == Q4_1:
+        b[..., 2:4] = np.frombuffer(np.float16(-65504.0).tobytes(), np.uint8)
+    x = torch.from_numpy(rng.integers(-1, 2, (rows, K)).astype(np.float16)).cuda()
+    want = x.double() @ (8188.0 * (q - 8.0)).view(N, K).T
+    got = gxlib.mul_mat_q4(torch.from_numpy(b.reshape(1, N, -1)).cuda(), x, type=kind, out_dtype=F32)
+    # (whole numbers below 2^24 after a division by 4)
+    assert torch.equal(got.double(), want)
