@@ -72,9 +72,9 @@ def mul_mat_q4(w, x, *, type: int, ids=None, offsets=None, order=None, n_rows: i
 
     ids (int32, any contiguous shape, at most 256 of them): row j = x[j //
     gather] times the matrix ids[j], to result row j; rows of negative ids are
-    left as they were (uninitialised in a result allocated here). offsets (and
-    order): the groups of group_rows, as in mul_mat_grouped. Neither: one matrix
-    for all rows."""
+    left as they were (uninitialised in a result allocated here); many rows of
+    one matrix are faster as a group. offsets (and order): the groups of
+    group_rows, as in mul_mat_grouped. Neither: one matrix for all rows."""
     return _q4("gx_mul_mat_q4", w, None, x, type, ids, offsets, order, n_rows, gather, scatter, (), out, out_dtype, stream)
 
 

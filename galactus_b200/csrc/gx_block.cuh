@@ -10,9 +10,10 @@
 // Every row is read once and every result written once; what lies between stays in
 // f32 registers (16 elements a thread). Two kernels:
 //   k_block       narrow rows: a warp each, without a barrier (65536 rows of 128, sum,
-//                 residual and next norm: 45 us, 109 with a CTA each). Others: a CTA per row, or a cluster of up to eight whose sums of squares
-//                 are exchanged through their shared memories (wide rows, or so few
-//                 wide rows that most SMs would idle): latency bound. One token:
+//                 residual and next norm: 45 us, 109 with a CTA each). Others: a CTA per
+//                 row, or a cluster of up to eight whose sums of squares are exchanged
+//                 through their shared memories (wide rows, or so few wide rows that
+//                 most SMs would idle): latency bound. One token:
 //                 2.2 us (2880 elements, a norm), 3.4 us (2048 x 8 experts, with
 //                 residual and next norm), of which a launch alone is about 2.
 //   k_block_rows  many rows: HBM bound, as far as the instructions keep up. 8192 rows

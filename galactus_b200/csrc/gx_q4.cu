@@ -25,9 +25,11 @@ static_assert(kSlotEnd <= kKernelSlots, "one slot per kernel");
 static_assert(gx::kQ4MaxIds == GX_Q4_MAX_IDS && gx::kBlockMaxWidth == GX_BLOCK_MAX_WIDTH, "limits of the header");
 
 // Rows of a group above which matrix tiles are made for the tensor cores. In us
-// with 8, 16, 24, 32 and 48 rows: 64 tokens x 8 of 128 experts, 1536 x 4096, 123,
-// 123, 114, 119, 126; 1031 tokens x 8 of 64, 1024 x 2048, 176, 172, 172, 170, 176;
-// one matrix of 4096 x 14336 with 32 rows 45, 44, 45, 56, 55.
+// with 16, 24, 32 and 48 rows: 64 tokens x 8 of 128 experts, 1536 x 4096, 117, 121,
+// 125, 124; 1031 tokens x 8 of 64, 1024 x 2048, 172, 172, 176, 180; gated, 2048 tokens
+// x 8 of 128, 4096 x 1536, 1001, 1010, 1013, 1032; one matrix of 4096 x 14336 with 32
+// rows 44, 45, 56, 55. (16 and 24 differ by as much as a case does from run to run;
+// below the border no sum is of a weight's parts.)
 constexpr int64_t kTileRows = 24;
 
 // A launch that may begin while the kernel before it on the stream ends: the

@@ -25,13 +25,16 @@
 //     warp 2800 cycles for 32 of them.
 //   - Few jobs: warps share a job's K (p.share) and add their sums in their order, so
 //     the same call gives the same bits.
-// What bounds it: instructions. A step is 178 of them, 87 cycles per SM, 83 of those
-// on the units for shifts, masks, byte permutations and conversions alone (64 lanes
-// a cycle): 3.5 TB/s of weights, 264 MB in 74 us where the copies by themselves take
-// 47. 19 tokens x 8 of 64 experts, gated, 2048 x 1024, Q4_1: 46 us, 1.9 TB/s (two and
-// three tiles of rows for the popular experts); one token, 8 of 128, 768 x 2048: 9.3 us,
-// set-up and one round of jobs; 2880 x 2880, 4 experts, gated: 23 us, of which the
-// copies of 16 bytes take 20.
+// What bounds it: instructions and their latency. 264 MB of Q4_0 and one BF16 row: 76
+// us, 3.5 TB/s (F16 67, 3.9; the copies by themselves 47). A step is some 180 of them
+// and 86 cycles per SM, 2.2 a cycle of four that could be; no unit is full (the one for
+// shifts, masks and permutations 51 %, tensor cores 28 %, DRAM 36 %). A warp issues
+// every 5.6 cycles, four warps to a scheduler: 1.0 goes to the operation before, 0.9 to
+// other warps' turns, 0.8 to full units, 0.7 to fetching instructions.
+// 19 tokens x 8 of 64 experts, gated, 2048 x 1024, Q4_1: 46 us, 1.9 TB/s (two and three
+// tiles of rows for the popular experts); one token, 8 of 128, 768 x 2048: 9.3 us, set-up
+// and one round of jobs; 2880 x 2880, 4 experts, gated: 23 us, of which the copies of
+// 16 bytes take 20.
 #pragma once
 
 #include <climits>
@@ -112,8 +115,9 @@ __device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 // or 64 sum x taken off behind, what the tensor cores cut off was that of sums up to
 // sixteen times the result: rows of mean 1, 1024 elements, 1.7e-6 of a Q4_0 result and
 // 8.7e-7 of a Q4_1 one where f32 sums leave 1.8e-7. It rounds nothing, and a Q4_0
-// step needs no product for sum x. BF16's 16 + q, and 24 or 16 sum x behind, stays at
-// 1.1e-7 and 1.8e-7.)
+// step needs no product for sum x: 264 MB and one row 70 -> 67 us; Q4_1 keeps those
+// products, 77 -> 81. BF16's 16 + q, and 24 or 16 sum x behind, stays at 1.1e-7 and
+// 1.8e-7.)
 // (Left shifts are products, which run beside the units for shifts, masks and
 // byte permutations: those are what the kernel needs most.)
 __device__ __forceinline__ uint32_t q4_times(uint32_t w, uint32_t by) {

@@ -379,10 +379,13 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
  *   Q4_1  { f16 d; f16 m; u8 qs[16] }  w = d q + m
  * gx_mul_mat_id refuses these types (it promises ggml's bits, with activations
  * quantised to 8 bits); here rows keep their 16 bits, products are exact, sums
- * are f32 and the result is rounded once to type_dst (F32, F16, BF16). (Calls of
- * more than 24 rows without ids take a Q4_1 weight, d q + m, to 22 bits with F16
- * rows, and to 24 or, for 16-bit results, 16 with BF16 rows; a weight must lie in
- * the range of the rows' type.)
+ * are f32 and the result is rounded once to type_dst (F32, F16, BF16). (The tensor
+ * cores cut their sums where f32 would round them: f32 results are as far from the
+ * exact ones as f32 sums are up to 24 rows of a matrix, and some 6e-7 of their size
+ * above. There a weight is two or three 16-bit parts: Q4_0's d (q - 8) whole, Q4_1's
+ * d q + m to 22 bits with F16 rows, and to 24 or, for 16-bit results, 16 with BF16
+ * rows. With F16 rows it must not be beyond 65504, which shorter groups and calls
+ * with ids do not ask.)
  *   dst row of j = W_e (b row of j)
  * The matrix of a row is named in one of three ways:
  *   ids      device i32 [n_rows], n_rows <= GX_Q4_MAX_IDS: row j's expert (decode:
@@ -390,14 +393,16 @@ int gx_lora_mul_mat(const gx_lora_desc * desc, const void * x, int64_t ne11, int
  *            k where b has a row per token, 1 or 0 where it has one per pair), dst
  *            row j; order and offsets are NULL, scatter is not read. A negative id
  *            leaves its row of dst as it was; one >= n_as is reported
- *            (gx_device_error) and its row left too.
+ *            (gx_device_error) and its row left too. Each eight rows of an expert
+ *            read its matrix anew: many rows of one are faster as a group.
  *   offsets  device i32 [n_as + 1] and order as gx_group_rows gives them, any
  *            number of rows, with gather and scatter as in gx_mul_mat_grouped
  *   neither  n_as = 1: all n_rows rows with the one matrix (a dense projection)
  * Offsets, row indexes and what is reported: as gx_mul_mat_grouped (borders that
  * name more rows than n_rows are reported, and groups of one kind, short or long,
  * may be computed all the same). A row of b with an infinity or a NaN makes its
- * own results NaN, and no other.
+ * own results infinite or NaN, and no other. Behind a wait that ran out
+ * (GX_DEVERR_TIMEOUT) results are NaN.
  * Requires ne00 % 64 == 0, ne00 <= GX_Q4_MAX_K; 16-byte aligned as, b and nb11; nb01 and nb02
  * multiples of 4; n_as <= 8192. dst may not overlap an input. The calls follow
  * one another on a stream without a gap (programmatic launches), can be
@@ -423,8 +428,10 @@ int gx_mul_mat_q4_glu(int type, const void * gate, const void * up, int64_t ne00
  * norm(v) = v / sqrt(mean(v^2) + eps) * its weight (ggml's rms_norm and mul).
  * All in f32 (the sum over s in slot order with a rounding per product and per
  * add, as gx_combine), each result rounded once; next is the norm of the f32
- * out. Rows have F32, F16 or BF16 elements; sums of their squares must be finite
- * in f32. Results may lie in place of an input with the same type and strides;
+ * out. Rows (fewer than 2^28 - 8192) have F32, F16 or BF16 elements; sums of their
+ * squares must be finite in f32 (where one is not, elements are zero, and NaN where
+ * they are infinite). Behind a wait that ran out (GX_DEVERR_TIMEOUT) results are NaN.
+ * Results may lie in place of an input with the same type and strides;
  * otherwise nothing may overlap a result. */
 #define GX_BLOCK_MAX_WIDTH 65536
 #define GX_GATE_NONE    0
